@@ -59,6 +59,12 @@ extern "C" {
  * halves the volume's footprint and the bytes its staging reads. */
 #define TP_F16S 2
 
+/* The matching operators' storage types besides TP_F32 (binary16 and bfloat16
+ * rows; every value is widened exactly to fp32 and results are rounded once).
+ * No projector takes them. */
+#define TP_F16 3
+#define TP_BF16 4
+
 #define TP_LINEAR 0
 #define TP_CUBIC 1
 
@@ -285,6 +291,86 @@ int tp_from_fourier(int dtype, int dim, int64_t batch, int64_t boxsize, int64_t 
  * out may alias data. */
 int tp_normalize_reconstruction(int dtype, const void* data, const void* weights, int64_t elems, double reg,
                                 void* out, void* stream);
+
+/* ---------------------------------------------------------------- matching
+ *
+ * What a caller does between projecting references and backprojecting images:
+ * scores of images against references, posteriors over the scored hypotheses,
+ * and images in class order.  No counterpart in the reference.  `work` is
+ * device memory of at least the matching tp_*_work() bytes (16-byte aligned,
+ * uninitialised, free again once the call's work on the stream is done; it may
+ * be NULL where that is 0). */
+
+/* Rows in 8-bit blocks: x [rows, cols] (TP_F32, TP_F16 or TP_BF16; rows
+ * `row_stride` elements apart, values of a row adjacent) becomes
+ *   codes   [rows, 128 * nb] e4m3 bytes, nb = ceil(cols / 128), zero past cols
+ *   scales  [nb, tp_scale_rows(rows)] bytes: 127 + e, 127 for the padding rows
+ * with e the least exponent >= -127 that keeps a block's largest finite
+ * magnitude within 448 * 2^e (0 for a block of zeros), and a value's code that
+ * of x * 2^-e to nearest even (NaN for one that is not finite). */
+int64_t tp_scale_rows(int64_t rows);
+int tp_quantize_blocks(int dtype, const void* x, int64_t rows, int64_t cols, int64_t row_stride, void* codes,
+                       void* scales, void* stream);
+
+/* scores[m, n] = bias[n] + <row m of a, row n of b>, both in 8-bit blocks, summed
+ * in fp32 (bias fp32, optional; scores TP_F32 or TP_BF16). */
+int64_t tp_block_scores_work(int64_t rows_a, int64_t rows_b, int64_t blocks);
+int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, const void* codes_b,
+                    const void* scales_b, int64_t rows_b, int64_t blocks, const void* bias, int out_dtype,
+                    void* scores, void* work, int64_t work_bytes, void* stream);
+
+/* Log probabilities of rows of scores [rows, candidates] (TP_F32, TP_F16 or
+ * TP_BF16, rows `row_stride` apart): p = softmax(scores / temperature) over
+ * the allowed candidates.
+ *   given      [rows, givens] int64, optional: candidates whose log probability is
+ *              wanted; -1 for none (0 is returned), NaN for any other out of range
+ *   mask       optional bytes, nonzero where allowed: [candidates] with mask_stride
+ *              0, else rows mask_stride apart.  What a masked place holds is not used
+ *   top        0 .. 64 best alternatives, ties to the lowest index; -1 / -inf past
+ *              the allowed ones (scores of -inf count as not allowed)
+ * Outputs fp32: given_log_probs [rows, givens], entropy [rows], log_sum [rows] (of
+ * exp(score / temperature)), top_log_probs [rows, top]; top_index int64 [rows, top];
+ * stats [rows, 4], which the gradient reads.  A row that allows nothing has
+ * log_sum and log probabilities -inf and entropy 0. */
+int64_t tp_log_probs_work(int64_t rows, int64_t candidates, int64_t top);
+int tp_log_probs(int dtype, const void* scores, int64_t rows, int64_t candidates, int64_t row_stride,
+                 const void* given, int64_t givens, const void* mask, int64_t mask_stride, int64_t top,
+                 double temperature, void* given_log_probs, void* entropy, void* log_sum, void* top_log_probs,
+                 void* top_index, void* stats, void* work, int64_t work_bytes, void* stream);
+
+/* d_scores [rows, candidates] (row-major, of `dtype`) from the upstream gradients
+ * of the four fp32 outputs, each optional; zero where masked. */
+int tp_log_probs_back(int dtype, const void* scores, int64_t rows, int64_t candidates, int64_t row_stride,
+                      const void* given, int64_t givens, const void* mask, int64_t mask_stride, int64_t top,
+                      double temperature, const void* top_index, const void* stats, const void* d_given,
+                      const void* d_entropy, const void* d_log_sum, const void* d_top, void* d_scores, void* stream);
+
+/* Slots sorted by class, stably: class_ids [slots] (id_bytes 4 or 8) ->
+ *   order    [slots] int32: the slot at each place
+ *   slot     [slots] int32: the place of each slot
+ *   offsets  [classes + 1] int32: each class's first place, then the end of all
+ * 1 .. 4096 classes; ids outside [0, classes) are dropped: their slots follow all
+ * others. */
+int64_t tp_sort_by_class_work(int64_t slots, int64_t classes);
+int tp_sort_by_class(int id_bytes, const void* class_ids, int64_t slots, int64_t classes, void* order, void* slot,
+                     void* offsets, void* work, int64_t work_bytes, void* stream);
+
+/* Rows to their places and back, each the other's adjoint.  x and out [rows, cols];
+ * sorted [rows * k, cols] in class order; slot [rows, k] and `kept` (the address
+ * of offsets[classes]) from tp_sort_by_class; weights [rows, k] fp32, optional (ones).
+ *   tp_spread_rows  sorted[slot[t, j]] = weights[t, j] * x[t], zero where dropped
+ *   tp_gather_rows  out[t] = sum over j of weights[t, j] * sorted[slot[t, j]], in
+ *                   fp32, without the dropped
+ * With `other` and d_weights (both or neither) each also gives the weights'
+ * gradient, fp32, 0 where dropped: tp_spread_rows d_weights[t, j] =
+ * <x[t], other[slot[t, j]]> with other [rows * k, cols], tp_gather_rows
+ * <other[t], sorted[slot[t, j]]> with other [rows, cols]. */
+int tp_spread_rows(int dtype, const void* x, int64_t rows, int64_t cols, int64_t k, const void* slot,
+                   const void* kept, const void* weights, void* sorted, const void* other, void* d_weights,
+                   void* stream);
+int tp_gather_rows(int dtype, const void* sorted, int64_t rows, int64_t cols, int64_t k, const void* slot,
+                   const void* kept, const void* weights, void* out, const void* other, void* d_weights,
+                   void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,8 +5,8 @@ Outputs (both inside torch_projectors/, so they travel with the tree):
   libtorch_projectors_hip.so  the HIP kernels + the C ABI of
                               include/torch_projectors_hip.h (hipcc, gfx950)
   _C.so                       the PyTorch dispatcher registration
-                              (csrc/torch_projectors.cpp), linked against the
-                              library above with an $ORIGIN rpath
+                              (csrc/torch_projectors.cpp, csrc/torch_matching.cpp),
+                              linked against the library above with an $ORIGIN rpath
 
 Kernel flags: -O3, no fast-math, -ffp-contract=off (sample coordinates and
 stencil weights must round exactly like the reference CPU code), and packed
@@ -29,6 +29,7 @@ BUILD = os.path.join(HERE, "_build")
 HIP_SRC = os.path.join(HERE, "csrc", "hip")
 LIB = os.path.join(PKG, "libtorch_projectors_hip.so")
 EXT = os.path.join(PKG, "_C.so")
+EXT_SRC = ("torch_projectors.cpp", "torch_matching.cpp")
 
 ARCH = os.environ.get("TP_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
@@ -92,11 +93,19 @@ def _torch_flags():
     return inc, defs, libs
 
 
-def build_ext():
+def build_ext(jobs=8):
     inc, defs, libs = _torch_flags()
-    src = os.path.join(HERE, "csrc", "torch_projectors.cpp")
+    os.makedirs(BUILD, exist_ok=True)
+
+    def compile_one(name):
+        obj = os.path.join(BUILD, name + ".o")
+        _run([HIPCC, "-O2", "-fPIC", "-std=c++17", "-w", *defs, *inc, "-c", os.path.join(HERE, "csrc", name), "-o", obj])
+        return obj
+
+    with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        objs = list(ex.map(compile_one, EXT_SRC))
     tmp = EXT + ".tmp"
-    _run([HIPCC, "-O2", "-fPIC", "-std=c++17", "-shared", "-w", *defs, *inc, src, "-o", tmp,
+    _run([HIPCC, "-fPIC", "-shared", *objs, "-o", tmp,
           f"-L{PKG}", "-ltorch_projectors_hip", "-Wl,-rpath,$ORIGIN", *libs])
     os.replace(tmp, EXT)
     return EXT
@@ -105,7 +114,7 @@ def build_ext():
 def build(jobs=8, only_lib=False, quiet=False):
     out = [build_lib(jobs)]
     if not only_lib:
-        out.append(build_ext())
+        out.append(build_ext(jobs))
     if not quiet:
         for p in out:
             print("built", os.path.relpath(p, ROOT))

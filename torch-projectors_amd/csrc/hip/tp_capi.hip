@@ -23,6 +23,7 @@
 
 #include "../../../include/torch_projectors_hip.h"
 #include "tp_launch.hh"
+#include "tp_match.hh"
 
 namespace {
 
@@ -1044,6 +1045,48 @@ int backproject_back(int dim, int dtype, const void* gdata, const void* gw, int6
                     "backprojection backward launch");
 }
 
+// ------------------------------------------------------------------ matching
+int match_dtype(int dtype) {
+    if (dtype != TP_F32 && dtype != TP_F16 && dtype != TP_BF16)
+        return fail("dtype must be TP_F32, TP_F16 or TP_BF16");
+    return TP_OK;
+}
+
+int probs_args(int dtype, const void* scores, int64_t rows, int64_t candidates, int64_t row_stride, const void* given,
+               int64_t givens, const void* mask, int64_t mask_stride, int64_t top, double temperature,
+               tp::ProbsArgs& a) {
+    TP_TRY(match_dtype(dtype));
+    if (rows < 0 || givens < 0) return fail("rows and givens must be non-negative");
+    if (candidates < 1) return fail("there must be at least one candidate");
+    if (rows > kInt32Max || candidates > kInt32Max) return fail("rows and candidates must be < 2^31");
+    if (row_stride < 0 || mask_stride < 0) return fail("strides must be non-negative");
+    if (top < 0 || top > tp::kMaxTop) return fail("top must be in [0, 64]");
+    // (as the kernels hold it: not 0 or infinite in fp32)
+    const float t = float(temperature);
+    if (!(t >= 1e-30f && t <= 1e30f)) return fail("temperature must be in [1e-30, 1e30]");
+    if (givens && rows) TP_TRY(need(given, "given"));
+    a = tp::ProbsArgs{dtype, scores, rows, candidates, row_stride, static_cast<const int64_t*>(given), givens,
+                      static_cast<const uint8_t*>(mask), mask_stride, int(top), t};
+    return TP_OK;
+}
+
+int route_args(int dtype, int64_t rows, int64_t cols, int64_t k, const void* slot, const void* kept,
+               const void* weights, const void* other, const void* d_weights, tp::RouteArgs& a) {
+    TP_TRY(match_dtype(dtype));
+    if (rows < 0 || cols < 0 || k < 0) return fail("rows, cols and k must be non-negative");
+    if (rows > kInt32Max || cols > kInt32Max || k > kInt32Max || (k && rows > kInt32Max / k))
+        return fail("rows * k and cols must be < 2^31");
+    if (rows && k) {
+        TP_TRY(need(slot, "slot"));
+        TP_TRY(need(kept, "kept"));
+        if (cols && (other != nullptr) != (d_weights != nullptr))
+            return fail("other and d_weights must be given together");
+    }
+    a = tp::RouteArgs{dtype, rows, cols, int(k), static_cast<const int*>(slot), static_cast<const int*>(kept),
+                      static_cast<const float*>(weights)};
+    return TP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1319,6 +1362,166 @@ int tp_normalize_reconstruction(int dtype, const void* data, const void* weights
     TP_TRY(need(out, "out"));
     return launched(tp::launch_normalize(dtype, data, weights, elems, reg, out, static_cast<hipStream_t>(stream)),
                     "normalisation launch");
+}
+
+// ------------------------------------------------------------------ matching
+int64_t tp_scale_rows(int64_t rows) { return rows < 0 ? 0 : tp::scale_rows(rows); }
+
+int tp_quantize_blocks(int dtype, const void* x, int64_t rows, int64_t cols, int64_t row_stride, void* codes,
+                       void* scales, void* stream) {
+    g_err.clear();
+    TP_TRY(match_dtype(dtype));
+    if (rows < 0 || cols < 0) return fail("rows and cols must be non-negative");
+    if (row_stride < 0) return fail("row_stride must be non-negative");
+    if (rows > kInt32Max || cols > kInt32Max) return fail("rows and cols must be < 2^31");
+    if (rows == 0 || cols == 0) return TP_OK;
+    TP_TRY(need(x, "x"));
+    TP_TRY(need(codes, "codes"));
+    TP_TRY(need(scales, "scales"));
+    return launched(tp::launch_quantize_blocks(dtype, x, rows, cols, row_stride, codes, scales,
+                                               static_cast<hipStream_t>(stream)),
+                    "quantisation launch");
+}
+
+int64_t tp_block_scores_work(int64_t rows_a, int64_t rows_b, int64_t blocks) {
+    if (rows_a <= 0 || rows_b <= 0 || blocks <= 0) return 0;
+    return tp::block_scores_work(rows_a, rows_b, blocks);
+}
+
+int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, const void* codes_b,
+                    const void* scales_b, int64_t rows_b, int64_t blocks, const void* bias, int out_dtype,
+                    void* scores, void* work, int64_t work_bytes, void* stream) {
+    g_err.clear();
+    if (out_dtype != TP_F32 && out_dtype != TP_BF16) return fail("out_dtype must be TP_F32 or TP_BF16");
+    if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
+    if (blocks < 1) return fail("blocks must be positive");
+    if (rows_a > kInt32Max || rows_b > kInt32Max || blocks > kInt32Max / tp::kScaleBlock)
+        return fail("rows and columns must be < 2^31");
+    if (rows_a == 0 || rows_b == 0) return TP_OK;
+    TP_TRY(need(codes_a, "codes_a"));
+    TP_TRY(need(scales_a, "scales_a"));
+    TP_TRY(need(codes_b, "codes_b"));
+    TP_TRY(need(scales_b, "scales_b"));
+    TP_TRY(need(scores, "scores"));
+    const int64_t need_bytes = tp::block_scores_work(rows_a, rows_b, blocks);
+    if (need_bytes) TP_TRY(need(work, "work"));
+    if (work_bytes < need_bytes) return fail("work is smaller than tp_block_scores_work");
+    return launched(tp::launch_block_scores(codes_a, scales_a, rows_a, codes_b, scales_b, rows_b, blocks, bias,
+                                            out_dtype, scores, work, static_cast<hipStream_t>(stream)),
+                    "score launch");
+}
+
+int64_t tp_log_probs_work(int64_t rows, int64_t candidates, int64_t top) {
+    if (rows <= 0 || candidates <= 0 || top < 0 || top > tp::kMaxTop) return 0;
+    return tp::log_probs_work(rows, candidates, int(top));
+}
+
+int tp_log_probs(int dtype, const void* scores, int64_t rows, int64_t candidates, int64_t row_stride,
+                 const void* given, int64_t givens, const void* mask, int64_t mask_stride, int64_t top,
+                 double temperature, void* given_log_probs, void* entropy, void* log_sum, void* top_log_probs,
+                 void* top_index, void* stats, void* work, int64_t work_bytes, void* stream) {
+    g_err.clear();
+    tp::ProbsArgs a;
+    TP_TRY(probs_args(dtype, scores, rows, candidates, row_stride, given, givens, mask, mask_stride, top, temperature,
+                      a));
+    if (rows == 0) return TP_OK;
+    TP_TRY(need(scores, "scores"));
+    if (givens) TP_TRY(need(given_log_probs, "given_log_probs"));
+    TP_TRY(need(entropy, "entropy"));
+    TP_TRY(need(log_sum, "log_sum"));
+    if (top) {
+        TP_TRY(need(top_log_probs, "top_log_probs"));
+        TP_TRY(need(top_index, "top_index"));
+    }
+    TP_TRY(need(stats, "stats"));
+    const int64_t need_bytes = tp::log_probs_work(rows, candidates, int(top));
+    if (need_bytes) TP_TRY(need(work, "work"));
+    if (work_bytes < need_bytes) return fail("work is smaller than tp_log_probs_work");
+    return launched(tp::launch_log_probs(a, static_cast<float*>(given_log_probs), static_cast<float*>(entropy),
+                                         static_cast<float*>(log_sum), static_cast<float*>(top_log_probs),
+                                         static_cast<int64_t*>(top_index), static_cast<float*>(stats), work,
+                                         static_cast<hipStream_t>(stream)),
+                    "log probability launch");
+}
+
+int tp_log_probs_back(int dtype, const void* scores, int64_t rows, int64_t candidates, int64_t row_stride,
+                      const void* given, int64_t givens, const void* mask, int64_t mask_stride, int64_t top,
+                      double temperature, const void* top_index, const void* stats, const void* d_given,
+                      const void* d_entropy, const void* d_log_sum, const void* d_top, void* d_scores, void* stream) {
+    g_err.clear();
+    tp::ProbsArgs a;
+    TP_TRY(probs_args(dtype, scores, rows, candidates, row_stride, given, givens, mask, mask_stride, top, temperature,
+                      a));
+    if (rows == 0) return TP_OK;
+    TP_TRY(need(scores, "scores"));
+    TP_TRY(need(stats, "stats"));
+    TP_TRY(need(d_scores, "d_scores"));
+    if (d_top && top) TP_TRY(need(top_index, "top_index"));
+    return launched(tp::launch_log_probs_back(a, static_cast<const float*>(stats),
+                                              static_cast<const int64_t*>(top_index),
+                                              static_cast<const float*>(d_given),
+                                              static_cast<const float*>(d_entropy),
+                                              static_cast<const float*>(d_log_sum), static_cast<const float*>(d_top),
+                                              d_scores, static_cast<hipStream_t>(stream)),
+                    "log probability gradient launch");
+}
+
+int64_t tp_sort_by_class_work(int64_t slots, int64_t classes) {
+    if (slots <= 0 || classes < 1 || classes > tp::kMaxClasses) return 0;
+    return tp::sort_by_class_work(slots, classes);
+}
+
+int tp_sort_by_class(int id_bytes, const void* class_ids, int64_t slots, int64_t classes, void* order, void* slot,
+                     void* offsets, void* work, int64_t work_bytes, void* stream) {
+    g_err.clear();
+    if (id_bytes != 4 && id_bytes != 8) return fail("class ids must be 4 or 8 bytes each");
+    if (slots < 0 || slots > (int64_t(1) << 30)) return fail("the number of slots must be in [0, 2^30]");
+    if (classes < 1 || classes > tp::kMaxClasses) return fail("the number of classes must be in [1, 4096]");
+    TP_TRY(need(offsets, "offsets"));
+    if (slots) {
+        TP_TRY(need(class_ids, "class_ids"));
+        TP_TRY(need(order, "order"));
+        TP_TRY(need(slot, "slot"));
+    }
+    const int64_t need_bytes = tp_sort_by_class_work(slots, classes);
+    if (need_bytes) TP_TRY(need(work, "work"));
+    if (work_bytes < need_bytes) return fail("work is smaller than tp_sort_by_class_work");
+    return launched(tp::launch_sort_by_class(id_bytes, class_ids, slots, int(classes), static_cast<int*>(order),
+                                             static_cast<int*>(slot), static_cast<int*>(offsets), work,
+                                             static_cast<hipStream_t>(stream)),
+                    "class sort launch");
+}
+
+int tp_spread_rows(int dtype, const void* x, int64_t rows, int64_t cols, int64_t k, const void* slot,
+                   const void* kept, const void* weights, void* sorted, const void* other, void* d_weights,
+                   void* stream) {
+    g_err.clear();
+    tp::RouteArgs a;
+    TP_TRY(route_args(dtype, rows, cols, k, slot, kept, weights, other, d_weights, a));
+    if (rows == 0 || k == 0 || (cols == 0 && !d_weights)) return TP_OK;
+    if (cols) {
+        TP_TRY(need(x, "x"));
+        TP_TRY(need(sorted, "sorted"));
+    }
+    return launched(tp::launch_spread_rows(a, x, sorted, other, static_cast<float*>(d_weights),
+                                           static_cast<hipStream_t>(stream)),
+                    "row spreading launch");
+}
+
+int tp_gather_rows(int dtype, const void* sorted, int64_t rows, int64_t cols, int64_t k, const void* slot,
+                   const void* kept, const void* weights, void* out, const void* other, void* d_weights,
+                   void* stream) {
+    g_err.clear();
+    tp::RouteArgs a;
+    TP_TRY(route_args(dtype, rows, cols, k, slot, kept, weights, other, d_weights, a));
+    if (rows == 0 || (cols == 0 && !d_weights)) return TP_OK;
+    if (cols) {
+        if (k) TP_TRY(need(sorted, "sorted"));
+        TP_TRY(need(out, "out"));
+    }
+    return launched(tp::launch_gather_rows(a, sorted, out, other, static_cast<float*>(d_weights),
+                                           static_cast<hipStream_t>(stream)),
+                    "row gathering launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,307 @@
+// PyTorch dispatcher registration of the matching operators
+// (torch_projectors/matching.py): scores in 8-bit blocks, log probabilities,
+// rows sorted by class.  No counterpart in the reference.  The ops join the
+// namespace that torch_projectors.cpp defines; each checks its arguments,
+// allocates its outputs and workspace from PyTorch's allocator, and calls the
+// C ABI on PyTorch's current stream.
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/library.h>
+#include <torch/torch.h>
+
+#include <tuple>
+
+#include "../../include/torch_projectors_hip.h"
+
+namespace {
+
+using at::Tensor;
+using c10::optional;
+
+constexpr int64_t kBlock = 128;
+
+void* current_stream(const c10::Device& dev) {
+    return static_cast<void*>(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream());
+}
+
+void check_rc(int rc) { TORCH_CHECK(rc == TP_OK, "torch_projectors HIP backend: ", tp_last_error()); }
+
+int dtype_code(const Tensor& t, const char* what) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return TP_F32;
+        case at::kHalf: return TP_F16;
+        case at::kBFloat16: return TP_BF16;
+        default: TORCH_CHECK(false, what, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+    }
+}
+
+void same_device(const Tensor& t, const c10::Device& dev) {
+    TORCH_CHECK(t.device() == dev, "all tensors must be on the same GPU (", dev, "), got one on ", t.device());
+}
+
+Tensor workspace(int64_t bytes, const c10::Device& dev) {
+    return bytes ? at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev)) : Tensor();
+}
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// ------------------------------------------------------------------ 8-bit blocks
+std::tuple<Tensor, Tensor> quantize_blocks(const Tensor& x) {
+    TORCH_CHECK(x.dim() == 2, "quantize_blocks: x must be (rows, values)");
+    TORCH_CHECK(x.size(1) >= 1, "quantize_blocks: rows must hold at least one value");
+    const int dt = dtype_code(x, "quantize_blocks: x");
+    const auto dev = x.device();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    // rows may lie any distance apart; the values of one have to be adjacent
+    const Tensor v = (x.size(1) == 1 || x.stride(1) == 1) && x.stride(0) >= 0 ? x : x.contiguous();
+    const int64_t R = v.size(0), nb = (v.size(1) + kBlock - 1) / kBlock;
+    Tensor codes = at::empty({R, nb * kBlock}, x.options().dtype(at::kFloat8_e4m3fn));
+    Tensor scales = at::empty({nb, tp_scale_rows(R)}, x.options().dtype(at::kByte));
+    check_rc(tp_quantize_blocks(dt, v.data_ptr(), R, v.size(1), v.stride(0), codes.data_ptr(), scales.data_ptr(),
+                                current_stream(dev)));
+    return {codes, scales};
+}
+
+void check_blocks(const Tensor& codes, const Tensor& scales, const char* what) {
+    TORCH_CHECK(codes.scalar_type() == at::kFloat8_e4m3fn && codes.dim() == 2 && codes.size(1) >= kBlock &&
+                    codes.size(1) % kBlock == 0,
+                what, ": codes must be float8_e4m3fn (rows, 128 * blocks)");
+    TORCH_CHECK(scales.scalar_type() == at::kByte && scales.dim() == 2 && scales.size(0) == codes.size(1) / kBlock &&
+                    scales.size(1) == tp_scale_rows(codes.size(0)),
+                what, ": scales must be uint8 (blocks, rows padded to 16)");
+}
+
+// images: float rows, quantised here, or codes with their scales
+Tensor block_scores(const Tensor& images, const optional<Tensor>& image_scales, const Tensor& codes,
+                    const Tensor& scales, const optional<Tensor>& bias, at::ScalarType out_dtype) {
+    check_blocks(codes, scales, "references");
+    TORCH_CHECK(out_dtype == at::kFloat || out_dtype == at::kBFloat16,
+                "block_scores: out_dtype must be float32 or bfloat16");
+    const auto dev = codes.device();
+    same_device(scales, dev);
+    same_device(images, dev);
+    Tensor a, sa;
+    if (image_scales.has_value()) {
+        check_blocks(images, *image_scales, "images");
+        same_device(*image_scales, dev);
+        a = images.contiguous();
+        sa = image_scales->contiguous();
+    } else {
+        std::tie(a, sa) = quantize_blocks(images);
+    }
+    TORCH_CHECK(a.size(1) == codes.size(1), "block_scores: images have ", a.size(1) / kBlock,
+                " blocks a row, references ", codes.size(1) / kBlock);
+    const int64_t M = a.size(0), N = codes.size(0), nb = codes.size(1) / kBlock;
+    Tensor f;
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N && bias->scalar_type() == at::kFloat,
+                    "block_scores: bias must be float32 (references)");
+        same_device(*bias, dev);
+        f = bias->contiguous();
+    }
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Tensor b = codes.contiguous(), sb = scales.contiguous();
+    Tensor out = at::empty({M, N}, codes.options().dtype(out_dtype));
+    const int64_t bytes = tp_block_scores_work(M, N, nb);
+    const Tensor work = workspace(bytes, dev);
+    check_rc(tp_block_scores(a.data_ptr(), sa.data_ptr(), M, b.data_ptr(), sb.data_ptr(), N, nb, ptr(f),
+                             out_dtype == at::kFloat ? TP_F32 : TP_BF16, out.data_ptr(), ptr(work), bytes,
+                             current_stream(dev)));
+    return out;
+}
+
+// ------------------------------------------------------------------ log probabilities
+struct Probs {
+    int dt;
+    Tensor scores, given, mask;
+    int64_t T, V, stride, G = 0, mask_stride = 0;
+};
+Probs probs(const Tensor& scores, const optional<Tensor>& given, const optional<Tensor>& mask) {
+    Probs p;
+    TORCH_CHECK(scores.dim() == 2, "log_probs: scores must be (rows, candidates)");
+    TORCH_CHECK(scores.size(1) >= 1, "log_probs: there must be at least one candidate");
+    p.dt = dtype_code(scores, "log_probs: scores");
+    const auto dev = scores.device();
+    p.T = scores.size(0);
+    p.V = scores.size(1);
+    p.scores = p.V == 1 || scores.stride(1) == 1 ? scores : scores.contiguous();
+    p.stride = p.scores.stride(0);
+    if (given.has_value()) {
+        TORCH_CHECK(given->scalar_type() == at::kLong && given->dim() == 2 && given->size(0) == p.T,
+                    "log_probs: given must be int64 with the scores' leading dimensions");
+        same_device(*given, dev);
+        p.given = given->contiguous();
+        p.G = given->size(1);
+    }
+    if (mask.has_value()) {
+        TORCH_CHECK(mask->scalar_type() == at::kBool && mask->dim() == 2 && mask->size(1) == p.V &&
+                        (mask->size(0) == p.T || mask->size(0) == 1),
+                    "log_probs: mask must be bool (candidates) or of the scores' shape");
+        same_device(*mask, dev);
+        p.mask = p.V == 1 || mask->stride(1) == 1 ? *mask : mask->contiguous();
+        p.mask_stride = mask->size(0) == 1 ? 0 : p.mask.stride(0);
+    }
+    return p;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs(const Tensor& scores, const optional<Tensor>& given,
+                                                                     const optional<Tensor>& mask, int64_t top,
+                                                                     double temperature) {
+    const Probs p = probs(scores, given, mask);
+    TORCH_CHECK(top >= 0 && top <= 64, "log_probs: top must be in [0, 64]");
+    const auto dev = scores.device();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const auto f32 = scores.options().dtype(at::kFloat);
+    Tensor given_out = at::empty({p.T, p.G}, f32), entropy = at::empty({p.T}, f32), log_sum = at::empty({p.T}, f32);
+    Tensor top_out = at::empty({p.T, top}, f32), top_index = at::empty({p.T, top}, f32.dtype(at::kLong));
+    Tensor stats = at::empty({p.T, 4}, f32);
+    const int64_t bytes = tp_log_probs_work(p.T, p.V, top);
+    const Tensor work = workspace(bytes, dev);
+    check_rc(tp_log_probs(p.dt, p.scores.data_ptr(), p.T, p.V, p.stride, ptr(p.given), p.G, ptr(p.mask),
+                          p.mask_stride, top, temperature, given_out.data_ptr(), entropy.data_ptr(),
+                          log_sum.data_ptr(), top_out.data_ptr(), top_index.data_ptr(), stats.data_ptr(), ptr(work),
+                          bytes, current_stream(dev)));
+    return {given_out, entropy, log_sum, top_out, top_index, stats};
+}
+
+Tensor log_probs_back(const Tensor& scores, const optional<Tensor>& given, const optional<Tensor>& mask,
+                      const Tensor& top_index, const Tensor& stats, double temperature,
+                      const optional<Tensor>& d_given, const optional<Tensor>& d_entropy,
+                      const optional<Tensor>& d_log_sum, const optional<Tensor>& d_top) {
+    const Probs p = probs(scores, given, mask);
+    const auto dev = scores.device();
+    const int64_t top = top_index.dim() == 2 ? top_index.size(1) : -1;
+    TORCH_CHECK(top >= 0 && top <= 64 && top_index.size(0) == p.T && top_index.scalar_type() == at::kLong,
+                "log_probs_back: top_index must be int64 (rows, top)");
+    TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.dim() == 2 && stats.size(0) == p.T && stats.size(1) == 4,
+                "log_probs_back: stats must be float32 (rows, 4)");
+    auto upstream = [&](const optional<Tensor>& g, int64_t n, const char* what) {
+        if (!g.has_value()) return Tensor();
+        TORCH_CHECK(g->scalar_type() == at::kFloat && g->numel() == n, "log_probs_back: ", what,
+                    " must be float32 of its output's shape");
+        same_device(*g, dev);
+        return g->contiguous();
+    };
+    const Tensor dg = upstream(d_given, p.T * p.G, "d_given"), dh = upstream(d_entropy, p.T, "d_entropy");
+    const Tensor dl = upstream(d_log_sum, p.T, "d_log_sum"), dt = upstream(d_top, p.T * top, "d_top");
+    same_device(top_index, dev);
+    same_device(stats, dev);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Tensor index = top_index.contiguous(), st = stats.contiguous();
+    Tensor out = at::empty({p.T, p.V}, scores.options());
+    check_rc(tp_log_probs_back(p.dt, p.scores.data_ptr(), p.T, p.V, p.stride, ptr(p.given), p.G, ptr(p.mask),
+                               p.mask_stride, top, temperature, index.data_ptr(), st.data_ptr(),
+                               p.G ? ptr(dg) : nullptr, ptr(dh), ptr(dl), top ? ptr(dt) : nullptr, out.data_ptr(),
+                               current_stream(dev)));
+    return out;
+}
+
+// ------------------------------------------------------------------ rows by class
+std::tuple<Tensor, Tensor, Tensor> sort_by_class(const Tensor& classes, int64_t num_classes) {
+    TORCH_CHECK(classes.dim() == 2, "sort_by_class: classes must be (rows, choices)");
+    TORCH_CHECK(classes.scalar_type() == at::kLong || classes.scalar_type() == at::kInt,
+                "sort_by_class: classes must be int64 or int32, got ", classes.scalar_type());
+    TORCH_CHECK(num_classes >= 1 && num_classes <= 4096, "sort_by_class: num_classes must be in [1, 4096]");
+    const auto dev = classes.device();
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Tensor ids = classes.contiguous();
+    const auto i32 = classes.options().dtype(at::kInt);
+    const int64_t n = ids.numel();
+    Tensor order = at::empty({n}, i32), slot = at::empty(ids.sizes(), i32), offsets = at::empty({num_classes + 1}, i32);
+    const int64_t bytes = tp_sort_by_class_work(n, num_classes);
+    const Tensor work = workspace(bytes, dev);
+    check_rc(tp_sort_by_class(int(ids.element_size()), ids.data_ptr(), n, num_classes, order.data_ptr(),
+                              slot.data_ptr(), offsets.data_ptr(), ptr(work), bytes, current_stream(dev)));
+    return {order, slot, offsets};
+}
+
+struct Route {
+    Tensor slot, offsets, weights;
+    int64_t T, k;
+    const void* kept() const { return static_cast<const int*>(offsets.data_ptr()) + offsets.numel() - 1; }
+};
+Route route(const Tensor& slot, const Tensor& offsets, const optional<Tensor>& weights, const c10::Device& dev) {
+    TORCH_CHECK(slot.scalar_type() == at::kInt && slot.dim() == 2, "slot must be int32 (rows, choices)");
+    TORCH_CHECK(offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.numel() >= 2,
+                "offsets must be int32 (classes + 1)");
+    same_device(slot, dev);
+    same_device(offsets, dev);
+    Route r{slot.contiguous(), offsets.contiguous(), Tensor(), slot.size(0), slot.size(1)};
+    if (weights.has_value()) {
+        TORCH_CHECK(weights->scalar_type() == at::kFloat && weights->sizes() == slot.sizes(),
+                    "weights must be float32 (rows, choices)");
+        same_device(*weights, dev);
+        r.weights = weights->contiguous();
+    }
+    return r;
+}
+// rows of a tensor: n along dimension 0, the rest of it one row
+int64_t row_size(const Tensor& t, int64_t n, const char* what) {
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == n, what, " must be (", n, ", values)");
+    return t.size(1);
+}
+
+// x [T, D] -> sorted [T k, D]; with other [T k, D] also the weights' gradient <x[t], other[slot]>
+std::tuple<Tensor, Tensor> spread_rows(const Tensor& x, const Tensor& slot, const Tensor& offsets,
+                                       const optional<Tensor>& weights, const optional<Tensor>& other) {
+    const auto dev = x.device();
+    const Route r = route(slot, offsets, weights, dev);
+    const int64_t D = row_size(x, r.T, "rows");
+    const int dt = dtype_code(x, "rows");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Tensor v = x.contiguous();
+    Tensor sorted = at::empty({r.T * r.k, D}, x.options()), o, dw;
+    if (other.has_value()) {
+        TORCH_CHECK(other->scalar_type() == x.scalar_type(), "both sides' rows must have the same dtype");
+        TORCH_CHECK(row_size(*other, r.T * r.k, "sorted rows") == D, "both sides' rows must have the same size");
+        same_device(*other, dev);
+        o = other->contiguous();
+        dw = at::empty(slot.sizes(), x.options().dtype(at::kFloat));
+    }
+    check_rc(tp_spread_rows(dt, v.data_ptr(), r.T, D, r.k, r.slot.data_ptr(), r.kept(), ptr(r.weights),
+                            sorted.data_ptr(), ptr(o), ptr(dw), current_stream(dev)));
+    return {sorted, dw.defined() ? dw : at::empty({0}, x.options().dtype(at::kFloat))};
+}
+
+// sorted [T k, D] -> out [T, D]; with other [T, D] also the weights' gradient <other[t], sorted[slot]>
+std::tuple<Tensor, Tensor> gather_rows(const Tensor& sorted, const Tensor& slot, const Tensor& offsets,
+                                       const optional<Tensor>& weights, const optional<Tensor>& other) {
+    const auto dev = sorted.device();
+    const Route r = route(slot, offsets, weights, dev);
+    const int64_t D = row_size(sorted, r.T * r.k, "sorted rows");
+    const int dt = dtype_code(sorted, "sorted rows");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Tensor v = sorted.contiguous();
+    Tensor out = at::empty({r.T, D}, sorted.options()), o, dw;
+    if (other.has_value()) {
+        TORCH_CHECK(other->scalar_type() == sorted.scalar_type(), "both sides' rows must have the same dtype");
+        TORCH_CHECK(row_size(*other, r.T, "rows") == D, "both sides' rows must have the same size");
+        same_device(*other, dev);
+        o = other->contiguous();
+        dw = at::empty(slot.sizes(), sorted.options().dtype(at::kFloat));
+    }
+    check_rc(tp_gather_rows(dt, v.data_ptr(), r.T, D, r.k, r.slot.data_ptr(), r.kept(), ptr(r.weights),
+                            out.data_ptr(), ptr(o), ptr(dw), current_stream(dev)));
+    return {out, dw.defined() ? dw : at::empty({0}, sorted.options().dtype(at::kFloat))};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(torch_projectors, m) {
+    m.def("quantize_blocks(Tensor x) -> (Tensor, Tensor)");
+    m.def("block_scores(Tensor images, Tensor? image_scales, Tensor codes, Tensor scales, Tensor? bias, ScalarType out_dtype) -> Tensor");
+    m.def("log_probs(Tensor scores, Tensor? given, Tensor? mask, int top, float temperature) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("log_probs_back(Tensor scores, Tensor? given, Tensor? mask, Tensor top_index, Tensor stats, float temperature, Tensor? d_given, Tensor? d_entropy, Tensor? d_log_sum, Tensor? d_top) -> Tensor");
+    m.def("sort_by_class(Tensor classes, int num_classes) -> (Tensor, Tensor, Tensor)");
+    m.def("spread_rows(Tensor x, Tensor slot, Tensor offsets, Tensor? weights, Tensor? other) -> (Tensor, Tensor)");
+    m.def("gather_rows(Tensor sorted, Tensor slot, Tensor offsets, Tensor? weights, Tensor? other) -> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(torch_projectors, CUDA, m) {
+    m.impl("quantize_blocks", &quantize_blocks);
+    m.impl("block_scores", &block_scores);
+    m.impl("log_probs", &log_probs);
+    m.impl("log_probs_back", &log_probs_back);
+    m.impl("sort_by_class", &sort_by_class);
+    m.impl("spread_rows", &spread_rows);
+    m.impl("gather_rows", &gather_rows);
+}

@@ -14,6 +14,7 @@ LIBRARY_PATH = os.path.join(_HERE, "libtorch_projectors_hip.so")
 
 TP_OK, TP_ERR_INVALID, TP_ERR_HIP = 0, 1, 2
 TP_F32, TP_F64, TP_F16S = 0, 1, 2
+TP_F16, TP_BF16 = 3, 4  # the matching operators' storage types besides TP_F32
 TP_LINEAR, TP_CUBIC = 0, 1
 
 _P, _I, _L, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
@@ -40,6 +41,14 @@ SIGNATURES = {
     "tp_to_fourier": [_I, _I, _L, _L, _L, _L, _P, _P, _P, _L, _P],
     "tp_from_fourier": [_I, _I, _L, _L, _L, _L, _P, _P, _D, _P, _P, _L, _P],
     "tp_normalize_reconstruction": [_I, _P, _P, _L, _D, _P, _P],
+    # matching
+    "tp_quantize_blocks": [_I, _P, _L, _L, _L, _P, _P, _P],
+    "tp_block_scores": [_P, _P, _L, _P, _P, _L, _L, _P, _I, _P, _P, _L, _P],
+    "tp_log_probs": [_I, _P, _L, _L, _L, _P, _L, _P, _L, _L, _D, _P, _P, _P, _P, _P, _P, _P, _L, _P],
+    "tp_log_probs_back": [_I, _P, _L, _L, _L, _P, _L, _P, _L, _L, _D, _P, _P, _P, _P, _P, _P, _P, _P],
+    "tp_sort_by_class": [_I, _P, _L, _L, _P, _P, _P, _P, _L, _P],
+    "tp_spread_rows": [_I, _P, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P],
+    "tp_gather_rows": [_I, _P, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P],
 }
 # helpers returning a size: name -> argument types
 SIZE_HELPERS = {
@@ -47,6 +56,10 @@ SIZE_HELPERS = {
     "tp_padded_boxsize": [_L, _D],
     "tp_cropped_boxsize": [_L, _D],
     "tp_fused_fourier_work": [_I, _I, _I, _L, _L, _L],
+    "tp_scale_rows": [_L],
+    "tp_block_scores_work": [_L, _L, _L],
+    "tp_log_probs_work": [_L, _L, _L],
+    "tp_sort_by_class_work": [_L, _L],
 }
 # which gathers this thread's calls take (for tests and measurements): name -> argument types
 ROUTE_BY_SIZE, ROUTE_TILES, ROUTE_PER_PIXEL = range(3)
