@@ -1395,8 +1395,9 @@ int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, c
     if (out_dtype != TP_F32 && out_dtype != TP_BF16) return fail("out_dtype must be TP_F32 or TP_BF16");
     if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
     if (blocks < 1) return fail("blocks must be positive");
-    if (rows_a > kInt32Max || rows_b > kInt32Max || blocks > kInt32Max / tp::kScaleBlock)
-        return fail("rows and columns must be < 2^31");
+    if (rows_a > kInt32Max || rows_b > kInt32Max) return fail("row counts must be < 2^31");
+    // (the codes of 256 rows are one buffer of less than 2^32 bytes)
+    if (blocks > 65536) return fail("blocks must be at most 65536");
     if (rows_a == 0 || rows_b == 0) return TP_OK;
     TP_TRY(need(codes_a, "codes_a"));
     TP_TRY(need(scales_a, "scales_a"));

@@ -30,36 +30,63 @@ __device__ __forceinline__ int block_exponent(float most) {
     return most == 0.0f ? 0 : max(f > 0.875f ? x - 8 : x - 9, -127);
 }
 
-// Codes of two values: to nearest even, NaN for what is not finite.
-__device__ __forceinline__ uint32_t codes2(float x, float y, int e) {
-    // 2^-e in two factors: e reaches -127, and 2^127 is the largest power of two
+// Codes of eight values: to nearest even, NaN for what is not finite.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], int e) {
     const float f = ldexpf(1.0f, -e);
-    const uint32_t two = __builtin_amdgcn_cvt_pk_fp8_f32(x * f, y * f, 0, false) & 0xffffu;
-    const uint32_t nx = isfinite(x) ? 0u : 0x7fu, ny = isfinite(y) ? 0u : 0x7f00u;
-    return two | nx | ny;
+    uint32_t c[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float* v = x + 4 * h;
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * f, v[1] * f, 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * f, v[3] * f, w, true);
+        c[h] = uint32_t(w);
+    }
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) finite = finite && isfinite(x[i]);
+    if (!finite) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!isfinite(x[i])) c[i / 4] |= 0x7fu << (i % 4 * 8);
+    }
+    return uint2{c[0], c[1]};
 }
 
-// A wavefront per block of a row, two values per lane.
+// 16 lanes per block of a row, eight values each.  Memory bound: reads each value once, writes a byte for it.
 template <class S>
 __global__ __launch_bounds__(256) void k_quantize(const typename S::Bits* __restrict__ x, int64_t rows, int64_t cols,
-                                                  int64_t stride, int64_t nb, int64_t srows,
-                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); item < srows * nb; item += int64_t(gridDim.x) * 4) {
-    const int64_t r = item / nb, b = item % nb;
-    if (r >= rows) {  // the padding rows' scales
-        if (lane == 0) scales[b * srows + r] = 127;
-        continue;
-    }
-    const int64_t c = b * kScaleBlock + 2 * lane;
-    const float u = c < cols ? S::widen(x[r * stride + c]) : 0.0f;
-    const float v = c + 1 < cols ? S::widen(x[r * stride + c + 1]) : 0.0f;
-    float most = fmaxf(isfinite(u) ? fabsf(u) : 0.0f, isfinite(v) ? fabsf(v) : 0.0f);
+                                                  int64_t stride, int nb, int64_t srows, uint8_t* __restrict__ codes,
+                                                  uint8_t* __restrict__ scales) {
+    const int part = threadIdx.x & 15;
+    const uint32_t span = (nb + 15) / 16;  // workgroups of a row
+    for (int64_t g = blockIdx.x; g < srows * span; g += gridDim.x) {
+        const int64_t r = g / span, b = (g - r * span) * 16 + (threadIdx.x >> 4);
+        if (b >= nb) continue;
+        if (r >= rows) {  // the padding rows' scales
+            if (part == 0) scales[b * srows + r] = 127;
+            continue;
+        }
+        const int64_t c = b * kScaleBlock + 8 * part;
+        const typename S::Bits* p = x + r * stride + c;
+        float v[8];
+        if (c + 8 <= cols) {
+            Pack<S> w[8 / Pack<S>::n];
 #pragma unroll
-    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-    const int e = block_exponent(most);
-    if (lane == 0) scales[b * srows + r] = uint8_t(e + 127);
-    reinterpret_cast<uint16_t*>(codes + r * nb * kScaleBlock + b * kScaleBlock)[lane] = uint16_t(codes2(u, v, e));
+            for (int i = 0; i < 8 / Pack<S>::n; ++i) w[i] = load_pack<S>(p + i * Pack<S>::n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = S::widen(w[i / Pack<S>::n].v[i % Pack<S>::n]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? S::widen(p[i]) : 0.0f;
+        }
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, isfinite(v[i]) ? fabsf(v[i]) : 0.0f);
+#pragma unroll
+        for (int d = 8; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+        const int e = block_exponent(most);
+        if (part == 0) scales[b * srows + r] = uint8_t(e + 127);
+        *reinterpret_cast<uint2*>(codes + (r * nb + b) * kScaleBlock + 8 * part) = codes8(v, e);
     }
 }
 
@@ -79,64 +106,340 @@ __device__ __forceinline__ v8bf widen8(int lo, int hi, float scale) {
     return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A wavefront computes 16 rows x 64 columns, operands straight from memory.  Rows and columns past the
-// end read the last one's and are not stored.
-template <class O>
-__global__ __launch_bounds__(256) void k_scores(const uint8_t* __restrict__ a, const uint8_t* __restrict__ sa,
-                                                int64_t M, int64_t sra, const uint8_t* __restrict__ b,
-                                                const uint8_t* __restrict__ sb, int64_t N, int64_t srb, int64_t nb,
-                                                const float* __restrict__ bias, typename O::Bits* __restrict__ out) {
-    const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
-    const int64_t tn = (N + 63) / 64, K = nb * kScaleBlock;
-    for (int64_t tile = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); tile < (M + 15) / 16 * tn;
-         tile += int64_t(gridDim.x) * 4) {
-        const int64_t m0 = tile / tn * 16, n0 = tile % tn * 64, am = min(m0 + r16, M - 1);
-        const uint8_t* pa = a + am * K + q * 8;
-        const uint8_t* pb[4];
-        int64_t bn[4];
-        v4f acc[4];
+// What the kernels of the product share: [splits] ranges of the nb blocks are one workgroup each, and
+// where there are several their sums go to part [splits][M][N], which k_scores_join adds up.
+struct ScoreArgs {
+    const uint8_t *a, *sa, *b, *sb;
+    int64_t M, N, sra, srb;
+    int nb, splits;
+    const float* bias;
+    void* out;
+    float* part;
+    __device__ __forceinline__ int first(uint32_t split) const { return int(int64_t(nb) * split / splits); }
+};
+
+template <class O> __device__ __forceinline__ void store_score(const ScoreArgs& g, uint32_t split, int64_t m, int64_t n, float v) {
+    if (g.splits > 1)
+        g.part[(int64_t(split) * g.M + m) * g.N + n] = v;
+    else
+        static_cast<typename O::Bits*>(g.out)[m * g.N + n] = O::round(v + (g.bias ? g.bias[n] : 0.0f));
+}
+
+template <class O> __global__ __launch_bounds__(256) void k_scores_join(ScoreArgs g) {
+    const int64_t MN = g.M * g.N;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < MN; i += int64_t(gridDim.x) * 256) {
+        float v = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < g.splits; ++s) v += g.part[s * MN + i];
+        if (g.bias) v += g.bias[uint64_t(i) < (uint64_t(1) << 32) ? uint32_t(i) % uint32_t(g.N) : i % g.N];
+        static_cast<typename O::Bits*>(g.out)[i] = O::round(v);
+    }
+}
+
+// Few images (at most 16 FM): as fast as the references' codes can be read.  A workgroup takes 16 references,
+// each of its wavefronts every eighth block of them, straight from memory into operands: kAhead blocks'
+// loads are in flight at once (8 KB a wavefront, 64 KB a CU).
+constexpr int kFewWaves = 8, kAhead = 4;
+
+template <int FM, class O>
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_scores_few(ScoreArgs g) {
+    __shared__ float sums[kFewWaves][FM * 16][16];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q = lane >> 4;
+    const uint32_t groups = uint32_t((g.N + 15) / 16), split = blockIdx.x / groups;
+    const int64_t n0 = int64_t(blockIdx.x % groups) * 16, K = int64_t(g.nb) * kScaleBlock;
+    const int k0 = g.first(split), k1 = g.first(split + 1);
+    // rows past the end read the last one's codes and are not stored
+    const int64_t bn = min(n0 + r, g.N - 1);
+    const uint8_t* pb = g.b + bn * K + q * 16;
+    const uint8_t* sb = g.sb + bn;
+    const uint8_t* pa[FM];
+    const uint8_t* sa[FM];
+    v4f acc[FM];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bn[i] = min(n0 + 16 * i + r16, N - 1);
-            pb[i] = b + bn[i] * K + q * 8;
-            acc[i] = v4f{0, 0, 0, 0};
+    for (int f = 0; f < FM; ++f) {
+        const int64_t am = min(int64_t(f * 16 + r), g.M - 1);
+        pa[f] = g.a + am * K + q * 16;
+        sa[f] = g.sa + am;
+        acc[f] = v4f{0, 0, 0, 0};
+    }
+    for (int k = k0 + wave; k < k1; k += kFewWaves * kAhead) {
+        int4 cb[kAhead][2], ca[kAhead][FM][2];
+        uint32_t eb[kAhead], ea[kAhead][FM];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t at = min(k + u * kFewWaves, k1 - 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) cb[u][h] = *reinterpret_cast<const int4*>(pb + at * kScaleBlock + h * 64);
+            eb[u] = sb[at * g.srb];
+#pragma unroll
+            for (int f = 0; f < FM; ++f) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    ca[u][f][h] = *reinterpret_cast<const int4*>(pa[f] + at * kScaleBlock + h * 64);
+                ea[u][f] = sa[f][at * g.sra];
+            }
         }
-        for (int64_t k = 0; k < nb; ++k) {
-            const float ea = scale_of(sa[k * sra + am]);
-            float eb[4];
+        __builtin_amdgcn_sched_barrier(0);  // all loads before the first use
 #pragma unroll
-            for (int i = 0; i < 4; ++i) eb[i] = scale_of(sb[k * srb + bn[i]]);
+        for (int u = 0; u < kAhead; ++u) {
+            if (k + u * kFewWaves >= k1) break;
+            const float fb = scale_of(eb[u]);
 #pragma unroll
-            for (int h = 0; h < kScaleBlock; h += 32) {
-                const int2 ca = *reinterpret_cast<const int2*>(pa + k * kScaleBlock + h);
-                const v8bf fa = widen8(ca.x, ca.y, ea);
+            for (int h = 0; h < 2; ++h) {
+                const v8bf b0 = widen8(cb[u][h].x, cb[u][h].y, fb), b1 = widen8(cb[u][h].z, cb[u][h].w, fb);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int2 cb = *reinterpret_cast<const int2*>(pb[i] + k * kScaleBlock + h);
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, widen8(cb.x, cb.y, eb[i]), acc[i], 0, 0, 0);
+                for (int f = 0; f < FM; ++f) {
+                    const float fa = scale_of(ea[u][f]);
+                    const int4 c = ca[u][f][h];
+                    acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(c.x, c.y, fa), b0, acc[f], 0, 0, 0);
+                    acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(c.z, c.w, fa), b1, acc[f], 0, 0, 0);
                 }
             }
         }
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t n = n0 + 16 * i + r16;
-            if (n >= N) continue;
-            const float off = bias ? bias[n] : 0.0f;
+    for (int f = 0; f < FM; ++f)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t m = m0 + 4 * q + j;
-                if (m < M) out[m * N + n] = O::round(acc[i][j] + off);
+        for (int j = 0; j < 4; ++j) sums[wave][f * 16 + 4 * q + j][r] = acc[f][j];
+    __syncthreads();
+    for (int i = tid; i < FM * 256; i += 64 * kFewWaves) {
+        const int64_t m = i >> 4, n = n0 + (i & 15);
+        if (m >= g.M || n >= g.N) continue;
+        float v = 0;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w) v += sums[w][m][i & 15];
+        store_score<O>(g, split, m, n, v);
+    }
+}
+
+// The product in tiles: a workgroup of WM x WN wavefronts computes BM x BN scores.
+// Codes of one block of a tile's rows in LDS: 128 bytes a row, whose 16-byte chunks are permuted among
+// themselves (chunk c of row r at place c ^ key(r)), so that the eight lanes that read one chunk of eight
+// rows reach all banks.
+template <int BM, int BN> struct alignas(16) Stage {
+    uint8_t a[BM * kScaleBlock], b[BN * kScaleBlock];
+    uint32_t sa[64], sb[64];  // scale bytes (the first BM and BN are used)
+};
+
+using LocalPtr = __attribute__((address_space(3))) void*;
+
+// The codes of `rows` rows from p on as a buffer: reads past its end give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t codes_buffer(const uint8_t* p, int64_t rows, int64_t K) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, int(uint32_t(rows * K)), 0x00027000);
+}
+
+// N loads of a wavefront to LDS, 8 rows of 128 bytes each; off: each lane's byte offsets from `at` on.
+template <int N>
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t src, const uint32_t (&off)[N], int at, uint8_t* dst) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (LocalPtr)(dst + i * 1024), 16, int(off[i]), at, 0, 0);
+}
+
+// The scales of rows `first` .. first + F - 1 (F divides first and 4) from the stage's bytes.  They are read
+// as words: before a load of single bytes, which may alias anything, the compiler waits for all loads to LDS.
+template <int F> __device__ __forceinline__ void scales_of(const uint32_t* words, int first, float (&s)[F]) {
+    const uint32_t w = words[first >> 2] >> (8 * (first & 3));
+#pragma unroll
+    for (int f = 0; f < F; ++f) s[f] = scale_of((w >> (8 * f)) & 255u);
+}
+
+using v16f = __attribute__((ext_vector_type(16))) float;
+
+template <int FM, int FN>
+__device__ __forceinline__ void tile_step(const uint8_t* __restrict__ ca, const uint8_t* __restrict__ cb, int key,
+                                          int q, const uint32_t* __restrict__ sa, const uint32_t* __restrict__ sb,
+                                          int ra0, int rb0, v16f (&acc)[FM][FN]) {
+    float ea[FM], eb[FN];
+    scales_of<FM>(sa, ra0, ea);
+    scales_of<FN>(sb, rb0, eb);
+    // operands of one quarter of the block are read from LDS while the one before is multiplied, or, where
+    // there are registers for it, all at once
+    constexpr int D = FM + FN <= 4 ? 4 : 2;
+    int4 ra[D][FM], rb[D][FN];
+    auto read = [&](int t) {
+        const int at = ((2 * t + q) ^ key) * 16;
+#pragma unroll
+        for (int f = 0; f < FM; ++f) ra[t % D][f] = *reinterpret_cast<const int4*>(ca + f * kScaleBlock + at);
+#pragma unroll
+        for (int f = 0; f < FN; ++f) rb[t % D][f] = *reinterpret_cast<const int4*>(cb + f * kScaleBlock + at);
+    };
+#pragma unroll
+    for (int t = 0; t < D - 1; ++t) read(t);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (t + D - 1 < 4) read(t + D - 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v8bf fa[FM], fb[FN];
+#pragma unroll
+            for (int f = 0; f < FM; ++f) {
+                const int4 c = ra[t % D][f];
+                fa[f] = h ? widen8(c.z, c.w, ea[f]) : widen8(c.x, c.y, ea[f]);
+            }
+#pragma unroll
+            for (int f = 0; f < FN; ++f) {
+                const int4 c = rb[t % D][f];
+                fb[f] = h ? widen8(c.z, c.w, eb[f]) : widen8(c.x, c.y, eb[f]);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        }
+        if (D == 2) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Wait until this wavefront's loads to LDS have arrived, then for the other wavefronts.
+__device__ __forceinline__ void stage_ready() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A wavefront's rows of 32 x 32 fragments lie F apart (fragment f has rows F r + f), so that one load brings
+// the scales of a lane's rows and a lane's F columns are neighbours in the output.
+template <int BM, int BN, int WM, int WN, class O>
+__global__ __launch_bounds__(64 * WM * WN) void k_scores_tile(ScoreArgs g, uint32_t tm, uint32_t tn) {
+    constexpr int W = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
+    constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // loads of a wavefront for a stage
+    static_assert(LA * W * 8 == BM && LB * W * 8 == BN, "whole loads");
+    __shared__ Stage<BM, BN> stages[2];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, q = lane >> 5;
+    const int wm = wave / WN, wn = wave % WN;
+    // workgroups are dealt to the XCDs in turn: each XCD takes a contiguous run of the items, whose tiles
+    // share rows and columns in its L2
+    const uint32_t items = gridDim.x, x = blockIdx.x & 7, per = items >> 3, more = items & 7;
+    uint32_t item = x * per + min(x, more) + (blockIdx.x >> 3);
+    const uint32_t split = item / (tm * tn);
+    item -= split * tm * tn;
+    // tiles in bands of 4 along M, column by column
+    const uint32_t band = item / (4 * tn), at = item - band * 4 * tn, height = min(4u, tm - band * 4);
+    const int64_t m0 = int64_t(band * 4u + at % height) * BM, n0 = int64_t(at / height) * BN;
+    const int k0 = g.first(split), k1 = g.first(split + 1);
+    const int64_t K = int64_t(g.nb) * kScaleBlock;
+
+    uint32_t oa[LA], ob[LB];
+    const int row8 = lane >> 3, place = lane & 7;
+#pragma unroll
+    for (int i = 0; i < LA; ++i) {
+        const int row = (wave * LA + i) * 8 + row8;
+        oa[i] = uint32_t(row * K) + (place ^ ((row / FM) & 7)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+        const int row = (wave * LB + i) * 8 + row8;
+        ob[i] = uint32_t(row * K) + (place ^ ((row / FN) & 7)) * 16;
+    }
+    // rows past the end read zeros
+    const auto ga = codes_buffer(g.a + m0 * K, min(int64_t(BM), g.M - m0), K);
+    const auto gb = codes_buffer(g.b + n0 * K, min(int64_t(BN), g.N - n0), K);
+    const int ra = (wm * 32 + r) * FM, rb = (wn * 32 + r) * FN;  // a lane's first row and column of the tile
+    v16f acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+    // two stages in turn: while one is multiplied the other is filled (three and four were no faster: a
+    // stage's loads take less than its products, and the LDS holds fewer workgroups)
+    const int lane4 = lane * 4;
+    auto load = [&](Stage<BM, BN>& st, int k) {
+        to_lds(ga, oa, k * kScaleBlock, st.a + wave * LA * 1024);
+        to_lds(gb, ob, k * kScaleBlock, st.b + wave * LB * 1024);
+        // (every wavefront brings all scales: the same bytes to the same place)
+        const auto sa = codes_buffer(g.sa + k * g.sra + m0, 1, g.sra - m0);
+        const auto sb = codes_buffer(g.sb + k * g.srb + n0, 1, g.srb - n0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(sa, (LocalPtr)st.sa, 4, lane4, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (LocalPtr)st.sb, 4, lane4, 0, 0, 0);
+    };
+    load(stages[0], k0);
+#pragma unroll 1
+    for (int k = k0; k < k1; ++k) {
+        const int cur = (k - k0) & 1;
+        stage_ready();
+        if (k + 1 < k1) load(stages[cur ^ 1], k + 1);
+        const Stage<BM, BN>& st = stages[cur];
+        tile_step<FM, FN>(st.a + ra * kScaleBlock, st.b + rb * kScaleBlock, r & 7, q, st.sa, st.sb, ra, rb, acc);
+    }
+
+    const int64_t n = n0 + rb;
+    const bool whole = n + FN <= g.N;
+    float off[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) off[j] = g.bias && n + j < g.N ? g.bias[n + j] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int64_t m = m0 + (wm * 32 + (e / 4) * 8 + q * 4 + e % 4) * FM + i;
+            if (m >= g.M) continue;
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    if (n + j < g.N) store_score<O>(g, split, m, n + j, acc[i][j][e]);
+            } else if (g.splits > 1) {
+                float v[FN];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) v[j] = acc[i][j][e];
+                __builtin_memcpy(g.part + (int64_t(split) * g.M + m) * g.N + n, v, sizeof v);
+            } else {
+                typename O::Bits v[FN];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) v[j] = O::round(acc[i][j][e] + off[j]);
+                __builtin_memcpy(static_cast<typename O::Bits*>(g.out) + m * g.N + n, v, sizeof v);
+            }
+        }
+}
+
+// ------------------------------------------------------------------ which kernel
+// Few images: k_scores_few.  Else the tile and the number of ranges of the blocks with the least time by a
+// count of steps (one block of K for one tile).  A CU with n workgroups of a tile takes n step_us for a step
+// of each, but no less than alone_us: one workgroup alone waits for LDS and for its own products.  Measured:
+// 4096 x 8192 x 16640 (full CUs) 64: 1283 us, 128: 997, 256: 869; 333 x 1999 x 8280 64: 36, 128: 75, 256: 175
+// us in one range, 29, 33 and 64 in four.  Several ranges cost a launch and their sums written and read.
+struct ScorePlan {
+    int few, tile, splits;  // few: FM of k_scores_few, or 0; tile: index of kTiles
+};
+struct TileKind {
+    int bm, bn;
+    double step_us, alone_us;
+};
+constexpr TileKind kTiles[] = {{64, 64, 0.31, 0.48}, {128, 128, 0.96, 1.1}, {256, 256, 3.3, 2.5}};
+constexpr int kCus = 256, kMaxSplits = 16;
+
+ScorePlan score_plan(int64_t M, int64_t N, int64_t nb) {
+    if (M <= 32) return {M <= 16 ? 1 : 2, 0, 1};
+    ScorePlan best{0, 0, 1};
+    double least = 1e300;
+    for (int t = 0; t < 3; ++t) {
+        const TileKind& kind = kTiles[t];
+        const int64_t tiles = ((M + kind.bm - 1) / kind.bm) * ((N + kind.bn - 1) / kind.bn);
+        for (int s = 1; s <= kMaxSplits && s <= nb; ++s) {
+            const double each = double((tiles * s + kCus - 1) / kCus);
+            double us = ((nb + s - 1) / s + 2) * (each * kind.step_us > kind.alone_us ? each * kind.step_us : kind.alone_us);
+            if (s > 1) us += 4.0 + double(M) * N * (8 * s + 4) / 4.5e6;
+            if (us < least) {
+                least = us;
+                best = {0, t, s};
             }
         }
     }
+    return best;
 }
 
 }  // namespace
 
 hipError_t launch_quantize_blocks(int dt, const void* x, int64_t rows, int64_t cols, int64_t stride, void* codes,
                                   void* scales, hipStream_t s) {
-    const int64_t nb = (cols + kScaleBlock - 1) / kScaleBlock, sr = scale_rows(rows);
-    const dim3 grid(match_grid((sr * nb + 3) / 4));
+    const int nb = int((cols + kScaleBlock - 1) / kScaleBlock);
+    const int64_t sr = scale_rows(rows);
+    const dim3 grid(match_grid(sr * ((nb + 15) / 16)));
     auto* c = static_cast<uint8_t*>(codes);
     auto* e = static_cast<uint8_t*>(scales);
     switch (dt) {
@@ -152,24 +455,41 @@ hipError_t launch_quantize_blocks(int dt, const void* x, int64_t rows, int64_t c
     return hipGetLastError();
 }
 
-int64_t block_scores_work(int64_t, int64_t, int64_t) { return 0; }
+int64_t block_scores_work(int64_t M, int64_t N, int64_t nb) {
+    const ScorePlan p = score_plan(M, N, nb);
+    return p.splits > 1 ? p.splits * M * N * int64_t(sizeof(float)) : 0;
+}
+
+template <class O> hipError_t scores(const ScoreArgs& g, const ScorePlan& p, hipStream_t s) {
+    if (p.few) {
+        const dim3 grid(unsigned((g.N + 15) / 16) * p.splits);
+        if (p.few == 1)
+            k_scores_few<1, O><<<grid, 64 * kFewWaves, 0, s>>>(g);
+        else
+            k_scores_few<2, O><<<grid, 64 * kFewWaves, 0, s>>>(g);
+    } else {
+        const TileKind& kind = kTiles[p.tile];
+        const uint32_t tm = uint32_t((g.M + kind.bm - 1) / kind.bm), tn = uint32_t((g.N + kind.bn - 1) / kind.bn);
+        const dim3 grid(tm * tn * p.splits);
+        if (p.tile == 0)
+            k_scores_tile<64, 64, 2, 2, O><<<grid, 256, 0, s>>>(g, tm, tn);
+        else if (p.tile == 1)
+            k_scores_tile<128, 128, 2, 2, O><<<grid, 256, 0, s>>>(g, tm, tn);
+        else
+            k_scores_tile<256, 256, 2, 4, O><<<grid, 512, 0, s>>>(g, tm, tn);
+    }
+    if (hipError_t e = hipGetLastError()) return e;
+    if (p.splits > 1) k_scores_join<O><<<match_grid((g.M * g.N + 255) / 256), 256, 0, s>>>(g);
+    return hipGetLastError();
+}
 
 hipError_t launch_block_scores(const void* a, const void* sa, int64_t M, const void* b, const void* sb, int64_t N,
-                               int64_t nb, const void* bias, int out_dt, void* out, void*, hipStream_t s) {
-    const int64_t tiles = (M + 15) / 16 * ((N + 63) / 64);
-    const dim3 grid(match_grid((tiles + 3) / 4));
-    const auto* pa = static_cast<const uint8_t*>(a);
-    const auto* pb = static_cast<const uint8_t*>(b);
-    const auto* ea = static_cast<const uint8_t*>(sa);
-    const auto* eb = static_cast<const uint8_t*>(sb);
-    const auto* f = static_cast<const float*>(bias);
-    if (out_dt == TP_F32)
-        k_scores<F32><<<grid, 256, 0, s>>>(pa, ea, M, scale_rows(M), pb, eb, N, scale_rows(N), nb, f,
-                                           static_cast<uint32_t*>(out));
-    else
-        k_scores<BF16><<<grid, 256, 0, s>>>(pa, ea, M, scale_rows(M), pb, eb, N, scale_rows(N), nb, f,
-                                            static_cast<uint16_t*>(out));
-    return hipGetLastError();
+                               int64_t nb, const void* bias, int out_dt, void* out, void* work, hipStream_t s) {
+    const ScorePlan p = score_plan(M, N, nb);
+    const ScoreArgs g{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(sa), static_cast<const uint8_t*>(b),
+                      static_cast<const uint8_t*>(sb), M, N, scale_rows(M), scale_rows(N), int(nb), p.splits,
+                      static_cast<const float*>(bias), out, static_cast<float*>(work)};
+    return out_dt == TP_F32 ? scores<F32>(g, p, s) : scores<BF16>(g, p, s);
 }
 
 }  // namespace tp
