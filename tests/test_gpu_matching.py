@@ -524,3 +524,12 @@ def test_another_stream_and_a_graph(m):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[n])), n
         assert all(torch.equal(a, b) for a, b in zip(_all(m, states[n]), want[n])), n  # eager work in between
+
+
+def test_probs_many_givens(m):
+    """More given and listed candidates than a wavefront has lanes, with repeats."""
+    g = gen(21)
+    x = torch.randn(3, 900, generator=g) * 2
+    given = torch.randint(0, 60, (3, 100), generator=g)
+    given[torch.rand(3, 100, generator=g) < 0.1] = -1
+    _probs_check(m, x, given, 40, 1.2)

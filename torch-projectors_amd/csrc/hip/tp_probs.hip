@@ -8,30 +8,39 @@
 // Sums are fp32.
 //   d x = c ( p (dL - sum dG - sum dT - dH (log p + H)) + what is given or listed at x )
 //
-// Alternatives: a wavefront keeps its `top` best as sorted keys, one per lane: the score's bits in an order that
-// integers have, then the complement of its index, so ties go to the lowest index.  A score above the last
-// key's is inserted by the lanes' common effort: its place is a population count, the keys behind it move
-// one lane up.  In rows in no particular order that happens about top (1 + ln(n / top)) times for n scores.
+// Alternatives: a wavefront keeps its best as sorted keys, one per lane: the score's bits in an order that
+// integers have, then the complement of its index, so ties go to the lowest index.  Scores above the top-th
+// key's are candidates; of a tile with many (the first; rising rows) only those that reach a floor below
+// which none can be listed: a value that `top` of the lanes' own largest reach.  Candidates go through LDS,
+// 64 at a time, and are merged by counting: each one's place is the number of keys and of other candidates
+// above it, each key moves up by the number of candidates above it.  (Counting over broadcast reads of LDS, in
+// all lanes at once, is faster from about 16 candidates on, but most tiles have one or two.)
+//
+// Split: a row is one wavefront's, or 2, 4 or 8 of a workgroup's, or, where rows are few, several workgroups',
+// whose sums and keys k_probs_join joins.  Memory bound: a tile of 16 scores a lane is in flight for every
+// wavefront of a CU.
 //
 // Scores of -inf count as not allowed.  A NaN makes the row's results NaN.
 #include "../../../include/torch_projectors_hip.h"
 #include "tp_match.hh"
 
+#include <algorithm>
+
 namespace tp {
 namespace {
 
-constexpr int kProbsBlock = 256, kProbsWaves = kProbsBlock / 64;
+constexpr int kProbsBlock = 512, kProbsWaves = kProbsBlock / 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
-__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+__host__ __device__ __forceinline__ constexpr float neg_inf() { return -__builtin_inff(); }
 
 // The larger of two, NaN if either is.
 __device__ __forceinline__ float max_or_nan(float a, float b) { return a != a ? a : (b > a || b != b ? b : a); }
 
-// Larger keys are better: the score, then the lower index.  0 is no candidate.
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
+// Larger keys are better: the score's bits in the order of the scores, then the lower index.  0 is no candidate.
+__device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);  // -0 and 0 are equal
-    return (uint64_t(b & 0x80000000u ? ~b : b | 0x80000000u) << 32) | ~index;
+    return b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float score_of(uint64_t key) {
     const uint32_t o = uint32_t(key >> 32);
@@ -39,200 +48,517 @@ __device__ __forceinline__ float score_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~uint32_t(key); }
 
-// Insert a key (uniform over the wavefront) into the sorted keys, one per lane.
-__device__ __forceinline__ void insert(uint64_t& mine, uint64_t key, int lane) {
-    const int place = __popcll(__ballot(mine > key));
-    const uint64_t before = __shfl_up(mine, 1);
-    if (lane >= place) mine = lane == place ? key : before;
+__device__ __forceinline__ uint32_t read_lane(uint32_t v, int lane) {
+    return uint32_t(__builtin_amdgcn_readlane(int(v), lane));
 }
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+    return uint64_t(read_lane(uint32_t(v >> 32), lane)) << 32 | read_lane(uint32_t(v), lane);
+}
+// The value that a DPP control brings, `none` where it brings none.
+template <int CTRL> __device__ __forceinline__ uint32_t brought(uint32_t v, uint32_t none) {
+    return uint32_t(__builtin_amdgcn_update_dpp(int(none), int(v), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL> __device__ __forceinline__ float brought(float v, float none) {
+    return __uint_as_float(brought<CTRL>(__float_as_uint(v), __float_as_uint(none)));
+}
+// Each lane's f over the lanes up to it (none: f's neutral value): row_shr:1, 2, 4, 8, then row_bcast:15 to
+// rows 1 and 3 and row_bcast:31 to rows 2 and 3.
+template <class T, class F> __device__ __forceinline__ T scanned(T v, T none, F f) {
+    v = f(v, brought<0x111>(v, none));
+    v = f(v, brought<0x112>(v, none));
+    v = f(v, brought<0x114>(v, none));
+    v = f(v, brought<0x118>(v, none));
+    const int lane = threadIdx.x & 63;
+    const T b = brought<0x142>(v, none);
+    v = lane & 16 ? f(v, b) : v;
+    const T c = brought<0x143>(v, none);
+    return lane & 32 ? f(v, c) : v;
+}
+// f over all lanes.
+template <class F> __device__ __forceinline__ float reduced(float v, float none, F f) {
+    return __uint_as_float(read_lane(__float_as_uint(scanned(v, none, f)), 63));
+}
+
+// Number of lanes below this one whose bit is set.
+__device__ __forceinline__ int below(uint64_t lanes) {
+    return int(__builtin_amdgcn_mbcnt_hi(uint32_t(lanes >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(lanes), 0)));
+}
+// A value (in order_of's order) that at least k lanes reach, with its low 16 bits zero: the largest such.
+__device__ __forceinline__ uint32_t floor_of(uint32_t order, int k) {
+    uint32_t at = 0;
+#pragma unroll 1
+    for (uint32_t bit = 0x80000000u; bit > 0x8000u; bit >>= 1)
+        if (__popcll(__ballot(order >= (at | bit))) >= k) at |= bit;
+    return at;
+}
+
+// A wavefront's LDS.  Only it reads and writes it, in order; the fences keep the compiler to that.
+constexpr int kLaneScores = 16;                 // of a tile
+constexpr int kTileScores = 64 * kLaneScores;
+struct Room {
+    uint64_t found[kTileScores];  // candidates
+    uint64_t keys[64];
+};
+__device__ __forceinline__ void lds_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// The best keys of a wavefront, sorted, and the score of the top-th (-inf while there are fewer).  Keys past the
+// top-th are kept in the lanes that are there anyway.
+struct Best {
+    uint64_t key = 0;
+    float least = neg_inf();
+
+    // Merge the lanes' keys for which `set` holds a bit.
+    __device__ __forceinline__ void take(uint64_t set, uint64_t theirs, Room& room, int lane) {
+        if (!set) return;
+        int up = 0, rank = 0, above = 0;
+        for (uint64_t left = set; left; left &= left - 1) {
+            const int from = __ffsll(static_cast<long long>(left)) - 1;
+            const uint64_t k = read_lane(theirs, from);
+            const int keys = __popcll(__ballot(key > k));
+            if (lane == from) above = keys;
+            up += key < k ? 1 : 0;
+            rank += theirs < k ? 1 : 0;
+        }
+        const bool in = (set >> lane) & 1;
+        room.keys[lane] = 0;
+        lds_order();
+        if (key && lane + up < 64) room.keys[lane + up] = key;
+        if (in && above + rank < 64) room.keys[above + rank] = theirs;
+        lds_order();
+        key = room.keys[lane];
+        lds_order();
+    }
+    __device__ __forceinline__ uint64_t last(int top) const { return read_lane(key, top - 1); }
+    __device__ __forceinline__ void settle(int top) {
+        const uint64_t k = last(top);
+        least = k ? score_of(k) : neg_inf();
+    }
+};
 
 // Sums over scores relative to their largest: z in units of 1 / (c log2 e), i.e. exponents of 2.
 struct Sums {
     float m, s, u;
 };
-// exp2 of z clamped to where it is 0, so that z exp2(z) is 0 and not NaN for -inf.
+// z is clamped to where its exponential is 0, so that z exp2(z) is 0 and not NaN for -inf.
 __device__ __forceinline__ void add_score(Sums& a, float x, float c2) {
     const float z = fmaxf((x - a.m) * c2, -200.0f), e = __builtin_amdgcn_exp2f(z);
     a.s += e;
-    a.u += z * e;
+    a.u = __builtin_fmaf(z, e, a.u);
 }
 // The sums of a relative to m >= a.m.
 __device__ __forceinline__ Sums moved(const Sums& a, float m, float c2) {
-    if (a.s == 0.0f) return Sums{m, 0.0f, 0.0f};
     const float z = fmaxf((a.m - m) * c2, -200.0f), f = __builtin_amdgcn_exp2f(z);
-    return Sums{m, a.s * f, (a.u + a.s * z) * f};
+    return Sums{m, a.s * f, __builtin_fmaf(a.s, z, a.u) * f};
 }
 __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c2) {
     const float m = max_or_nan(a.m, b.m);
     const Sums p = moved(a, m, c2), q = moved(b, m, c2);
     return Sums{m, p.s + q.s, p.u + q.u};
 }
+// All lanes' sums joined: their largest m first, then one rescaling, then plain sums.
+__device__ __forceinline__ Sums wave_joined(Sums a, float c2) {
+    const float m = reduced(a.m, neg_inf(), [](float x, float y) { return max_or_nan(x, y); });
+    a = moved(a, m, c2);
+    const auto add = [](float x, float y) { return x + y; };
+    return Sums{m, reduced(a.s, 0.0f, add), reduced(a.u, 0.0f, add)};
+}
 
-// One workgroup per row.
+// A lane's scores of the tile at v0: packs of neighbours, lane after lane.  Masked ones and those from v1 on
+// are -inf.
+template <class S> __device__ __forceinline__ int64_t tile_index(int64_t v0, int lane, int i) {
+    return v0 + (i / Pack<S>::n * 64 + lane) * Pack<S>::n + i % Pack<S>::n;
+}
 template <class S>
-__global__ __launch_bounds__(kProbsBlock) void k_probs(ProbsArgs a, float* __restrict__ given_out,
-                                                       float* __restrict__ entropy, float* __restrict__ log_sum,
-                                                       float* __restrict__ top_out, int64_t* __restrict__ top_index,
-                                                       float* __restrict__ stats) {
-    __shared__ Sums part[kProbsWaves];
-    __shared__ uint64_t keys[kProbsWaves][kMaxTop];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
-    const auto* x = static_cast<const typename S::Bits*>(a.scores) + t * a.stride;
-    const uint8_t* mask = a.mask ? a.mask + t * a.mask_stride : nullptr;
-    const float c2 = kLog2e / a.temperature;
-    Sums mine{neg_inf(), 0.0f, 0.0f};
-    uint64_t key = 0;
-    float least = neg_inf();  // the last listed score: only larger ones are listed (they have later indices)
-    for (int64_t v0 = wave * 64; v0 < a.V; v0 += kProbsBlock) {
-        const int64_t v = v0 + lane;
-        float f = neg_inf();
-        if (v < a.V && (!mask || mask[v])) f = S::widen(x[v]);
-        const float m = max_or_nan(mine.m, f);
-        if (m != mine.m) mine = moved(mine, m, c2);
-        if (f != neg_inf()) add_score(mine, f, c2);
-        if (a.top) {
-            uint64_t better = __ballot(f > least);
-            while (better) {
-                const int from = __ffsll(static_cast<long long>(better)) - 1;
-                better &= better - 1;
-                insert(key, key_of(__shfl(f, from), uint32_t(v0 + from)), lane);
-            }
-            const uint64_t last = __shfl(key, a.top - 1);
-            least = last ? score_of(last) : neg_inf();
-        }
-    }
+__device__ __forceinline__ void load_tile(const typename S::Bits* x, const uint8_t* mask, int64_t v0, int64_t v1,
+                                          int lane, float (&f)[kLaneScores]) {
+    constexpr int n = Pack<S>::n, P = kLaneScores / n;
+    if (v0 + kTileScores <= v1) {
+        Pack<S> w[P];
 #pragma unroll
-    for (int d = 32; d; d >>= 1)
-        mine = joined(mine, Sums{__shfl_xor(mine.m, d), __shfl_xor(mine.s, d), __shfl_xor(mine.u, d)}, c2);
-    if (lane == 0) part[wave] = mine;
-    keys[wave][lane] = lane < a.top ? key : 0;
-    __syncthreads();
-    if (wave == 0) {
-    for (int w = 1; w < kProbsWaves; ++w) {
-        mine = joined(mine, part[w], c2);
-        for (int j = 0; j < a.top; ++j)
-            if (keys[w][j]) insert(key, keys[w][j], lane);
-    }
-    const bool none = mine.m == neg_inf();
-    const float m = mine.m;
-    const float ls = m == __builtin_inff() ? __builtin_nanf("") : logf(mine.s);
-    if (lane == 0) {
-        const float H = none ? 0.0f : !isfinite(m) ? __builtin_nanf("") : ls - mine.u * kLn2 / mine.s;
-        entropy[t] = H;
-        log_sum[t] = isfinite(m) ? m / a.temperature + ls : m;
-        float* st = stats + t * kProbsStats;
-        st[0] = m;
-        st[1] = ls;
-        st[2] = H;
-        st[3] = 0.0f;
-    }
-    for (int64_t g = lane; g < a.G; g += 64) {
-        const int64_t v = a.given[t * a.G + g];
-        float lp = 0.0f;
-        if (v != -1) {
-            if (v < 0 || v >= a.V) lp = __builtin_nanf("");
-            else if (m != m) lp = m;
-            else if (none || (mask && !mask[v])) lp = neg_inf();
-            else lp = (S::widen(x[v]) - m) / a.temperature - ls;
+        for (int p = 0; p < P; ++p) w[p] = load_pack<S>(x + tile_index<S>(v0, lane, p * n));
+#pragma unroll
+        for (int i = 0; i < kLaneScores; ++i) f[i] = S::widen(w[i / n].v[i % n]);
+    } else {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int64_t v = tile_index<S>(v0, lane, p * n);
+            if (v + n <= v1) {
+                const Pack<S> w = load_pack<S>(x + v);
+#pragma unroll
+                for (int i = 0; i < n; ++i) f[p * n + i] = S::widen(w.v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < n; ++i) f[p * n + i] = v + i < v1 ? S::widen(x[v + i]) : neg_inf();
+            }
         }
-        given_out[t * a.G + g] = lp;
     }
-    if (lane < a.top) {
-        top_out[t * a.top + lane] = m != m ? m : key ? (score_of(key) - m) / a.temperature - ls : neg_inf();
-        top_index[t * a.top + lane] = key ? int64_t(index_of(key)) : -1;
-    }
-    }
-    __syncthreads();  // the next row's sums overwrite this one's
+    if (mask) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int64_t v = tile_index<S>(v0, lane, p * n);
+            uint8_t b[n];
+            if (v + n <= v1) {
+                __builtin_memcpy(b, mask + v, n);
+            } else {
+#pragma unroll
+                for (int i = 0; i < n; ++i) b[i] = v + i < v1 ? mask[v + i] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < n; ++i)
+                if (!b[i]) f[p * n + i] = neg_inf();
+        }
     }
 }
 
-// One workgroup per row: every score's gradient but that of the given and listed ones, then those.
+// Scores [v0, v1) of a row, by one wavefront.
 template <class S>
-__global__ __launch_bounds__(kProbsBlock) void k_probs_back(ProbsArgs a, const float* __restrict__ stats,
+__device__ __forceinline__ void scan_scores(const typename S::Bits* x, const uint8_t* mask, int64_t v0, int64_t v1,
+                                            float c2, int top, int lane, Room& room, Sums& sums, Best& best) {
+    for (; v0 < v1; v0 += kTileScores) {
+        float f[kLaneScores];
+        load_tile<S>(x, mask, v0, v1, lane, f);
+        float most = f[0];
+#pragma unroll
+        for (int i = 1; i < kLaneScores; ++i) most = max_or_nan(most, f[i]);
+        sums = moved(sums, max_or_nan(sums.m, most), c2);
+#pragma unroll
+        for (int i = 0; i < kLaneScores; ++i) add_score(sums, f[i], c2);
+        if (!top) continue;
+        if (__ballot(most != most)) {  // (the largest without the NaN)
+            most = f[0];
+#pragma unroll
+            for (int i = 1; i < kLaneScores; ++i) most = fmaxf(most, f[i]);
+            if (most != most) most = neg_inf();
+        }
+        const uint64_t lanes = __ballot(most > best.least);
+        if (!lanes) continue;
+        const uint32_t floor = __popcll(lanes) > 4 ? floor_of(order_of(most), top) : 0;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kLaneScores; ++i) {
+            const uint32_t o = order_of(f[i]);
+            const bool in = f[i] > best.least && o >= floor;
+            const uint64_t set = __ballot(in);
+            if (in) room.found[n + below(set)] = uint64_t(o) << 32 | uint32_t(~uint32_t(tile_index<S>(v0, lane, i)));
+            n += __popcll(set);
+        }
+        lds_order();
+        for (int i = 0; i < n; i += 64) {
+            const uint64_t k = i + lane < n ? room.found[i + lane] : 0;
+            best.take(__ballot(k > best.last(top)), k, room, lane);
+        }
+        best.settle(top);
+    }
+}
+
+// Merge the keys from p on: 64 N at a time, of more than 64 those that a floor found as in a tile leaves.
+template <int N>
+__device__ __forceinline__ void join_keys(Best& best, const uint64_t* p, int count, int top, Room& room, int lane) {
+    for (int i0 = 0; i0 < count; i0 += 64 * N) {
+        uint64_t k[N], most = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) k[i] = i0 + i * 64 + lane < count ? p[i0 + i * 64 + lane] : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) most = max(most, k[i]);
+        const uint32_t floor = count - i0 > 64 ? floor_of(uint32_t(most >> 32), top) : 0;
+        const uint64_t last = best.last(top);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool in = k[i] > last && uint32_t(k[i] >> 32) >= floor;
+            const uint64_t set = __ballot(in);
+            if (in) room.found[n + below(set)] = k[i];
+            n += __popcll(set);
+        }
+        lds_order();
+        for (int i = 0; i < n; i += 64) {
+            const uint64_t mine = i + lane < n ? room.found[i + lane] : 0;
+            best.take(__ballot(mine > best.last(top)), mine, room, lane);
+        }
+    }
+}
+
+struct ProbsOut {
+    float *given, *entropy, *log_sum, *top;
+    int64_t* top_index;
+    float* stats;
+};
+
+// A lane's given candidate of row t: its index, and its score (-inf where masked or out of range).
+__device__ __forceinline__ int64_t given_index(const ProbsArgs& a, int64_t t, int64_t g) {
+    return g < a.G ? a.given[t * a.G + g] : -1;
+}
+template <class S> __device__ __forceinline__ float given_score(const ProbsArgs& a, int64_t t, int64_t v) {
+    if (v < 0 || v >= a.V || (a.mask && !a.mask[t * a.mask_stride + v])) return neg_inf();
+    return S::widen(static_cast<const typename S::Bits*>(a.scores)[t * a.stride + v]);
+}
+
+// The results of row t, by one wavefront, from its sums and keys.
+template <class S>
+__device__ __forceinline__ void write_row(const ProbsArgs& a, const ProbsOut& o, int64_t t, const Sums& sums, uint64_t key,
+                                          int64_t given, float given_x, int lane) {
+    const float m = sums.m, c = 1.0f / a.temperature;
+    const bool none = m == neg_inf();
+    const float ls = m == __builtin_inff() ? __builtin_nanf("") : __builtin_amdgcn_logf(sums.s) * kLn2;  // (s >= 1)
+    if (lane == 0) {
+        const float H = none ? 0.0f : !isfinite(m) ? __builtin_nanf("") : ls - sums.u * kLn2 / sums.s;
+        o.entropy[t] = H;
+        o.log_sum[t] = isfinite(m) ? __builtin_fmaf(m, c, ls) : m;
+        *reinterpret_cast<float4*>(o.stats + t * kProbsStats) = float4{m, ls, H, 0.0f};
+    }
+    for (int64_t g = lane; g < a.G; g += 64) {
+        const int64_t v = g < 64 ? given : given_index(a, t, g);
+        const float x = g < 64 ? given_x : given_score<S>(a, t, v);
+        float lp = 0.0f;
+        if (v != -1) {
+            if (v < 0 || v >= a.V) lp = __builtin_nanf("");
+            else lp = none ? m : x == neg_inf() && m == m ? x : (x - m) * c - ls;
+        }
+        o.given[t * a.G + g] = lp;
+    }
+    if (lane < a.top) {
+        o.top[t * a.top + lane] = m != m ? m : key ? (score_of(key) - m) * c - ls : neg_inf();
+        o.top_index[t * a.top + lane] = key ? int64_t(index_of(key)) : -1;
+    }
+}
+
+// What the workgroups of a row leave for k_probs_join where there are several: their sums, and their keys.
+struct Parts {
+    Sums* sums;      // [T][blocks]
+    uint64_t* keys;  // [T][blocks][top]
+};
+
+// `waves` wavefronts per row: 1, 2, 4, 8, or a multiple of 8 (several workgroups, whose parts are joined).
+template <class S>
+__global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut o, int waves, int64_t span, Parts parts) {
+    __shared__ Sums sums_of[kProbsWaves];
+    __shared__ Room rooms[kProbsWaves];
+    __shared__ uint64_t keys_of[kProbsWaves * kMaxTop];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int group = waves < kProbsWaves ? waves : kProbsWaves;  // wavefronts of a row in the workgroup
+    const int blocks = waves / group;                             // workgroups of a row
+    const float c2 = kLog2e / a.temperature;
+    const int64_t items = waves < kProbsWaves ? (a.T * waves + kProbsWaves - 1) / kProbsWaves : a.T * blocks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t at = item * kProbsWaves + wave, t = at / waves;  // wavefront `at % waves` of row t
+        const bool in = t < a.T, writes = in && wave % group == 0;
+        Sums sums{neg_inf(), 0.0f, 0.0f};
+        Best best;
+        const int64_t given = writes && blocks == 1 ? given_index(a, t, lane) : -1;
+        float given_x = neg_inf();
+        if (in) {
+            const auto* x = static_cast<const typename S::Bits*>(a.scores) + t * a.stride;
+            const int64_t v0 = at % waves * span, v1 = min(v0 + span, a.V);
+            scan_scores<S>(x, a.mask ? a.mask + t * a.mask_stride : nullptr, v0, v1, c2, a.top, lane, rooms[wave], sums,
+                           best);
+            given_x = given_score<S>(a, t, given);
+            sums = wave_joined(sums, c2);
+        }
+        if (group > 1) {
+            if (lane == 0) sums_of[wave] = sums;
+            if (lane < a.top) keys_of[wave * a.top + lane] = best.key;
+            __syncthreads();
+            if (writes) {
+                for (int w = wave + 1; w < wave + group; ++w) sums = joined(sums, sums_of[w], c2);
+                if (a.top) join_keys<2>(best, keys_of + (wave + 1) * a.top, (group - 1) * a.top, a.top, rooms[wave], lane);
+            }
+            __syncthreads();
+        }
+        if (!writes) continue;
+        if (blocks == 1) {
+            write_row<S>(a, o, t, sums, best.key, given, given_x, lane);
+        } else {
+            if (lane == 0) parts.sums[item] = sums;
+            if (lane < a.top) parts.keys[item * a.top + lane] = best.key;
+        }
+    }
+}
+
+// One wavefront per row: its `blocks` parts.
+template <class S>
+__global__ __launch_bounds__(64) void k_probs_join(ProbsArgs a, ProbsOut o, int blocks, Parts parts) {
+    __shared__ Room room;
+    const int lane = threadIdx.x;
+    const float c2 = kLog2e / a.temperature;
+    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
+        const int64_t given = given_index(a, t, lane);
+        const Sums* of = parts.sums + t * blocks;
+        Sums sums = lane < blocks ? of[lane] : Sums{neg_inf(), 0.0f, 0.0f};
+        Best best;
+        if (a.top) join_keys<16>(best, parts.keys + t * blocks * a.top, blocks * a.top, a.top, room, lane);
+        const float given_x = given_score<S>(a, t, given);
+        for (int b = lane + 64; b < blocks; b += 64) sums = joined(sums, of[b], c2);
+        sums = wave_joined(sums, c2);
+        write_row<S>(a, o, t, sums, best.key, given, given_x, lane);
+    }
+}
+
+// Wavefronts of a row, and the scores of each: as many as fill the card (16 on each CU), none with less than a
+// tile.
+struct ProbsPlan {
+    int waves;
+    int64_t span;
+};
+ProbsPlan probs_plan(int64_t T, int64_t V) {
+    const int64_t tiles = (V + kTileScores - 1) / kTileScores;
+    const int64_t most = std::min<int64_t>((4096 + T - 1) / T, tiles);
+    int64_t w = 1;
+    while (w < most && w < kProbsWaves) w *= 2;
+    if (most > kProbsWaves) w = (most + kProbsWaves - 1) / kProbsWaves * kProbsWaves;
+    const int64_t span = (tiles + w - 1) / w * kTileScores;
+    return {int(w), span};
+}
+
+// The gradient: a wavefront per stretch of a row (four tiles, or one where that leaves CUs idle).  Every
+// score's share but that of the given and listed ones first, then those scores' once more with it, each by one
+// lane.  Memory bound: reads and writes each score once.
+constexpr int kBackBlock = 256, kBackWaves = kBackBlock / 64;
+int64_t back_span(int64_t T, int64_t V) {
+    return (T * ((V + kTileScores - 1) / kTileScores) >= 16384 ? 4 : 1) * int64_t(kTileScores);
+}
+
+template <class S>
+__global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t span, const float* __restrict__ stats,
                                                             const int64_t* __restrict__ top_index,
                                                             const float* __restrict__ d_given,
                                                             const float* __restrict__ d_entropy,
                                                             const float* __restrict__ d_log_sum,
                                                             const float* __restrict__ d_top,
                                                             typename S::Bits* __restrict__ d_scores) {
-    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
-    const auto* x = static_cast<const typename S::Bits*>(a.scores) + t * a.stride;
-    auto* d = d_scores + t * a.V;
-    const uint8_t* mask = a.mask ? a.mask + t * a.mask_stride : nullptr;
-    const float m = stats[t * kProbsStats], ls = stats[t * kProbsStats + 1], H = stats[t * kProbsStats + 2];
-    const float c = 1.0f / a.temperature, c2 = kLog2e / a.temperature, ls2 = ls * kLog2e;
-    const bool none = m == neg_inf();
+    const int lane = threadIdx.x & 63;
+    const float c = 1.0f / a.temperature, c2 = kLog2e / a.temperature;
     const int64_t G = d_given ? a.G : 0;
     const int K = d_top ? a.top : 0;
-    float all = d_log_sum ? d_log_sum[t] : 0.0f;
-    for (int64_t g = 0; g < G; ++g)
-        if (a.given[t * G + g] != -1) all -= d_given[t * G + g];
-    for (int j = 0; j < K; ++j)
-        if (top_index[t * K + j] >= 0) all -= d_top[t * K + j];
-    const float dH = d_entropy ? d_entropy[t] : 0.0f;
-    // the gradient of score v without what is given or listed there
-    auto smooth = [&](int64_t v) {
-        if (none || (mask && !mask[v])) return 0.0f;
-        const float lp2 = (S::widen(x[v]) - m) * c2 - ls2, p = __builtin_amdgcn_exp2f(lp2);
-        return p * (all - dH * (fmaxf(lp2, -200.0f) * kLn2 + H));
-    };
-    for (int64_t v = threadIdx.x; v < a.V; v += kProbsBlock) d[v] = S::round(c * smooth(v));
-    __syncthreads();
-    for (int64_t i = threadIdx.x; i < G + K; i += kProbsBlock) {
-        auto at = [&](int64_t j) { return j < G ? a.given[t * G + j] : top_index[t * K + j - G]; };
-        const int64_t v = at(i);
-        if (none || v < 0 || v >= a.V || (mask && !mask[v])) continue;
-        float sum = 0.0f;
-        bool first = true;
-        for (int64_t j = 0; j < G + K; ++j)
-            if (at(j) == v) {
-                if (j < i) first = false;
-                sum += j < G ? d_given[t * G + j] : d_top[t * K + j - G];
+    const int64_t spans = (a.V + span - 1) / span;
+    for (int64_t item = int64_t(blockIdx.x) * kBackWaves + (threadIdx.x >> 6); item < a.T * spans;
+         item += int64_t(gridDim.x) * kBackWaves) {
+        const int64_t t = item / spans, first = (item - t * spans) * span, end = min(first + span, a.V);
+        const auto* x = static_cast<const typename S::Bits*>(a.scores) + t * a.stride;
+        auto* d = d_scores + t * a.V;
+        const uint8_t* mask = a.mask ? a.mask + t * a.mask_stride : nullptr;
+        // a lane's given or listed candidate and its upstream gradient (the first 64; more are read again below)
+        const int64_t n = G + K;
+        auto index_at = [&](int64_t j) { return j < G ? a.given[t * G + j] : top_index[t * K + j - G]; };
+        auto up_at = [&](int64_t j) { return j < G ? d_given[t * G + j] : d_top[t * K + j - G]; };
+        const int64_t mine = lane < n ? index_at(lane) : -1;
+        const float up = lane < n ? up_at(lane) : 0.0f;
+        const float4 st = *reinterpret_cast<const float4*>(stats + t * kProbsStats);
+        const float dL = d_log_sum ? d_log_sum[t] : 0.0f, dH = d_entropy ? d_entropy[t] : 0.0f;
+        float f[kLaneScores];
+        load_tile<S>(x, mask, first, end, lane, f);
+        const bool fix = mine >= first && mine < end && !(mask && !mask[mine]);
+        const float at_mine = fix ? S::widen(x[mine]) : 0.0f;
+        const float m = st.x, ls = st.y, H = st.z, ls2 = ls * kLog2e;
+        const bool none = m == neg_inf();
+        float all = mine != -1 ? -up : 0.0f;
+        for (int64_t j = lane + 64; j < n; j += 64)
+            if (index_at(j) != -1) all -= up_at(j);
+        all = wave_sum(all) + dL;
+        // the gradient of score f without what is given or listed there; 0 where not allowed
+        auto smooth = [&](float f) {
+            const float lp2 = fmaxf((f - m) * c2 - ls2, -200.0f), p = __builtin_amdgcn_exp2f(lp2);
+            return p * (all - dH * __builtin_fmaf(lp2, kLn2, H));
+        };
+        const bool broken = !(ls == ls);  // a NaN or +inf in the row: so are its gradients
+        for (int64_t v0 = first; v0 < end; v0 += kTileScores) {
+            if (v0 != first) load_tile<S>(x, mask, v0, end, lane, f);
+            constexpr int P = Pack<S>::n;
+#pragma unroll
+            for (int p = 0; p < kLaneScores / P; ++p) {
+                Pack<S> w;
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float g = c * smooth(f[p * P + i]);
+                    w.v[i] = S::round(none ? 0.0f : broken ? __builtin_nanf("") : g);
+                }
+                const int64_t v = tile_index<S>(v0, lane, p * P);
+                if (v + P <= end) {
+                    store_pack<S>(d + v, w);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        if (v + i < end) d[v + i] = w.v[i];
+                }
             }
-        if (first) d[v] = S::round(c * (smooth(v) + sum));
+        }
+        if (none || broken) continue;
+        // (the stores above come before those below: one wavefront's, in order)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (n <= 64) {
+            // what is given or listed at the same score is summed by the first lane that holds it
+            float sum = 0.0f;
+            bool is_first = true;
+            for (int l = 0; l < int(n); ++l) {
+                const bool same = read_lane(uint64_t(mine), l) == uint64_t(mine);
+                if (same) sum += __uint_as_float(read_lane(__float_as_uint(up), l));
+                if (same && l < lane) is_first = false;
+            }
+            if (fix && is_first) d[mine] = S::round(c * (smooth(at_mine) + sum));
+            continue;
+        }
+        for (int64_t i = lane; i < n; i += 64) {
+            const int64_t v = index_at(i);
+            if (v < first || v >= end || (mask && !mask[v])) continue;
+            float sum = 0.0f;
+            bool is_first = true;
+            for (int64_t j = 0; j < n; ++j)
+                if (index_at(j) == v) {
+                    if (j < i) is_first = false;
+                    sum += up_at(j);
+                }
+            if (is_first) d[v] = S::round(c * (smooth(S::widen(x[v])) + sum));
+        }
     }
-    }
+}
+
+template <class S>
+hipError_t probs(const ProbsArgs& a, const ProbsOut& o, void* work, hipStream_t s) {
+    const ProbsPlan p = probs_plan(a.T, a.V);
+    const int64_t blocks = p.waves / kProbsWaves;
+    auto* keys = static_cast<uint64_t*>(work);
+    const Parts parts{reinterpret_cast<Sums*>(keys + a.T * blocks * a.top), keys};
+    const int64_t items = p.waves < kProbsWaves ? (a.T * p.waves + kProbsWaves - 1) / kProbsWaves : a.T * blocks;
+    k_probs<S><<<match_grid(items), kProbsBlock, 0, s>>>(a, o, p.waves, p.span, parts);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (blocks > 1) k_probs_join<S><<<match_grid(a.T), 64, 0, s>>>(a, o, int(blocks), parts);
+    return hipGetLastError();
+}
+
+template <class S>
+hipError_t probs_back(const ProbsArgs& a, const float* stats, const int64_t* top_index, const float* d_given,
+                      const float* d_entropy, const float* d_log_sum, const float* d_top, void* d_scores,
+                      hipStream_t s) {
+    const int64_t span = back_span(a.T, a.V), items = a.T * ((a.V + span - 1) / span);
+    k_probs_back<S><<<match_grid((items + kBackWaves - 1) / kBackWaves), kBackBlock, 0, s>>>(
+        a, span, stats, top_index, d_given, d_entropy, d_log_sum, d_top, static_cast<typename S::Bits*>(d_scores));
+    return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t log_probs_work(int64_t, int64_t, int) { return 0; }
+int64_t log_probs_work(int64_t T, int64_t V, int top) {
+    const ProbsPlan p = probs_plan(T, V);
+    return p.waves > kProbsWaves ? T * (p.waves / kProbsWaves) * (int64_t(sizeof(Sums)) + 8 * int64_t(top)) : 0;
+}
 
 hipError_t launch_log_probs(const ProbsArgs& a, float* given_out, float* entropy, float* log_sum, float* top_out,
-                            int64_t* top_index, float* stats, void*, hipStream_t s) {
-    const dim3 grid(match_grid(a.T));
+                            int64_t* top_index, float* stats, void* work, hipStream_t s) {
+    const ProbsOut o{given_out, entropy, log_sum, top_out, top_index, stats};
     switch (a.dt) {
-        case TP_F32:
-            k_probs<F32><<<grid, kProbsBlock, 0, s>>>(a, given_out, entropy, log_sum, top_out, top_index, stats);
-            break;
-        case TP_F16:
-            k_probs<F16><<<grid, kProbsBlock, 0, s>>>(a, given_out, entropy, log_sum, top_out, top_index, stats);
-            break;
-        default:
-            k_probs<BF16><<<grid, kProbsBlock, 0, s>>>(a, given_out, entropy, log_sum, top_out, top_index, stats);
+        case TP_F32: return probs<F32>(a, o, work, s);
+        case TP_F16: return probs<F16>(a, o, work, s);
+        default: return probs<BF16>(a, o, work, s);
     }
-    return hipGetLastError();
 }
 
 hipError_t launch_log_probs_back(const ProbsArgs& a, const float* stats, const int64_t* top_index,
                                  const float* d_given, const float* d_entropy, const float* d_log_sum,
                                  const float* d_top, void* d_scores, hipStream_t s) {
-    const dim3 grid(match_grid(a.T));
     switch (a.dt) {
-        case TP_F32:
-            k_probs_back<F32><<<grid, kProbsBlock, 0, s>>>(a, stats, top_index, d_given, d_entropy, d_log_sum, d_top,
-                                                           static_cast<uint32_t*>(d_scores));
-            break;
-        case TP_F16:
-            k_probs_back<F16><<<grid, kProbsBlock, 0, s>>>(a, stats, top_index, d_given, d_entropy, d_log_sum, d_top,
-                                                           static_cast<uint16_t*>(d_scores));
-            break;
-        default:
-            k_probs_back<BF16><<<grid, kProbsBlock, 0, s>>>(a, stats, top_index, d_given, d_entropy, d_log_sum, d_top,
-                                                            static_cast<uint16_t*>(d_scores));
+        case TP_F32: return probs_back<F32>(a, stats, top_index, d_given, d_entropy, d_log_sum, d_top, d_scores, s);
+        case TP_F16: return probs_back<F16>(a, stats, top_index, d_given, d_entropy, d_log_sum, d_top, d_scores, s);
+        default: return probs_back<BF16>(a, stats, top_index, d_given, d_entropy, d_log_sum, d_top, d_scores, s);
     }
-    return hipGetLastError();
 }
 
 }  // namespace tp

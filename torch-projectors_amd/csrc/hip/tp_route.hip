@@ -14,213 +14,512 @@
 #include "../../../include/torch_projectors_hip.h"
 #include "tp_match.hh"
 
+#include <algorithm>
+
 namespace tp {
 namespace {
 
 // ------------------------------------------------------------------ sort
-constexpr int kSortWaves = 4;
+// A workgroup of W wavefronts sorts up to 64 W kGroups slots: each wavefront takes consecutive groups of 64, keeps
+// their classes and their ranks among its own slots of that class in registers, and its counts per class in
+// LDS.  Few slots are one workgroup's (16 wavefronts hold 8192); of more, a first kernel counts each workgroup's
+// stretch, and the second, knowing every stretch's counts, places it.
+constexpr int kGroups = 8, kMaxSortWaves = 16, kOneSort = 64 * kMaxSortWaves * kGroups;
+constexpr int kDirectStretches = 64;  // as many are summed by every workgroup of the second kernel by itself
 
 template <class I> __device__ __forceinline__ int class_of(const I* ids, int64_t i, int E) {
     const I c = ids[i];
     return c >= 0 && c < I(E) ? int(c) : E;
 }
 
-// One workgroup sorts all slots: counts per wavefront, their prefix sums in (class, wavefront) order, places.
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(v, d);
+        v += lane >= d ? u : 0;
+    }
+    return v;
+}
+
+// Places slots [i0, i1) (i1 - i0 at most 64 waves kGroups a turn; several turns where there are more).
+// before: for each class the slots of earlier stretches, all: those of all stretches (null: there is one).
 template <class I>
-__global__ __launch_bounds__(64 * kSortWaves) void k_sort_one(const I* __restrict__ ids, int n, int E,
-                                                              int* __restrict__ order, int* __restrict__ slot,
-                                                              int* __restrict__ offsets) {
-    extern __shared__ int cnt[];  // [kSortWaves][E + 1], then [E + 1] of totals
-    int* total = cnt + kSortWaves * (E + 1);
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int groups = (n + 63) / 64, per = (groups + kSortWaves - 1) / kSortWaves;
-    const int g0 = wave * per, g1 = min(g0 + per, groups);
-    int* mine = cnt + wave * (E + 1);
-    for (int i = tid; i < kSortWaves * (E + 1); i += 64 * kSortWaves) cnt[i] = 0;
-    __syncthreads();
-    for (int g = g0; g < g1; ++g) {
-        const int i = g * 64 + lane;
-        if (i < n) atomicAdd(&mine[class_of(ids, i, E)], 1);
-    }
-    __syncthreads();
-    for (int c = tid; c <= E; c += 64 * kSortWaves) {
-        int t = 0;
-        for (int w = 0; w < kSortWaves; ++w) t += cnt[w * (E + 1) + c];
-        total[c] = t;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        int at = 0;
-        for (int c = 0; c <= E; ++c) {
-            const int t = total[c];
-            total[c] = at;
-            at += t;
-        }
-    }
-    __syncthreads();
-    for (int c = tid; c <= E; c += 64 * kSortWaves) {
-        int at = total[c];
-        offsets[c] = at;
-        for (int w = 0; w < kSortWaves; ++w) {
-            const int t = cnt[w * (E + 1) + c];
-            cnt[w * (E + 1) + c] = at;
-            at += t;
-        }
-    }
-    __syncthreads();
+__global__ __launch_bounds__(64 * kMaxSortWaves) void k_sort_place(const I* __restrict__ ids, int64_t n, int64_t stretch,
+                                                                   int E, const int* __restrict__ counts, int stretches,
+                                                                   bool summed, int* __restrict__ order,
+                                                                   int* __restrict__ slot, int* __restrict__ offsets) {
+    extern __shared__ int lds[];
+    const int C = E + 1, waves = blockDim.x >> 6, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    int* cnt = lds;               // [waves][C]: counts, then places of the wavefront's next slots
+    int* base = lds + waves * C;  // [C]: place of the workgroup's next slot of a class
+    __shared__ int wave_total[kMaxSortWaves];
+    __shared__ int carry;
+    const int64_t i0 = int64_t(blockIdx.x) * stretch, i1 = min(i0 + stretch, n);
     const int bits = 32 - __clz(E);
-    for (int g = g0; g < g1; ++g) {
-        const int i = g * 64 + lane;
-        const bool in = i < n;
-        const int c = in ? class_of(ids, i, E) : -1;
-        uint64_t same = __ballot(in);
-        for (int b = 0; b < bits; ++b) {
-            const uint64_t set = __ballot((c >> b) & 1);
-            same &= (c >> b) & 1 ? set : ~set;
+
+    // base: an exclusive scan of the classes' totals, plus what earlier stretches hold (one stretch: the scan
+    // follows the counting below)
+    auto scan_classes = [&](auto total, auto done) {
+        if (tid == 0) carry = 0;
+        for (int c0 = 0; c0 < C; c0 += int(blockDim.x)) {
+            const int c = c0 + tid, t = c < C ? total(c) : 0, s = wave_scan(t);
+            if (lane == 63) wave_total[wave] = s;
+            __syncthreads();
+            int at = carry + s - t;
+            for (int w = 0; w < wave; ++w) at += wave_total[w];
+            if (c < C) done(c, at);
+            __syncthreads();
+            if (tid == int(blockDim.x) - 1) carry = at + t;
+            __syncthreads();
         }
-        if (in) {
-            const int place = mine[c] + __popcll(same & ((uint64_t(1) << lane) - 1));
-            order[place] = i;
-            slot[i] = place;
-            // the last lane of each class moves its counter on, after all lanes have read it
-            __builtin_amdgcn_wave_barrier();
-            if (lane == 63 - __clzll(same)) mine[c] = place + 1;
-        }
-        __builtin_amdgcn_wave_barrier();
+    };
+    if (counts) {
+        scan_classes(
+            [&](int c) {
+                if (summed) {  // counts: [stretch][C] of earlier stretches' slots, then the totals
+                    base[c] = counts[int64_t(blockIdx.x) * C + c];
+                    return counts[int64_t(stretches) * C + c];
+                }
+                int earlier = 0, all = 0;
+                for (int b = 0; b < stretches; ++b) {
+                    const int v = counts[int64_t(b) * C + c];
+                    all += v;
+                    earlier += b < int(blockIdx.x) ? v : 0;
+                }
+                base[c] = earlier;
+                return all;
+            },
+            [&](int c, int at) {
+                base[c] += at;
+                if (blockIdx.x == 0) offsets[c] = at;
+            });
     }
+    for (int64_t turn = i0; turn < i1 || turn == i0; turn += int64_t(waves) * 64 * kGroups) {
+        for (int i = tid; i < waves * C; i += blockDim.x) cnt[i] = 0;
+        __syncthreads();
+        int cls[kGroups], rank[kGroups];
+        int* mine = cnt + wave * C;
+        const int64_t first = turn + int64_t(wave) * 64 * kGroups;
+        // a short stretch is dealt to the wavefronts in equal shares
+        const int groups = int(min(int64_t(kGroups), (i1 - turn + 64 * waves - 1) / (64 * waves)));
+        const int64_t start = groups == kGroups ? first : turn + int64_t(wave) * 64 * groups;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int64_t i = start + g * 64 + lane;
+            cls[g] = g < groups && i < i1 ? class_of(ids, i, E) : -1;
+        }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            if (g >= groups) break;
+            const int c = cls[g];
+            uint64_t same = __ballot(c >= 0);
+            if (c >= 0) {
+                for (int b = 0; b < bits; ++b) {
+                    const uint64_t set = __ballot((c >> b) & 1);
+                    same &= (c >> b) & 1 ? set : ~set;
+                }
+                const int old = mine[c];
+                rank[g] = old + __popcll(same & ((uint64_t(1) << lane) - 1));
+                // the last lane of each class counts on, after all lanes have read
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                if (lane == 63 - __clzll(same)) mine[c] = rank[g] + 1;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
+        }
+        __syncthreads();
+        auto to_places = [&](int c, int at) {  // wavefronts' counts of class c to their first places
+            for (int w = 0; w < waves; ++w) {
+                const int t = cnt[w * C + c];
+                cnt[w * C + c] = at;
+                at += t;
+            }
+            return at;
+        };
+        if (counts) {
+            for (int c = tid; c < C; c += blockDim.x) base[c] = to_places(c, base[c]);
+            __syncthreads();
+        } else {
+            scan_classes(
+                [&](int c) {
+                    int t = 0;
+                    for (int w = 0; w < waves; ++w) t += cnt[w * C + c];
+                    return t;
+                },
+                [&](int c, int at) {
+                    offsets[c] = at;
+                    to_places(c, at);
+                });
+        }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            if (g >= groups || cls[g] < 0) continue;
+            const int64_t i = start + g * 64 + lane;
+            const int place = mine[cls[g]] + rank[g];
+            order[place] = int(i);
+            slot[i] = place;
+        }
+        __syncthreads();
+    }
+}
+
+// counts[b][c]: slots of class c in stretch b.
+template <class I>
+__global__ __launch_bounds__(1024) void k_sort_count(const I* __restrict__ ids, int64_t n, int64_t stretch, int E,
+                                                     int* __restrict__ counts) {
+    extern __shared__ int lds[];
+    const int C = E + 1;
+    for (int c = threadIdx.x; c < C; c += blockDim.x) lds[c] = 0;
+    __syncthreads();
+    const int64_t i1 = min(int64_t(blockIdx.x + 1) * stretch, n);
+    for (int64_t i = int64_t(blockIdx.x) * stretch + threadIdx.x; i < i1; i += blockDim.x)
+        atomicAdd(&lds[class_of(ids, i, E)], 1);  // (a count: in any order the same)
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += blockDim.x) counts[int64_t(blockIdx.x) * C + c] = lds[c];
+}
+
+// Many stretches: their counts to the sums of earlier ones, and the totals after them.  64 classes a workgroup, whose
+// wavefronts take consecutive stretches.
+__global__ __launch_bounds__(1024) void k_sort_sum(int* __restrict__ counts, int stretches, int C) {
+    __shared__ int part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+    const int b0 = int(int64_t(stretches) * wave / 16), b1 = int(int64_t(stretches) * (wave + 1) / 16);
+    int sum = 0;
+    if (c < C)
+        for (int b = b0; b < b1; ++b) sum += counts[int64_t(b) * C + c];
+    part[wave][lane] = sum;
+    __syncthreads();
+    if (c >= C) return;
+    int at = 0;
+    for (int w = 0; w < wave; ++w) at += part[w][lane];
+    for (int b = b0; b < b1; ++b) {
+        const int v = counts[int64_t(b) * C + c];
+        counts[int64_t(b) * C + c] = at;
+        at += v;
+    }
+    if (wave == 15) counts[int64_t(stretches) * C + c] = at;
+}
+
+// Wavefronts of the placing workgroups (LDS holds a count per class for each), and the slots of each.
+struct SortPlan {
+    int waves, stretches;
+    int64_t stretch;
+};
+SortPlan sort_plan(int64_t n, int E) {
+    int waves = E <= 1024 ? kMaxSortWaves : 4;
+    const int64_t hold = int64_t(waves) * 64 * kGroups;
+    if (n <= hold) {
+        while (waves > 1 && int64_t(waves / 2) * 64 >= n) waves /= 2;
+        return {waves, 1, std::max<int64_t>(n, 1)};
+    }
+    // at most 2048 stretches, of whole turns
+    const int64_t turns = (n + hold - 1) / hold, each = (turns + 2047) / 2048;
+    return {waves, int((turns + each - 1) / each), each * hold};
+}
+
+template <class I>
+hipError_t sort(const I* ids, int64_t n, int E, int* order, int* slot, int* offsets, int* counts, hipStream_t s) {
+    const SortPlan p = sort_plan(n, E);
+    const int C = E + 1;
+    const bool summed = p.stretches > kDirectStretches;
+    if (p.stretches > 1) {
+        k_sort_count<I><<<p.stretches, 1024, C * sizeof(int), s>>>(ids, n, p.stretch, E, counts);
+        if (summed) k_sort_sum<<<(C + 63) / 64, 1024, 0, s>>>(counts, p.stretches, C);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    const size_t lds = size_t(p.waves + 1) * C * sizeof(int);
+    if (lds > 65536)
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_sort_place<I>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)))
+            return e;
+    k_sort_place<I><<<p.stretches, 64 * p.waves, lds, s>>>(ids, n, p.stretch, E, p.stretches > 1 ? counts : nullptr,
+                                                           p.stretches, summed, order, slot, offsets);
+    return hipGetLastError();
 }
 
 // ------------------------------------------------------------------ rows
-constexpr int kRowBlock = 256;
+// Both directions go by rows, not places: W wavefronts take a row (or a stretch of it), whose k places they know,
+// so that the row is read (spread) or written (gather) once whatever k is.  Memory bound.  Values move 16 bytes a
+// lane at a time, whatever the rows' alignment; of up to KB choices the loads are in flight together, and the
+// products for the weights' gradient stay in registers.  More than KB choices: spread goes over the row again for
+// each KB of them, gather reads KB at a time and does the products in a second look.
+template <class S> struct Values {
+    static constexpr int n = Pack<S>::n;
+    float v[n];
+};
+template <class S> __device__ __forceinline__ Values<S> load_values(const typename S::Bits* p, int64_t left) {
+    Values<S> r;
+    if (left >= Values<S>::n) {
+        const Pack<S> w = load_pack<S>(p);
+#pragma unroll
+        for (int i = 0; i < Values<S>::n; ++i) r.v[i] = S::widen(w.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Values<S>::n; ++i) r.v[i] = i < left ? S::widen(p[i]) : 0.0f;
+    }
+    return r;
+}
+template <class S> __device__ __forceinline__ void store_values(typename S::Bits* p, int64_t left, const Values<S>& r) {
+    Pack<S> w;
+#pragma unroll
+    for (int i = 0; i < Values<S>::n; ++i) w.v[i] = S::round(r.v[i]);
+    if (left >= Values<S>::n) {
+        store_pack<S>(p, w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Values<S>::n; ++i)
+            if (i < left) p[i] = w.v[i];
+    }
+}
 
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-    v = wave_sum(v);
+// The places of KB choices of a row and what they weigh.
+template <int KB> struct Places {
+    int64_t at[KB];  // first value of the row there
+    float w[KB];
+    bool in[KB], real[KB];
+};
+template <int KB>
+__device__ __forceinline__ Places<KB> places_of(const RouteArgs& a, int64_t t, int j0, int kept) {
+    Places<KB> p;
+#pragma unroll
+    for (int u = 0; u < KB; ++u) {
+        p.real[u] = j0 + u < a.k;
+        const int64_t s = t * a.k + j0 + u;
+        const int at = p.real[u] ? a.slot[s] : 0;
+        p.in[u] = p.real[u] && at < kept;
+        p.at[u] = int64_t(at) * a.D;
+        p.w[u] = p.real[u] && a.weights ? a.weights[s] : 1.0f;
+    }
+    return p;
+}
+
+// Sums of the W wavefronts of a row, the same in all of them.
+template <int W, int KB> __device__ __forceinline__ void row_sums(float (&v)[KB], float (*lds)[KB]) {
+#pragma unroll
+    for (int u = 0; u < KB; ++u) v[u] = wave_sum(v[u]);
+    if (W == 1) return;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int u = 0; u < KB; ++u) lds[threadIdx.x >> 6][u] = v[u];
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+#pragma unroll
+    for (int u = 0; u < KB; ++u) {
+        v[u] = lds[0][u];
+#pragma unroll
+        for (int w = 1; w < W; ++w) v[u] += lds[w][u];
+    }
     __syncthreads();
-    float t = 0;
-    for (int w = 0; w < kRowBlock / 64; ++w) t += lds[w];
-    return t;
 }
 
-// One workgroup per row.
-template <class S, bool DOT>
-__global__ __launch_bounds__(kRowBlock) void k_spread_rows(RouteArgs a, const typename S::Bits* __restrict__ x,
-                                                           typename S::Bits* __restrict__ sorted,
-                                                           const typename S::Bits* __restrict__ rows,
-                                                           float* __restrict__ d_weights) {
-    __shared__ float lds[kRowBlock / 64];
-    const int kept = *a.kept;
-    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x)
-    for (int j = 0; j < a.k; ++j) {
-        const int at = a.slot[t * a.k + j];
-        const bool in = at < kept;
-        const float w = a.weights ? a.weights[t * a.k + j] : 1.0f;
-        float dot = 0;
-        for (int64_t d = threadIdx.x; d < a.D; d += kRowBlock) {
-            const float v = S::widen(x[t * a.D + d]);
-            sorted[int64_t(at) * a.D + d] = S::round(in ? w * v : 0.0f);
-            if (DOT) dot += in ? v * S::widen(rows[int64_t(at) * a.D + d]) : 0.0f;
-        }
-        if (DOT) {
-            dot = block_sum(dot, lds);
-            if (threadIdx.x == 0) d_weights[t * a.k + j] = dot;
+// W wavefronts per item: a workgroup of 256 with four items (W = 1), or one item of W wavefronts.  An item is a
+// stretch of `span` values of a row; `parts` of them are a row (one with DOT).
+template <int W> constexpr int row_block() { return W == 1 ? 256 : 64 * W; }
+struct RowItem {
+    int64_t t, d0, d1;
+};
+template <int W> __device__ __forceinline__ bool row_item(const RouteArgs& a, int64_t item0, int64_t span, int parts, RowItem& r) {
+    const int64_t item = item0 + (W == 1 ? __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)) : 0);
+    if (item >= a.T * parts) return false;
+    r.t = parts == 1 ? item : item / parts;
+    r.d0 = (item - r.t * parts) * span;
+    r.d1 = min(r.d0 + span, a.D);
+    return true;
+}
+
+template <class S, int W, int KB, bool DOT>
+__global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int64_t span, int parts,
+                                                                const typename S::Bits* __restrict__ x,
+                                                                typename S::Bits* __restrict__ sorted,
+                                                                const typename S::Bits* __restrict__ rows,
+                                                                float* __restrict__ d_weights) {
+    constexpr int n = Values<S>::n, items = W == 1 ? 4 : 1;
+    __shared__ float lds[W][KB];
+    const int kept = *a.kept, lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    for (int64_t item0 = int64_t(blockIdx.x) * items; item0 < a.T * parts; item0 += int64_t(gridDim.x) * items) {
+        RowItem r;
+        if (!row_item<W>(a, item0, span, parts, r)) break;
+        for (int j0 = 0; j0 < a.k; j0 += KB) {
+            const Places<KB> p = places_of<KB>(a, r.t, j0, kept);
+            float dot[KB] = {};
+            for (int64_t d = r.d0 + lane * n; d < r.d1; d += W * 64 * n) {
+                const int64_t left = r.d1 - d;
+                const Values<S> v = load_values<S>(x + r.t * a.D + d, left);
+                Values<S> o[KB];
+                if (DOT) {
+#pragma unroll
+                    for (int u = 0; u < KB; ++u) {
+                        if (p.in[u]) o[u] = load_values<S>(rows + p.at[u] + d, left);
+                        else o[u] = Values<S>{};
+                    }
+#pragma unroll
+                    for (int u = 0; u < KB; ++u)
+                        if (p.in[u])
+#pragma unroll
+                            for (int i = 0; i < n; ++i) dot[u] = __builtin_fmaf(v.v[i], o[u].v[i], dot[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < KB; ++u) {
+                    if (!p.real[u]) continue;
+#pragma unroll
+                    for (int i = 0; i < n; ++i) o[u].v[i] = p.in[u] ? p.w[u] * v.v[i] : 0.0f;
+                    store_values<S>(sorted + p.at[u] + d, left, o[u]);
+                }
+            }
+            if (DOT) {
+                row_sums<W, KB>(dot, lds);
+                if (lane == 0)
+#pragma unroll
+                    for (int u = 0; u < KB; ++u)
+                        if (p.real[u]) d_weights[r.t * a.k + j0 + u] = dot[u];
+            }
         }
     }
 }
 
-template <class S, bool DOT>
-__global__ __launch_bounds__(kRowBlock) void k_gather_rows(RouteArgs a, const typename S::Bits* __restrict__ rows,
-                                                           typename S::Bits* __restrict__ out,
-                                                           const typename S::Bits* __restrict__ x,
-                                                           float* __restrict__ d_weights) {
-    __shared__ float lds[kRowBlock / 64];
-    const int kept = a.k ? *a.kept : 0;
-    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
-    for (int64_t d = threadIdx.x; d < a.D; d += kRowBlock) {
-        float sum = 0;
-        for (int j = 0; j < a.k; ++j) {
-            const int at = a.slot[t * a.k + j];
-            if (at >= kept) continue;
-            const float w = a.weights ? a.weights[t * a.k + j] : 1.0f;
-            sum += w * S::widen(rows[int64_t(at) * a.D + d]);
+template <class S, int W, int KB, bool DOT>
+__global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int64_t span, int parts,
+                                                                const typename S::Bits* __restrict__ rows,
+                                                                typename S::Bits* __restrict__ out,
+                                                                const typename S::Bits* __restrict__ x,
+                                                                float* __restrict__ d_weights) {
+    constexpr int n = Values<S>::n, items = W == 1 ? 4 : 1;
+    __shared__ float lds[W][KB];
+    const int kept = a.k ? *a.kept : 0, lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    for (int64_t item0 = int64_t(blockIdx.x) * items; item0 < a.T * parts; item0 += int64_t(gridDim.x) * items) {
+        RowItem r;
+        if (!row_item<W>(a, item0, span, parts, r)) break;
+        Places<KB> p = places_of<KB>(a, r.t, 0, kept);
+        float dot[KB] = {};
+        for (int64_t d = r.d0 + lane * n; d < r.d1; d += W * 64 * n) {
+            const int64_t left = r.d1 - d;
+            Values<S> sum{}, v{}, o[KB];
+            for (int j0 = 0; j0 < a.k; j0 += KB) {
+                if (a.k > KB) p = places_of<KB>(a, r.t, j0, kept);
+#pragma unroll
+                for (int u = 0; u < KB; ++u) {
+                    if (p.in[u]) o[u] = load_values<S>(rows + p.at[u] + d, left);
+                    else o[u] = Values<S>{};
+                }
+                if (DOT && a.k <= KB) v = load_values<S>(x + r.t * a.D + d, left);
+#pragma unroll
+                for (int u = 0; u < KB; ++u)
+                    if (p.in[u])
+#pragma unroll
+                        for (int i = 0; i < n; ++i) {
+                            sum.v[i] += p.w[u] * o[u].v[i];
+                            if (DOT) dot[u] = __builtin_fmaf(v.v[i], o[u].v[i], dot[u]);
+                        }
+            }
+            store_values<S>(out + r.t * a.D + d, left, sum);
         }
-        out[t * a.D + d] = S::round(sum);
-    }
-    if (DOT)
-        for (int j = 0; j < a.k; ++j) {
-            const int at = a.slot[t * a.k + j];
-            float dot = 0;
-            if (at < kept)
-                for (int64_t d = threadIdx.x; d < a.D; d += kRowBlock)
-                    dot += S::widen(x[t * a.D + d]) * S::widen(rows[int64_t(at) * a.D + d]);
-            dot = block_sum(dot, lds);
-            if (threadIdx.x == 0) d_weights[t * a.k + j] = dot;
+        if (!DOT) continue;
+        for (int j0 = 0; j0 < a.k; j0 += KB) {
+            if (a.k > KB) {
+                p = places_of<KB>(a, r.t, j0, kept);
+#pragma unroll
+                for (int u = 0; u < KB; ++u) dot[u] = 0.0f;
+                for (int64_t d = r.d0 + lane * n; d < r.d1; d += W * 64 * n) {
+                    const int64_t left = r.d1 - d;
+                    const Values<S> v = load_values<S>(x + r.t * a.D + d, left);
+#pragma unroll
+                    for (int u = 0; u < KB; ++u) {
+                        if (!p.in[u]) continue;
+                        const Values<S> o = load_values<S>(rows + p.at[u] + d, left);
+#pragma unroll
+                        for (int i = 0; i < n; ++i) dot[u] = __builtin_fmaf(v.v[i], o.v[i], dot[u]);
+                    }
+                }
+            }
+            row_sums<W, KB>(dot, lds);
+            if (lane == 0)
+#pragma unroll
+                for (int u = 0; u < KB; ++u)
+                    if (p.real[u]) d_weights[r.t * a.k + j0 + u] = dot[u];
         }
     }
 }
 
-template <class S>
-hipError_t spread(const RouteArgs& a, const void* x, void* sorted, const void* rows, float* d_weights, hipStream_t s) {
+// Wavefronts of a row: one while a row is at most 4 KB (four loads a lane), else 4, or 16 where rows are so few
+// that CUs would idle (with the weights' gradient, whose sums need the whole row in one workgroup); without it a
+// row of few is cut into stretches instead.
+struct RowPlan {
+    int waves, parts;
+    int64_t span;
+};
+RowPlan row_plan(const RouteArgs& a, int size, bool dot) {
+    const int64_t bytes = a.D * size;
+    RowPlan p{bytes <= 4096 ? 1 : 4, 1, a.D};
+    if (a.T * p.waves >= 2048 || bytes <= 1024) return p;
+    if (dot) {
+        p.waves = bytes <= 4096 ? 4 : 16;
+        return p;
+    }
+    p.waves = 1;
+    const int64_t want = (2048 + a.T - 1) / a.T, step = 1024 / size;  // a wavefront's values at once
+    p.span = ((a.D + want - 1) / want + step - 1) / step * step;
+    p.parts = int((a.D + p.span - 1) / p.span);
+    return p;
+}
+
+#define TP_ROWS(kernel, W, KB)                                                                                      \
+    (dot ? kernel<S, W, KB, true><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, in, to, other, d_weights)     \
+         : kernel<S, W, KB, false><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, in, to, nullptr, nullptr))
+#define TP_ROWS_BY_K(kernel, W) (a.k <= 2 ? TP_ROWS(kernel, W, 2) : TP_ROWS(kernel, W, 4))
+
+template <class S, bool SPREAD>
+hipError_t move_rows(const RouteArgs& a, const void* in_, void* to_, const void* other_, float* d_weights, hipStream_t s) {
     using B = typename S::Bits;
-    const dim3 grid(match_grid(a.T));
-    if (d_weights)
-        k_spread_rows<S, true><<<grid, kRowBlock, 0, s>>>(a, static_cast<const B*>(x), static_cast<B*>(sorted),
-                                                          static_cast<const B*>(rows), d_weights);
-    else
-        k_spread_rows<S, false><<<grid, kRowBlock, 0, s>>>(a, static_cast<const B*>(x), static_cast<B*>(sorted),
-                                                           nullptr, nullptr);
+    const auto* in = static_cast<const B*>(in_);
+    auto* to = static_cast<B*>(to_);
+    const auto* other = static_cast<const B*>(other_);
+    const bool dot = d_weights != nullptr;
+    const RowPlan p = row_plan(a, sizeof(B), dot);
+    const int64_t items = a.T * p.parts;
+    const unsigned grid = match_grid(p.waves == 1 ? (items + 3) / 4 : items);
+    if (SPREAD) {
+        if (p.waves == 1) TP_ROWS_BY_K(k_spread_rows, 1);
+        else if (p.waves == 4) TP_ROWS_BY_K(k_spread_rows, 4);
+        else TP_ROWS_BY_K(k_spread_rows, 16);
+    } else {
+        if (p.waves == 1) TP_ROWS_BY_K(k_gather_rows, 1);
+        else if (p.waves == 4) TP_ROWS_BY_K(k_gather_rows, 4);
+        else TP_ROWS_BY_K(k_gather_rows, 16);
+    }
     return hipGetLastError();
 }
-
-template <class S>
-hipError_t gather(const RouteArgs& a, const void* rows, void* out, const void* x, float* d_weights, hipStream_t s) {
-    using B = typename S::Bits;
-    const dim3 grid(match_grid(a.T));
-    if (d_weights)
-        k_gather_rows<S, true><<<grid, kRowBlock, 0, s>>>(a, static_cast<const B*>(rows), static_cast<B*>(out),
-                                                          static_cast<const B*>(x), d_weights);
-    else
-        k_gather_rows<S, false><<<grid, kRowBlock, 0, s>>>(a, static_cast<const B*>(rows), static_cast<B*>(out),
-                                                           nullptr, nullptr);
-    return hipGetLastError();
-}
+#undef TP_ROWS
+#undef TP_ROWS_BY_K
 
 }  // namespace
 
-int64_t sort_by_class_work(int64_t, int64_t) { return 0; }
+int64_t sort_by_class_work(int64_t slots, int64_t classes) {
+    const SortPlan p = sort_plan(slots, int(classes));
+    return p.stretches > 1 ? (int64_t(p.stretches) + 1) * (classes + 1) * int64_t(sizeof(int)) : 0;
+}
 
 hipError_t launch_sort_by_class(int id_bytes, const void* ids, int64_t slots, int E, int* order, int* slot,
-                                int* offsets, void*, hipStream_t s) {
-    const size_t lds = size_t(kSortWaves + 1) * (E + 1) * sizeof(int);
-    const void* f = id_bytes == 4 ? reinterpret_cast<const void*>(&k_sort_one<int32_t>)
-                                  : reinterpret_cast<const void*>(&k_sort_one<int64_t>);
-    if (lds > 65536)
-        if (hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds))) return e;
-    if (id_bytes == 4)
-        k_sort_one<int32_t><<<1, 64 * kSortWaves, lds, s>>>(static_cast<const int32_t*>(ids), int(slots), E, order,
-                                                            slot, offsets);
-    else
-        k_sort_one<int64_t><<<1, 64 * kSortWaves, lds, s>>>(static_cast<const int64_t*>(ids), int(slots), E, order,
-                                                            slot, offsets);
-    return hipGetLastError();
+                                int* offsets, void* work, hipStream_t s) {
+    auto* counts = static_cast<int*>(work);
+    return id_bytes == 4 ? sort(static_cast<const int32_t*>(ids), slots, E, order, slot, offsets, counts, s)
+                         : sort(static_cast<const int64_t*>(ids), slots, E, order, slot, offsets, counts, s);
 }
 
 hipError_t launch_spread_rows(const RouteArgs& a, const void* x, void* sorted, const void* rows, float* d_weights,
                               hipStream_t s) {
     switch (a.dt) {
-        case TP_F32: return spread<F32>(a, x, sorted, rows, d_weights, s);
-        case TP_F16: return spread<F16>(a, x, sorted, rows, d_weights, s);
-        default: return spread<BF16>(a, x, sorted, rows, d_weights, s);
+        case TP_F32: return move_rows<F32, true>(a, x, sorted, rows, d_weights, s);
+        case TP_F16: return move_rows<F16, true>(a, x, sorted, rows, d_weights, s);
+        default: return move_rows<BF16, true>(a, x, sorted, rows, d_weights, s);
     }
 }
 
 hipError_t launch_gather_rows(const RouteArgs& a, const void* rows, void* out, const void* x, float* d_weights,
                               hipStream_t s) {
     switch (a.dt) {
-        case TP_F32: return gather<F32>(a, rows, out, x, d_weights, s);
-        case TP_F16: return gather<F16>(a, rows, out, x, d_weights, s);
-        default: return gather<BF16>(a, rows, out, x, d_weights, s);
+        case TP_F32: return move_rows<F32, false>(a, rows, out, x, d_weights, s);
+        case TP_F16: return move_rows<F16, false>(a, rows, out, x, d_weights, s);
+        default: return move_rows<BF16, false>(a, rows, out, x, d_weights, s);
     }
 }
 
