@@ -4,6 +4,7 @@
 // namespace that torch_projectors.cpp defines; each checks its arguments,
 // allocates its outputs and workspace from PyTorch's allocator, and calls the
 // C ABI on PyTorch's current stream.
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
@@ -39,9 +40,19 @@ void same_device(const Tensor& t, const c10::Device& dev) {
     TORCH_CHECK(t.device() == dev, "all tensors must be on the same GPU (", dev, "), got one on ", t.device());
 }
 
-Tensor workspace(int64_t bytes, const c10::Device& dev) {
-    return bytes ? at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev)) : Tensor();
+// An output or a workspace, straight from the GPU's allocator (at::empty's way there through the dispatcher
+// costs as much again, and a small call is as long as its host side).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const c10::Device& dev) {
+    return Tensor(at::detail::empty_cuda(sizes, dtype, dev, c10::nullopt));
 }
+Tensor workspace(int64_t bytes, const c10::Device& dev) { return bytes ? fresh({bytes}, at::kByte, dev) : Tensor(); }
+
+// The op's device, and no autograd inside it.
+struct Scope {
+    c10::hip::HIPGuardMasqueradingAsCUDA guard;
+    at::AutoDispatchBelowADInplaceOrView no_autograd;
+    explicit Scope(const c10::Device& dev) : guard(dev) {}
+};
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // ------------------------------------------------------------------ 8-bit blocks
@@ -50,12 +61,12 @@ std::tuple<Tensor, Tensor> quantize_blocks(const Tensor& x) {
     TORCH_CHECK(x.size(1) >= 1, "quantize_blocks: rows must hold at least one value");
     const int dt = dtype_code(x, "quantize_blocks: x");
     const auto dev = x.device();
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Scope scope(dev);
     // rows may lie any distance apart; the values of one have to be adjacent
     const Tensor v = (x.size(1) == 1 || x.stride(1) == 1) && x.stride(0) >= 0 ? x : x.contiguous();
     const int64_t R = v.size(0), nb = (v.size(1) + kBlock - 1) / kBlock;
-    Tensor codes = at::empty({R, nb * kBlock}, x.options().dtype(at::kFloat8_e4m3fn));
-    Tensor scales = at::empty({nb, tp_scale_rows(R)}, x.options().dtype(at::kByte));
+    Tensor codes = fresh({R, nb * kBlock}, at::kFloat8_e4m3fn, dev);
+    Tensor scales = fresh({nb, tp_scale_rows(R)}, at::kByte, dev);
     check_rc(tp_quantize_blocks(dt, v.data_ptr(), R, v.size(1), v.stride(0), codes.data_ptr(), scales.data_ptr(),
                                 current_stream(dev)));
     return {codes, scales};
@@ -98,9 +109,9 @@ Tensor block_scores(const Tensor& images, const optional<Tensor>& image_scales, 
         same_device(*bias, dev);
         f = bias->contiguous();
     }
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Scope scope(dev);
     const Tensor b = codes.contiguous(), sb = scales.contiguous();
-    Tensor out = at::empty({M, N}, codes.options().dtype(out_dtype));
+    Tensor out = fresh({M, N}, out_dtype, dev);
     const int64_t bytes = tp_block_scores_work(M, N, nb);
     const Tensor work = workspace(bytes, dev);
     check_rc(tp_block_scores(a.data_ptr(), sa.data_ptr(), M, b.data_ptr(), sb.data_ptr(), N, nb, ptr(f),
@@ -126,19 +137,21 @@ Probs probs(const Tensor& scores, const optional<Tensor>& given, const optional<
     p.scores = p.V == 1 || scores.stride(1) == 1 ? scores : scores.contiguous();
     p.stride = p.scores.stride(0);
     if (given.has_value()) {
-        TORCH_CHECK(given->scalar_type() == at::kLong && given->dim() == 2 && given->size(0) == p.T,
+        TORCH_CHECK(given->scalar_type() == at::kLong && (given->dim() == 1 || given->dim() == 2) &&
+                        given->size(0) == p.T,
                     "log_probs: given must be int64 with the scores' leading dimensions");
         same_device(*given, dev);
         p.given = given->contiguous();
-        p.G = given->size(1);
+        p.G = given->dim() == 1 ? 1 : given->size(1);
     }
     if (mask.has_value()) {
-        TORCH_CHECK(mask->scalar_type() == at::kBool && mask->dim() == 2 && mask->size(1) == p.V &&
-                        (mask->size(0) == p.T || mask->size(0) == 1),
+        const int64_t d = mask->dim();
+        TORCH_CHECK(mask->scalar_type() == at::kBool && (d == 1 || d == 2) && mask->size(d - 1) == p.V &&
+                        (d == 1 || mask->size(0) == p.T),
                     "log_probs: mask must be bool (candidates) or of the scores' shape");
         same_device(*mask, dev);
-        p.mask = p.V == 1 || mask->stride(1) == 1 ? *mask : mask->contiguous();
-        p.mask_stride = mask->size(0) == 1 ? 0 : p.mask.stride(0);
+        p.mask = p.V == 1 || mask->stride(d - 1) == 1 ? *mask : mask->contiguous();
+        p.mask_stride = d == 1 ? 0 : p.mask.stride(0);
     }
     return p;
 }
@@ -149,15 +162,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs(const Tenso
     const Probs p = probs(scores, given, mask);
     TORCH_CHECK(top >= 0 && top <= 64, "log_probs: top must be in [0, 64]");
     const auto dev = scores.device();
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
-    const auto f32 = scores.options().dtype(at::kFloat);
-    Tensor given_out = at::empty({p.T, p.G}, f32), entropy = at::empty({p.T}, f32), log_sum = at::empty({p.T}, f32);
-    Tensor top_out = at::empty({p.T, top}, f32), top_index = at::empty({p.T, top}, f32.dtype(at::kLong));
-    Tensor stats = at::empty({p.T, 4}, f32);
+    const Scope scope(dev);
+    Tensor given_out = given.has_value() ? fresh(given->sizes(), at::kFloat, dev) : Tensor();
+    Tensor entropy = fresh({p.T}, at::kFloat, dev), log_sum = fresh({p.T}, at::kFloat, dev);
+    Tensor top_out = fresh({p.T, top}, at::kFloat, dev), top_index = fresh({p.T, top}, at::kLong, dev);
+    Tensor stats = fresh({p.T, 4}, at::kFloat, dev);
     const int64_t bytes = tp_log_probs_work(p.T, p.V, top);
     const Tensor work = workspace(bytes, dev);
     check_rc(tp_log_probs(p.dt, p.scores.data_ptr(), p.T, p.V, p.stride, ptr(p.given), p.G, ptr(p.mask),
-                          p.mask_stride, top, temperature, given_out.data_ptr(), entropy.data_ptr(),
+                          p.mask_stride, top, temperature, ptr(given_out), entropy.data_ptr(),
                           log_sum.data_ptr(), top_out.data_ptr(), top_index.data_ptr(), stats.data_ptr(), ptr(work),
                           bytes, current_stream(dev)));
     return {given_out, entropy, log_sum, top_out, top_index, stats};
@@ -185,9 +198,9 @@ Tensor log_probs_back(const Tensor& scores, const optional<Tensor>& given, const
     const Tensor dl = upstream(d_log_sum, p.T, "d_log_sum"), dt = upstream(d_top, p.T * top, "d_top");
     same_device(top_index, dev);
     same_device(stats, dev);
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Scope scope(dev);
     const Tensor index = top_index.contiguous(), st = stats.contiguous();
-    Tensor out = at::empty({p.T, p.V}, scores.options());
+    Tensor out = fresh({p.T, p.V}, scores.scalar_type(), dev);
     check_rc(tp_log_probs_back(p.dt, p.scores.data_ptr(), p.T, p.V, p.stride, ptr(p.given), p.G, ptr(p.mask),
                                p.mask_stride, top, temperature, index.data_ptr(), st.data_ptr(),
                                p.G ? ptr(dg) : nullptr, ptr(dh), ptr(dl), top ? ptr(dt) : nullptr, out.data_ptr(),
@@ -197,16 +210,16 @@ Tensor log_probs_back(const Tensor& scores, const optional<Tensor>& given, const
 
 // ------------------------------------------------------------------ rows by class
 std::tuple<Tensor, Tensor, Tensor> sort_by_class(const Tensor& classes, int64_t num_classes) {
-    TORCH_CHECK(classes.dim() == 2, "sort_by_class: classes must be (rows, choices)");
+    TORCH_CHECK(classes.dim() == 1 || classes.dim() == 2, "sort_by_class: classes must be (rows) or (rows, choices)");
     TORCH_CHECK(classes.scalar_type() == at::kLong || classes.scalar_type() == at::kInt,
                 "sort_by_class: classes must be int64 or int32, got ", classes.scalar_type());
     TORCH_CHECK(num_classes >= 1 && num_classes <= 4096, "sort_by_class: num_classes must be in [1, 4096]");
     const auto dev = classes.device();
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Scope scope(dev);
     const Tensor ids = classes.contiguous();
-    const auto i32 = classes.options().dtype(at::kInt);
     const int64_t n = ids.numel();
-    Tensor order = at::empty({n}, i32), slot = at::empty(ids.sizes(), i32), offsets = at::empty({num_classes + 1}, i32);
+    Tensor order = fresh({n}, at::kInt, dev), slot = fresh({ids.size(0), ids.dim() == 1 ? 1 : ids.size(1)}, at::kInt, dev);
+    Tensor offsets = fresh({num_classes + 1}, at::kInt, dev);
     const int64_t bytes = tp_sort_by_class_work(n, num_classes);
     const Tensor work = workspace(bytes, dev);
     check_rc(tp_sort_by_class(int(ids.element_size()), ids.data_ptr(), n, num_classes, order.data_ptr(),
@@ -240,48 +253,48 @@ int64_t row_size(const Tensor& t, int64_t n, const char* what) {
     return t.size(1);
 }
 
-// x [T, D] -> sorted [T k, D]; with other [T k, D] also the weights' gradient <x[t], other[slot]>
+// x [T, D] -> sorted [T k, D]; with other [T k, D] also the weights' gradient <x[t], other[slot]> (else None)
 std::tuple<Tensor, Tensor> spread_rows(const Tensor& x, const Tensor& slot, const Tensor& offsets,
                                        const optional<Tensor>& weights, const optional<Tensor>& other) {
     const auto dev = x.device();
     const Route r = route(slot, offsets, weights, dev);
     const int64_t D = row_size(x, r.T, "rows");
     const int dt = dtype_code(x, "rows");
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Scope scope(dev);
     const Tensor v = x.contiguous();
-    Tensor sorted = at::empty({r.T * r.k, D}, x.options()), o, dw;
+    Tensor sorted = fresh({r.T * r.k, D}, x.scalar_type(), dev), o, dw;
     if (other.has_value()) {
         TORCH_CHECK(other->scalar_type() == x.scalar_type(), "both sides' rows must have the same dtype");
         TORCH_CHECK(row_size(*other, r.T * r.k, "sorted rows") == D, "both sides' rows must have the same size");
         same_device(*other, dev);
         o = other->contiguous();
-        dw = at::empty(slot.sizes(), x.options().dtype(at::kFloat));
+        dw = fresh(slot.sizes(), at::kFloat, dev);
     }
     check_rc(tp_spread_rows(dt, v.data_ptr(), r.T, D, r.k, r.slot.data_ptr(), r.kept(), ptr(r.weights),
                             sorted.data_ptr(), ptr(o), ptr(dw), current_stream(dev)));
-    return {sorted, dw.defined() ? dw : at::empty({0}, x.options().dtype(at::kFloat))};
+    return {sorted, dw};
 }
 
-// sorted [T k, D] -> out [T, D]; with other [T, D] also the weights' gradient <other[t], sorted[slot]>
+// sorted [T k, D] -> out [T, D]; with other [T, D] also the weights' gradient <other[t], sorted[slot]> (else None)
 std::tuple<Tensor, Tensor> gather_rows(const Tensor& sorted, const Tensor& slot, const Tensor& offsets,
                                        const optional<Tensor>& weights, const optional<Tensor>& other) {
     const auto dev = sorted.device();
     const Route r = route(slot, offsets, weights, dev);
     const int64_t D = row_size(sorted, r.T * r.k, "sorted rows");
     const int dt = dtype_code(sorted, "sorted rows");
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+    const Scope scope(dev);
     const Tensor v = sorted.contiguous();
-    Tensor out = at::empty({r.T, D}, sorted.options()), o, dw;
+    Tensor out = fresh({r.T, D}, sorted.scalar_type(), dev), o, dw;
     if (other.has_value()) {
         TORCH_CHECK(other->scalar_type() == sorted.scalar_type(), "both sides' rows must have the same dtype");
         TORCH_CHECK(row_size(*other, r.T, "rows") == D, "both sides' rows must have the same size");
         same_device(*other, dev);
         o = other->contiguous();
-        dw = at::empty(slot.sizes(), sorted.options().dtype(at::kFloat));
+        dw = fresh(slot.sizes(), at::kFloat, dev);
     }
     check_rc(tp_gather_rows(dt, v.data_ptr(), r.T, D, r.k, r.slot.data_ptr(), r.kept(), ptr(r.weights),
                             out.data_ptr(), ptr(o), ptr(dw), current_stream(dev)));
-    return {out, dw.defined() ? dw : at::empty({0}, sorted.options().dtype(at::kFloat))};
+    return {out, dw};
 }
 
 }  // namespace
@@ -304,4 +317,12 @@ TORCH_LIBRARY_IMPL(torch_projectors, CUDA, m) {
     m.impl("sort_by_class", &sort_by_class);
     m.impl("spread_rows", &spread_rows);
     m.impl("gather_rows", &gather_rows);
+}
+
+// The autograd Functions of matching.py call these ops with gradients off; without a registration of its own the
+// Autograd key would go through PyTorch's checks of every argument first (2 us of a call's 7).
+TORCH_LIBRARY_IMPL(torch_projectors, Autograd, m) {
+    for (const char* name : {"quantize_blocks", "block_scores", "log_probs", "log_probs_back", "sort_by_class",
+                             "spread_rows", "gather_rows"})
+        m.impl(name, torch::CppFunction::makeFallthrough());
 }

@@ -44,9 +44,9 @@ def _real_rows(x, what):
         raise ValueError(f"{what} must have at least 1 dimension")
     if x.is_complex():
         x = torch.view_as_real(x.resolve_conj())
-    if x.is_neg():
+    elif x.is_neg():
         x = x.resolve_neg()
-    return x if x.dim() == 2 else x.reshape(x.shape[0], x[0].numel() if x.shape[0] else _numel(x.shape[1:]))
+    return x if x.dim() == 2 else x.reshape(x.shape[0], _numel(x.shape[1:]))
 
 
 def _numel(shape):
@@ -62,7 +62,7 @@ def quantize_blocks(x: torch.Tensor) -> BlockScaled:
     A block's scale is the least power of two that keeps its largest finite magnitude within 448 times
     it; the codes are rounded to nearest even.  Values that are not finite become NaN.  Not
     differentiable."""
-    return BlockScaled(*_OPS.quantize_blocks(_real_rows(x.detach(), "x")))
+    return BlockScaled(*_OPS.quantize_blocks.default(_real_rows(x, "x")))
 
 
 def block_scores(images, references, bias: Optional[torch.Tensor] = None,
@@ -79,10 +79,8 @@ def block_scores(images, references, bias: Optional[torch.Tensor] = None,
     if isinstance(images, BlockScaled):
         images, image_scales = images
     else:
-        images, image_scales = _real_rows(images.detach(), "images"), None
-    if bias is not None:
-        bias = bias.detach()
-    return _OPS.block_scores(images, image_scales, references.codes, references.scales, bias, out_dtype)
+        images, image_scales = _real_rows(images, "images"), None
+    return _OPS.block_scores.default(images, image_scales, references.codes, references.scales, bias, out_dtype)
 
 
 # ----------------------------------------------------------------------------- log probabilities
@@ -105,7 +103,7 @@ class LogProbs(NamedTuple):
 class _LogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, scores, given, mask, top, temperature):
-        *out, stats = _OPS.log_probs(scores, given, mask, top, temperature)
+        *out, stats = _OPS.log_probs.default(scores, given, mask, top, temperature)
         ctx.save_for_backward(scores, given, mask, out[4], stats)
         ctx.temperature = temperature
         ctx.mark_non_differentiable(out[4])
@@ -116,7 +114,7 @@ class _LogProbs(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_given, d_entropy, d_log_sum, d_top, _):
         scores, given, mask, top_index, stats = ctx.saved_tensors
-        d_scores = _OPS.log_probs_back(scores, given, mask, top_index, stats, ctx.temperature, d_given, d_entropy,
+        d_scores = _OPS.log_probs_back.default(scores, given, mask, top_index, stats, ctx.temperature, d_given, d_entropy,
                                        d_log_sum, d_top)
         return d_scores, None, None, None, None
 
@@ -137,26 +135,26 @@ def log_probs(scores: torch.Tensor, given: Optional[torch.Tensor] = None, top: i
     if scores.dim() < 1:
         raise ValueError("Scores must have at least 1 dimension (..., candidates)")
     lead, V = scores.shape[:-1], scores.shape[-1]
-    rows = scores if scores.dim() == 2 else scores.reshape(_numel(lead), V)
-    if given is not None:
-        if given.shape[:len(lead)] != lead or given.dim() > len(lead) + 1:
-            raise ValueError(f"Given candidates {tuple(given.shape)} must have the scores' leading dimensions "
-                             f"{tuple(lead)} and at most one more")
-        shape = given.shape
-        given = given.reshape(rows.shape[0], 1 if given.dim() == len(lead) else shape[-1])
-    if mask is not None:
-        if mask.shape != scores.shape and mask.shape != (V,):
-            raise ValueError(f"Mask {tuple(mask.shape)} must have the scores' shape {tuple(scores.shape)} or be ({V},)")
-        mask = mask.unsqueeze(0) if mask.dim() == 1 else mask.reshape(rows.shape[0], V)
-    if torch.is_grad_enabled() and scores.requires_grad:
-        out = _LogProbs.apply(rows, given, mask, top, temperature)
-    else:
-        out = _OPS.log_probs(rows, given, mask, top, temperature)
-    g, entropy, log_sum, best, index = out[:5]
-    g = None if given is None else g.view(shape)
+    if given is not None and (given.shape[:len(lead)] != lead or given.dim() > len(lead) + 1):
+        raise ValueError(f"Given candidates {tuple(given.shape)} must have the scores' leading dimensions "
+                         f"{tuple(lead)} and at most one more")
+    if mask is not None and mask.shape != scores.shape and mask.shape != (V,):
+        raise ValueError(f"Mask {tuple(mask.shape)} must have the scores' shape {tuple(scores.shape)} or be ({V},)")
     if len(lead) == 1:
-        return LogProbs(g, entropy, log_sum, best, index)
-    return LogProbs(g, entropy.view(lead), log_sum.view(lead), best.view(*lead, top), index.view(*lead, top))
+        return LogProbs(*_log_probs(scores, given, mask, top, temperature))
+    T = _numel(lead)
+    flat = given if given is None else given.reshape(T) if given.dim() == len(lead) else given.reshape(T, given.shape[-1])
+    g, entropy, log_sum, best, index = _log_probs(scores.reshape(T, V), flat,
+                                                  mask if mask is None or mask.dim() == 1 and len(lead) else
+                                                  mask.reshape(T, V), top, temperature)
+    return LogProbs(None if g is None else g.view(given.shape), entropy.view(lead), log_sum.view(lead),
+                    best.view(*lead, top), index.view(*lead, top))
+
+
+def _log_probs(rows, given, mask, top, temperature):
+    if rows.requires_grad and torch.is_grad_enabled():
+        return _LogProbs.apply(rows, given, mask, top, temperature)
+    return _OPS.log_probs.default(rows, given, mask, top, temperature)[:5]
 
 
 # ----------------------------------------------------------------------------- rows by class
@@ -178,20 +176,20 @@ def sort_by_class(classes: torch.Tensor, num_classes: int) -> ClassOrder:
     class's slots.  Choices outside [0, num_classes), num_classes at most 4096, are dropped."""
     if classes.dim() not in (1, 2):
         raise ValueError("Classes must be (rows) or (rows, choices)")
-    return ClassOrder(*_OPS.sort_by_class(classes if classes.dim() == 2 else classes.unsqueeze(1), num_classes))
+    return ClassOrder(*_OPS.sort_by_class.default(classes, num_classes))
 
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, slot, offsets, weights):
         ctx.save_for_backward(x if weights is not None and weights.requires_grad else None, slot, offsets, weights)
-        return _OPS.spread_rows(x, slot, offsets, weights, None)[0]
+        return _OPS.spread_rows.default(x, slot, offsets, weights, None)[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_sorted):
         x, slot, offsets, weights = ctx.saved_tensors
-        d_x, d_weights = _OPS.gather_rows(d_sorted, slot, offsets, weights, x)
+        d_x, d_weights = _OPS.gather_rows.default(d_sorted, slot, offsets, weights, x)
         return d_x, None, None, (None if x is None else d_weights)
 
 
@@ -199,46 +197,44 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, slot, offsets, weights):
         ctx.save_for_backward(y if weights is not None and weights.requires_grad else None, slot, offsets, weights)
-        return _OPS.gather_rows(y, slot, offsets, weights, None)[0]
+        return _OPS.gather_rows.default(y, slot, offsets, weights, None)[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_sum):
         y, slot, offsets, weights = ctx.saved_tensors
-        d_y, d_weights = _OPS.spread_rows(d_sum, slot, offsets, weights, y)
+        d_y, d_weights = _OPS.spread_rows.default(d_sum, slot, offsets, weights, y)
         return d_y, None, None, (None if y is None else d_weights)
 
 
 def _move(function, op, x, n, order, weights, what):
+    slot, offsets = order.slot, order.offsets
     if x.dim() < 1 or x.shape[0] != n:
         raise ValueError(f"{what} must have {n} rows, got shape {tuple(x.shape)}")
-    if weights is not None:
-        if weights.shape != order.slot.shape and weights.shape != order.slot.shape[:1]:
-            raise ValueError(f"Weights {tuple(weights.shape)} must have the classes' shape {tuple(order.slot.shape)}")
-        if weights.dim() == 1:
-            if order.slot.shape[1] != 1:
-                raise ValueError(f"Weights {tuple(weights.shape)} must have the classes' shape "
-                                 f"{tuple(order.slot.shape)}")
-            weights = weights.unsqueeze(1)
-    shape, is_complex = x.shape, x.is_complex()
+    if weights is not None and weights.shape != slot.shape:
+        if weights.dim() != 1 or (weights.shape[0], 1) != slot.shape:
+            raise ValueError(f"Weights {tuple(weights.shape)} must have the classes' shape {tuple(slot.shape)}")
+        weights = weights.unsqueeze(1)
     rows = _real_rows(x, what)
     if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
-        out = function.apply(rows, order.slot, order.offsets, weights)
+        out = function.apply(rows, slot, offsets, weights)
     else:
-        out = op(rows, order.slot, order.offsets, weights, None)[0]
-    if is_complex:
-        return torch.view_as_complex(out.view(out.shape[0], *shape[1:], 2))
-    return out if len(shape) == 2 else out.view(out.shape[0], *shape[1:])
+        out = op(rows, slot, offsets, weights, None)[0]
+    if rows is x:
+        return out
+    if x.is_complex():
+        return torch.view_as_complex(out.view(out.shape[0], *x.shape[1:], 2))
+    return out.view(out.shape[0], *x.shape[1:])
 
 
 def dispatch(x: torch.Tensor, order: ClassOrder, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rows x [T, ...] (float32, float16, bfloat16 or complex64) in class order: [T k, ...], row t at
     each of its places slot[t, j], times weights[t, j] (float32 [T, k]) where given; zero rows where
     dropped.  Differentiable in x and weights."""
-    return _move(_Dispatch, _OPS.spread_rows, x, order.slot.shape[0], order, weights, "x")
+    return _move(_Dispatch, _OPS.spread_rows.default, x, order.slot.shape[0], order, weights, "x")
 
 
 def combine(y: torch.Tensor, order: ClassOrder, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rows y [T k, ...] in class order back to [T, ...]: sum_j weights[t, j] y[slot[t, j]] in float32,
     rounded once, without the dropped ones.  Differentiable in y and weights."""
-    return _move(_Combine, _OPS.gather_rows, y, order.order.shape[0], order, weights, "y")
+    return _move(_Combine, _OPS.gather_rows.default, y, order.order.shape[0], order, weights, "y")
