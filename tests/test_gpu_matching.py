@@ -488,6 +488,26 @@ def test_rows_gradient_against_differences(m, which):
         assert abs(slope - (value(*plus) - value(*minus)) / (2 * h)) <= 1e-6 * size / h
 
 
+def test_gradients_once(m):
+    """A graph of the gradients is refused where it is used, not before; what needs no gradient gets none."""
+    x = torch.randn(3, 20, device=DEV, requires_grad=True)
+    (d,) = torch.autograd.grad(m.log_probs(x).log_sum.sum(), x, create_graph=True)
+    assert torch.isfinite(d).all()
+    with pytest.raises(RuntimeError, match="once"):
+        d.square().sum().backward()
+    order = m.sort_by_class(torch.tensor([[0, 1], [1, 1], [0, 0]], device=DEV), 2)
+    w = torch.rand(3, 2, device=DEV, requires_grad=True)
+    (d,) = torch.autograd.grad(m.dispatch(x, order, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        d.sum().backward()
+    (dw,) = torch.autograd.grad(m.combine(torch.ones(6, 5, device=DEV), order, w).sum(), w)
+    assert torch.equal(dw, torch.full((3, 2), 5.0, device=DEV))
+    with torch.no_grad():
+        assert not m.log_probs(x, top=2).top.requires_grad and not m.dispatch(x, order, w).requires_grad
+    out = m.log_probs(x, top=2)
+    assert out.top.requires_grad and not out.top_index.requires_grad and out.given is None
+
+
 # ----------------------------------------------------------------------------- streams and graphs
 def _all(m, s):
     scores = m.block_scores(s["x"], m.BlockScaled(s["codes"], s["scales"]), bias=s["bias"])

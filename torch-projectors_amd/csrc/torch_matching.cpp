@@ -7,6 +7,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 #include <torch/torch.h>
 
@@ -297,6 +298,87 @@ std::tuple<Tensor, Tensor> gather_rows(const Tensor& sorted, const Tensor& slot,
     return {out, dw};
 }
 
+// ------------------------------------------------------------------ gradients
+// Autograd in C++: a backward in Python would have the engine's thread wait for the interpreter (30 us a step).
+
+// The gradients are computed without a graph of their own: asking for one fails where it is used.
+torch::autograd::variable_list once(torch::autograd::variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    auto refuse = std::make_shared<torch::autograd::DelayedError>(
+        "torch_projectors: the matching operators are differentiable once", int64_t(grads.size()));
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().requires_grad_();
+    return (*refuse)(std::move(grads));
+}
+optional<Tensor> given_or_none(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
+bool wants(const Tensor& t) { return t.requires_grad(); }
+bool wants(const optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct LogProbsGrad : torch::autograd::Function<LogProbsGrad> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& scores, const optional<Tensor>& given,
+                                 const optional<Tensor>& mask, int64_t top, double temperature) {
+        auto [g, entropy, log_sum, best, index, stats] = log_probs(scores, given, mask, top, temperature);
+        ctx->save_for_backward({scores, given.value_or(Tensor()), mask.value_or(Tensor()), index, stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->mark_non_differentiable({index, stats});
+        ctx->set_materialize_grads(false);
+        if (!g.defined()) return {entropy, log_sum, best, index, stats};
+        return {entropy, log_sum, best, index, stats, g};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list d) {
+        const auto v = ctx->get_saved_variables();
+        Tensor out;
+        {
+            at::AutoGradMode off(false);
+            auto up = [&](size_t i) { return i < d.size() ? given_or_none(d[i]) : c10::nullopt; };
+            out = log_probs_back(v[0], given_or_none(v[1]), given_or_none(v[2]), v[3], v[4],
+                                 ctx->saved_data["temperature"].toDouble(), up(5), up(0), up(1), up(2));
+        }
+        return once({out, Tensor(), Tensor(), Tensor(), Tensor()});
+    }
+};
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs_grad(const Tensor& scores,
+                                                                          const optional<Tensor>& given,
+                                                                          const optional<Tensor>& mask, int64_t top,
+                                                                          double temperature) {
+    if (!at::GradMode::is_enabled() || !wants(scores)) return log_probs(scores, given, mask, top, temperature);
+    auto r = LogProbsGrad::apply(scores, given, mask, top, temperature);
+    return {r.size() > 5 ? r[5] : Tensor(), r[0], r[1], r[2], r[3], r[4]};
+}
+
+// SPREAD: rows to their places; else back.  Each one's backward is the other.
+template <bool SPREAD> struct RowsGrad : torch::autograd::Function<RowsGrad<SPREAD>> {
+    static std::tuple<Tensor, Tensor> move(bool spread, const Tensor& x, const Tensor& slot, const Tensor& offsets,
+                                           const optional<Tensor>& weights, const optional<Tensor>& other) {
+        return spread ? spread_rows(x, slot, offsets, weights, other) : gather_rows(x, slot, offsets, weights, other);
+    }
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& slot, const Tensor& offsets,
+                          const optional<Tensor>& weights) {
+        ctx->save_for_backward({wants(weights) ? x : Tensor(), slot, offsets, weights.value_or(Tensor())});
+        return std::get<0>(move(SPREAD, x, slot, offsets, weights, c10::nullopt));
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list d) {
+        const auto v = ctx->get_saved_variables();
+        Tensor dx, dw;
+        if (d[0].defined()) {
+            at::AutoGradMode off(false);
+            std::tie(dx, dw) = move(!SPREAD, d[0], v[1], v[2], given_or_none(v[3]), given_or_none(v[0]));
+        }
+        return once({dx, Tensor(), Tensor(), dw});
+    }
+};
+template <bool SPREAD>
+std::tuple<Tensor, Tensor> rows_grad(const Tensor& x, const Tensor& slot, const Tensor& offsets,
+                                     const optional<Tensor>& weights, const optional<Tensor>& other) {
+    using F = RowsGrad<SPREAD>;
+    if (!at::GradMode::is_enabled() || other.has_value() || !(wants(x) || wants(weights)))
+        return F::move(SPREAD, x, slot, offsets, weights, other);
+    return {F::apply(x, slot, offsets, weights), Tensor()};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(torch_projectors, m) {
@@ -319,10 +401,11 @@ TORCH_LIBRARY_IMPL(torch_projectors, CUDA, m) {
     m.impl("gather_rows", &gather_rows);
 }
 
-// The autograd Functions of matching.py call these ops with gradients off; without a registration of its own the
-// Autograd key would go through PyTorch's checks of every argument first (2 us of a call's 7).
-TORCH_LIBRARY_IMPL(torch_projectors, Autograd, m) {
-    for (const char* name : {"quantize_blocks", "block_scores", "log_probs", "log_probs_back", "sort_by_class",
-                             "spread_rows", "gather_rows"})
+// What is differentiable takes its gradient from above; the others are called as they are.
+TORCH_LIBRARY_IMPL(torch_projectors, AutogradCUDA, m) {
+    m.impl("log_probs", &log_probs_grad);
+    m.impl("spread_rows", &rows_grad<true>);
+    m.impl("gather_rows", &rows_grad<false>);
+    for (const char* name : {"quantize_blocks", "block_scores", "log_probs_back", "sort_by_class"})
         m.impl(name, torch::CppFunction::makeFallthrough());
 }

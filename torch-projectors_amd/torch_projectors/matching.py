@@ -16,7 +16,7 @@ with its weights.  In training, `log_probs` of `images @ projections.T` carries 
 likelihood (`log_sum`) back to volumes and poses.
 
 All run on the GPU only (a CPU tensor raises NotImplementedError), on the current stream, without a
-synchronisation; they can be captured in a graph.
+synchronisation; they can be captured in a graph.  What is differentiable is so once.
 """
 from typing import NamedTuple, Optional
 
@@ -100,25 +100,6 @@ class LogProbs(NamedTuple):
     top_index: torch.Tensor
 
 
-class _LogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, scores, given, mask, top, temperature):
-        *out, stats = _OPS.log_probs.default(scores, given, mask, top, temperature)
-        ctx.save_for_backward(scores, given, mask, out[4], stats)
-        ctx.temperature = temperature
-        ctx.mark_non_differentiable(out[4])
-        ctx.set_materialize_grads(False)
-        return tuple(out)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_given, d_entropy, d_log_sum, d_top, _):
-        scores, given, mask, top_index, stats = ctx.saved_tensors
-        d_scores = _OPS.log_probs_back.default(scores, given, mask, top_index, stats, ctx.temperature, d_given, d_entropy,
-                                       d_log_sum, d_top)
-        return d_scores, None, None, None, None
-
-
 def log_probs(scores: torch.Tensor, given: Optional[torch.Tensor] = None, top: int = 0, temperature: float = 1.0,
               mask: Optional[torch.Tensor] = None) -> LogProbs:
     """Log probabilities of the softmax of scores [..., V] / temperature (float32, float16 or bfloat16).
@@ -141,20 +122,14 @@ def log_probs(scores: torch.Tensor, given: Optional[torch.Tensor] = None, top: i
     if mask is not None and mask.shape != scores.shape and mask.shape != (V,):
         raise ValueError(f"Mask {tuple(mask.shape)} must have the scores' shape {tuple(scores.shape)} or be ({V},)")
     if len(lead) == 1:
-        return LogProbs(*_log_probs(scores, given, mask, top, temperature))
+        return LogProbs(*_OPS.log_probs.default(scores, given, mask, top, temperature)[:5])
     T = _numel(lead)
     flat = given if given is None else given.reshape(T) if given.dim() == len(lead) else given.reshape(T, given.shape[-1])
-    g, entropy, log_sum, best, index = _log_probs(scores.reshape(T, V), flat,
-                                                  mask if mask is None or mask.dim() == 1 and len(lead) else
-                                                  mask.reshape(T, V), top, temperature)
+    if mask is not None and mask.shape == scores.shape:
+        mask = mask.reshape(T, V)
+    g, entropy, log_sum, best, index, _ = _OPS.log_probs.default(scores.reshape(T, V), flat, mask, top, temperature)
     return LogProbs(None if g is None else g.view(given.shape), entropy.view(lead), log_sum.view(lead),
                     best.view(*lead, top), index.view(*lead, top))
-
-
-def _log_probs(rows, given, mask, top, temperature):
-    if rows.requires_grad and torch.is_grad_enabled():
-        return _LogProbs.apply(rows, given, mask, top, temperature)
-    return _OPS.log_probs.default(rows, given, mask, top, temperature)[:5]
 
 
 # ----------------------------------------------------------------------------- rows by class
@@ -179,35 +154,7 @@ def sort_by_class(classes: torch.Tensor, num_classes: int) -> ClassOrder:
     return ClassOrder(*_OPS.sort_by_class.default(classes, num_classes))
 
 
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, slot, offsets, weights):
-        ctx.save_for_backward(x if weights is not None and weights.requires_grad else None, slot, offsets, weights)
-        return _OPS.spread_rows.default(x, slot, offsets, weights, None)[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_sorted):
-        x, slot, offsets, weights = ctx.saved_tensors
-        d_x, d_weights = _OPS.gather_rows.default(d_sorted, slot, offsets, weights, x)
-        return d_x, None, None, (None if x is None else d_weights)
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, slot, offsets, weights):
-        ctx.save_for_backward(y if weights is not None and weights.requires_grad else None, slot, offsets, weights)
-        return _OPS.gather_rows.default(y, slot, offsets, weights, None)[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_sum):
-        y, slot, offsets, weights = ctx.saved_tensors
-        d_y, d_weights = _OPS.spread_rows.default(d_sum, slot, offsets, weights, y)
-        return d_y, None, None, (None if y is None else d_weights)
-
-
-def _move(function, op, x, n, order, weights, what):
+def _move(op, x, n, order, weights, what):
     slot, offsets = order.slot, order.offsets
     if x.dim() < 1 or x.shape[0] != n:
         raise ValueError(f"{what} must have {n} rows, got shape {tuple(x.shape)}")
@@ -216,10 +163,7 @@ def _move(function, op, x, n, order, weights, what):
             raise ValueError(f"Weights {tuple(weights.shape)} must have the classes' shape {tuple(slot.shape)}")
         weights = weights.unsqueeze(1)
     rows = _real_rows(x, what)
-    if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
-        out = function.apply(rows, slot, offsets, weights)
-    else:
-        out = op(rows, slot, offsets, weights, None)[0]
+    out = op(rows, slot, offsets, weights, None)[0]
     if rows is x:
         return out
     if x.is_complex():
@@ -231,10 +175,10 @@ def dispatch(x: torch.Tensor, order: ClassOrder, weights: Optional[torch.Tensor]
     """Rows x [T, ...] (float32, float16, bfloat16 or complex64) in class order: [T k, ...], row t at
     each of its places slot[t, j], times weights[t, j] (float32 [T, k]) where given; zero rows where
     dropped.  Differentiable in x and weights."""
-    return _move(_Dispatch, _OPS.spread_rows.default, x, order.slot.shape[0], order, weights, "x")
+    return _move(_OPS.spread_rows.default, x, order.slot.shape[0], order, weights, "x")
 
 
 def combine(y: torch.Tensor, order: ClassOrder, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rows y [T k, ...] in class order back to [T, ...]: sum_j weights[t, j] y[slot[t, j]] in float32,
     rounded once, without the dropped ones.  Differentiable in y and weights."""
-    return _move(_Combine, _OPS.gather_rows.default, y, order.order.shape[0], order, weights, "y")
+    return _move(_OPS.gather_rows.default, y, order.order.shape[0], order, weights, "y")
