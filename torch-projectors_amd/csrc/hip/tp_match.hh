@@ -114,6 +114,19 @@ template <class S> __device__ __forceinline__ Pack<S> load_pack(const typename S
 template <class S> __device__ __forceinline__ void store_pack(typename S::Bits* p, const Pack<S>& r) {
     __builtin_memcpy(p, &r, 16);
 }
+// The same for what will not be used again before the caches have lost it anyway (streaming).
+template <class S> struct PackBits {
+    using Any = uint32_t __attribute__((ext_vector_type(4)));
+    using At = uint32_t __attribute__((ext_vector_type(4), aligned(sizeof(typename S::Bits))));
+};
+template <class S> __device__ __forceinline__ Pack<S> stream_pack(const typename S::Bits* p) {
+    const typename PackBits<S>::Any w = __builtin_nontemporal_load(reinterpret_cast<const typename PackBits<S>::At*>(p));
+    return __builtin_bit_cast(Pack<S>, w);
+}
+template <class S> __device__ __forceinline__ void stream_pack(typename S::Bits* p, const Pack<S>& r) {
+    __builtin_nontemporal_store(__builtin_bit_cast(typename PackBits<S>::Any, r),
+                                reinterpret_cast<typename PackBits<S>::At*>(p));
+}
 
 // Sum over a wavefront, the same in every lane (fixed order).
 __device__ __forceinline__ float wave_sum(float v) {

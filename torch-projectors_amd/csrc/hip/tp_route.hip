@@ -83,6 +83,7 @@ __global__ __launch_bounds__(64 * kMaxSortWaves) void k_sort_place(const I* __re
                     return counts[int64_t(stretches) * C + c];
                 }
                 int earlier = 0, all = 0;
+#pragma unroll 16
                 for (int b = 0; b < stretches; ++b) {
                     const int v = counts[int64_t(b) * C + c];
                     all += v;
@@ -213,9 +214,10 @@ SortPlan sort_plan(int64_t n, int E) {
         while (waves > 1 && int64_t(waves / 2) * 64 >= n) waves /= 2;
         return {waves, 1, std::max<int64_t>(n, 1)};
     }
-    // at most 2048 stretches, of whole turns
-    const int64_t turns = (n + hold - 1) / hold, each = (turns + 2047) / 2048;
-    return {waves, int((turns + each - 1) / each), each * hold};
+    // about 32 stretches, or as many of a whole turn as there are, or 2048 of several turns
+    const int64_t group = int64_t(waves) * 64, turns = (n + hold - 1) / hold, each = (turns + 2047) / 2048;
+    const int64_t stretch = turns <= 32 ? ((n + 31) / 32 + group - 1) / group * group : each * hold;
+    return {waves, int((n + stretch - 1) / stretch), stretch};
 }
 
 template <class I>
@@ -243,15 +245,17 @@ hipError_t sort(const I* ids, int64_t n, int E, int* order, int* slot, int* offs
 // so that the row is read (spread) or written (gather) once whatever k is.  Memory bound.  Values move 16 bytes a
 // lane at a time, whatever the rows' alignment; of up to KB choices the loads are in flight together, and the
 // products for the weights' gradient stay in registers.  More than KB choices: spread goes over the row again for
-// each KB of them, gather reads KB at a time and does the products in a second look.
+// each KB of them (four at once are faster than eight: 16384 x 8 rows of 512 bfloat16 65 against 84 us with the
+// weights' gradient), gather reads KB at a time and does the products in a second look (so there KB is up to eight:
+// 48 against 69 us).
 template <class S> struct Values {
     static constexpr int n = Pack<S>::n;
     float v[n];
 };
-template <class S> __device__ __forceinline__ Values<S> load_values(const typename S::Bits* p, int64_t left) {
+template <class S> __device__ __forceinline__ Values<S> load_values(const typename S::Bits* p, int64_t left, bool stream) {
     Values<S> r;
     if (left >= Values<S>::n) {
-        const Pack<S> w = load_pack<S>(p);
+        const Pack<S> w = stream ? stream_pack<S>(p) : load_pack<S>(p);
 #pragma unroll
         for (int i = 0; i < Values<S>::n; ++i) r.v[i] = S::widen(w.v[i]);
     } else {
@@ -260,12 +264,14 @@ template <class S> __device__ __forceinline__ Values<S> load_values(const typena
     }
     return r;
 }
-template <class S> __device__ __forceinline__ void store_values(typename S::Bits* p, int64_t left, const Values<S>& r) {
+template <class S>
+__device__ __forceinline__ void store_values(typename S::Bits* p, int64_t left, const Values<S>& r, bool stream) {
     Pack<S> w;
 #pragma unroll
     for (int i = 0; i < Values<S>::n; ++i) w.v[i] = S::round(r.v[i]);
     if (left >= Values<S>::n) {
-        store_pack<S>(p, w);
+        if (stream) stream_pack<S>(p, w);
+        else store_pack<S>(p, w);
     } else {
 #pragma unroll
         for (int i = 0; i < Values<S>::n; ++i)
@@ -328,7 +334,7 @@ template <int W> __device__ __forceinline__ bool row_item(const RouteArgs& a, in
 }
 
 template <class S, int W, int KB, bool DOT>
-__global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int64_t span, int parts,
+__global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int64_t span, int parts, bool stream,
                                                                 const typename S::Bits* __restrict__ x,
                                                                 typename S::Bits* __restrict__ sorted,
                                                                 const typename S::Bits* __restrict__ rows,
@@ -344,12 +350,12 @@ __global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int
             float dot[KB] = {};
             for (int64_t d = r.d0 + lane * n; d < r.d1; d += W * 64 * n) {
                 const int64_t left = r.d1 - d;
-                const Values<S> v = load_values<S>(x + r.t * a.D + d, left);
+                const Values<S> v = load_values<S>(x + r.t * a.D + d, left, stream && a.k <= KB);
                 Values<S> o[KB];
                 if (DOT) {
 #pragma unroll
                     for (int u = 0; u < KB; ++u) {
-                        if (p.in[u]) o[u] = load_values<S>(rows + p.at[u] + d, left);
+                        if (p.in[u]) o[u] = load_values<S>(rows + p.at[u] + d, left, stream);
                         else o[u] = Values<S>{};
                     }
 #pragma unroll
@@ -363,7 +369,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int
                     if (!p.real[u]) continue;
 #pragma unroll
                     for (int i = 0; i < n; ++i) o[u].v[i] = p.in[u] ? p.w[u] * v.v[i] : 0.0f;
-                    store_values<S>(sorted + p.at[u] + d, left, o[u]);
+                    store_values<S>(sorted + p.at[u] + d, left, o[u], stream);
                 }
             }
             if (DOT) {
@@ -378,7 +384,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int
 }
 
 template <class S, int W, int KB, bool DOT>
-__global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int64_t span, int parts,
+__global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int64_t span, int parts, bool stream,
                                                                 const typename S::Bits* __restrict__ rows,
                                                                 typename S::Bits* __restrict__ out,
                                                                 const typename S::Bits* __restrict__ x,
@@ -398,10 +404,10 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
                 if (a.k > KB) p = places_of<KB>(a, r.t, j0, kept);
 #pragma unroll
                 for (int u = 0; u < KB; ++u) {
-                    if (p.in[u]) o[u] = load_values<S>(rows + p.at[u] + d, left);
+                    if (p.in[u]) o[u] = load_values<S>(rows + p.at[u] + d, left, stream);
                     else o[u] = Values<S>{};
                 }
-                if (DOT && a.k <= KB) v = load_values<S>(x + r.t * a.D + d, left);
+                if (DOT && a.k <= KB) v = load_values<S>(x + r.t * a.D + d, left, stream);
 #pragma unroll
                 for (int u = 0; u < KB; ++u)
                     if (p.in[u])
@@ -411,7 +417,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
                             if (DOT) dot[u] = __builtin_fmaf(v.v[i], o[u].v[i], dot[u]);
                         }
             }
-            store_values<S>(out + r.t * a.D + d, left, sum);
+            store_values<S>(out + r.t * a.D + d, left, sum, stream);
         }
         if (!DOT) continue;
         for (int j0 = 0; j0 < a.k; j0 += KB) {
@@ -421,11 +427,11 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
                 for (int u = 0; u < KB; ++u) dot[u] = 0.0f;
                 for (int64_t d = r.d0 + lane * n; d < r.d1; d += W * 64 * n) {
                     const int64_t left = r.d1 - d;
-                    const Values<S> v = load_values<S>(x + r.t * a.D + d, left);
+                    const Values<S> v = load_values<S>(x + r.t * a.D + d, left, stream);
 #pragma unroll
                     for (int u = 0; u < KB; ++u) {
                         if (!p.in[u]) continue;
-                        const Values<S> o = load_values<S>(rows + p.at[u] + d, left);
+                        const Values<S> o = load_values<S>(rows + p.at[u] + d, left, stream);
 #pragma unroll
                         for (int i = 0; i < n; ++i) dot[u] = __builtin_fmaf(v.v[i], o.v[i], dot[u]);
                     }
@@ -439,6 +445,11 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
         }
     }
 }
+
+// Sorted rows of at least this size, what the XCDs' L2s hold together, are streamed past the caches.  Measured on
+// 16384 x 4 rows of 4096 bfloat16 (537 MB): spread 221 us through the caches, 128 streamed; weighted gather 159
+// and 118; on 2048 x 2 rows of 4224 fp32 (69 MB) 33 and 23, 26 and 24.
+constexpr int64_t kStreamBytes = int64_t(32) << 20;
 
 // Wavefronts of a row: one while a row is at most 4 KB (four loads a lane), else 4, or 16 where rows are so few
 // that CUs would idle (with the weights' gradient, whose sums need the whole row in one workgroup); without it a
@@ -463,8 +474,10 @@ RowPlan row_plan(const RouteArgs& a, int size, bool dot) {
 }
 
 #define TP_ROWS(kernel, W, KB)                                                                                      \
-    (dot ? kernel<S, W, KB, true><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, in, to, other, d_weights)     \
-         : kernel<S, W, KB, false><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, in, to, nullptr, nullptr))
+    (dot ? kernel<S, W, KB, true><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, stream, in, to, other,        \
+                                                                          d_weights)                                \
+         : kernel<S, W, KB, false><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, stream, in, to, nullptr,      \
+                                                                           nullptr))
 #define TP_ROWS_BY_K(kernel, W) (a.k <= 2 ? TP_ROWS(kernel, W, 2) : TP_ROWS(kernel, W, 4))
 
 template <class S, bool SPREAD>
@@ -476,11 +489,16 @@ hipError_t move_rows(const RouteArgs& a, const void* in_, void* to_, const void*
     const bool dot = d_weights != nullptr;
     const RowPlan p = row_plan(a, sizeof(B), dot);
     const int64_t items = a.T * p.parts;
+    const bool stream = a.T * a.k * a.D * int64_t(sizeof(B)) >= kStreamBytes;
     const unsigned grid = match_grid(p.waves == 1 ? (items + 3) / 4 : items);
     if (SPREAD) {
         if (p.waves == 1) TP_ROWS_BY_K(k_spread_rows, 1);
         else if (p.waves == 4) TP_ROWS_BY_K(k_spread_rows, 4);
         else TP_ROWS_BY_K(k_spread_rows, 16);
+    } else if (dot && a.k > 4) {
+        if (p.waves == 1) TP_ROWS(k_gather_rows, 1, 8);
+        else if (p.waves == 4) TP_ROWS(k_gather_rows, 4, 8);
+        else TP_ROWS(k_gather_rows, 16, 8);
     } else {
         if (p.waves == 1) TP_ROWS_BY_K(k_gather_rows, 1);
         else if (p.waves == 4) TP_ROWS_BY_K(k_gather_rows, 4);
