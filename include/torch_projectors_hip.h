@@ -319,6 +319,13 @@ int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, c
                     const void* scales_b, int64_t rows_b, int64_t blocks, const void* bias, int out_dtype,
                     void* scores, void* work, int64_t work_bytes, void* stream);
 
+/* The same with rows x [rows_a, cols] (TP_F32, TP_F16 or TP_BF16, `row_stride`
+ * elements apart) for a, quantised as tp_quantize_blocks does on the way. */
+int64_t tp_score_images_work(int64_t rows_a, int64_t rows_b, int64_t cols);
+int tp_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, int64_t row_stride, const void* codes_b,
+                    const void* scales_b, int64_t rows_b, const void* bias, int out_dtype, void* scores, void* work,
+                    int64_t work_bytes, void* stream);
+
 /* Log probabilities of rows of scores [rows, candidates] (TP_F32, TP_F16 or
  * TP_BF16, rows `row_stride` apart): p = softmax(scores / temperature) over
  * the allowed candidates.
@@ -330,7 +337,7 @@ int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, c
  *              the allowed ones (scores of -inf count as not allowed)
  * Outputs fp32: given_log_probs [rows, givens], entropy [rows], log_sum [rows] (of
  * exp(score / temperature)), top_log_probs [rows, top]; top_index int64 [rows, top];
- * stats [rows, 4], which the gradient reads.  A row that allows nothing has
+ * stats [rows, 4], which the gradient reads (optional: NULL where none will).  A row that allows nothing has
  * log_sum and log probabilities -inf and entropy 0. */
 int64_t tp_log_probs_work(int64_t rows, int64_t candidates, int64_t top);
 int tp_log_probs(int dtype, const void* scores, int64_t rows, int64_t candidates, int64_t row_stride,

@@ -78,8 +78,12 @@ A, NULL = _P(256), _P(None)
         (dict(dt=1), "dtype"), (dict(V=0), "at least one"), (dict(top=65), "top"), (dict(top=-1), "top"),
         (dict(temp=0.0), "temperature"), (dict(temp=-1.0), "temperature"), (dict(temp=math.nan), "temperature"),
         (dict(temp=math.inf), "temperature"), (dict(temp=1e-300), "temperature"), (dict(G=1), "given"),
-        (dict(stride=-1), "strides"), (dict(T=1 << 31), "2^31"), (dict(x=NULL), "scores"), (dict(ti=NULL), "top_index"),
-        (dict(st=NULL), "stats")]),
+        (dict(stride=-1), "strides"), (dict(T=1 << 31), "2^31"), (dict(x=NULL), "scores"), (dict(ti=NULL), "top_index")]),
+    ("tp_score_images", dict(dt=0, x=A, M=2, cols=200, stride=200, b=A, sb=A, N=3, bias=NULL, odt=4, out=A, work=A,
+                             bytes=1 << 40, stream=NULL), [
+        (dict(dt=1), "dtype"), (dict(odt=3), "out_dtype"), (dict(cols=0), "cols"), (dict(cols=1 << 24), "blocks"),
+        (dict(M=-1), "non-negative"), (dict(stride=-1), "row_stride"), (dict(x=NULL), "x"), (dict(work=NULL), "work"),
+        (dict(bytes=10), "work is smaller"), (dict(sb=NULL), "scales_b"), (dict(out=NULL), "scores")]),
     ("tp_log_probs_back", dict(dt=0, x=A, T=2, V=3, stride=3, given=NULL, G=0, mask=NULL, ms=0, top=1, temp=1.0, ti=A, st=A,
                                dg=NULL, dh=NULL, dl=NULL, dt_=A, out=A, stream=NULL), [
         (dict(dt=2), "dtype"), (dict(ti=NULL), "top_index"), (dict(st=NULL), "stats"), (dict(out=NULL), "d_scores"),

@@ -1412,6 +1412,35 @@ int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, c
                     "score launch");
 }
 
+int64_t tp_score_images_work(int64_t rows_a, int64_t rows_b, int64_t cols) {
+    if (rows_a <= 0 || rows_b <= 0 || cols <= 0) return 0;
+    return tp::score_images_work(rows_a, rows_b, cols);
+}
+
+int tp_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, int64_t row_stride, const void* codes_b,
+                    const void* scales_b, int64_t rows_b, const void* bias, int out_dtype, void* scores, void* work,
+                    int64_t work_bytes, void* stream) {
+    g_err.clear();
+    TP_TRY(match_dtype(dtype));
+    if (out_dtype != TP_F32 && out_dtype != TP_BF16) return fail("out_dtype must be TP_F32 or TP_BF16");
+    if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
+    if (cols < 1) return fail("cols must be positive");
+    if (row_stride < 0) return fail("row_stride must be non-negative");
+    if (rows_a > kInt32Max || rows_b > kInt32Max) return fail("row counts must be < 2^31");
+    if (tp::block_count(cols) > 65536) return fail("blocks must be at most 65536");
+    if (rows_a == 0 || rows_b == 0) return TP_OK;
+    TP_TRY(need(x, "x"));
+    TP_TRY(need(codes_b, "codes_b"));
+    TP_TRY(need(scales_b, "scales_b"));
+    TP_TRY(need(scores, "scores"));
+    const int64_t need_bytes = tp::score_images_work(rows_a, rows_b, cols);
+    if (need_bytes) TP_TRY(need(work, "work"));
+    if (work_bytes < need_bytes) return fail("work is smaller than tp_score_images_work");
+    return launched(tp::launch_score_images(dtype, x, rows_a, cols, row_stride, codes_b, scales_b, rows_b, bias,
+                                            out_dtype, scores, work, static_cast<hipStream_t>(stream)),
+                    "score launch");
+}
+
 int64_t tp_log_probs_work(int64_t rows, int64_t candidates, int64_t top) {
     if (rows <= 0 || candidates <= 0 || top < 0 || top > tp::kMaxTop) return 0;
     return tp::log_probs_work(rows, candidates, int(top));
@@ -1434,7 +1463,6 @@ int tp_log_probs(int dtype, const void* scores, int64_t rows, int64_t candidates
         TP_TRY(need(top_log_probs, "top_log_probs"));
         TP_TRY(need(top_index, "top_index"));
     }
-    TP_TRY(need(stats, "stats"));
     const int64_t need_bytes = tp::log_probs_work(rows, candidates, int(top));
     if (need_bytes) TP_TRY(need(work, "work"));
     if (work_bytes < need_bytes) return fail("work is smaller than tp_log_probs_work");

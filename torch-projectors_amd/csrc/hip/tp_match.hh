@@ -15,6 +15,8 @@ constexpr int kScaleRows = 16;    // rows of the scales are padded to this
 
 inline int64_t scale_rows(int64_t rows) { return (rows + kScaleRows - 1) / kScaleRows * kScaleRows; }
 
+inline int64_t block_count(int64_t cols) { return (cols + kScaleBlock - 1) / kScaleBlock; }
+
 // x [rows, cols] of `dt`, rows `stride` elements apart -> codes [rows, 128 nb], scales [nb, scale_rows(rows)].
 hipError_t launch_quantize_blocks(int dt, const void* x, int64_t rows, int64_t cols, int64_t stride, void* codes,
                                   void* scales, hipStream_t s);
@@ -24,6 +26,13 @@ int64_t block_scores_work(int64_t M, int64_t N, int64_t nb);
 // out [M, N] (TP_F32 or TP_BF16) = bias[n] + sum over blocks; bias fp32 or null.
 hipError_t launch_block_scores(const void* a, const void* sa, int64_t M, const void* b, const void* sb, int64_t N,
                                int64_t nb, const void* bias, int out_dt, void* out, void* work, hipStream_t s);
+
+// The same for rows x [M, cols] of `dt`, `stride` apart, that are quantised first (one row: by the product's own
+// kernel, on its way; bytes of work for codes and scales otherwise, then launch_block_scores').
+int64_t score_images_work(int64_t M, int64_t N, int64_t cols);
+hipError_t launch_score_images(int dt, const void* x, int64_t M, int64_t cols, int64_t stride, const void* b,
+                               const void* sb, int64_t N, const void* bias, int out_dt, void* out, void* work,
+                               hipStream_t s);
 
 // ------------------------------------------------------------------ log probabilities (tp_probs.hip)
 constexpr int kMaxTop = 64;  // a wavefront keeps one alternative per lane
@@ -39,7 +48,7 @@ struct ProbsArgs {
     int top;
     float temperature;
 };
-// Statistics of a row that the gradient reads: the largest allowed score, ln of the sum of
+// Statistics of a row that the gradient reads (null where none will): the largest allowed score, ln of the sum of
 // exp((x - largest) / temperature), the entropy, and an unused word.
 constexpr int kProbsStats = 4;
 

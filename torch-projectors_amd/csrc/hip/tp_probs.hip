@@ -11,10 +11,10 @@
 // Alternatives: a wavefront keeps its best as sorted keys, one per lane: the score's bits in an order that
 // integers have, then the complement of its index, so ties go to the lowest index.  Scores above the top-th
 // key's are candidates; of a tile with many (the first; rising rows) only those that reach a floor below
-// which none can be listed: a value that `top` of the lanes' own largest reach.  Candidates go through LDS,
-// 64 at a time, and are merged by counting: each one's place is the number of keys and of other candidates
-// above it, each key moves up by the number of candidates above it.  (Counting over broadcast reads of LDS, in
-// all lanes at once, is faster from about 16 candidates on, but most tiles have one or two.)
+// which none can be listed: the top-th largest of the lanes' own largest.  Candidates go through LDS and are
+// merged by counting: a key's place is the number of keys above it, which all lanes count at once over
+// broadcast reads (about 15 cycles a key; handing one key after another around through scalar registers takes
+// 100, but does not depend on `top`, and is left for few candidates of long lists).
 //
 // Split: a row is one wavefront's, or 2, 4 or 8 of a workgroup's, or, where rows are few, several workgroups',
 // whose sums and keys k_probs_join joins.  Memory bound: a tile of 16 scores a lane is in flight for every
@@ -83,55 +83,89 @@ template <class F> __device__ __forceinline__ float reduced(float v, float none,
 __device__ __forceinline__ int below(uint64_t lanes) {
     return int(__builtin_amdgcn_mbcnt_hi(uint32_t(lanes >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(lanes), 0)));
 }
-// A value (in order_of's order) that at least k lanes reach, with its low 16 bits zero: the largest such.
-__device__ __forceinline__ uint32_t floor_of(uint32_t order, int k) {
-    uint32_t at = 0;
-#pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit > 0x8000u; bit >>= 1)
-        if (__popcll(__ballot(order >= (at | bit))) >= k) at |= bit;
-    return at;
-}
-
 // A wavefront's LDS.  Only it reads and writes it, in order; the fences keep the compiler to that.
 constexpr int kLaneScores = 16;                 // of a tile
 constexpr int kTileScores = 64 * kLaneScores;
-struct Room {
-    uint64_t found[kTileScores];  // candidates
+struct alignas(16) Room {
+    uint64_t found[kTileScores + 4];  // candidates, then zeros up to the next multiple of 4
     uint64_t keys[64];
+    uint32_t order[64];
 };
 __device__ __forceinline__ void lds_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-// The best keys of a wavefront, sorted, and the score of the top-th (-inf while there are fewer).  Keys past the
-// top-th are kept in the lanes that are there anyway.
+// A value that at least k lanes reach: the k-th largest without its last 6 bits.
+__device__ __forceinline__ uint32_t floor_of(uint32_t v, int k, Room& room, int lane) {
+    const uint32_t mine = (v & ~63u) | uint32_t(63 - lane);  // no two are equal
+    room.order[lane] = mine;
+    lds_order();
+    int above = 0;
+#pragma unroll
+    for (int l = 0; l < 64; l += 4) {
+        const uint4 o = *reinterpret_cast<const uint4*>(room.order + l);
+        above += (o.x > mine ? 1 : 0) + (o.y > mine ? 1 : 0) + (o.z > mine ? 1 : 0) + (o.w > mine ? 1 : 0);
+    }
+    lds_order();
+    return read_lane(mine, __ffsll(static_cast<long long>(__ballot(above == k - 1))) - 1) & ~63u;
+}
+// How many of the n keys from p on (zeros after them up to a multiple of 4; p 16-byte aligned) are above `key`.
+__device__ __forceinline__ int above(uint64_t key, const uint64_t* p, int n) {
+    int a = 0;
+    for (int j = 0; j < n; j += 4) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(p + j), y = *reinterpret_cast<const ulonglong2*>(p + j + 2);
+        a += (x.x > key ? 1 : 0) + (x.y > key ? 1 : 0) + (y.x > key ? 1 : 0) + (y.y > key ? 1 : 0);
+    }
+    return a;
+}
+
+// The best keys of a wavefront, sorted, one per lane below top, and the score of the top-th (-inf while there are
+// fewer).
 struct Best {
     uint64_t key = 0;
     float least = neg_inf();
 
-    // Merge the lanes' keys for which `set` holds a bit.
-    __device__ __forceinline__ void take(uint64_t set, uint64_t theirs, Room& room, int lane) {
-        if (!set) return;
-        int up = 0, rank = 0, above = 0;
-        for (uint64_t left = set; left; left &= left - 1) {
-            const int from = __ffsll(static_cast<long long>(left)) - 1;
-            const uint64_t k = read_lane(theirs, from);
-            const int keys = __popcll(__ballot(key > k));
-            if (lane == from) above = keys;
-            up += key < k ? 1 : 0;
-            rank += theirs < k ? 1 : 0;
+    // Merge room.found[0, n).
+    __device__ __forceinline__ void take(int n, int top, Room& room, int lane) {
+        if (lane < 4) room.found[n + lane] = 0;
+        lds_order();
+        if (top <= 32 && top <= 6 * n + 12) {
+            const int step = (64 - top) & ~3;
+            for (int i = 0; i < n; i += step) {
+                const int count = min(step, n - i);
+                const uint64_t mine = lane < top ? key : lane - top < count ? room.found[i + lane - top] : 0;
+                room.keys[lane] = key;
+                lds_order();
+                const int place = above(mine, room.found + i, count) + above(mine, room.keys, top);
+                lds_order();
+                room.keys[lane] = 0;
+                if (mine && place < top) room.keys[place] = mine;
+                lds_order();
+                key = room.keys[lane];
+                lds_order();
+            }
+        } else {
+            for (int i = 0; i < n; i += 64) {
+                const uint64_t theirs = i + lane < n ? room.found[i + lane] : 0;
+                const uint64_t set = __ballot(theirs > read_lane(key, top - 1));
+                int up = 0, rank = 0, more = 0;
+                for (uint64_t left = set; left; left &= left - 1) {
+                    const int from = __ffsll(static_cast<long long>(left)) - 1;
+                    const uint64_t k = read_lane(theirs, from);
+                    const int keys = __popcll(__ballot(key > k));
+                    if (lane == from) more = keys;
+                    up += key < k ? 1 : 0;
+                    rank += theirs < k ? 1 : 0;
+                }
+                room.keys[lane] = 0;
+                lds_order();
+                if (key && lane + up < top) room.keys[lane + up] = key;
+                if (((set >> lane) & 1) && more + rank < top) room.keys[more + rank] = theirs;
+                lds_order();
+                key = room.keys[lane];
+                lds_order();
+            }
         }
-        const bool in = (set >> lane) & 1;
-        room.keys[lane] = 0;
-        lds_order();
-        if (key && lane + up < 64) room.keys[lane + up] = key;
-        if (in && above + rank < 64) room.keys[above + rank] = theirs;
-        lds_order();
-        key = room.keys[lane];
-        lds_order();
-    }
-    __device__ __forceinline__ uint64_t last(int top) const { return read_lane(key, top - 1); }
-    __device__ __forceinline__ void settle(int top) {
-        const uint64_t k = last(top);
-        least = k ? score_of(k) : neg_inf();
+        const uint64_t last = read_lane(key, top - 1);
+        least = last ? score_of(last) : neg_inf();
     }
 };
 
@@ -232,7 +266,7 @@ __device__ __forceinline__ void scan_scores(const typename S::Bits* x, const uin
         }
         const uint64_t lanes = __ballot(most > best.least);
         if (!lanes) continue;
-        const uint32_t floor = __popcll(lanes) > 4 ? floor_of(order_of(most), top) : 0;
+        const uint32_t floor = __popcll(lanes) > 4 ? floor_of(order_of(most), top, room, lane) : 0;
         int n = 0;
 #pragma unroll
         for (int i = 0; i < kLaneScores; ++i) {
@@ -242,39 +276,31 @@ __device__ __forceinline__ void scan_scores(const typename S::Bits* x, const uin
             if (in) room.found[n + below(set)] = uint64_t(o) << 32 | uint32_t(~uint32_t(tile_index<S>(v0, lane, i)));
             n += __popcll(set);
         }
-        lds_order();
-        for (int i = 0; i < n; i += 64) {
-            const uint64_t k = i + lane < n ? room.found[i + lane] : 0;
-            best.take(__ballot(k > best.last(top)), k, room, lane);
-        }
-        best.settle(top);
+        best.take(n, top, room, lane);
     }
 }
 
-// Merge the keys from p on: 64 N at a time, of more than 64 those that a floor found as in a tile leaves.
-template <int N>
+// Merge the keys from p on, 1024 at a time, of which a floor is found as in a tile.
 __device__ __forceinline__ void join_keys(Best& best, const uint64_t* p, int count, int top, Room& room, int lane) {
+    constexpr int N = kLaneScores;
     for (int i0 = 0; i0 < count; i0 += 64 * N) {
         uint64_t k[N], most = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) k[i] = i0 + i * 64 + lane < count ? p[i0 + i * 64 + lane] : 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) most = max(most, k[i]);
-        const uint32_t floor = count - i0 > 64 ? floor_of(uint32_t(most >> 32), top) : 0;
-        const uint64_t last = best.last(top);
+        const uint32_t floor = floor_of(uint32_t(most >> 32), top, room, lane);
+        const uint64_t last = read_lane(best.key, top - 1);
         int n = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            if (i0 + i * 64 >= count) break;
             const bool in = k[i] > last && uint32_t(k[i] >> 32) >= floor;
             const uint64_t set = __ballot(in);
             if (in) room.found[n + below(set)] = k[i];
             n += __popcll(set);
         }
-        lds_order();
-        for (int i = 0; i < n; i += 64) {
-            const uint64_t mine = i + lane < n ? room.found[i + lane] : 0;
-            best.take(__ballot(mine > best.last(top)), mine, room, lane);
-        }
+        best.take(n, top, room, lane);
     }
 }
 
@@ -304,7 +330,7 @@ __device__ __forceinline__ void write_row(const ProbsArgs& a, const ProbsOut& o,
         const float H = none ? 0.0f : !isfinite(m) ? __builtin_nanf("") : ls - sums.u * kLn2 / sums.s;
         o.entropy[t] = H;
         o.log_sum[t] = isfinite(m) ? __builtin_fmaf(m, c, ls) : m;
-        *reinterpret_cast<float4*>(o.stats + t * kProbsStats) = float4{m, ls, H, 0.0f};
+        if (o.stats) *reinterpret_cast<float4*>(o.stats + t * kProbsStats) = float4{m, ls, H, 0.0f};
     }
     for (int64_t g = lane; g < a.G; g += 64) {
         const int64_t v = g < 64 ? given : given_index(a, t, g);
@@ -333,7 +359,8 @@ template <class S>
 __global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut o, int waves, int64_t span, Parts parts) {
     __shared__ Sums sums_of[kProbsWaves];
     __shared__ Room rooms[kProbsWaves];
-    __shared__ uint64_t keys_of[kProbsWaves * kMaxTop];
+    __shared__ uint64_t keys_of[kProbsWaves * kMaxTop], best_of[kMaxTop];
+    __shared__ int places[kProbsWaves * kMaxTop];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int group = waves < kProbsWaves ? waves : kProbsWaves;  // wavefronts of a row in the workgroup
     const int blocks = waves / group;                             // workgroups of a row
@@ -357,10 +384,32 @@ __global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut 
         if (group > 1) {
             if (lane == 0) sums_of[wave] = sums;
             if (lane < a.top) keys_of[wave * a.top + lane] = best.key;
+            const int keys = kProbsWaves * a.top;
+            if (group == kProbsWaves && threadIdx.x < kMaxTop) best_of[threadIdx.x] = 0;
+            if (int(threadIdx.x) < keys) places[threadIdx.x] = 0;
             __syncthreads();
+            if (group == kProbsWaves && a.top) {
+                // a key's place among all wavefronts' keys, counted by 2^s lanes
+                const int s = 31 - __clz(kProbsBlock / keys), i = threadIdx.x >> s, p = threadIdx.x & ((1 << s) - 1);
+                const uint64_t mine = i < keys ? keys_of[i] : 0;
+                if (mine) {
+                    int more = 0;
+#pragma unroll 4
+                    for (int j = p; j < keys; j += 1 << s) more += keys_of[j] > mine ? 1 : 0;
+                    atomicAdd(&places[i], more);
+                }
+                __syncthreads();
+                if (mine && p == 0 && places[i] < a.top) best_of[places[i]] = mine;
+                __syncthreads();
+                best.key = best_of[lane];
+            }
             if (writes) {
-                for (int w = wave + 1; w < wave + group; ++w) sums = joined(sums, sums_of[w], c2);
-                if (a.top) join_keys<2>(best, keys_of + (wave + 1) * a.top, (group - 1) * a.top, a.top, rooms[wave], lane);
+                sums = wave_joined(lane < group ? sums_of[wave + lane] : Sums{neg_inf(), 0.0f, 0.0f}, c2);
+                if (group < kProbsWaves && a.top)
+                    for (int w = wave + 1; w < wave + group; ++w) {
+                        if (lane < a.top) rooms[wave].found[lane] = keys_of[w * a.top + lane];
+                        best.take(a.top, a.top, rooms[wave], lane);
+                    }
             }
             __syncthreads();
         }
@@ -385,7 +434,7 @@ __global__ __launch_bounds__(64) void k_probs_join(ProbsArgs a, ProbsOut o, int 
         const Sums* of = parts.sums + t * blocks;
         Sums sums = lane < blocks ? of[lane] : Sums{neg_inf(), 0.0f, 0.0f};
         Best best;
-        if (a.top) join_keys<16>(best, parts.keys + t * blocks * a.top, blocks * a.top, a.top, room, lane);
+        if (a.top) join_keys(best, parts.keys + t * blocks * a.top, blocks * a.top, a.top, room, lane);
         const float given_x = given_score<S>(a, t, given);
         for (int b = lane + 64; b < blocks; b += 64) sums = joined(sums, of[b], c2);
         sums = wave_joined(sums, c2);
@@ -394,7 +443,8 @@ __global__ __launch_bounds__(64) void k_probs_join(ProbsArgs a, ProbsOut o, int 
 }
 
 // Wavefronts of a row, and the scores of each: as many as fill the card (16 on each CU), none with less than a
-// tile.
+// tile; a whole workgroup's where that leaves none waiting (its join is the faster one: 1 x 4096 with 8
+// alternatives 7.5 us by 4 of 8 wavefronts, 6.6 by 8, half of them without scores).
 struct ProbsPlan {
     int waves;
     int64_t span;
@@ -404,6 +454,7 @@ ProbsPlan probs_plan(int64_t T, int64_t V) {
     const int64_t most = std::min<int64_t>((4096 + T - 1) / T, tiles);
     int64_t w = 1;
     while (w < most && w < kProbsWaves) w *= 2;
+    if (w > 1 && T <= 512) w = kProbsWaves;
     if (most > kProbsWaves) w = (most + kProbsWaves - 1) / kProbsWaves * kProbsWaves;
     const int64_t span = (tiles + w - 1) / w * kTileScores;
     return {int(w), span};

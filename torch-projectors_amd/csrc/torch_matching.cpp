@@ -57,14 +57,18 @@ struct Scope {
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // ------------------------------------------------------------------ 8-bit blocks
+// Rows any distance apart, the values of each adjacent.
+Tensor rows_of(const Tensor& x, const char* what) {
+    TORCH_CHECK(x.dim() == 2, what, " must be (rows, values)");
+    TORCH_CHECK(x.size(1) >= 1, what, ": rows must hold at least one value");
+    return x.size(1) == 1 || x.stride(1) == 1 ? x : x.contiguous();
+}
+
 std::tuple<Tensor, Tensor> quantize_blocks(const Tensor& x) {
-    TORCH_CHECK(x.dim() == 2, "quantize_blocks: x must be (rows, values)");
-    TORCH_CHECK(x.size(1) >= 1, "quantize_blocks: rows must hold at least one value");
     const int dt = dtype_code(x, "quantize_blocks: x");
     const auto dev = x.device();
     const Scope scope(dev);
-    // rows may lie any distance apart; the values of one have to be adjacent
-    const Tensor v = (x.size(1) == 1 || x.stride(1) == 1) && x.stride(0) >= 0 ? x : x.contiguous();
+    const Tensor v = rows_of(x, "quantize_blocks: x");
     const int64_t R = v.size(0), nb = (v.size(1) + kBlock - 1) / kBlock;
     Tensor codes = fresh({R, nb * kBlock}, at::kFloat8_e4m3fn, dev);
     Tensor scales = fresh({nb, tp_scale_rows(R)}, at::kByte, dev);
@@ -82,7 +86,7 @@ void check_blocks(const Tensor& codes, const Tensor& scales, const char* what) {
                 what, ": scales must be uint8 (blocks, rows padded to 16)");
 }
 
-// images: float rows, quantised here, or codes with their scales
+// images: float rows, quantised on the way, or codes with their scales
 Tensor block_scores(const Tensor& images, const optional<Tensor>& image_scales, const Tensor& codes,
                     const Tensor& scales, const optional<Tensor>& bias, at::ScalarType out_dtype) {
     check_blocks(codes, scales, "references");
@@ -91,18 +95,8 @@ Tensor block_scores(const Tensor& images, const optional<Tensor>& image_scales, 
     const auto dev = codes.device();
     same_device(scales, dev);
     same_device(images, dev);
-    Tensor a, sa;
-    if (image_scales.has_value()) {
-        check_blocks(images, *image_scales, "images");
-        same_device(*image_scales, dev);
-        a = images.contiguous();
-        sa = image_scales->contiguous();
-    } else {
-        std::tie(a, sa) = quantize_blocks(images);
-    }
-    TORCH_CHECK(a.size(1) == codes.size(1), "block_scores: images have ", a.size(1) / kBlock,
-                " blocks a row, references ", codes.size(1) / kBlock);
-    const int64_t M = a.size(0), N = codes.size(0), nb = codes.size(1) / kBlock;
+    const Scope scope(dev);
+    const int64_t N = codes.size(0), nb = codes.size(1) / kBlock;
     Tensor f;
     if (bias.has_value()) {
         TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N && bias->scalar_type() == at::kFloat,
@@ -110,14 +104,31 @@ Tensor block_scores(const Tensor& images, const optional<Tensor>& image_scales, 
         same_device(*bias, dev);
         f = bias->contiguous();
     }
-    const Scope scope(dev);
     const Tensor b = codes.contiguous(), sb = scales.contiguous();
+    const int out_dt = out_dtype == at::kFloat ? TP_F32 : TP_BF16;
+    auto same_blocks = [&](int64_t blocks) {
+        TORCH_CHECK(blocks == nb, "block_scores: images have ", blocks, " blocks a row, references ", nb);
+    };
+    if (image_scales.has_value()) {
+        check_blocks(images, *image_scales, "images");
+        same_blocks(images.size(1) / kBlock);
+        same_device(*image_scales, dev);
+        const Tensor a = images.contiguous(), sa = image_scales->contiguous();
+        const int64_t M = a.size(0), bytes = tp_block_scores_work(M, N, nb);
+        Tensor out = fresh({M, N}, out_dtype, dev);
+        const Tensor work = workspace(bytes, dev);
+        check_rc(tp_block_scores(a.data_ptr(), sa.data_ptr(), M, b.data_ptr(), sb.data_ptr(), N, nb, ptr(f), out_dt,
+                                 out.data_ptr(), ptr(work), bytes, current_stream(dev)));
+        return out;
+    }
+    const int dt = dtype_code(images, "block_scores: images");
+    const Tensor a = rows_of(images, "block_scores: images");
+    same_blocks((a.size(1) + kBlock - 1) / kBlock);
+    const int64_t M = a.size(0), bytes = tp_score_images_work(M, N, a.size(1));
     Tensor out = fresh({M, N}, out_dtype, dev);
-    const int64_t bytes = tp_block_scores_work(M, N, nb);
     const Tensor work = workspace(bytes, dev);
-    check_rc(tp_block_scores(a.data_ptr(), sa.data_ptr(), M, b.data_ptr(), sb.data_ptr(), N, nb, ptr(f),
-                             out_dtype == at::kFloat ? TP_F32 : TP_BF16, out.data_ptr(), ptr(work), bytes,
-                             current_stream(dev)));
+    check_rc(tp_score_images(dt, a.data_ptr(), M, a.size(1), a.stride(0), b.data_ptr(), sb.data_ptr(), N, ptr(f),
+                             out_dt, out.data_ptr(), ptr(work), bytes, current_stream(dev)));
     return out;
 }
 
@@ -157,9 +168,10 @@ Probs probs(const Tensor& scores, const optional<Tensor>& given, const optional<
     return p;
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs(const Tensor& scores, const optional<Tensor>& given,
-                                                                     const optional<Tensor>& mask, int64_t top,
-                                                                     double temperature) {
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs_of(const Tensor& scores,
+                                                                        const optional<Tensor>& given,
+                                                                        const optional<Tensor>& mask, int64_t top,
+                                                                        double temperature, bool with_stats) {
     const Probs p = probs(scores, given, mask);
     TORCH_CHECK(top >= 0 && top <= 64, "log_probs: top must be in [0, 64]");
     const auto dev = scores.device();
@@ -167,14 +179,20 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs(const Tenso
     Tensor given_out = given.has_value() ? fresh(given->sizes(), at::kFloat, dev) : Tensor();
     Tensor entropy = fresh({p.T}, at::kFloat, dev), log_sum = fresh({p.T}, at::kFloat, dev);
     Tensor top_out = fresh({p.T, top}, at::kFloat, dev), top_index = fresh({p.T, top}, at::kLong, dev);
-    Tensor stats = fresh({p.T, 4}, at::kFloat, dev);
+    Tensor stats = with_stats ? fresh({p.T, 4}, at::kFloat, dev) : Tensor();
     const int64_t bytes = tp_log_probs_work(p.T, p.V, top);
     const Tensor work = workspace(bytes, dev);
     check_rc(tp_log_probs(p.dt, p.scores.data_ptr(), p.T, p.V, p.stride, ptr(p.given), p.G, ptr(p.mask),
                           p.mask_stride, top, temperature, ptr(given_out), entropy.data_ptr(),
-                          log_sum.data_ptr(), top_out.data_ptr(), top_index.data_ptr(), stats.data_ptr(), ptr(work),
+                          log_sum.data_ptr(), top_out.data_ptr(), top_index.data_ptr(), ptr(stats), ptr(work),
                           bytes, current_stream(dev)));
     return {given_out, entropy, log_sum, top_out, top_index, stats};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs(const Tensor& scores, const optional<Tensor>& given,
+                                                                     const optional<Tensor>& mask, int64_t top,
+                                                                     double temperature) {
+    return log_probs_of(scores, given, mask, top, temperature, true);
 }
 
 Tensor log_probs_back(const Tensor& scores, const optional<Tensor>& given, const optional<Tensor>& mask,
@@ -344,7 +362,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs_grad(const 
                                                                           const optional<Tensor>& given,
                                                                           const optional<Tensor>& mask, int64_t top,
                                                                           double temperature) {
-    if (!at::GradMode::is_enabled() || !wants(scores)) return log_probs(scores, given, mask, top, temperature);
+    if (!at::GradMode::is_enabled() || !wants(scores))  // (no statistics: None)
+        return log_probs_of(scores, given, mask, top, temperature, false);
     auto r = LogProbsGrad::apply(scores, given, mask, top, temperature);
     return {r.size() > 5 ? r[5] : Tensor(), r[0], r[1], r[2], r[3], r[4]};
 }

@@ -44,6 +44,7 @@ SIGNATURES = {
     # matching
     "tp_quantize_blocks": [_I, _P, _L, _L, _L, _P, _P, _P],
     "tp_block_scores": [_P, _P, _L, _P, _P, _L, _L, _P, _I, _P, _P, _L, _P],
+    "tp_score_images": [_I, _P, _L, _L, _L, _P, _P, _L, _P, _I, _P, _P, _L, _P],
     "tp_log_probs": [_I, _P, _L, _L, _L, _P, _L, _P, _L, _L, _D, _P, _P, _P, _P, _P, _P, _P, _L, _P],
     "tp_log_probs_back": [_I, _P, _L, _L, _L, _P, _L, _P, _L, _L, _D, _P, _P, _P, _P, _P, _P, _P, _P],
     "tp_sort_by_class": [_I, _P, _L, _L, _P, _P, _P, _P, _L, _P],
@@ -58,6 +59,7 @@ SIZE_HELPERS = {
     "tp_fused_fourier_work": [_I, _I, _I, _L, _L, _L],
     "tp_scale_rows": [_L],
     "tp_block_scores_work": [_L, _L, _L],
+    "tp_score_images_work": [_L, _L, _L],
     "tp_log_probs_work": [_L, _L, _L],
     "tp_sort_by_class_work": [_L, _L],
 }
