@@ -71,7 +71,7 @@ def block_scores(images, references, bias: Optional[torch.Tensor] = None,
 
     images [M, ...] and references [N, ...] are BlockScaled, or rows that are quantised here; of complex
     rows the real part of the inner product is taken (their real pairs' product).  With rfft images,
-    which hold one half of a symmetric plane, scale either side's columns other than x = 0 by two for the
+    which hold one half of a symmetric plane, scale either side's columns other than x = 0 and n / 2 by two for the
     whole plane's product; with bias = -|reference|^2 / 2 the scores are the log likelihoods of unit noise
     up to a constant per image.  bias float32 [N]; out_dtype float32 or bfloat16.  Not differentiable."""
     if not isinstance(references, BlockScaled):
