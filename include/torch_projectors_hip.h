@@ -313,7 +313,8 @@ int tp_quantize_blocks(int dtype, const void* x, int64_t rows, int64_t cols, int
                        void* scales, void* stream);
 
 /* scores[m, n] = bias[n] + <row m of a, row n of b>, both in 8-bit blocks, summed
- * in fp32 (bias fp32, optional; scores TP_F32 or TP_BF16; 1 to 65536 blocks). */
+ * in fp32 (bias fp32, optional; scores TP_F32 or TP_BF16; at most 2^26 rows on
+ * either side, 1 to 65536 blocks). */
 int64_t tp_block_scores_work(int64_t rows_a, int64_t rows_b, int64_t blocks);
 int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, const void* codes_b,
                     const void* scales_b, int64_t rows_b, int64_t blocks, const void* bias, int out_dtype,

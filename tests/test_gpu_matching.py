@@ -553,3 +553,31 @@ def test_probs_many_givens(m):
     given = torch.randint(0, 60, (3, 100), generator=g)
     given[torch.rand(3, 100, generator=g) < 0.1] = -1
     _probs_check(m, x, given, 40, 1.2)
+
+
+def test_rows_foreign_slots_stay_in_bounds(m):
+    """Places outside the sorted rows (an order from elsewhere) are not read, nor is anything written there."""
+    order = m.sort_by_class(torch.tensor([0, 1, 0, 1], device=DEV), 2)
+    bad = order._replace(slot=torch.tensor([[0], [-5], [1 << 30], [2]], dtype=torch.int32, device=DEV))
+    x = torch.ones(4, 33, device=DEV)
+    s = m.dispatch(x, bad)
+    assert (s[0] == 1).all() and (s[2] == 1).all()
+    w = torch.full((4, 1), 2.0, device=DEV, requires_grad=True)
+    back = m.combine(x, bad, w)
+    assert torch.equal(back[:, 0].detach().cpu(), torch.tensor([2.0, 0, 0, 2.0]))
+    (dw,) = torch.autograd.grad(back.sum(), w)
+    assert torch.equal(dw.cpu(), torch.tensor([[33.0], [0], [0], [33.0]]))
+
+
+def test_one_image_of_every_type(m):
+    """A single image takes its own kernel: the same scores as from its blocks."""
+    g = gen(31)
+    refs = m.quantize_blocks(torch.randn(37, 515, generator=g).to(DEV))
+    for dtype in (F32, F16, BF16):
+        x = torch.randn(3, 515, generator=g).to(dtype)[1:2]
+        x[0, 100] = 0.0
+        for out in (F32, BF16):
+            got = m.block_scores(x.to(DEV), refs, out_dtype=out)
+            assert torch.equal(got, m.block_scores(m.quantize_blocks(x.to(DEV)), refs, out_dtype=out))
+        x[0, 300] = math.nan
+        assert m.block_scores(x.to(DEV), refs).isnan().all()

@@ -71,7 +71,7 @@ A, NULL = _P(256), _P(None)
         (dict(dt=1), "dtype"), (dict(dt=9), "dtype"), (dict(rows=-1), "non-negative"), (dict(cols=1 << 31), "2^31"),
         (dict(stride=-3), "row_stride"), (dict(x=NULL), "x"), (dict(codes=NULL), "codes"), (dict(scales=NULL), "scales")]),
     ("tp_block_scores", dict(a=A, sa=A, M=2, b=A, sb=A, N=3, nb=1, bias=NULL, dt=0, out=A, work=A, bytes=1 << 40, stream=NULL), [
-        (dict(dt=3), "out_dtype"), (dict(nb=0), "blocks"), (dict(M=-1), "non-negative"), (dict(nb=1 << 25), "blocks"),
+        (dict(dt=3), "out_dtype"), (dict(nb=0), "blocks"), (dict(M=-1), "non-negative"), (dict(N=1 << 27), "2^26"), (dict(nb=1 << 25), "blocks"),
         (dict(a=NULL), "codes_a"), (dict(sb=NULL), "scales_b"), (dict(out=NULL), "scores")]),
     ("tp_log_probs", dict(dt=0, x=A, T=2, V=3, stride=3, given=NULL, G=0, mask=NULL, ms=0, top=1, temp=1.0, go=A, h=A, l=A,
                           to=A, ti=A, st=A, work=A, bytes=1 << 40, stream=NULL), [

@@ -1395,7 +1395,7 @@ int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, c
     if (out_dtype != TP_F32 && out_dtype != TP_BF16) return fail("out_dtype must be TP_F32 or TP_BF16");
     if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
     if (blocks < 1) return fail("blocks must be positive");
-    if (rows_a > kInt32Max || rows_b > kInt32Max) return fail("row counts must be < 2^31");
+    if (rows_a > tp::kMaxScoreRows || rows_b > tp::kMaxScoreRows) return fail("row counts must be at most 2^26");
     // (the codes of 256 rows are one buffer of less than 2^32 bytes)
     if (blocks > 65536) return fail("blocks must be at most 65536");
     if (rows_a == 0 || rows_b == 0) return TP_OK;
@@ -1426,7 +1426,7 @@ int tp_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, int6
     if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
     if (cols < 1) return fail("cols must be positive");
     if (row_stride < 0) return fail("row_stride must be non-negative");
-    if (rows_a > kInt32Max || rows_b > kInt32Max) return fail("row counts must be < 2^31");
+    if (rows_a > tp::kMaxScoreRows || rows_b > tp::kMaxScoreRows) return fail("row counts must be at most 2^26");
     if (tp::block_count(cols) > 65536) return fail("blocks must be at most 65536");
     if (rows_a == 0 || rows_b == 0) return TP_OK;
     TP_TRY(need(x, "x"));

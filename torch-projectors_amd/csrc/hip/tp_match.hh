@@ -12,6 +12,7 @@ namespace tp {
 // ------------------------------------------------------------------ 8-bit blocks (tp_scores.hip)
 constexpr int kScaleBlock = 128;  // values that share a scale
 constexpr int kScaleRows = 16;    // rows of the scales are padded to this
+constexpr int64_t kMaxScoreRows = int64_t(1) << 26;  // of either side (a launch has fewer than 2^32 lanes)
 
 inline int64_t scale_rows(int64_t rows) { return (rows + kScaleRows - 1) / kScaleRows * kScaleRows; }
 
@@ -135,6 +136,11 @@ template <class S> __device__ __forceinline__ Pack<S> stream_pack(const typename
 template <class S> __device__ __forceinline__ void stream_pack(typename S::Bits* p, const Pack<S>& r) {
     __builtin_nontemporal_store(__builtin_bit_cast(typename PackBits<S>::Any, r),
                                 reinterpret_cast<typename PackBits<S>::At*>(p));
+}
+
+// n / d for n >= 0: in 32 bits where that will do (a 64-bit division is some 100 instructions).
+__device__ __forceinline__ int64_t over(int64_t n, uint32_t d) {
+    return uint64_t(n) >> 32 ? int64_t(uint64_t(n) / d) : int64_t(uint32_t(n) / d);
 }
 
 // Sum over a wavefront, the same in every lane (fixed order).

@@ -367,15 +367,15 @@ __global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut 
     const float c2 = kLog2e / a.temperature;
     const int64_t items = waves < kProbsWaves ? (a.T * waves + kProbsWaves - 1) / kProbsWaves : a.T * blocks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t at = item * kProbsWaves + wave, t = at / waves;  // wavefront `at % waves` of row t
-        const bool in = t < a.T, writes = in && wave % group == 0;
+        const int64_t at = item * kProbsWaves + wave, t = over(at, waves), part = at - t * waves;  // wavefront `part` of row t
+        const bool in = t < a.T, writes = in && (wave & (group - 1)) == 0;
         Sums sums{neg_inf(), 0.0f, 0.0f};
         Best best;
         const int64_t given = writes && blocks == 1 ? given_index(a, t, lane) : -1;
         float given_x = neg_inf();
         if (in) {
             const auto* x = static_cast<const typename S::Bits*>(a.scores) + t * a.stride;
-            const int64_t v0 = at % waves * span, v1 = min(v0 + span, a.V);
+            const int64_t v0 = part * span, v1 = min(v0 + span, a.V);
             scan_scores<S>(x, a.mask ? a.mask + t * a.mask_stride : nullptr, v0, v1, c2, a.top, lane, rooms[wave], sums,
                            best);
             given_x = given_score<S>(a, t, given);
@@ -480,10 +480,10 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
     const float c = 1.0f / a.temperature, c2 = kLog2e / a.temperature;
     const int64_t G = d_given ? a.G : 0;
     const int K = d_top ? a.top : 0;
-    const int64_t spans = (a.V + span - 1) / span;
+    const uint32_t spans = uint32_t(over(a.V + span - 1, uint32_t(span)));
     for (int64_t item = int64_t(blockIdx.x) * kBackWaves + (threadIdx.x >> 6); item < a.T * spans;
          item += int64_t(gridDim.x) * kBackWaves) {
-        const int64_t t = item / spans, first = (item - t * spans) * span, end = min(first + span, a.V);
+        const int64_t t = over(item, spans), first = (item - t * spans) * span, end = min(first + span, a.V);
         const auto* x = static_cast<const typename S::Bits*>(a.scores) + t * a.stride;
         auto* d = d_scores + t * a.V;
         const uint8_t* mask = a.mask ? a.mask + t * a.mask_stride : nullptr;

@@ -283,18 +283,19 @@ __device__ __forceinline__ void store_values(typename S::Bits* p, int64_t left, 
 template <int KB> struct Places {
     int64_t at[KB];  // first value of the row there
     float w[KB];
-    bool in[KB], real[KB];
+    bool in[KB], real[KB];  // is not dropped; is a choice at all
 };
 template <int KB>
 __device__ __forceinline__ Places<KB> places_of(const RouteArgs& a, int64_t t, int j0, int kept) {
     Places<KB> p;
 #pragma unroll
     for (int u = 0; u < KB; ++u) {
-        p.real[u] = j0 + u < a.k;
         const int64_t s = t * a.k + j0 + u;
-        const int at = p.real[u] ? a.slot[s] : 0;
-        p.in[u] = p.real[u] && at < kept;
-        p.at[u] = int64_t(at) * a.D;
+        p.real[u] = j0 + u < a.k;
+        const uint32_t at = p.real[u] ? uint32_t(a.slot[s]) : 0u, last = uint32_t(a.T * a.k) - 1u;
+        // (a place from elsewhere is read nowhere, and not written outside the sorted rows)
+        p.in[u] = p.real[u] && at < uint32_t(kept) && at <= last;
+        p.at[u] = int64_t(min(at, last)) * a.D;
         p.w[u] = p.real[u] && a.weights ? a.weights[s] : 1.0f;
     }
     return p;
@@ -327,7 +328,7 @@ struct RowItem {
 template <int W> __device__ __forceinline__ bool row_item(const RouteArgs& a, int64_t item0, int64_t span, int parts, RowItem& r) {
     const int64_t item = item0 + (W == 1 ? __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)) : 0);
     if (item >= a.T * parts) return false;
-    r.t = parts == 1 ? item : item / parts;
+    r.t = parts == 1 ? item : over(item, parts);
     r.d0 = (item - r.t * parts) * span;
     r.d1 = min(r.d0 + span, a.D);
     return true;
@@ -498,7 +499,7 @@ hipError_t move_rows(const RouteArgs& a, const void* in_, void* to_, const void*
     } else if (dot && a.k > 4) {
         if (p.waves == 1) TP_ROWS(k_gather_rows, 1, 8);
         else if (p.waves == 4) TP_ROWS(k_gather_rows, 4, 8);
-        else TP_ROWS(k_gather_rows, 16, 8);
+        else TP_ROWS(k_gather_rows, 16, 4);  // (8 do not fit its registers)
     } else {
         if (p.waves == 1) TP_ROWS_BY_K(k_gather_rows, 1);
         else if (p.waves == 4) TP_ROWS_BY_K(k_gather_rows, 4);

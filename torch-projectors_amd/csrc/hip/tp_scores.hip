@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256) void k_quantize(const typename S::Bits* __rest
     const int part = threadIdx.x & 15;
     const uint32_t span = (nb + 15) / 16;  // workgroups of a row
     for (int64_t g = blockIdx.x; g < srows * span; g += gridDim.x) {
-        const int64_t r = g / span, b = (g - r * span) * 16 + (threadIdx.x >> 4);
+        const int64_t r = over(g, span), b = (g - r * span) * 16 + (threadIdx.x >> 4);
         if (b >= nb) continue;
         if (r >= rows) {  // the padding rows' scales
             if (part == 0) scales[b * srows + r] = 127;
@@ -162,9 +162,7 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
     __shared__ float sums[kFewWaves][FM * 16][16];
     __shared__ __attribute__((aligned(16))) uint8_t codes[kOne ? kFewWaves : 1][kOne ? kAhead : 1][kScaleBlock];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q = lane >> 4;
-    const uint32_t groups = uint32_t((g.N + 15) / 16), split = blockIdx.x / groups;
-    const int64_t n0 = int64_t(blockIdx.x % groups) * 16, K = int64_t(g.nb) * kScaleBlock;
-    const int k0 = g.first(split), k1 = g.first(split + 1);
+    const int64_t n0 = int64_t(blockIdx.x) * 16, K = int64_t(g.nb) * kScaleBlock;
     // rows past the end read the last one's codes and are not stored
     const int64_t bn = min(n0 + r, g.N - 1);
     const uint8_t* pb = g.b + bn * K + q * 16;
@@ -179,13 +177,13 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
         sa[f] = kOne ? nullptr : g.sa + am;
         acc[f] = v4f{0, 0, 0, 0};
     }
-    for (int k = k0 + wave; k < k1; k += kFewWaves * kAhead) {
+    for (int k = wave; k < g.nb; k += kFewWaves * kAhead) {
         int4 cb[kAhead][2], ca[kAhead][FM][2];
         uint32_t eb[kAhead], ea[kAhead][FM];
         float image[kOne ? kAhead : 1][2];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int64_t at = min(k + u * kFewWaves, k1 - 1);
+            const int64_t at = min(k + u * kFewWaves, g.nb - 1);
 #pragma unroll
             for (int h = 0; h < 2; ++h) cb[u][h] = *reinterpret_cast<const int4*>(pb + at * kScaleBlock + h * 64);
             eb[u] = sb[at * g.srb];
@@ -226,7 +224,7 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            if (k + u * kFewWaves >= k1) break;
+            if (k + u * kFewWaves >= g.nb) break;
             const float fb = scale_of(eb[u]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -252,7 +250,7 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
         float v = 0;
 #pragma unroll
         for (int w = 0; w < kFewWaves; ++w) v += sums[w][m][i & 15];
-        store_score<O>(g, split, m, n, v);
+        store_score<O>(g, 0, m, n, v);
     }
 }
 
@@ -336,9 +334,10 @@ __device__ __forceinline__ void tile_step(const uint8_t* __restrict__ ca, const 
     }
 }
 
-// Wait until this wavefront's loads to LDS have arrived, then for the other wavefronts.
+// Wait until this wavefront's loads to LDS have arrived, and its reads of the stage that is filled next, then for the
+// other wavefronts.
 __device__ __forceinline__ void stage_ready() {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -506,7 +505,7 @@ int64_t block_scores_work(int64_t M, int64_t N, int64_t nb) {
 
 template <class O> hipError_t scores(const ScoreArgs& g, const ScorePlan& p, hipStream_t s) {
     if (p.few) {
-        const dim3 grid(unsigned((g.N + 15) / 16) * p.splits);
+        const dim3 grid(unsigned((g.N + 15) / 16));
         if (p.few == 1)
             k_scores_few<1, O, void><<<grid, 64 * kFewWaves, 0, s>>>(g, OneImage{});
         else
@@ -536,8 +535,8 @@ hipError_t launch_block_scores(const void* a, const void* sa, int64_t M, const v
     return out_dt == TP_F32 ? scores<F32>(g, p, s) : scores<BF16>(g, p, s);
 }
 
-// One image is quantised by k_scores_few itself: 256 references of 4224 values 7.6 us in two launches, 5.4 in
-// one; 4096 of 16640 18.5 and 16.0.
+// One image is quantised by k_scores_few itself: 256 references of 4224 values 7.6 us in two launches, 5.9 in
+// one; 4096 of 16640 18.5 and 14.8.
 int64_t score_images_work(int64_t M, int64_t N, int64_t cols) {
     if (M == 1) return 0;
     const int64_t nb = block_count(cols);
