@@ -288,19 +288,20 @@ template <int F> __device__ __forceinline__ void scales_of(const uint32_t* words
 
 using v16f = __attribute__((ext_vector_type(16))) float;
 
-template <int FM, int FN>
-__device__ __forceinline__ void tile_step(const uint8_t* __restrict__ ca, const uint8_t* __restrict__ cb, int key,
+// NT quarters of a block from quarter t0 on.  fill starts the loads of the next block: its instructions go where the
+// first operands are on their way from LDS.
+template <int FM, int FN, int NT, class Fill>
+__device__ __forceinline__ void tile_step(const uint8_t* __restrict__ ca, const uint8_t* __restrict__ cb, int t0, int key,
                                           int q, const uint32_t* __restrict__ sa, const uint32_t* __restrict__ sb,
-                                          int ra0, int rb0, v16f (&acc)[FM][FN]) {
+                                          int ra0, int rb0, v16f (&acc)[FM][FN], Fill fill) {
     float ea[FM], eb[FN];
     scales_of<FM>(sa, ra0, ea);
     scales_of<FN>(sb, rb0, eb);
-    // operands of one quarter of the block are read from LDS while the one before is multiplied, or, where
-    // there are registers for it, all at once
-    constexpr int D = FM + FN <= 4 ? 4 : 2;
+    // of a whole block the operands of one quarter are read from LDS while the one before is multiplied
+    constexpr int D = NT <= 2 ? 1 : 2;
     int4 ra[D][FM], rb[D][FN];
     auto read = [&](int t) {
-        const int at = ((2 * t + q) ^ key) * 16;
+        const int at = ((2 * (t0 + t) + q) ^ key) * 16;
 #pragma unroll
         for (int f = 0; f < FM; ++f) ra[t % D][f] = *reinterpret_cast<const int4*>(ca + f * kScaleBlock + at);
 #pragma unroll
@@ -309,8 +310,9 @@ __device__ __forceinline__ void tile_step(const uint8_t* __restrict__ ca, const 
 #pragma unroll
     for (int t = 0; t < D - 1; ++t) read(t);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        if (t + D - 1 < 4) read(t + D - 1);
+    for (int t = 0; t < NT; ++t) {
+        if (t + D - 1 < NT) read(t + D - 1);
+        if (t == 0) fill();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             v8bf fa[FM], fb[FN];
@@ -330,7 +332,7 @@ __device__ __forceinline__ void tile_step(const uint8_t* __restrict__ ca, const 
                 for (int j = 0; j < FN; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
         }
-        if (D == 2) __builtin_amdgcn_sched_barrier(0);
+        if (NT > 2) __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -345,14 +347,17 @@ __device__ __forceinline__ void stage_ready() {
 
 // A wavefront's rows of 32 x 32 fragments lie F apart (fragment f has rows F r + f), so that one load brings
 // the scales of a lane's rows and a lane's F columns are neighbours in the output.
-template <int BM, int BN, int WM, int WN, class O>
-__global__ __launch_bounds__(64 * WM * WN) void k_scores_tile(ScoreArgs g, uint32_t tm, uint32_t tn) {
-    constexpr int W = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
+// KW > 1: as many wavefronts share a part of the tile, each with its quarters of every block, so that no value is
+// widened twice; their sums are added in LDS at the end.
+// (tiles of 128 x 128 keep to 128 registers: two workgroups of 8 wavefronts per CU)
+template <int BM, int BN, int WM, int WN, int KW, class O>
+__global__ __launch_bounds__(64 * WM * WN * KW, BM * BN == 128 * 128 ? 4 : 1) void k_scores_tile(ScoreArgs g, uint32_t tm, uint32_t tn) {
+    constexpr int W = WM * WN * KW, FM = BM / WM / 32, FN = BN / WN / 32;
     constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // loads of a wavefront for a stage
     static_assert(LA * W * 8 == BM && LB * W * 8 == BN, "whole loads");
     __shared__ Stage<BM, BN> stages[2];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, q = lane >> 5;
-    const int wm = wave / WN, wn = wave % WN;
+    const int kw = wave % KW, wm = wave / KW / WN, wn = wave / KW % WN;
     // workgroups are dealt to the XCDs in turn: each XCD takes a contiguous run of the items, whose tiles
     // share rows and columns in its L2
     const uint32_t items = gridDim.x, x = blockIdx.x & 7, per = items >> 3, more = items & 7;
@@ -392,23 +397,59 @@ __global__ __launch_bounds__(64 * WM * WN) void k_scores_tile(ScoreArgs g, uint3
     // two stages in turn: while one is multiplied the other is filled (three and four were no faster: a
     // stage's loads take less than its products, and the LDS holds fewer workgroups)
     const int lane4 = lane * 4;
+    const uint8_t *sa = g.sa + k0 * g.sra + m0, *sb = g.sb + k0 * g.srb + n0;  // the next block's scales
     auto load = [&](Stage<BM, BN>& st, int k) {
         to_lds(ga, oa, k * kScaleBlock, st.a + wave * LA * 1024);
         to_lds(gb, ob, k * kScaleBlock, st.b + wave * LB * 1024);
         // (every wavefront brings all scales: the same bytes to the same place)
-        const auto sa = codes_buffer(g.sa + k * g.sra + m0, 1, g.sra - m0);
-        const auto sb = codes_buffer(g.sb + k * g.srb + n0, 1, g.srb - n0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(sa, (LocalPtr)st.sa, 4, lane4, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (LocalPtr)st.sb, 4, lane4, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(codes_buffer(sa, 1, g.sra - m0), (LocalPtr)st.sa, 4, lane4, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(codes_buffer(sb, 1, g.srb - n0), (LocalPtr)st.sb, 4, lane4, 0, 0, 0);
+        sa += g.sra;
+        sb += g.srb;
     };
     load(stages[0], k0);
 #pragma unroll 1
     for (int k = k0; k < k1; ++k) {
         const int cur = (k - k0) & 1;
         stage_ready();
-        if (k + 1 < k1) load(stages[cur ^ 1], k + 1);
         const Stage<BM, BN>& st = stages[cur];
-        tile_step<FM, FN>(st.a + ra * kScaleBlock, st.b + rb * kScaleBlock, r & 7, q, st.sa, st.sb, ra, rb, acc);
+        tile_step<FM, FN, 4 / KW>(st.a + ra * kScaleBlock, st.b + rb * kScaleBlock, kw * (4 / KW), r & 7, q, st.sa, st.sb,
+                                  ra, rb, acc, [&] {
+                                      if (k + 1 < k1) load(stages[cur ^ 1], k + 1);
+                                  });
+    }
+
+    // a wavefront's share of its part's results: elements e0 .. e0 + EN - 1 of each fragment
+    constexpr int EN = 16 / KW;
+    const int e0 = kw * EN;
+    float sum[FM][FN][EN];
+    if constexpr (KW == 1) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < EN; ++e) sum[i][j][e] = acc[i][j][e];
+    } else {
+        float* room = reinterpret_cast<float*>(stages);
+        static_assert(sizeof(stages) >= size_t(W) * 4096, "a fragment of every wavefront");
+        const float* part = room + (wave - kw) * 1024 + e0 * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) room[wave * 1024 + e * 64 + lane] = acc[i][j][e];
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < EN; ++e) {
+                    float v = part[e * 64];
+#pragma unroll
+                    for (int w = 1; w < KW; ++w) v += part[w * 1024 + e * 64];
+                    sum[i][j][e] = v;
+                }
+            }
     }
 
     const int64_t n = n0 + rb;
@@ -419,22 +460,23 @@ __global__ __launch_bounds__(64 * WM * WN) void k_scores_tile(ScoreArgs g, uint3
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int64_t m = m0 + (wm * 32 + (e / 4) * 8 + q * 4 + e % 4) * FM + i;
+        for (int e = 0; e < EN; ++e) {
+            const int at_e = e0 + e;
+            const int64_t m = m0 + (wm * 32 + (at_e / 4) * 8 + q * 4 + at_e % 4) * FM + i;
             if (m >= g.M) continue;
             if (!whole) {
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
-                    if (n + j < g.N) store_score<O>(g, split, m, n + j, acc[i][j][e]);
+                    if (n + j < g.N) store_score<O>(g, split, m, n + j, sum[i][j][e]);
             } else if (g.splits > 1) {
                 float v[FN];
 #pragma unroll
-                for (int j = 0; j < FN; ++j) v[j] = acc[i][j][e];
+                for (int j = 0; j < FN; ++j) v[j] = sum[i][j][e];
                 __builtin_memcpy(g.part + (int64_t(split) * g.M + m) * g.N + n, v, sizeof v);
             } else {
                 typename O::Bits v[FN];
 #pragma unroll
-                for (int j = 0; j < FN; ++j) v[j] = O::round(acc[i][j][e] + off[j]);
+                for (int j = 0; j < FN; ++j) v[j] = O::round(sum[i][j][e] + off[j]);
                 __builtin_memcpy(static_cast<typename O::Bits*>(g.out) + m * g.N + n, v, sizeof v);
             }
         }
@@ -444,8 +486,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_scores_tile(ScoreArgs g, uint3
 // Few images: k_scores_few.  Else the tile and the number of ranges of the blocks with the least time by a
 // count of steps (one block of K for one tile).  A CU with n workgroups of a tile takes n step_us for a step
 // of each, but no less than alone_us: one workgroup alone waits for LDS and for its own products.  Measured:
-// 4096 x 8192 x 16640 (full CUs) 64: 1283 us, 128: 997, 256: 869; 333 x 1999 x 8280 64: 36, 128: 75, 256: 175
-// us in one range, 29, 33 and 64 in four.  Several ranges cost a launch and their sums written and read.
+// 4096 x 8192 x 16640 (full CUs) 64: 1160 us, 128: 910, 256: 810; 2000 x 2000 x 4224 48, 42 and 100; 333 x 1999 x
+// 8280 in one range 38, 63 and 175 us, in four 26, 29 and 63.  Several ranges cost a launch and their sums written
+// and read.  Against every tile and 1 to 16 ranges on 25 sizes from 33 x 8192 to 4096 x 8192 the choice is within
+// 7 % of the best.
 struct ScorePlan {
     int few, tile, splits;  // few: FM of k_scores_few, or 0; tile: index of kTiles
 };
@@ -453,7 +497,7 @@ struct TileKind {
     int bm, bn;
     double step_us, alone_us;
 };
-constexpr TileKind kTiles[] = {{64, 64, 0.31, 0.48}, {128, 128, 0.96, 1.1}, {256, 256, 3.3, 2.5}};
+constexpr TileKind kTiles[] = {{64, 64, 0.28, 0.50}, {128, 128, 0.87, 1.0}, {256, 256, 3.1, 2.6}};
 constexpr int kCus = 256, kMaxSplits = 16;
 
 ScorePlan score_plan(int64_t M, int64_t N, int64_t nb) {
@@ -515,11 +559,11 @@ template <class O> hipError_t scores(const ScoreArgs& g, const ScorePlan& p, hip
         const uint32_t tm = uint32_t((g.M + kind.bm - 1) / kind.bm), tn = uint32_t((g.N + kind.bn - 1) / kind.bn);
         const dim3 grid(tm * tn * p.splits);
         if (p.tile == 0)
-            k_scores_tile<64, 64, 2, 2, O><<<grid, 256, 0, s>>>(g, tm, tn);
+            k_scores_tile<64, 64, 1, 1, 4, O><<<grid, 256, 0, s>>>(g, tm, tn);
         else if (p.tile == 1)
-            k_scores_tile<128, 128, 2, 2, O><<<grid, 256, 0, s>>>(g, tm, tn);
+            k_scores_tile<128, 128, 2, 2, 2, O><<<grid, 512, 0, s>>>(g, tm, tn);
         else
-            k_scores_tile<256, 256, 2, 4, O><<<grid, 512, 0, s>>>(g, tm, tn);
+            k_scores_tile<256, 256, 2, 4, 1, O><<<grid, 512, 0, s>>>(g, tm, tn);
     }
     if (hipError_t e = hipGetLastError()) return e;
     if (p.splits > 1) k_scores_join<O><<<match_grid((g.M * g.N + 255) / 256), 256, 0, s>>>(g);
