@@ -255,9 +255,10 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 }
 
 // The product in tiles: a workgroup of WM x WN wavefronts computes BM x BN scores.
-// Codes of one block of a tile's rows in LDS: 128 bytes a row, whose 16-byte chunks are permuted among
-// themselves (chunk c of row r at place c ^ key(r)), so that the eight lanes that read one chunk of eight
-// rows reach all banks.
+// Codes of one block of a tile's rows in LDS: 128 bytes a row, fragment after fragment (fragment f of a part of
+// the tile has its rows F r + f, r < 32), and the 16-byte chunks of a row permuted among themselves (chunk c of row
+// r of a fragment at place c ^ ((r / 2) & 7)), so that the 16 lanes that read one chunk of 16 rows at a time reach
+// each of the 64 banks once.
 template <int BM, int BN> struct alignas(16) Stage {
     uint8_t a[BM * kScaleBlock], b[BN * kScaleBlock];
     uint32_t sa[64], sb[64];  // scale bytes (the first BM and BN are used)
@@ -303,9 +304,9 @@ __device__ __forceinline__ void tile_step(const uint8_t* __restrict__ ca, const 
     auto read = [&](int t) {
         const int at = ((2 * (t0 + t) + q) ^ key) * 16;
 #pragma unroll
-        for (int f = 0; f < FM; ++f) ra[t % D][f] = *reinterpret_cast<const int4*>(ca + f * kScaleBlock + at);
+        for (int f = 0; f < FM; ++f) ra[t % D][f] = *reinterpret_cast<const int4*>(ca + f * 32 * kScaleBlock + at);
 #pragma unroll
-        for (int f = 0; f < FN; ++f) rb[t % D][f] = *reinterpret_cast<const int4*>(cb + f * kScaleBlock + at);
+        for (int f = 0; f < FN; ++f) rb[t % D][f] = *reinterpret_cast<const int4*>(cb + f * 32 * kScaleBlock + at);
     };
 #pragma unroll
     for (int t = 0; t < D - 1; ++t) read(t);
@@ -372,16 +373,14 @@ __global__ __launch_bounds__(64 * WM * WN * KW, BM * BN == 128 * 128 ? 4 : 1) vo
 
     uint32_t oa[LA], ob[LB];
     const int row8 = lane >> 3, place = lane & 7;
+    auto offset = [&](int slot, int F) {  // of a row's place in LDS and this lane's chunk there
+        const int r = slot & 31, f = (slot >> 5) % F, part = (slot >> 5) / F;
+        return uint32_t(((part * 32 + r) * F + f) * K) + (place ^ ((r >> 1) & 7)) * 16;
+    };
 #pragma unroll
-    for (int i = 0; i < LA; ++i) {
-        const int row = (wave * LA + i) * 8 + row8;
-        oa[i] = uint32_t(row * K) + (place ^ ((row / FM) & 7)) * 16;
-    }
+    for (int i = 0; i < LA; ++i) oa[i] = offset((wave * LA + i) * 8 + row8, FM);
 #pragma unroll
-    for (int i = 0; i < LB; ++i) {
-        const int row = (wave * LB + i) * 8 + row8;
-        ob[i] = uint32_t(row * K) + (place ^ ((row / FN) & 7)) * 16;
-    }
+    for (int i = 0; i < LB; ++i) ob[i] = offset((wave * LB + i) * 8 + row8, FN);
     // rows past the end read zeros
     const auto ga = codes_buffer(g.a + m0 * K, min(int64_t(BM), g.M - m0), K);
     const auto gb = codes_buffer(g.b + n0 * K, min(int64_t(BN), g.N - n0), K);
@@ -413,8 +412,8 @@ __global__ __launch_bounds__(64 * WM * WN * KW, BM * BN == 128 * 128 ? 4 : 1) vo
         const int cur = (k - k0) & 1;
         stage_ready();
         const Stage<BM, BN>& st = stages[cur];
-        tile_step<FM, FN, 4 / KW>(st.a + ra * kScaleBlock, st.b + rb * kScaleBlock, kw * (4 / KW), r & 7, q, st.sa, st.sb,
-                                  ra, rb, acc, [&] {
+        tile_step<FM, FN, 4 / KW>(st.a + (wm * 32 * FM + r) * kScaleBlock, st.b + (wn * 32 * FN + r) * kScaleBlock,
+                                  kw * (4 / KW), (r >> 1) & 7, q, st.sa, st.sb, ra, rb, acc, [&] {
                                       if (k + 1 < k1) load(stages[cur ^ 1], k + 1);
                                   });
     }
