@@ -297,9 +297,10 @@ int tp_normalize_reconstruction(int dtype, const void* data, const void* weights
  * What a caller does between projecting references and backprojecting images:
  * scores of images against references, posteriors over the scored hypotheses,
  * and images in class order.  No counterpart in the reference.  `work` is
- * device memory of at least the matching tp_*_work() bytes (16-byte aligned,
- * uninitialised, free again once the call's work on the stream is done; it may
- * be NULL where that is 0). */
+ * device memory of at least the matching tp_*_work() bytes (uninitialised,
+ * free again once the call's work on the stream is done; it may be NULL where
+ * that is 0).  work, codes, scales and stats are 16-byte aligned, everything
+ * else as its type. */
 
 /* Rows in 8-bit blocks: x [rows, cols] (TP_F32, TP_F16 or TP_BF16; rows
  * `row_stride` elements apart, values of a row adjacent) becomes

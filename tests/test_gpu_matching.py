@@ -581,3 +581,42 @@ def test_one_image_of_every_type(m):
             assert torch.equal(got, m.block_scores(m.quantize_blocks(x.to(DEV)), refs, out_dtype=out))
         x[0, 300] = math.nan
         assert m.block_scores(x.to(DEV), refs).isnan().all()
+
+
+def test_views_that_hold_other_values(m):
+    """Negative and conjugate views count as what they show, in values, weights and upstream gradients."""
+    g = gen(41)
+    c = torch.randn(6, 40, dtype=torch.complex64, generator=g).to(DEV)
+    view = c.conj().imag
+    plain = view.resolve_neg().contiguous()
+    assert view.is_neg() and not plain.is_neg()
+    for a, b in zip(m.log_probs(view, top=3), m.log_probs(plain, top=3)):
+        assert a is b is None or torch.equal(a, b)
+    x, y = (v.detach().requires_grad_() for v in (view, plain))
+    up = torch.randn(6, dtype=torch.complex64, generator=g).to(DEV).conj().imag
+    dx, = torch.autograd.grad(m.log_probs(x).entropy, x, up)
+    dy, = torch.autograd.grad(m.log_probs(y).entropy, y, up.resolve_neg())
+    assert torch.equal(dx, dy)
+    q, r = m.quantize_blocks(view), m.quantize_blocks(plain)
+    assert torch.equal(q.codes.view(torch.uint8), r.codes.view(torch.uint8)) and torch.equal(q.scales, r.scales)
+    bias = torch.randn(6, dtype=torch.complex64, generator=g).to(DEV).conj().imag
+    assert torch.equal(m.block_scores(view, r, bias=bias), m.block_scores(plain, r, bias=bias.resolve_neg()))
+    order = m.sort_by_class(torch.randint(0, 3, (6, 2), generator=g).to(DEV), 3)
+    w = torch.randn(6, 2, dtype=torch.complex64, generator=g).to(DEV).conj().imag
+    s = m.dispatch(plain, order, w.resolve_neg())
+    assert torch.equal(m.dispatch(view, order, w), s)
+    assert torch.equal(m.combine(-(-s), order, w), m.combine(s, order, w.resolve_neg()))
+    assert torch.equal(m.dispatch(c.conj(), order, w), m.dispatch(c.conj().resolve_conj(), order, w.resolve_neg()))
+
+
+def test_blocks_from_any_address(m):
+    g = gen(42)
+    x = torch.randn(40, 300, generator=g).to(DEV)
+    q = m.quantize_blocks(torch.randn(70, 300, generator=g).to(DEV))
+    moved = []
+    for t in q:
+        room = torch.empty(t.numel() + 3, dtype=torch.uint8, device=DEV)[3:]
+        room.copy_(t.view(torch.uint8).flatten())
+        moved.append(room.view(t.dtype).view(t.shape))
+    assert moved[0].data_ptr() % 16
+    assert torch.equal(m.block_scores(x, m.BlockScaled(*moved)), m.block_scores(x, q))

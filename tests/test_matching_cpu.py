@@ -105,6 +105,25 @@ def test_c_abi_refuses_before_anything_is_enqueued(name, good, bad):
         _refused(name, list({**good, **change}.values()), msg)
 
 
+ODD = _P(264)
+
+
+@pytest.mark.parametrize("name,args,places", [
+    ("tp_quantize_blocks", [0, A, 2, 3, 3, A, A, NULL], {5: "codes", 6: "scales"}),
+    ("tp_block_scores", [A, A, 2, A, A, 3, 1, NULL, 0, A, A, 1 << 40, NULL],
+     {0: "codes_a", 1: "scales_a", 3: "codes_b", 4: "scales_b", 10: "work"}),
+    ("tp_score_images", [0, A, 2, 200, 200, A, A, 3, NULL, 4, A, A, 1 << 40, NULL],
+     {5: "codes_b", 6: "scales_b", 11: "work"}),
+    ("tp_log_probs", [0, A, 2, 3, 3, NULL, 0, NULL, 0, 1, 1.0, A, A, A, A, A, A, A, 1 << 40, NULL],
+     {16: "stats", 17: "work"}),
+    ("tp_log_probs_back", [0, A, 2, 3, 3, NULL, 0, NULL, 0, 1, 1.0, A, A, NULL, NULL, NULL, A, A, NULL], {12: "stats"}),
+    ("tp_sort_by_class", [8, A, 4, 3, A, A, A, A, 1 << 40, NULL], {7: "work"}),
+])
+def test_c_abi_refuses_what_is_not_aligned(name, args, places):
+    for i, what in places.items():
+        _refused(name, [*args[:i], ODD, *args[i + 1:]], f"{what} must be 16-byte aligned")
+
+
 def test_c_abi_refuses_small_workspaces():
     M, N, nb = 1, 16, 130
     need = capi.lib().tp_block_scores_work(M, N, nb)

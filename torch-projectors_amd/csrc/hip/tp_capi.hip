@@ -448,6 +448,10 @@ int need(const void* p, const char* name) {
     if (!p) return fail(std::string(name) + " must not be NULL");
     return TP_OK;
 }
+// What kernels read or write 16 bytes at a time from its first byte on.
+int aligned16(const void* p, const char* name) {
+    return reinterpret_cast<uintptr_t>(p) % 16 ? fail(std::string(name) + " must be 16-byte aligned") : TP_OK;
+}
 
 #define TP_TRY(expr)                 \
     do {                             \
@@ -1378,6 +1382,8 @@ int tp_quantize_blocks(int dtype, const void* x, int64_t rows, int64_t cols, int
     TP_TRY(need(x, "x"));
     TP_TRY(need(codes, "codes"));
     TP_TRY(need(scales, "scales"));
+    TP_TRY(aligned16(codes, "codes"));
+    TP_TRY(aligned16(scales, "scales"));
     return launched(tp::launch_quantize_blocks(dtype, x, rows, cols, row_stride, codes, scales,
                                                static_cast<hipStream_t>(stream)),
                     "quantisation launch");
@@ -1404,6 +1410,11 @@ int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, c
     TP_TRY(need(codes_b, "codes_b"));
     TP_TRY(need(scales_b, "scales_b"));
     TP_TRY(need(scores, "scores"));
+    TP_TRY(aligned16(codes_a, "codes_a"));
+    TP_TRY(aligned16(scales_a, "scales_a"));
+    TP_TRY(aligned16(codes_b, "codes_b"));
+    TP_TRY(aligned16(scales_b, "scales_b"));
+    TP_TRY(aligned16(work, "work"));
     const int64_t need_bytes = tp::block_scores_work(rows_a, rows_b, blocks);
     if (need_bytes) TP_TRY(need(work, "work"));
     if (work_bytes < need_bytes) return fail("work is smaller than tp_block_scores_work");
@@ -1433,6 +1444,9 @@ int tp_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, int6
     TP_TRY(need(codes_b, "codes_b"));
     TP_TRY(need(scales_b, "scales_b"));
     TP_TRY(need(scores, "scores"));
+    TP_TRY(aligned16(codes_b, "codes_b"));
+    TP_TRY(aligned16(scales_b, "scales_b"));
+    TP_TRY(aligned16(work, "work"));
     const int64_t need_bytes = tp::score_images_work(rows_a, rows_b, cols);
     if (need_bytes) TP_TRY(need(work, "work"));
     if (work_bytes < need_bytes) return fail("work is smaller than tp_score_images_work");
@@ -1463,6 +1477,8 @@ int tp_log_probs(int dtype, const void* scores, int64_t rows, int64_t candidates
         TP_TRY(need(top_log_probs, "top_log_probs"));
         TP_TRY(need(top_index, "top_index"));
     }
+    TP_TRY(aligned16(stats, "stats"));
+    TP_TRY(aligned16(work, "work"));
     const int64_t need_bytes = tp::log_probs_work(rows, candidates, int(top));
     if (need_bytes) TP_TRY(need(work, "work"));
     if (work_bytes < need_bytes) return fail("work is smaller than tp_log_probs_work");
@@ -1484,6 +1500,7 @@ int tp_log_probs_back(int dtype, const void* scores, int64_t rows, int64_t candi
     if (rows == 0) return TP_OK;
     TP_TRY(need(scores, "scores"));
     TP_TRY(need(stats, "stats"));
+    TP_TRY(aligned16(stats, "stats"));
     TP_TRY(need(d_scores, "d_scores"));
     if (d_top && top) TP_TRY(need(top_index, "top_index"));
     return launched(tp::launch_log_probs_back(a, static_cast<const float*>(stats),
@@ -1512,6 +1529,7 @@ int tp_sort_by_class(int id_bytes, const void* class_ids, int64_t slots, int64_t
         TP_TRY(need(order, "order"));
         TP_TRY(need(slot, "slot"));
     }
+    TP_TRY(aligned16(work, "work"));
     const int64_t need_bytes = tp_sort_by_class_work(slots, classes);
     if (need_bytes) TP_TRY(need(work, "work"));
     if (work_bytes < need_bytes) return fail("work is smaller than tp_sort_by_class_work");

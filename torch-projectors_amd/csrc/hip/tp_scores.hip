@@ -60,7 +60,8 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], int e) {
     return uint2{c[0], c[1]};
 }
 
-// 16 lanes per block of a row, eight values each.  Memory bound: reads each value once, writes a byte for it.
+// 16 lanes per block of a row, eight values each.  Memory bound: reads each value once, writes a byte for it
+// (4096 x 16640 fp32 in 61 us, 5.6 TB/s).
 template <class S>
 __global__ __launch_bounds__(256) void k_quantize(const typename S::Bits* __restrict__ x, int64_t rows, int64_t cols,
                                                   int64_t stride, int nb, int64_t srows, uint8_t* __restrict__ codes,
@@ -146,7 +147,8 @@ template <class O> __global__ __launch_bounds__(256) void k_scores_join(ScoreArg
 
 // Few images (at most 16 FM): as fast as the references' codes can be read.  A workgroup takes 16 references,
 // each of its wavefronts every eighth block of them, straight from memory into operands: kAhead blocks'
-// loads are in flight at once (8 KB a wavefront, 64 KB a CU).
+// loads are in flight at once (8 KB a wavefront, 64 KB a CU).  One image against 4096 references of 16640
+// values: 14.8 us, 4.7 TB/s.
 constexpr int kFewWaves = 8, kAhead = 4;
 
 // A row that a wavefront quantises itself, block by block: no launch and no memory for its codes.
@@ -254,7 +256,9 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
     }
 }
 
-// The product in tiles: a workgroup of WM x WN wavefronts computes BM x BN scores.
+// The product in tiles: a workgroup of WM x WN x KW wavefronts computes BM x BN scores.  4096 x 8192 x 16640 by
+// tiles of 256 x 256 takes 810 to 850 us (1.31 to 1.38 PFLOP/s, the rate of a bfloat16 library product on this
+// card): the matrix units are busy for two thirds of the cycles, at a clock that the power limit holds at 1.9 GHz.
 // Codes of one block of a tile's rows in LDS: 128 bytes a row, fragment after fragment (fragment f of a part of
 // the tile has its rows F r + f, r < 32), and the 16-byte chunks of a row permuted among themselves (chunk c of row
 // r of a fragment at place c ^ ((r / 2) & 7)), so that the 16 lanes that read one chunk of 16 rows at a time reach
@@ -580,10 +584,12 @@ hipError_t launch_block_scores(const void* a, const void* sa, int64_t M, const v
 
 // One image is quantised by k_scores_few itself: 256 references of 4224 values 7.6 us in two launches, 5.9 in
 // one; 4096 of 16640 18.5 and 14.8.
+// (the sums of the product's ranges, then codes and scales from a 16-byte boundary on)
+int64_t sums_before_codes(int64_t M, int64_t N, int64_t nb) { return (block_scores_work(M, N, nb) + 15) / 16 * 16; }
 int64_t score_images_work(int64_t M, int64_t N, int64_t cols) {
     if (M == 1) return 0;
     const int64_t nb = block_count(cols);
-    return M * nb * kScaleBlock + nb * scale_rows(M) + block_scores_work(M, N, nb);
+    return sums_before_codes(M, N, nb) + M * nb * kScaleBlock + nb * scale_rows(M);
 }
 
 template <class S> hipError_t score_one(const ScoreArgs& g, const OneImage& one, int out_dt, hipStream_t s) {
@@ -606,9 +612,8 @@ hipError_t launch_score_images(int dt, const void* x, int64_t M, int64_t cols, i
         return dt == TP_F32 ? score_one<F32>(g, one, out_dt, s) : dt == TP_F16 ? score_one<F16>(g, one, out_dt, s)
                                                                                : score_one<BF16>(g, one, out_dt, s);
     }
-    // the sums of the product's ranges first: they are aligned most
     auto* part = static_cast<char*>(work);
-    auto* codes = part + block_scores_work(M, N, nb);
+    auto* codes = part + sums_before_codes(M, N, nb);
     auto* scales = codes + M * nb * kScaleBlock;
     if (hipError_t e = launch_quantize_blocks(dt, x, M, cols, stride, codes, scales, s)) return e;
     return launch_block_scores(codes, scales, M, b, sb, N, nb, bias, out_dt, out, part, s);

@@ -43,9 +43,7 @@ def _real_rows(x, what):
     if x.dim() < 1:
         raise ValueError(f"{what} must have at least 1 dimension")
     if x.is_complex():
-        x = torch.view_as_real(x.resolve_conj())
-    elif x.is_neg():
-        x = x.resolve_neg()
+        x = torch.view_as_real(x.resolve_conj().resolve_neg())
     return x if x.dim() == 2 else x.reshape(x.shape[0], _numel(x.shape[1:]))
 
 
