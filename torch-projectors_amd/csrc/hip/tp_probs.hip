@@ -89,23 +89,20 @@ constexpr int kTileScores = 64 * kLaneScores;
 struct alignas(16) Room {
     uint64_t found[kTileScores + 4];  // candidates, then zeros up to the next multiple of 4
     uint64_t keys[64];
-    uint32_t order[64];
 };
 __device__ __forceinline__ void lds_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-// A value that at least k lanes reach: the k-th largest without its last 6 bits.
-__device__ __forceinline__ uint32_t floor_of(uint32_t v, int k, Room& room, int lane) {
-    const uint32_t mine = (v & ~63u) | uint32_t(63 - lane);  // no two are equal
-    room.order[lane] = mine;
-    lds_order();
-    int above = 0;
-#pragma unroll
-    for (int l = 0; l < 64; l += 4) {
-        const uint4 o = *reinterpret_cast<const uint4*>(room.order + l);
-        above += (o.x > mine ? 1 : 0) + (o.y > mine ? 1 : 0) + (o.z > mine ? 1 : 0) + (o.w > mine ? 1 : 0);
+// A value that at least k lanes reach: the k-th largest without its last 12 bits, which two bits at a time are found
+// by counting the lanes that reach each of three values (some 40 cycles a step).
+__device__ __forceinline__ uint32_t floor_of(uint32_t v, int k) {
+    uint32_t f = 0;
+#pragma unroll 1
+    for (int b = 30; b >= 12; b -= 2) {
+        const uint32_t one = f | 1u << b, two = f | 2u << b, three = f | 3u << b;
+        const int n1 = __popcll(__ballot(v >= one)), n2 = __popcll(__ballot(v >= two)), n3 = __popcll(__ballot(v >= three));
+        f = n3 >= k ? three : n2 >= k ? two : n1 >= k ? one : f;
     }
-    lds_order();
-    return read_lane(mine, __ffsll(static_cast<long long>(__ballot(above == k - 1))) - 1) & ~63u;
+    return f;
 }
 // How many of the n keys from p on (zeros after them up to a multiple of 4; p 16-byte aligned) are above `key`.
 __device__ __forceinline__ int above(uint64_t key, const uint64_t* p, int n) {
@@ -114,6 +111,13 @@ __device__ __forceinline__ int above(uint64_t key, const uint64_t* p, int n) {
         const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(p + j), y = *reinterpret_cast<const ulonglong2*>(p + j + 2);
         a += (x.x > key ? 1 : 0) + (x.y > key ? 1 : 0) + (y.x > key ? 1 : 0) + (y.y > key ? 1 : 0);
     }
+    return a;
+}
+// The same of a sorted list of n keys.
+__device__ __forceinline__ int above_in_order(uint64_t key, const uint64_t* p, int n) {
+    int a = 0;
+#pragma unroll 1
+    for (int b = 1 << (31 - __clz(n)); b; b >>= 1) a += a + b <= n && p[min(a + b, n) - 1] > key ? b : 0;
     return a;
 }
 
@@ -127,23 +131,24 @@ struct Best {
     __device__ __forceinline__ void take(int n, int top, Room& room, int lane) {
         if (lane < 4) room.found[n + lane] = 0;
         lds_order();
-        if (top <= 32 && top <= 6 * n + 12) {
+        int i = 0;
+        if (!read_lane(key, 0)) {  // the first ones
+            const uint64_t mine = lane < n ? room.found[lane] : 0;
+            i = min(n, 64);
+            place(mine, above(mine, room.found, i), top, room, lane);
+        }
+        if (i == n) {
+        } else if (top <= 32 && top <= 6 * n + 12) {
             const int step = (64 - top) & ~3;
-            for (int i = 0; i < n; i += step) {
+            for (; i < n; i += step) {
                 const int count = min(step, n - i);
                 const uint64_t mine = lane < top ? key : lane - top < count ? room.found[i + lane - top] : 0;
                 room.keys[lane] = key;
                 lds_order();
-                const int place = above(mine, room.found + i, count) + above(mine, room.keys, top);
-                lds_order();
-                room.keys[lane] = 0;
-                if (mine && place < top) room.keys[place] = mine;
-                lds_order();
-                key = room.keys[lane];
-                lds_order();
+                place(mine, above(mine, room.found + i, count) + above(mine, room.keys, top), top, room, lane);
             }
         } else {
-            for (int i = 0; i < n; i += 64) {
+            for (; i < n; i += 64) {
                 const uint64_t theirs = i + lane < n ? room.found[i + lane] : 0;
                 const uint64_t set = __ballot(theirs > read_lane(key, top - 1));
                 int up = 0, rank = 0, more = 0;
@@ -166,6 +171,16 @@ struct Best {
         }
         const uint64_t last = read_lane(key, top - 1);
         least = last ? score_of(last) : neg_inf();
+    }
+
+    // Each lane's key, unless it is 0, to its place in the list.
+    __device__ __forceinline__ void place(uint64_t mine, int at, int top, Room& room, int lane) {
+        lds_order();
+        room.keys[lane] = 0;
+        if (mine && at < top) room.keys[at] = mine;
+        lds_order();
+        key = room.keys[lane];
+        lds_order();
     }
 };
 
@@ -266,38 +281,46 @@ __device__ __forceinline__ void scan_scores(const typename S::Bits* x, const uin
         }
         const uint64_t lanes = __ballot(most > best.least);
         if (!lanes) continue;
-        const uint32_t floor = __popcll(lanes) > 4 ? floor_of(order_of(most), top, room, lane) : 0;
+        const uint32_t floor = __popcll(lanes) > 4 ? floor_of(order_of(most), top) : 0;
+        const float from = score_of(uint64_t(max(floor, order_of(best.least) + 1)) << 32);  // (past +inf: a NaN)
         int n = 0;
 #pragma unroll
         for (int i = 0; i < kLaneScores; ++i) {
-            const uint32_t o = order_of(f[i]);
-            const bool in = f[i] > best.least && o >= floor;
-            const uint64_t set = __ballot(in);
-            if (in) room.found[n + below(set)] = uint64_t(o) << 32 | uint32_t(~uint32_t(tile_index<S>(v0, lane, i)));
+            const uint64_t set = __ballot(f[i] >= from);
+            if (!set) continue;
+            if (f[i] >= from)
+                room.found[n + below(set)] =
+                    uint64_t(order_of(f[i])) << 32 | uint32_t(~uint32_t(tile_index<S>(v0, lane, i)));
             n += __popcll(set);
         }
         best.take(n, top, room, lane);
     }
 }
 
-// Merge the keys from p on, 1024 at a time, of which a floor is found as in a tile.
-__device__ __forceinline__ void join_keys(Best& best, const uint64_t* p, int count, int top, Room& room, int lane) {
+// Merge the lists of `blocks` parts, `top` keys each, 1024 keys at a time, of which those below a floor are left out:
+// the top-th largest of the lists' first 64 keys (of more lists' first keys, of the lanes' largest).
+__device__ __forceinline__ void join_keys(Best& best, const uint64_t* p, int blocks, int top, Room& room, int lane) {
     constexpr int N = kLaneScores;
+    const int count = blocks * top;
+    uint64_t first = 0;
+    for (int b = lane; b < max(blocks, 64); b += 64) {
+        const int rank = b / blocks;
+        first = max(first, rank < top ? p[(b - rank * blocks) * top + rank] : 0);
+    }
+    uint32_t floor = 0;
     for (int i0 = 0; i0 < count; i0 += 64 * N) {
-        uint64_t k[N], most = 0;
+        uint64_t k[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) k[i] = i0 + i * 64 + lane < count ? p[i0 + i * 64 + lane] : 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) most = max(most, k[i]);
-        const uint32_t floor = floor_of(uint32_t(most >> 32), top, room, lane);
-        const uint64_t last = read_lane(best.key, top - 1);
+        if (i0 == 0) floor = floor_of(uint32_t(first >> 32), top);
+        const uint64_t from = max(read_lane(best.key, top - 1) + 1, uint64_t(floor) << 32);
         int n = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (i0 + i * 64 >= count) break;
-            const bool in = k[i] > last && uint32_t(k[i] >> 32) >= floor;
-            const uint64_t set = __ballot(in);
-            if (in) room.found[n + below(set)] = k[i];
+            const uint64_t set = __ballot(k[i] >= from);
+            if (!set) continue;
+            if (k[i] >= from) room.found[n + below(set)] = k[i];
             n += __popcll(set);
         }
         best.take(n, top, room, lane);
@@ -360,7 +383,6 @@ __global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut 
     __shared__ Sums sums_of[kProbsWaves];
     __shared__ Room rooms[kProbsWaves];
     __shared__ uint64_t keys_of[kProbsWaves * kMaxTop], best_of[kMaxTop];
-    __shared__ int places[kProbsWaves * kMaxTop];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int group = waves < kProbsWaves ? waves : kProbsWaves;  // wavefronts of a row in the workgroup
     const int blocks = waves / group;                             // workgroups of a row
@@ -384,22 +406,19 @@ __global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut 
         if (group > 1) {
             if (lane == 0) sums_of[wave] = sums;
             if (lane < a.top) keys_of[wave * a.top + lane] = best.key;
-            const int keys = kProbsWaves * a.top;
             if (group == kProbsWaves && threadIdx.x < kMaxTop) best_of[threadIdx.x] = 0;
-            if (int(threadIdx.x) < keys) places[threadIdx.x] = 0;
             __syncthreads();
             if (group == kProbsWaves && a.top) {
-                // a key's place among all wavefronts' keys, counted by 2^s lanes
-                const int s = 31 - __clz(kProbsBlock / keys), i = threadIdx.x >> s, p = threadIdx.x & ((1 << s) - 1);
+                // a key's place is the number of keys above it in the eight sorted lists, of which 2^s lanes search
+                // some each
+                const int keys = kProbsWaves * a.top, s = min(31 - __clz(kProbsBlock / keys), 3);
+                const int i = threadIdx.x >> s, p = threadIdx.x & ((1 << s) - 1);
                 const uint64_t mine = i < keys ? keys_of[i] : 0;
-                if (mine) {
-                    int more = 0;
-#pragma unroll 4
-                    for (int j = p; j < keys; j += 1 << s) more += keys_of[j] > mine ? 1 : 0;
-                    atomicAdd(&places[i], more);
-                }
-                __syncthreads();
-                if (mine && p == 0 && places[i] < a.top) best_of[places[i]] = mine;
+                int more = 0;
+                if (mine)
+                    for (int w = p; w < kProbsWaves; w += 1 << s) more += above_in_order(mine, keys_of + w * a.top, a.top);
+                for (int d = 1; d < 1 << s; d <<= 1) more += __shfl_xor(more, d);
+                if (mine && p == 0 && more < a.top) best_of[more] = mine;
                 __syncthreads();
                 best.key = best_of[lane];
             }
@@ -434,7 +453,7 @@ __global__ __launch_bounds__(64) void k_probs_join(ProbsArgs a, ProbsOut o, int 
         const Sums* of = parts.sums + t * blocks;
         Sums sums = lane < blocks ? of[lane] : Sums{neg_inf(), 0.0f, 0.0f};
         Best best;
-        if (a.top) join_keys(best, parts.keys + t * blocks * a.top, blocks * a.top, a.top, room, lane);
+        if (a.top) join_keys(best, parts.keys + t * blocks * a.top, blocks, a.top, room, lane);
         const float given_x = given_score<S>(a, t, given);
         for (int b = lane + 64; b < blocks; b += 64) sums = joined(sums, of[b], c2);
         sums = wave_joined(sums, c2);
