@@ -1070,7 +1070,7 @@ int probs_args(int dtype, const void* scores, int64_t rows, int64_t candidates, 
     if (!(t >= 1e-30f && t <= 1e30f)) return fail("temperature must be in [1e-30, 1e30]");
     if (givens && rows) TP_TRY(need(given, "given"));
     a = tp::ProbsArgs{dtype, scores, rows, candidates, row_stride, static_cast<const int64_t*>(given), givens,
-                      static_cast<const uint8_t*>(mask), mask_stride, int(top), t};
+                      static_cast<const uint8_t*>(mask), mask_stride, int(top), 1.0f / t, 1.44269504088896340736f / t};
     return TP_OK;
 }
 

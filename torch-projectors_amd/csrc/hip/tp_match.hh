@@ -47,7 +47,7 @@ struct ProbsArgs {
     const uint8_t* mask;         // [V] (mask_stride 0) or [T, V]: nonzero is allowed; null: all are
     int64_t mask_stride;
     int top;
-    float temperature;
+    float c, c2;  // 1 and log2 e, over the temperature
 };
 // Statistics of a row that the gradient reads (null where none will): the largest allowed score, ln of the sum of
 // exp((x - largest) / temperature), the entropy, and an unused word.

@@ -78,6 +78,9 @@ template <class T, class F> __device__ __forceinline__ T scanned(T v, T none, F 
 template <class F> __device__ __forceinline__ float reduced(float v, float none, F f) {
     return __uint_as_float(read_lane(__float_as_uint(scanned(v, none, f)), 63));
 }
+template <class F> __device__ __forceinline__ uint32_t reduced(uint32_t v, uint32_t none, F f) {
+    return read_lane(scanned(v, none, f), 63);
+}
 
 // Number of lanes below this one whose bit is set.
 __device__ __forceinline__ int below(uint64_t lanes) {
@@ -92,33 +95,42 @@ struct alignas(16) Room {
 };
 __device__ __forceinline__ void lds_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-// A value that at least k lanes reach: the k-th largest without its last 12 bits, which two bits at a time are found
-// by counting the lanes that reach each of three values (some 40 cycles a step).
-__device__ __forceinline__ uint32_t floor_of(uint32_t v, int k) {
-    uint32_t f = 0;
-#pragma unroll 1
-    for (int b = 30; b >= 12; b -= 2) {
-        const uint32_t one = f | 1u << b, two = f | 2u << b, three = f | 3u << b;
-        const int n1 = __popcll(__ballot(v >= one)), n2 = __popcll(__ballot(v >= two)), n3 = __popcll(__ballot(v >= three));
-        f = n3 >= k ? three : n2 >= k ? two : n1 >= k ? one : f;
+// A value that at least k of the lanes `in` reach, close to the k-th largest: the 12 bits below those that all of
+// them share are found one by one, by counting the lanes that reach a value (0 where they are fewer than k).
+__device__ __forceinline__ uint32_t floor_of(uint32_t v, bool in, int k) {
+    if (__popcll(__ballot(in)) < k) return 0;
+    const uint32_t hi = reduced(in ? v : 0u, 0u, [](uint32_t a, uint32_t b) { return max(a, b); });
+    const uint32_t lo = reduced(in ? v : ~0u, ~0u, [](uint32_t a, uint32_t b) { return min(a, b); });
+    if (hi == lo) return lo;
+    uint32_t bit = 0x80000000u >> __clz(hi ^ lo), f = hi & ~(2 * bit - 1);
+    v = in ? v : 0u;
+#pragma unroll
+    for (int i = 0; i < 12; ++i) {
+        f = __popcll(__ballot(v >= (f | bit))) >= k ? f | bit : f;
+        bit >>= 1;
     }
     return f;
 }
-// How many of the n keys from p on (zeros after them up to a multiple of 4; p 16-byte aligned) are above `key`.
-__device__ __forceinline__ int above(uint64_t key, const uint64_t* p, int n) {
+// How many of the n keys from p on (zeros after them up to a multiple of 4; p 16-byte aligned) are above `key`; U
+// fours of them are on their way at once.
+template <int U = 1> __device__ __forceinline__ int above(uint64_t key, const uint64_t* p, int n) {
     int a = 0;
+#pragma unroll U
     for (int j = 0; j < n; j += 4) {
         const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(p + j), y = *reinterpret_cast<const ulonglong2*>(p + j + 2);
         a += (x.x > key ? 1 : 0) + (x.y > key ? 1 : 0) + (y.x > key ? 1 : 0) + (y.y > key ? 1 : 0);
     }
     return a;
 }
-// The same of a sorted list of n keys.
-__device__ __forceinline__ int above_in_order(uint64_t key, const uint64_t* p, int n) {
-    int a = 0;
+
+// The same of two sorted lists of n keys, one after the other, by searching them.
+__device__ __forceinline__ int above_in_two(uint64_t key, const uint64_t* p, int n) {
+    int a[2] = {};
 #pragma unroll 1
-    for (int b = 1 << (31 - __clz(n)); b; b >>= 1) a += a + b <= n && p[min(a + b, n) - 1] > key ? b : 0;
-    return a;
+    for (int b = 1 << (31 - __clz(n)); b; b >>= 1)
+#pragma unroll
+        for (int l = 0; l < 2; ++l) a[l] += a[l] + b <= n && p[l * n + min(a[l] + b, n) - 1] > key ? b : 0;
+    return a[0] + a[1];
 }
 
 // The best keys of a wavefront, sorted, one per lane below top, and the score of the top-th (-inf while there are
@@ -281,7 +293,7 @@ __device__ __forceinline__ void scan_scores(const typename S::Bits* x, const uin
         }
         const uint64_t lanes = __ballot(most > best.least);
         if (!lanes) continue;
-        const uint32_t floor = __popcll(lanes) > 4 ? floor_of(order_of(most), top) : 0;
+        const uint32_t floor = __popcll(lanes) > 4 ? floor_of(order_of(most), most > best.least, top) : 0;
         const float from = score_of(uint64_t(max(floor, order_of(best.least) + 1)) << 32);  // (past +inf: a NaN)
         int n = 0;
 #pragma unroll
@@ -312,7 +324,7 @@ __device__ __forceinline__ void join_keys(Best& best, const uint64_t* p, int blo
         uint64_t k[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) k[i] = i0 + i * 64 + lane < count ? p[i0 + i * 64 + lane] : 0;
-        if (i0 == 0) floor = floor_of(uint32_t(first >> 32), top);
+        if (i0 == 0) floor = floor_of(uint32_t(first >> 32), first != 0, top);
         const uint64_t from = max(read_lane(best.key, top - 1) + 1, uint64_t(floor) << 32);
         int n = 0;
 #pragma unroll
@@ -346,7 +358,7 @@ template <class S> __device__ __forceinline__ float given_score(const ProbsArgs&
 template <class S>
 __device__ __forceinline__ void write_row(const ProbsArgs& a, const ProbsOut& o, int64_t t, const Sums& sums, uint64_t key,
                                           int64_t given, float given_x, int lane) {
-    const float m = sums.m, c = 1.0f / a.temperature;
+    const float m = sums.m, c = a.c;
     const bool none = m == neg_inf();
     const float ls = m == __builtin_inff() ? __builtin_nanf("") : __builtin_amdgcn_logf(sums.s) * kLn2;  // (s >= 1)
     if (lane == 0) {
@@ -377,20 +389,23 @@ struct Parts {
     uint64_t* keys;  // [T][blocks][top]
 };
 
-// `waves` wavefronts per row: 1, 2, 4, 8, or a multiple of 8 (several workgroups, whose parts are joined).
-template <class S>
-__global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut o, int waves, int64_t span, Parts parts) {
+// `group` wavefronts of a workgroup per row: 1, 2, 4 or 8, and with 8 `blocks` workgroups, whose parts are joined.
+template <class S, int group>
+__global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut o, int blocks, int64_t span, Parts parts) {
+    constexpr int rows = kProbsWaves / group;  // of a workgroup
     __shared__ Sums sums_of[kProbsWaves];
     __shared__ Room rooms[kProbsWaves];
-    __shared__ uint64_t keys_of[kProbsWaves * kMaxTop], best_of[kMaxTop];
+    __shared__ __attribute__((aligned(16))) uint64_t keys_of[kProbsWaves * kMaxTop], best_of[kMaxTop];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int group = waves < kProbsWaves ? waves : kProbsWaves;  // wavefronts of a row in the workgroup
-    const int blocks = waves / group;                             // workgroups of a row
-    const float c2 = kLog2e / a.temperature;
-    const int64_t items = waves < kProbsWaves ? (a.T * waves + kProbsWaves - 1) / kProbsWaves : a.T * blocks;
+    const float c2 = a.c2;
+    const int list = max((a.top + 3) & ~3, 8);  // keys and zeros of a wavefront in keys_of
+    const int s = 31 - __clz(kProbsBlock / kProbsWaves / list);
+    const int64_t items = rows > 1 ? (a.T + rows - 1) / rows : a.T * blocks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t at = item * kProbsWaves + wave, t = over(at, waves), part = at - t * waves;  // wavefront `part` of row t
-        const bool in = t < a.T, writes = in && (wave & (group - 1)) == 0;
+        // wavefront `part` of row t
+        const int64_t t = rows > 1 ? item * rows + wave / group : blocks == 1 ? item : over(item, blocks);
+        const int64_t part = rows > 1 ? wave % group : (item - t * blocks) * kProbsWaves + wave;
+        const bool in = rows == 1 || t < a.T, writes = in && wave % group == 0;
         Sums sums{neg_inf(), 0.0f, 0.0f};
         Best best;
         const int64_t given = writes && blocks == 1 ? given_index(a, t, lane) : -1;
@@ -405,18 +420,19 @@ __global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut 
         }
         if (group > 1) {
             if (lane == 0) sums_of[wave] = sums;
-            if (lane < a.top) keys_of[wave * a.top + lane] = best.key;
+            if (lane < list) keys_of[wave * list + lane] = best.key;
             if (group == kProbsWaves && threadIdx.x < kMaxTop) best_of[threadIdx.x] = 0;
             __syncthreads();
             if (group == kProbsWaves && a.top) {
-                // a key's place is the number of keys above it in the eight sorted lists, of which 2^s lanes search
-                // some each
-                const int keys = kProbsWaves * a.top, s = min(31 - __clz(kProbsBlock / keys), 3);
+                // a key's place is the number of keys above it, of which 2^s lanes count some each (lists of more
+                // than 8 are searched)
                 const int i = threadIdx.x >> s, p = threadIdx.x & ((1 << s) - 1);
-                const uint64_t mine = i < keys ? keys_of[i] : 0;
+                const uint64_t mine = i < kProbsWaves * list ? keys_of[i] : 0;
                 int more = 0;
-                if (mine)
-                    for (int w = p; w < kProbsWaves; w += 1 << s) more += above_in_order(mine, keys_of + w * a.top, a.top);
+                if (s == 3)  // (list is 8)
+                    more = above<2>(mine, keys_of + 8 * p, 8);
+                else if (mine)
+                    for (int w = 2 * p; w < kProbsWaves; w += 2 << s) more += above_in_two(mine, keys_of + w * list, list);
                 for (int d = 1; d < 1 << s; d <<= 1) more += __shfl_xor(more, d);
                 if (mine && p == 0 && more < a.top) best_of[more] = mine;
                 __syncthreads();
@@ -426,7 +442,7 @@ __global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut 
                 sums = wave_joined(lane < group ? sums_of[wave + lane] : Sums{neg_inf(), 0.0f, 0.0f}, c2);
                 if (group < kProbsWaves && a.top)
                     for (int w = wave + 1; w < wave + group; ++w) {
-                        if (lane < a.top) rooms[wave].found[lane] = keys_of[w * a.top + lane];
+                        if (lane < a.top) rooms[wave].found[lane] = keys_of[w * list + lane];
                         best.take(a.top, a.top, rooms[wave], lane);
                     }
             }
@@ -447,7 +463,7 @@ template <class S>
 __global__ __launch_bounds__(64) void k_probs_join(ProbsArgs a, ProbsOut o, int blocks, Parts parts) {
     __shared__ Room room;
     const int lane = threadIdx.x;
-    const float c2 = kLog2e / a.temperature;
+    const float c2 = a.c2;
     for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
         const int64_t given = given_index(a, t, lane);
         const Sums* of = parts.sums + t * blocks;
@@ -496,7 +512,7 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
                                                             const float* __restrict__ d_top,
                                                             typename S::Bits* __restrict__ d_scores) {
     const int lane = threadIdx.x & 63;
-    const float c = 1.0f / a.temperature, c2 = kLog2e / a.temperature;
+    const float c = a.c, c2 = a.c2;
     const int64_t G = d_given ? a.G : 0;
     const int K = d_top ? a.top : 0;
     const uint32_t spans = uint32_t(over(a.V + span - 1, uint32_t(span)));
@@ -581,17 +597,26 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
     }
 }
 
-template <class S>
-hipError_t probs(const ProbsArgs& a, const ProbsOut& o, void* work, hipStream_t s) {
-    const ProbsPlan p = probs_plan(a.T, a.V);
-    const int64_t blocks = p.waves / kProbsWaves;
+template <class S, int group>
+hipError_t probs(const ProbsArgs& a, const ProbsOut& o, const ProbsPlan& p, void* work, hipStream_t s) {
+    constexpr int rows = kProbsWaves / group;
+    const int blocks = std::max(p.waves / kProbsWaves, 1);
     auto* keys = static_cast<uint64_t*>(work);
     const Parts parts{reinterpret_cast<Sums*>(keys + a.T * blocks * a.top), keys};
-    const int64_t items = p.waves < kProbsWaves ? (a.T * p.waves + kProbsWaves - 1) / kProbsWaves : a.T * blocks;
-    k_probs<S><<<match_grid(items), kProbsBlock, 0, s>>>(a, o, p.waves, p.span, parts);
+    k_probs<S, group><<<match_grid(rows > 1 ? (a.T + rows - 1) / rows : a.T * blocks), kProbsBlock, 0, s>>>(a, o, blocks,
+                                                                                                     p.span, parts);
     if (hipError_t e = hipGetLastError()) return e;
-    if (blocks > 1) k_probs_join<S><<<match_grid(a.T), 64, 0, s>>>(a, o, int(blocks), parts);
+    if (blocks > 1) k_probs_join<S><<<match_grid(a.T), 64, 0, s>>>(a, o, blocks, parts);
     return hipGetLastError();
+}
+template <class S> hipError_t probs(const ProbsArgs& a, const ProbsOut& o, void* work, hipStream_t s) {
+    const ProbsPlan p = probs_plan(a.T, a.V);
+    switch (p.waves) {
+        case 1: return probs<S, 1>(a, o, p, work, s);
+        case 2: return probs<S, 2>(a, o, p, work, s);
+        case 4: return probs<S, 4>(a, o, p, work, s);
+        default: return probs<S, 8>(a, o, p, work, s);
+    }
 }
 
 template <class S>
