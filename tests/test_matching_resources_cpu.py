@@ -30,7 +30,7 @@ def test_tiles_fit_the_lds(kernels, tile, per_cu):
 
 def test_two_workgroups_of_log_probabilities_per_cu(kernels):
     hits = [k for n, k in kernels["tp_probs.hip"].items() if "7k_probsI" in n]
-    assert len(hits) == 3
+    assert len(hits) == 12  # 3 types of the scores, 1, 2, 4 or 8 wavefronts a row
     for k in hits:
         # 512 lanes: two wavefronts per SIMD each
         assert k["Occupancy"] >= 4 and 2 * -(-k["LDS"] // GRANULE) * GRANULE <= LDS_PER_CU, k
