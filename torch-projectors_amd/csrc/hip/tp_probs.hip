@@ -34,8 +34,8 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417
 
 __host__ __device__ __forceinline__ constexpr float neg_inf() { return -__builtin_inff(); }
 
-// The larger of two, NaN if either is.
-__device__ __forceinline__ float max_or_nan(float a, float b) { return a != a ? a : (b > a || b != b ? b : a); }
+// The larger of two, NaN if either is (one instruction for two of these).
+__device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // Larger keys are better: the score's bits in the order of the scores, then the lower index.  0 is no candidate.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -150,6 +150,12 @@ struct Best {
             place(mine, above(mine, room.found, i), top, room, lane);
         }
         if (i == n) {
+        } else if (n <= 4) {
+            for (; i < n; ++i) {
+                const uint64_t k = room.found[i], before = uint64_t(brought<0x138>(uint32_t(key >> 32), ~0u)) << 32 |
+                                                           brought<0x138>(uint32_t(key), ~0u);  // wave_shr:1
+                key = lane >= top ? 0 : key > k ? key : before > k ? k : before;
+            }
         } else if (top <= 32 && top <= 6 * n + 12) {
             const int step = (64 - top) & ~3;
             for (; i < n; i += step) {
@@ -231,12 +237,17 @@ template <class S> __device__ __forceinline__ int64_t tile_index(int64_t v0, int
 }
 template <class S>
 __device__ __forceinline__ void load_tile(const typename S::Bits* x, const uint8_t* mask, int64_t v0, int64_t v1,
-                                          int lane, float (&f)[kLaneScores]) {
+                                          bool stream, int lane, float (&f)[kLaneScores]) {
     constexpr int n = Pack<S>::n, P = kLaneScores / n;
     if (v0 + kTileScores <= v1) {
         Pack<S> w[P];
+        if (stream) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) w[p] = load_pack<S>(x + tile_index<S>(v0, lane, p * n));
+            for (int p = 0; p < P; ++p) w[p] = stream_pack<S>(x + tile_index<S>(v0, lane, p * n));
+        } else {
+#pragma unroll
+            for (int p = 0; p < P; ++p) w[p] = load_pack<S>(x + tile_index<S>(v0, lane, p * n));
+        }
 #pragma unroll
         for (int i = 0; i < kLaneScores; ++i) f[i] = S::widen(w[i / n].v[i % n]);
     } else {
@@ -274,10 +285,10 @@ __device__ __forceinline__ void load_tile(const typename S::Bits* x, const uint8
 // Scores [v0, v1) of a row, by one wavefront.
 template <class S>
 __device__ __forceinline__ void scan_scores(const typename S::Bits* x, const uint8_t* mask, int64_t v0, int64_t v1,
-                                            float c2, int top, int lane, Room& room, Sums& sums, Best& best) {
+                                            float c2, int top, bool stream, int lane, Room& room, Sums& sums, Best& best) {
     for (; v0 < v1; v0 += kTileScores) {
         float f[kLaneScores];
-        load_tile<S>(x, mask, v0, v1, lane, f);
+        load_tile<S>(x, mask, v0, v1, stream, lane, f);
         float most = f[0];
 #pragma unroll
         for (int i = 1; i < kLaneScores; ++i) most = max_or_nan(most, f[i]);
@@ -391,7 +402,8 @@ struct Parts {
 
 // `group` wavefronts of a workgroup per row: 1, 2, 4 or 8, and with 8 `blocks` workgroups, whose parts are joined.
 template <class S, int group>
-__global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut o, int blocks, int64_t span, Parts parts) {
+__global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut o, int blocks, int64_t span, bool stream,
+                                                      Parts parts) {
     constexpr int rows = kProbsWaves / group;  // of a workgroup
     __shared__ Sums sums_of[kProbsWaves];
     __shared__ Room rooms[kProbsWaves];
@@ -413,8 +425,8 @@ __global__ __launch_bounds__(kProbsBlock, 4) void k_probs(ProbsArgs a, ProbsOut 
         if (in) {
             const auto* x = static_cast<const typename S::Bits*>(a.scores) + t * a.stride;
             const int64_t v0 = part * span, v1 = min(v0 + span, a.V);
-            scan_scores<S>(x, a.mask ? a.mask + t * a.mask_stride : nullptr, v0, v1, c2, a.top, lane, rooms[wave], sums,
-                           best);
+            scan_scores<S>(x, a.mask ? a.mask + t * a.mask_stride : nullptr, v0, v1, c2, a.top, stream,
+                           lane, rooms[wave], sums, best);
             given_x = given_score<S>(a, t, given);
             sums = wave_joined(sums, c2);
         }
@@ -504,7 +516,7 @@ int64_t back_span(int64_t T, int64_t V) {
 }
 
 template <class S>
-__global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t span, const float* __restrict__ stats,
+__global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t span, bool stream, const float* __restrict__ stats,
                                                             const int64_t* __restrict__ top_index,
                                                             const float* __restrict__ d_given,
                                                             const float* __restrict__ d_entropy,
@@ -531,7 +543,7 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
         const float4 st = *reinterpret_cast<const float4*>(stats + t * kProbsStats);
         const float dL = d_log_sum ? d_log_sum[t] : 0.0f, dH = d_entropy ? d_entropy[t] : 0.0f;
         float f[kLaneScores];
-        load_tile<S>(x, mask, first, end, lane, f);
+        load_tile<S>(x, mask, first, end, stream, lane, f);
         const bool fix = mine >= first && mine < end && !(mask && !mask[mine]);
         const float at_mine = fix ? S::widen(x[mine]) : 0.0f;
         const float m = st.x, ls = st.y, H = st.z, ls2 = ls * kLog2e;
@@ -540,26 +552,27 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
         for (int64_t j = lane + 64; j < n; j += 64)
             if (index_at(j) != -1) all -= up_at(j);
         all = wave_sum(all) + dL;
-        // the gradient of score f without what is given or listed there; 0 where not allowed
+        // the gradient of score f without what is given or listed there, c p (all - dH (ln p + H)); 0 where not allowed,
+        // and everywhere in a row that allows nothing; NaN in a row with a NaN or +inf
+        const bool plain = !none && ls == ls;
+        const float at_0 = plain ? c * __builtin_fmaf(-dH, H, all) : none ? 0.0f : __builtin_nanf("");
+        const float slope = plain ? c * -dH * kLn2 : 0.0f;
         auto smooth = [&](float f) {
-            const float lp2 = fmaxf((f - m) * c2 - ls2, -200.0f), p = __builtin_amdgcn_exp2f(lp2);
-            return p * (all - dH * __builtin_fmaf(lp2, kLn2, H));
+            const float lp2 = fmaxf((f - m) * c2 - ls2, -200.0f);
+            return __builtin_amdgcn_exp2f(lp2) * __builtin_fmaf(slope, lp2, at_0);
         };
-        const bool broken = !(ls == ls);  // a NaN or +inf in the row: so are its gradients
         for (int64_t v0 = first; v0 < end; v0 += kTileScores) {
-            if (v0 != first) load_tile<S>(x, mask, v0, end, lane, f);
+            if (v0 != first) load_tile<S>(x, mask, v0, end, stream, lane, f);
             constexpr int P = Pack<S>::n;
 #pragma unroll
             for (int p = 0; p < kLaneScores / P; ++p) {
                 Pack<S> w;
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const float g = c * smooth(f[p * P + i]);
-                    w.v[i] = S::round(none ? 0.0f : broken ? __builtin_nanf("") : g);
-                }
+                for (int i = 0; i < P; ++i) w.v[i] = S::round(smooth(f[p * P + i]));
                 const int64_t v = tile_index<S>(v0, lane, p * P);
                 if (v + P <= end) {
-                    store_pack<S>(d + v, w);
+                    if (stream) stream_pack<S>(d + v, w);
+                    else store_pack<S>(d + v, w);
                 } else {
 #pragma unroll
                     for (int i = 0; i < P; ++i)
@@ -567,7 +580,7 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
                 }
             }
         }
-        if (none || broken) continue;
+        if (!plain) continue;
         // (the stores above come before those below: one wavefront's, in order)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (n <= 64) {
@@ -579,7 +592,7 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
                 if (same) sum += __uint_as_float(read_lane(__float_as_uint(up), l));
                 if (same && l < lane) is_first = false;
             }
-            if (fix && is_first) d[mine] = S::round(c * (smooth(at_mine) + sum));
+            if (fix && is_first) d[mine] = S::round(__builtin_fmaf(c, sum, smooth(at_mine)));
             continue;
         }
         for (int64_t i = lane; i < n; i += 64) {
@@ -592,10 +605,16 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
                     if (j < i) is_first = false;
                     sum += up_at(j);
                 }
-            if (is_first) d[v] = S::round(c * (smooth(S::widen(x[v])) + sum));
+            if (is_first) d[v] = S::round(__builtin_fmaf(c, sum, smooth(S::widen(x[v]))));
         }
     }
 }
+
+// Scores of about the last cache's size (256 MB) or more are streamed past the caches.  Measured, forward and gradient:
+// 2000 x 33000 fp32 (251 MB) 171 us through the caches, 164 streamed; 4096 x 36864 (576 MB) 356 and 311; but
+// 4096 x 4300 (67 MB) 51 and 54.
+constexpr int64_t kStreamScores = int64_t(192) << 20;
+bool streams(const ProbsArgs& a, size_t size) { return a.T * a.V * int64_t(size) >= kStreamScores; }
 
 template <class S, int group>
 hipError_t probs(const ProbsArgs& a, const ProbsOut& o, const ProbsPlan& p, void* work, hipStream_t s) {
@@ -604,7 +623,7 @@ hipError_t probs(const ProbsArgs& a, const ProbsOut& o, const ProbsPlan& p, void
     auto* keys = static_cast<uint64_t*>(work);
     const Parts parts{reinterpret_cast<Sums*>(keys + a.T * blocks * a.top), keys};
     k_probs<S, group><<<match_grid(rows > 1 ? (a.T + rows - 1) / rows : a.T * blocks), kProbsBlock, 0, s>>>(a, o, blocks,
-                                                                                                     p.span, parts);
+                                                                                                     p.span, streams(a, sizeof(typename S::Bits)), parts);
     if (hipError_t e = hipGetLastError()) return e;
     if (blocks > 1) k_probs_join<S><<<match_grid(a.T), 64, 0, s>>>(a, o, blocks, parts);
     return hipGetLastError();
@@ -625,7 +644,7 @@ hipError_t probs_back(const ProbsArgs& a, const float* stats, const int64_t* top
                       hipStream_t s) {
     const int64_t span = back_span(a.T, a.V), items = a.T * ((a.V + span - 1) / span);
     k_probs_back<S><<<match_grid((items + kBackWaves - 1) / kBackWaves), kBackBlock, 0, s>>>(
-        a, span, stats, top_index, d_given, d_entropy, d_log_sum, d_top, static_cast<typename S::Bits*>(d_scores));
+        a, span, streams(a, sizeof(typename S::Bits)), stats, top_index, d_given, d_entropy, d_log_sum, d_top, static_cast<typename S::Bits*>(d_scores));
     return hipGetLastError();
 }
 
