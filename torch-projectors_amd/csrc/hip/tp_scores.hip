@@ -24,23 +24,26 @@ namespace {
 using v4f = __attribute__((ext_vector_type(4))) float;
 
 // ------------------------------------------------------------------ quantize
-// Exponent of a block with largest finite magnitude `most`: most = f 2^x with f in [0.5, 1), and
-// 448 = 0.875 2^9.
-__device__ __forceinline__ int block_exponent(float most) {
-    int x;
-    const float f = frexpf(most, &x);
-    return most == 0.0f ? 0 : max(f > 0.875f ? x - 8 : x - 9, -127);
+// Exponent of a block whose largest finite magnitude has these bits: 448 = 1.75 2^8, so one more where the mantissa
+// is past 1.75 (a carry).  Subnormal ones are far below 2^-127 448.
+__device__ __forceinline__ int block_exponent(uint32_t most) {
+    return most ? max(int((most + 0x1fffffu) >> 23) - 135, -127) : 0;
+}
+__device__ __forceinline__ float power_of_2(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }  // -126 .. 127
+// The bits of a finite value's magnitude (they are in the order of the magnitudes), 0 for others.
+__device__ __forceinline__ uint32_t magnitude(float x) {
+    const uint32_t m = __float_as_uint(x) & 0x7fffffffu;
+    return m < 0x7f800000u ? m : 0u;
 }
 
 // Codes of two values: to nearest even, NaN for what is not finite.
-__device__ __forceinline__ uint32_t codes2(float x, float y, int e) {
-    const float f = ldexpf(1.0f, -e);
+__device__ __forceinline__ uint32_t codes2(float x, float y, float f) {
     const uint32_t two = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(x * f, y * f, 0, false)) & 0xffffu;
     return two | (isfinite(x) ? 0u : 0x7fu) | (isfinite(y) ? 0u : 0x7f00u);
 }
 // Codes of eight values: to nearest even, NaN for what is not finite.
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], int e) {
-    const float f = ldexpf(1.0f, -e);
+    const float f = power_of_2(-e);
     uint32_t c[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -88,11 +91,11 @@ __global__ __launch_bounds__(256) void k_quantize(const typename S::Bits* __rest
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? S::widen(p[i]) : 0.0f;
         }
-        float most = 0.0f;
+        uint32_t most = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = fmaxf(most, isfinite(v[i]) ? fabsf(v[i]) : 0.0f);
+        for (int i = 0; i < 8; ++i) most = max(most, magnitude(v[i]));
 #pragma unroll
-        for (int d = 8; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+        for (int d = 8; d; d >>= 1) most = max(most, uint32_t(__shfl_xor(int(most), d)));
         const int e = block_exponent(most);
         if (part == 0) scales[b * srows + r] = uint8_t(e + 127);
         *reinterpret_cast<uint2*>(codes + (r * nb + b) * kScaleBlock + 8 * part) = codes8(v, e);
@@ -113,6 +116,18 @@ __device__ __forceinline__ v8bf widen8(int lo, int hi, float scale) {
     const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
     const v2bf d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
     return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Largest of a wavefront's values, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    // row_shr:1, 2, 4, 8, then row_bcast:15 and 31: lane 63 has seen all (0 where none is brought)
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x111, 0xf, 0xf, false)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x112, 0xf, 0xf, false)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x114, 0xf, 0xf, false)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xf, 0xf, false)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x142, 0xf, 0xf, false)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x143, 0xf, 0xf, false)));
+    return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
 }
 
 // What the kernels of the product share: [splits] ranges of the nb blocks are one workgroup each, and
@@ -162,8 +177,8 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
                                                                                                        OneImage one) {
     constexpr bool kOne = !std::is_same<S, void>::value;  // (M is 1; the image's codes and scales are not given)
     __shared__ float sums[kFewWaves][FM * 16][16];
-    __shared__ __attribute__((aligned(16))) uint8_t codes[kOne ? kFewWaves : 1][kOne ? kAhead : 1][kScaleBlock];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q = lane >> 4;
+    __shared__ __attribute__((aligned(16))) uint32_t wide[kOne ? kFewWaves : 1][kOne ? kAhead : 1][64];  // pairs of bfloat16
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int64_t n0 = int64_t(blockIdx.x) * 16, K = int64_t(g.nb) * kScaleBlock;
     // rows past the end read the last one's codes and are not stored
     const int64_t bn = min(n0 + r, g.N - 1);
@@ -180,6 +195,7 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
         acc[f] = v4f{0, 0, 0, 0};
     }
     for (int k = wave; k < g.nb; k += kFewWaves * kAhead) {
+        if constexpr (kOne) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         int4 cb[kAhead][2], ca[kAhead][FM][2];
         uint32_t eb[kAhead], ea[kAhead][FM];
         float image[kOne ? kAhead : 1][2];
@@ -190,10 +206,12 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
             for (int h = 0; h < 2; ++h) cb[u][h] = *reinterpret_cast<const int4*>(pb + at * kScaleBlock + h * 64);
             eb[u] = sb[at * g.srb];
             if constexpr (kOne) {
-                const int64_t c = at * kScaleBlock + 2 * lane;
-                const auto* x = static_cast<const typename S::Bits*>(one.x) + c;
-                image[u][0] = c < one.cols ? S::widen(x[0]) : 0.0f;
-                image[u][1] = c + 1 < one.cols ? S::widen(x[1]) : 0.0f;
+                const auto* x = static_cast<const typename S::Bits*>(one.x) + at * kScaleBlock;
+                const int last = int(min(one.cols - at * kScaleBlock, int64_t(kScaleBlock))) - 1;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) image[u][i] = S::widen(x[min(2 * lane + i, last)]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) image[u][i] = 2 * lane + i <= last ? image[u][i] : 0.0f;
                 continue;
             }
 #pragma unroll
@@ -210,18 +228,11 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const float v = image[u][0], w = image[u][1];
-                float most = fmaxf(isfinite(v) ? fabsf(v) : 0.0f, isfinite(w) ? fabsf(w) : 0.0f);
-#pragma unroll
-                for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-                const int e = block_exponent(most);
-                reinterpret_cast<uint16_t*>(codes[wave][u])[lane] = uint16_t(codes2(v, w, e));
-                ea[u][0] = uint32_t(e + 127);
+                const int e = block_exponent(wave_max(max(magnitude(v), magnitude(w))));
+                wide[wave][u][lane] = __builtin_bit_cast(
+                    uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(int(codes2(v, w, power_of_2(-e))),
+                                                                        scale_of(uint32_t(e + 127)), false));
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) ca[u][0][h] = *reinterpret_cast<const int4*>(codes[wave][u] + h * 64 + q * 16);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
 #pragma unroll
@@ -231,6 +242,12 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const v8bf b0 = widen8(cb[u][h].x, cb[u][h].y, fb), b1 = widen8(cb[u][h].z, cb[u][h].w, fb);
+                if constexpr (kOne) {
+                    const auto* a = reinterpret_cast<const v8bf*>(wide[wave][u] + h * 32 + q * 8);
+                    acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b0, acc[0], 0, 0, 0);
+                    acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b1, acc[0], 0, 0, 0);
+                    continue;
+                }
 #pragma unroll
                 for (int f = 0; f < FM; ++f) {
                     const float fa = scale_of(ea[u][f]);
