@@ -620,3 +620,61 @@ def test_blocks_from_any_address(m):
         moved.append(room.view(t.dtype).view(t.shape))
     assert moved[0].data_ptr() % 16
     assert torch.equal(m.block_scores(x, m.BlockScaled(*moved)), m.block_scores(x, q))
+
+
+@pytest.mark.parametrize("M,N,K,out_dtype,bias", [(16, 300, 16640, F32, True), (16, 4100, 1000, BF16, False),
+                                                  (24, 2000, 8320, F32, False), (20, 4099, 640, F32, True),
+                                                  (32, 150, 4224, BF16, True)])
+def test_scores_of_few_images(m, M, N, K, out_dtype, bias):
+    _scores_check(m, M, N, K, out_dtype, bias, seed=5)
+
+
+@pytest.mark.parametrize("n,E", [(2048, 4096), (2049, 4096), (4096, 16), (4097, 16), (5000, 1000), (8193, 64), (32768, 64),
+                                 (32769, 64), (140000, 4096), (530001, 64)])
+def test_sort_where_its_split_changes(m, n, E):
+    classes = (torch.rand(n, generator=gen(n)) ** 2 * (E + 1)).long()
+    got = m.sort_by_class(classes.to(DEV), E)
+    order = torch.sort(classes, stable=True)[1]
+    assert torch.equal(got.order.cpu().long(), order)
+    assert torch.equal(got.slot.cpu().long()[order, 0], torch.arange(n))
+    assert torch.equal(got.offsets.cpu().long(), torch.searchsorted(classes[order].contiguous(), torch.arange(E + 1)))
+
+
+@pytest.mark.parametrize("top", [1, 4, 12, 31, 33, 64])
+@pytest.mark.parametrize("kind", ["rising", "falling", "narrow", "few values", "one lane"])
+def test_probs_candidates_of_every_number(m, kind, top):
+    """Rows that bring many, few or clustered candidates to a wavefront's tile."""
+    V, g = 9001, gen(top)
+    x = torch.randn(3, V, generator=g)
+    if kind in ("rising", "falling"):
+        x = x.sort(1, descending=kind == "falling")[0]
+    elif kind == "narrow":
+        x = -20000 + x  # differ in the last bits only
+    elif kind == "few values":
+        x = x.sign() + (x > 2).float()
+    else:
+        x[:, 512:516] += 20  # neighbours, which one lane reads
+        x[:, 4096:4100] += 21
+    _probs_check(m, x, torch.randint(0, V, (3, 1), generator=g), top, 2.0)
+
+
+def test_probs_streamed(m):
+    """Scores larger than the caches: rows at both ends against the oracle."""
+    T, V = 1501, 36867  # 221 MB
+    for dtype in (F32, BF16):
+        n = T if dtype == F32 else 2 * T
+        x = (torch.randn(n, V, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV) * 2).to(dtype).requires_grad_()
+        given = torch.arange(n, device=DEV)
+        out = m.log_probs(x, given, top=9, temperature=1.5)
+        up = [torch.linspace(-1, 1, n, device=DEV), torch.linspace(0, 0.1, n, device=DEV), torch.linspace(0.5, 0, n, device=DEV),
+              torch.ones(n, 9, device=DEV) * 0.1]
+        (d,) = torch.autograd.grad([out.given, out.entropy, out.log_sum, out.top], [x], up)
+        rows = torch.tensor([0, 1, n // 2, n - 1])
+        at = rows.to(DEV)
+        want = R.log_probs(x.detach()[at].cpu(), given[at].cpu()[:, None], 9, 1.5, None,
+                           (up[0][at].cpu()[:, None], up[1][at].cpu(), up[2][at].cpu(), up[3][at].cpu()))
+        near(out.given[at][:, None], want["given"], 2e-5, "given")
+        near(out.log_sum[at], want["log_sum"], 2e-5, "log_sum")
+        near(out.entropy[at], want["entropy"], 4e-5, "entropy")
+        assert torch.equal(out.top_index[at].cpu(), want["top_index"])
+        near(d[at], want["d_scores"], 1e-5 + R.U[dtype] * want["d_scores"].abs() * 1.01, "d_scores")

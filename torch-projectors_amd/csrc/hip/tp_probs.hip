@@ -11,14 +11,17 @@
 // Alternatives: a wavefront keeps its best as sorted keys, one per lane: the score's bits in an order that
 // integers have, then the complement of its index, so ties go to the lowest index.  Scores above the top-th
 // key's are candidates; of a tile with many (the first; rising rows) only those that reach a floor below
-// which none can be listed: the top-th largest of the lanes' own largest.  Candidates go through LDS and are
-// merged by counting: a key's place is the number of keys above it, which all lanes count at once over
-// broadcast reads (about 15 cycles a key; handing one key after another around through scalar registers takes
-// 100, but does not depend on `top`, and is left for few candidates of long lists).
+// which none can be listed, close to the top-th largest of the lanes' own largest (without it 1 x 4096 with 8
+// alternatives takes 26 us instead of 5.3, 4096 x 36864 119 instead of 96).  Candidates go through LDS.  A few are
+// inserted one by one, the keys below moving up by a lane; more are merged by counting: a key's place is the
+// number of keys above it, which all lanes count at once over broadcast reads (4096 x 36864 bfloat16 with 32
+// alternatives: counting from 1 candidate on 84 us, from 13 on 76, never 78; 64 x 294912 fp32 31.4, 30.8 and 33.2).
+// More than 32 alternatives leave too few lanes for counting (4096 x 36864 with 64: 116 us, inserted 112).
 //
 // Split: a row is one wavefront's, or 2, 4 or 8 of a workgroup's, or, where rows are few, several workgroups',
-// whose sums and keys k_probs_join joins.  Memory bound: a tile of 16 scores a lane is in flight for every
-// wavefront of a CU.
+// whose sums and keys k_probs_join joins.  Large calls are bound by memory (4096 x 36864 fp32 with 8 alternatives
+// 96 us, 6.3 TB/s; bfloat16 73 us, by the instructions of a score), small ones by the chain from launch to result: of
+// the 5.3 us of 1 x 4096 a fifth each goes to the start, the loads and sums, and the selection, the rest to the joins.
 //
 // Scores of -inf count as not allowed.  A NaN makes the row's results NaN.
 #include "../../../include/torch_projectors_hip.h"
@@ -150,13 +153,13 @@ struct Best {
             place(mine, above(mine, room.found, i), top, room, lane);
         }
         if (i == n) {
-        } else if (n <= 4) {
+        } else if (n <= 12 || top > 32) {
             for (; i < n; ++i) {
                 const uint64_t k = room.found[i], before = uint64_t(brought<0x138>(uint32_t(key >> 32), ~0u)) << 32 |
                                                            brought<0x138>(uint32_t(key), ~0u);  // wave_shr:1
                 key = lane >= top ? 0 : key > k ? key : before > k ? k : before;
             }
-        } else if (top <= 32 && top <= 6 * n + 12) {
+        } else {
             const int step = (64 - top) & ~3;
             for (; i < n; i += step) {
                 const int count = min(step, n - i);
@@ -164,27 +167,6 @@ struct Best {
                 room.keys[lane] = key;
                 lds_order();
                 place(mine, above(mine, room.found + i, count) + above(mine, room.keys, top), top, room, lane);
-            }
-        } else {
-            for (; i < n; i += 64) {
-                const uint64_t theirs = i + lane < n ? room.found[i + lane] : 0;
-                const uint64_t set = __ballot(theirs > read_lane(key, top - 1));
-                int up = 0, rank = 0, more = 0;
-                for (uint64_t left = set; left; left &= left - 1) {
-                    const int from = __ffsll(static_cast<long long>(left)) - 1;
-                    const uint64_t k = read_lane(theirs, from);
-                    const int keys = __popcll(__ballot(key > k));
-                    if (lane == from) more = keys;
-                    up += key < k ? 1 : 0;
-                    rank += theirs < k ? 1 : 0;
-                }
-                room.keys[lane] = 0;
-                lds_order();
-                if (key && lane + up < top) room.keys[lane + up] = key;
-                if (((set >> lane) & 1) && more + rank < top) room.keys[more + rank] = theirs;
-                lds_order();
-                key = room.keys[lane];
-                lds_order();
             }
         }
         const uint64_t last = read_lane(key, top - 1);
@@ -518,8 +500,9 @@ __global__ __launch_bounds__(64) void k_probs_join(ProbsArgs a, ProbsOut o, int 
 }
 
 // Wavefronts of a row, and the scores of each: as many as fill the card (16 on each CU), none with less than a
-// tile; a whole workgroup's where that leaves none waiting (its join is the faster one: 1 x 4096 with 8
-// alternatives 7.5 us by 4 of 8 wavefronts, 6.6 by 8, half of them without scores).
+// tile; a whole workgroup's where each has a CU of its own (its join is the faster one, with half of the wavefronts
+// without scores: 1 x 4096 with 8 alternatives 6.3 us by 4 of 8 wavefronts, 5.4 by 8; 100 rows 7.3 and 5.8; but 512
+// rows of 2048 6.2 by 2, 6.8 by 8).
 struct ProbsPlan {
     int waves;
     int64_t span;
@@ -529,19 +512,16 @@ ProbsPlan probs_plan(int64_t T, int64_t V) {
     const int64_t most = std::min<int64_t>((4096 + T - 1) / T, tiles);
     int64_t w = 1;
     while (w < most && w < kProbsWaves) w *= 2;
-    if (w > 1 && T <= 512) w = kProbsWaves;
+    if (w > 1 && T <= 256) w = kProbsWaves;
     if (most > kProbsWaves) w = (most + kProbsWaves - 1) / kProbsWaves * kProbsWaves;
     const int64_t span = (tiles + w - 1) / w * kTileScores;
     return {int(w), span};
 }
 
-// The gradient: a wavefront per stretch of a row (four tiles, or one where that leaves CUs idle).  Every
-// score's share but that of the given and listed ones first, then those scores' once more with it, each by one
-// lane.  Memory bound: reads and writes each score once.
+// The gradient: a wavefront per stretch of a row.  Every score's share but that of the given and listed ones first,
+// then those scores' once more with it, each by one lane.  Memory bound: reads and writes each score once
+// (4096 x 36864 fp32 192 us, 6.3 TB/s).
 constexpr int kBackBlock = 256, kBackWaves = kBackBlock / 64;
-int64_t back_span(int64_t T, int64_t V) {
-    return (T * ((V + kTileScores - 1) / kTileScores) >= 16384 ? 4 : 1) * int64_t(kTileScores);
-}
 
 template <class S>
 __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t span, bool stream, const float* __restrict__ stats,
@@ -639,10 +619,19 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
 }
 
 // Scores of about the last cache's size (256 MB) or more are streamed past the caches.  Measured, forward and gradient:
-// 2000 x 33000 fp32 (251 MB) 171 us through the caches, 164 streamed; 4096 x 36864 (576 MB) 356 and 311; but
-// 4096 x 4300 (67 MB) 51 and 54.
+// 4096 x 36864 bfloat16 (288 MB) 180 us through the caches, 160 streamed, fp32 (576 MB) 351 and 308; but 1000 x 16384
+// fp32 (62 MB) 45 and 47.
 constexpr int64_t kStreamScores = int64_t(192) << 20;
 bool streams(const ProbsArgs& a, size_t size) { return a.T * a.V * int64_t(size) >= kStreamScores; }
+
+// Scores of a stretch of the gradient: 8 KB, but one tile where stretches would be fewer than eight to a CU, and of
+// fp32 scores that are streamed.  Measured with 1, 2 and 4 tiles: 4096 x 4300 fp32 30, 25 and 26 us, bfloat16 (8192
+// rows) 45, 35 and 31; streamed, 4096 x 36864 fp32 192, 195 and 213, bfloat16 140, 109 and 101; 8 x 294912 fp32
+// 6.7, 6.9 and 8.5.
+int64_t back_span(const ProbsArgs& a, size_t size) {
+    const int64_t tiles = a.T * ((a.V + kTileScores - 1) / kTileScores), most = 8192 / int64_t(size) / kTileScores;
+    return (tiles < 2048 * most || (size == 4 && streams(a, size)) ? 1 : most) * int64_t(kTileScores);
+}
 
 template <class S, int group>
 hipError_t probs(const ProbsArgs& a, const ProbsOut& o, const ProbsPlan& p, void* work, hipStream_t s) {
@@ -670,7 +659,7 @@ template <class S>
 hipError_t probs_back(const ProbsArgs& a, const float* stats, const int64_t* top_index, const float* d_given,
                       const float* d_entropy, const float* d_log_sum, const float* d_top, void* d_scores,
                       hipStream_t s) {
-    const int64_t span = back_span(a.T, a.V), items = a.T * ((a.V + span - 1) / span);
+    const int64_t span = back_span(a, sizeof(typename S::Bits)), items = a.T * ((a.V + span - 1) / span);
     k_probs_back<S><<<match_grid((items + kBackWaves - 1) / kBackWaves), kBackBlock, 0, s>>>(
         a, span, streams(a, sizeof(typename S::Bits)), stats, top_index, d_given, d_entropy, d_log_sum, d_top, static_cast<typename S::Bits*>(d_scores));
     return hipGetLastError();

@@ -22,10 +22,10 @@ namespace {
 // ------------------------------------------------------------------ sort
 // A workgroup of W wavefronts sorts up to 64 W kGroups slots: each wavefront takes consecutive groups of 64, keeps
 // their classes and their ranks among its own slots of that class in registers, and its counts per class in
-// LDS.  Few slots are one workgroup's (16 wavefronts hold 8192); of more, a first kernel counts each workgroup's
-// stretch, and the second, knowing every stretch's counts, places it.
-constexpr int kGroups = 8, kMaxSortWaves = 16, kOneSort = 64 * kMaxSortWaves * kGroups;
-constexpr int kDirectStretches = 64;  // as many are summed by every workgroup of the second kernel by itself
+// LDS.  Few slots are one workgroup's; of more, a first kernel counts each workgroup's stretch, and the last,
+// knowing every stretch's counts, places it.  Bound by the chain of launches, counts and scans, not by its bytes: 4096
+// slots 7 us, 65536 12, 8388608 112.
+constexpr int kGroups = 8, kMaxSortWaves = 16;
 
 template <class I> __device__ __forceinline__ int class_of(const I* ids, int64_t i, int E) {
     const I c = ids[i];
@@ -202,32 +202,37 @@ __global__ __launch_bounds__(1024) void k_sort_sum(int* __restrict__ counts, int
     if (wave == 15) counts[int64_t(stretches) * C + c] = at;
 }
 
-// Wavefronts of the placing workgroups (LDS holds a count per class for each), and the slots of each.
+// Wavefronts of the placing workgroups (LDS holds a count per class for each), the slots of each workgroup, and
+// whether the counts are summed by a kernel of their own or by every workgroup for itself.  Measured: one workgroup
+// or several, 4096 slots of 16 classes 7.6 and 8.0 us, 6000 of 64 10.4 and 9.2, 8192 of 1000 16.4 and 11.6; 16
+// stretches with their own sums or 64 summed, 16384 slots of 64 classes 10.2 and 10.5, 32768 11.1 and 10.9, 65536
+// 13.4 and 11.8, 131072 of 4096 classes (64 stretches) 157 and 35.
 struct SortPlan {
     int waves, stretches;
     int64_t stretch;
+    bool summed;
 };
 SortPlan sort_plan(int64_t n, int E) {
     int waves = E <= 1024 ? kMaxSortWaves : 4;
-    const int64_t hold = int64_t(waves) * 64 * kGroups;
-    if (n <= hold) {
+    const int64_t group = int64_t(waves) * 64, hold = group * kGroups;
+    if (n <= std::min<int64_t>(hold, 4096)) {
         while (waves > 1 && int64_t(waves / 2) * 64 >= n) waves /= 2;
-        return {waves, 1, std::max<int64_t>(n, 1)};
+        return {waves, 1, std::max<int64_t>(n, 1), false};
     }
-    // about 32 stretches, or as many of a whole turn as there are, or 2048 of several turns
-    const int64_t group = int64_t(waves) * 64, turns = (n + hold - 1) / hold, each = (turns + 2047) / 2048;
-    const int64_t stretch = turns <= 32 ? ((n + 31) / 32 + group - 1) / group * group : each * hold;
-    return {waves, int((n + stretch - 1) / stretch), stretch};
+    const bool summed = n > 32768 || E > 1024;
+    // equal stretches, or as many of a whole turn as there are, or 2048 of several turns
+    const int64_t count = summed ? 64 : 16, turns = (n + hold - 1) / hold, each = (turns + 2047) / 2048;
+    const int64_t stretch = turns <= count ? ((n + count - 1) / count + group - 1) / group * group : each * hold;
+    return {waves, int((n + stretch - 1) / stretch), stretch, summed};
 }
 
 template <class I>
 hipError_t sort(const I* ids, int64_t n, int E, int* order, int* slot, int* offsets, int* counts, hipStream_t s) {
     const SortPlan p = sort_plan(n, E);
     const int C = E + 1;
-    const bool summed = p.stretches > kDirectStretches;
     if (p.stretches > 1) {
         k_sort_count<I><<<p.stretches, 1024, C * sizeof(int), s>>>(ids, n, p.stretch, E, counts);
-        if (summed) k_sort_sum<<<(C + 63) / 64, 1024, 0, s>>>(counts, p.stretches, C);
+        if (p.summed) k_sort_sum<<<(C + 63) / 64, 1024, 0, s>>>(counts, p.stretches, C);
         if (hipError_t e = hipGetLastError()) return e;
     }
     const size_t lds = size_t(p.waves + 1) * C * sizeof(int);
@@ -236,7 +241,7 @@ hipError_t sort(const I* ids, int64_t n, int E, int* order, int* slot, int* offs
                                                hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)))
             return e;
     k_sort_place<I><<<p.stretches, 64 * p.waves, lds, s>>>(ids, n, p.stretch, E, p.stretches > 1 ? counts : nullptr,
-                                                           p.stretches, summed, order, slot, offsets);
+                                                           p.stretches, p.summed, order, slot, offsets);
     return hipGetLastError();
 }
 
@@ -447,24 +452,27 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
     }
 }
 
-// Sorted rows of at least this size, what the XCDs' L2s hold together, are streamed past the caches.  Measured on
-// 16384 x 4 rows of 4096 bfloat16 (537 MB): spread 221 us through the caches, 128 streamed; weighted gather 159
-// and 118; on 2048 x 2 rows of 4224 fp32 (69 MB) 33 and 23, 26 and 24.
+// Sorted rows of at least this size, what the XCDs' L2s hold together, are streamed past the caches.  Measured: 16384 x 4
+// rows of 4096 bfloat16 (537 MB) weighted gather 134 us through the caches, 121 streamed (spread 123 and 126); 2048 x 2
+// rows of 4224 fp32 (69 MB), spread then gather of one input after another 20 + 30 us through the caches, which the
+// gather finds full of what is yet to be written, 22 + 23 streamed (of the same input again and again 18 + 19 and
+// 22 + 23).
 constexpr int64_t kStreamBytes = int64_t(32) << 20;
 
-// Wavefronts of a row: one while a row is at most 4 KB (four loads a lane), else 4, or 16 where rows are so few
+// Wavefronts of a row: one while a row is at most 2.5 KB, else 4 (16384 x 2 rows of 2560 bytes: spread 25.3 us by one,
+// 26.1 by four, with the weights' gradient 38 and 44; of 4096 bytes 45 and 35, 66 and 58), or 16 where rows are so few
 // that CUs would idle (with the weights' gradient, whose sums need the whole row in one workgroup); without it a
-// row of few is cut into stretches instead.
+// row of few is cut into stretches instead (100 x 2 rows of 66560 bytes: 5.5 us, whole 9.3).
 struct RowPlan {
     int waves, parts;
     int64_t span;
 };
 RowPlan row_plan(const RouteArgs& a, int size, bool dot) {
     const int64_t bytes = a.D * size;
-    RowPlan p{bytes <= 4096 ? 1 : 4, 1, a.D};
+    RowPlan p{bytes <= 2560 ? 1 : 4, 1, a.D};
     if (a.T * p.waves >= 2048 || bytes <= 1024) return p;
     if (dot) {
-        p.waves = bytes <= 4096 ? 4 : 16;
+        p.waves = p.waves == 1 ? 4 : 16;
         return p;
     }
     p.waves = 1;

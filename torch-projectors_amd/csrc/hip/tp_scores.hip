@@ -503,13 +503,14 @@ __global__ __launch_bounds__(64 * WM * WN * KW, BM * BN == 128 * 128 ? 4 : 1) vo
 }
 
 // ------------------------------------------------------------------ which kernel
-// Few images: k_scores_few.  Else the tile and the number of ranges of the blocks with the least time by a
+// One image: k_scores_few.  Else the tile and the number of ranges of the blocks with the least time by a
 // count of steps (one block of K for one tile).  A CU with n workgroups of a tile takes n step_us for a step
 // of each, but no less than alone_us: one workgroup alone waits for LDS and for its own products.  Measured:
-// 4096 x 8192 x 16640 (full CUs) 64: 1160 us, 128: 910, 256: 810; 2000 x 2000 x 4224 48, 42 and 100; 333 x 1999 x
-// 8280 in one range 38, 63 and 175 us, in four 26, 29 and 63.  Several ranges cost a launch and their sums written
-// and read.  Against every tile and 1 to 16 ranges on 25 sizes from 33 x 8192 to 4096 x 8192 the choice is within
-// 7 % of the best.
+// 4096 x 8192 x 16640 (full CUs) 64: 1056 us, 128: 857, 256: 775; 2000 x 2000 x 4224 46, 37 and 93; 333 x 1999 x
+// 8280 in one range 37, 60 and 174 us, in four 24, 28 and 61.  Several ranges cost a launch and their sums written
+// and read.  Up to 32 images k_scores_few may be faster: 16 and 24 x 1000 x 4224 6.3 and 7.6 us (tiles 9.0 and 9.1),
+// but 24 x 4096 x 16640 23.6 (18.2).  Against every tile and 1 to 16 ranges on 28 sizes from 17 x 2000 to 4096 x 8192
+// the choice is within 8 % of the best.
 struct ScorePlan {
     int few, tile, splits;  // few: FM of k_scores_few, or 0; tile: index of kTiles
 };
@@ -521,15 +522,15 @@ constexpr TileKind kTiles[] = {{64, 64, 0.28, 0.50}, {128, 128, 0.87, 1.0}, {256
 constexpr int kCus = 256, kMaxSplits = 16;
 
 ScorePlan score_plan(int64_t M, int64_t N, int64_t nb) {
-    if (M <= 32) return {M <= 16 ? 1 : 2, 0, 1};
-    ScorePlan best{0, 0, 1};
-    double least = 1e300;
+    ScorePlan best{M <= 16 ? 1 : 2, 0, 1};
+    if (M == 1) return best;
+    double least = M > 32 ? 1e300 : (2.5 + (M <= 16 ? 0.12 : 0.15) * nb) * double((N + 16 * kCus - 1) / (16 * kCus));
     for (int t = 0; t < 3; ++t) {
         const TileKind& kind = kTiles[t];
         const int64_t tiles = ((M + kind.bm - 1) / kind.bm) * ((N + kind.bn - 1) / kind.bn);
         for (int s = 1; s <= kMaxSplits && s <= nb; ++s) {
             const double each = double((tiles * s + kCus - 1) / kCus);
-            double us = ((nb + s - 1) / s + 2) * (each * kind.step_us > kind.alone_us ? each * kind.step_us : kind.alone_us);
+            double us = 2.0 + ((nb + s - 1) / s + 2) * (each * kind.step_us > kind.alone_us ? each * kind.step_us : kind.alone_us);
             if (s > 1) us += 4.0 + double(M) * N * (8 * s + 4) / 4.5e6;
             if (us < least) {
                 least = us;
