@@ -164,6 +164,8 @@ struct Best {
             for (; i < n; i += step) {
                 const int count = min(step, n - i);
                 const uint64_t mine = lane < top ? key : lane - top < count ? room.found[i + lane - top] : 0;
+                // (of many equal ones most are below: 64 x 294912 of one value 27 us, 44 without)
+                if (!__ballot(lane >= top && mine > read_lane(key, top - 1))) continue;
                 room.keys[lane] = key;
                 lds_order();
                 place(mine, above(mine, room.found + i, count) + above(mine, room.keys, top), top, room, lane);
