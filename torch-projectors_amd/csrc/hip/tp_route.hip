@@ -247,7 +247,8 @@ hipError_t sort(const I* ids, int64_t n, int E, int* order, int* slot, int* offs
 
 // ------------------------------------------------------------------ rows
 // Both directions go by rows, not places: W wavefronts take a row (or a stretch of it), whose k places they know,
-// so that the row is read (spread) or written (gather) once whatever k is.  Memory bound.  Values move 16 bytes a
+// so that the row is read (spread) or written (gather) once whatever k is.  Memory bound: 16384 x 4 rows of 4096
+// bfloat16 spread in 120 us (5.6 TB/s), gathered in 114 (5.9).  Values move 16 bytes a
 // lane at a time, whatever the rows' alignment; of up to KB choices the loads are in flight together, and the
 // products for the weights' gradient stay in registers.  More than KB choices: spread goes over the row again for
 // each KB of them (four at once are faster than eight: 16384 x 8 rows of 512 bfloat16 65 against 84 us with the

@@ -64,7 +64,7 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], int e) {
 }
 
 // 16 lanes per block of a row, eight values each.  Memory bound: reads each value once, writes a byte for it
-// (4096 x 16640 fp32 in 61 us, 5.6 TB/s).
+// (4096 x 16640 fp32 in 61 us, 5.6 TB/s; streamed loads take 64).
 template <class S>
 __global__ __launch_bounds__(256) void k_quantize(const typename S::Bits* __restrict__ x, int64_t rows, int64_t cols,
                                                   int64_t stride, int nb, int64_t srows, uint8_t* __restrict__ codes,
@@ -163,7 +163,7 @@ template <class O> __global__ __launch_bounds__(256) void k_scores_join(ScoreArg
 // Few images (at most 16 FM): as fast as the references' codes can be read.  A workgroup takes 16 references,
 // each of its wavefronts every eighth block of them, straight from memory into operands: kAhead blocks'
 // loads are in flight at once (8 KB a wavefront, 64 KB a CU).  One image against 4096 references of 16640
-// values: 14.8 us, 4.7 TB/s.
+// values: 14.9 us, 4.6 TB/s; against 64 to 2048 12 us, as 16 wavefronts take, too: what a CU can have on its way.
 constexpr int kFewWaves = 8, kAhead = 4;
 
 // A row that a wavefront quantises itself, block by block: no launch and no memory for its codes.
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
 }
 
 // The product in tiles: a workgroup of WM x WN x KW wavefronts computes BM x BN scores.  4096 x 8192 x 16640 by
-// tiles of 256 x 256 takes 810 to 850 us (1.31 to 1.38 PFLOP/s, the rate of a bfloat16 library product on this
+// tiles of 256 x 256 takes 775 to 855 us (1.31 to 1.44 PFLOP/s; a bfloat16 library product 1.40 on this
 // card): the matrix units are busy for two thirds of the cycles, at a clock that the power limit holds at 1.9 GHz.
 // Codes of one block of a tile's rows in LDS: 128 bytes a row, fragment after fragment (fragment f of a part of
 // the tile has its rows F r + f, r < 32), and the 16-byte chunks of a row permuted among themselves (chunk c of row
@@ -414,8 +414,8 @@ __global__ __launch_bounds__(64 * WM * WN * KW, BM * BN == 128 * 128 ? 4 : 1) vo
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
-    // two stages in turn: while one is multiplied the other is filled (three and four were no faster: a
-    // stage's loads take less than its products, and the LDS holds fewer workgroups)
+    // two stages in turn: while one is multiplied the other is filled (333 x 1999 x 8280 by tiles of 64 x 64: two
+    // 25.7 us, three 26.0, four 30.8, as the LDS then holds fewer workgroups)
     const int lane4 = lane * 4;
     const uint8_t *sa = g.sa + k0 * g.sra + m0, *sb = g.sb + k0 * g.srb + n0;  // the next block's scales
     auto load = [&](Stage<BM, BN>& st, int k) {
@@ -600,8 +600,8 @@ hipError_t launch_block_scores(const void* a, const void* sa, int64_t M, const v
     return out_dt == TP_F32 ? scores<F32>(g, p, s) : scores<BF16>(g, p, s);
 }
 
-// One image is quantised by k_scores_few itself: 256 references of 4224 values 7.6 us in two launches, 5.9 in
-// one; 4096 of 16640 18.5 and 14.8.
+// One image is quantised by k_scores_few itself: 256 references of 4224 values 7.1 us in two launches, 5.2 in
+// one; 4096 of 16640 17.8 and 15.2.
 // (the sums of the product's ranges, then codes and scales from a 16-byte boundary on)
 int64_t sums_before_codes(int64_t M, int64_t N, int64_t nb) { return (block_scores_work(M, N, nb) + 15) / 16 * 16; }
 int64_t score_images_work(int64_t M, int64_t N, int64_t cols) {
