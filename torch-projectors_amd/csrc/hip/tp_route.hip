@@ -253,7 +253,9 @@ hipError_t sort(const I* ids, int64_t n, int E, int* order, int* slot, int* offs
 // products for the weights' gradient stay in registers.  More than KB choices: spread goes over the row again for
 // each KB of them (four at once are faster than eight: 16384 x 8 rows of 512 bfloat16 65 against 84 us with the
 // weights' gradient), gather reads KB at a time and does the products in a second look (so there KB is up to eight:
-// 48 against 69 us).
+// 48 against 69 us).  Spread without that gradient has two stretches of the row on their way, gather where a row has one or
+// two choices (2048 x 2 rows of 4224 fp32 23.1 and 23.4 us, so 21.7 and 21.0; 65536 x 2 of 300 58 and 53, so 51 and 42; but
+// gathers of four choices, 16384 x 4 of 4096 bfloat16, 120 us and 126).
 template <class S> struct Values {
     static constexpr int n = Pack<S>::n;
     float v[n];
@@ -346,7 +348,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int
                                                                 typename S::Bits* __restrict__ sorted,
                                                                 const typename S::Bits* __restrict__ rows,
                                                                 float* __restrict__ d_weights) {
-    constexpr int n = Values<S>::n, items = W == 1 ? 4 : 1;
+    constexpr int n = Values<S>::n, items = W == 1 ? 4 : 1, step = W * 64 * n, U = DOT ? 1 : 2;
     __shared__ float lds[W][KB];
     const int kept = *a.kept, lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
     for (int64_t item0 = int64_t(blockIdx.x) * items; item0 < a.T * parts; item0 += int64_t(gridDim.x) * items) {
@@ -355,28 +357,35 @@ __global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int
         for (int j0 = 0; j0 < a.k; j0 += KB) {
             const Places<KB> p = places_of<KB>(a, r.t, j0, kept);
             float dot[KB] = {};
-            for (int64_t d = r.d0 + lane * n; d < r.d1; d += W * 64 * n) {
-                const int64_t left = r.d1 - d;
-                const Values<S> v = load_values<S>(x + r.t * a.D + d, left, stream && a.k <= KB);
-                Values<S> o[KB];
-                if (DOT) {
+            for (int64_t d0 = r.d0 + lane * n; d0 < r.d1; d0 += U * step) {
+                Values<S> v[U];
 #pragma unroll
-                    for (int u = 0; u < KB; ++u) {
-                        if (p.in[u]) o[u] = load_values<S>(rows + p.at[u] + d, left, stream);
-                        else o[u] = Values<S>{};
+                for (int e = 0; e < U; ++e)
+                    v[e] = load_values<S>(x + r.t * a.D + d0 + e * step, r.d1 - d0 - e * step, stream && a.k <= KB);
+#pragma unroll
+                for (int e = 0; e < U; ++e) {
+                    const int64_t d = d0 + e * step, left = r.d1 - d;
+                    if (left <= 0) break;
+                    Values<S> o[KB];
+                    if (DOT) {
+#pragma unroll
+                        for (int u = 0; u < KB; ++u) {
+                            if (p.in[u]) o[u] = load_values<S>(rows + p.at[u] + d, left, stream);
+                            else o[u] = Values<S>{};
+                        }
+#pragma unroll
+                        for (int u = 0; u < KB; ++u)
+                            if (p.in[u])
+#pragma unroll
+                                for (int i = 0; i < n; ++i) dot[u] = __builtin_fmaf(v[e].v[i], o[u].v[i], dot[u]);
                     }
 #pragma unroll
-                    for (int u = 0; u < KB; ++u)
-                        if (p.in[u])
+                    for (int u = 0; u < KB; ++u) {
+                        if (!p.real[u]) continue;
 #pragma unroll
-                            for (int i = 0; i < n; ++i) dot[u] = __builtin_fmaf(v.v[i], o[u].v[i], dot[u]);
-                }
-#pragma unroll
-                for (int u = 0; u < KB; ++u) {
-                    if (!p.real[u]) continue;
-#pragma unroll
-                    for (int i = 0; i < n; ++i) o[u].v[i] = p.in[u] ? p.w[u] * v.v[i] : 0.0f;
-                    store_values<S>(sorted + p.at[u] + d, left, o[u], stream);
+                        for (int i = 0; i < n; ++i) o[u].v[i] = p.in[u] ? p.w[u] * v[e].v[i] : 0.0f;
+                        store_values<S>(sorted + p.at[u] + d, left, o[u], stream);
+                    }
                 }
             }
             if (DOT) {
@@ -396,7 +405,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
                                                                 typename S::Bits* __restrict__ out,
                                                                 const typename S::Bits* __restrict__ x,
                                                                 float* __restrict__ d_weights) {
-    constexpr int n = Values<S>::n, items = W == 1 ? 4 : 1;
+    constexpr int n = Values<S>::n, items = W == 1 ? 4 : 1, step = W * 64 * n, U = 2;
     __shared__ float lds[W][KB];
     const int kept = a.k ? *a.kept : 0, lane = W == 1 ? threadIdx.x & 63 : threadIdx.x;
     for (int64_t item0 = int64_t(blockIdx.x) * items; item0 < a.T * parts; item0 += int64_t(gridDim.x) * items) {
@@ -404,7 +413,31 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
         if (!row_item<W>(a, item0, span, parts, r)) break;
         Places<KB> p = places_of<KB>(a, r.t, 0, kept);
         float dot[KB] = {};
-        for (int64_t d = r.d0 + lane * n; d < r.d1; d += W * 64 * n) {
+        constexpr bool two = !DOT && KB == 2;  // stretches at once (the row has no more choices then)
+        if (two)
+            for (int64_t d0 = r.d0 + lane * n; d0 < r.d1; d0 += U * step) {
+                Values<S> o[U][KB];
+#pragma unroll
+                for (int e = 0; e < U; ++e)
+#pragma unroll
+                    for (int u = 0; u < KB; ++u) {
+                        if (p.in[u]) o[e][u] = load_values<S>(rows + p.at[u] + d0 + e * step, r.d1 - d0 - e * step, stream);
+                        else o[e][u] = Values<S>{};
+                    }
+#pragma unroll
+                for (int e = 0; e < U; ++e) {
+                    const int64_t d = d0 + e * step, left = r.d1 - d;
+                    if (left <= 0) break;
+                    Values<S> sum{};
+#pragma unroll
+                    for (int u = 0; u < KB; ++u)
+                        if (p.in[u])
+#pragma unroll
+                            for (int i = 0; i < n; ++i) sum.v[i] += p.w[u] * o[e][u].v[i];
+                    store_values<S>(out + r.t * a.D + d, left, sum, stream);
+                }
+            }
+        for (int64_t d = two ? r.d1 : r.d0 + lane * n; d < r.d1; d += step) {
             const int64_t left = r.d1 - d;
             Values<S> sum{}, v{}, o[KB];
             for (int j0 = 0; j0 < a.k; j0 += KB) {
@@ -432,7 +465,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
                 p = places_of<KB>(a, r.t, j0, kept);
 #pragma unroll
                 for (int u = 0; u < KB; ++u) dot[u] = 0.0f;
-                for (int64_t d = r.d0 + lane * n; d < r.d1; d += W * 64 * n) {
+                for (int64_t d = r.d0 + lane * n; d < r.d1; d += step) {
                     const int64_t left = r.d1 - d;
                     const Values<S> v = load_values<S>(x + r.t * a.D + d, left, stream);
 #pragma unroll
@@ -473,7 +506,7 @@ RowPlan row_plan(const RouteArgs& a, int size, bool dot) {
     RowPlan p{bytes <= 2560 ? 1 : 4, 1, a.D};
     if (a.T * p.waves >= 2048 || bytes <= 1024) return p;
     if (dot) {
-        p.waves = p.waves == 1 ? 4 : 16;
+        p.waves = bytes <= 4096 ? 4 : 16;
         return p;
     }
     p.waves = 1;
@@ -483,11 +516,11 @@ RowPlan row_plan(const RouteArgs& a, int size, bool dot) {
     return p;
 }
 
-#define TP_ROWS(kernel, W, KB)                                                                                      \
-    (dot ? kernel<S, W, KB, true><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, stream, in, to, other,        \
-                                                                          d_weights)                                \
-         : kernel<S, W, KB, false><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, stream, in, to, nullptr,      \
-                                                                           nullptr))
+#define TP_ROWS_DOT(kernel, W, KB) \
+    kernel<S, W, KB, true><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, stream, in, to, other, d_weights)
+#define TP_ROWS(kernel, W, KB)                                                                                       \
+    (dot ? TP_ROWS_DOT(kernel, W, KB)                                                                                \
+         : kernel<S, W, KB, false><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, stream, in, to, nullptr, nullptr))
 #define TP_ROWS_BY_K(kernel, W) (a.k <= 2 ? TP_ROWS(kernel, W, 2) : TP_ROWS(kernel, W, 4))
 
 template <class S, bool SPREAD>
@@ -506,9 +539,9 @@ hipError_t move_rows(const RouteArgs& a, const void* in_, void* to_, const void*
         else if (p.waves == 4) TP_ROWS_BY_K(k_spread_rows, 4);
         else TP_ROWS_BY_K(k_spread_rows, 16);
     } else if (dot && a.k > 4) {
-        if (p.waves == 1) TP_ROWS(k_gather_rows, 1, 8);
-        else if (p.waves == 4) TP_ROWS(k_gather_rows, 4, 8);
-        else TP_ROWS(k_gather_rows, 16, 4);  // (8 do not fit its registers)
+        if (p.waves == 1) TP_ROWS_DOT(k_gather_rows, 1, 8);
+        else if (p.waves == 4) TP_ROWS_DOT(k_gather_rows, 4, 8);
+        else TP_ROWS_DOT(k_gather_rows, 16, 4);  // (8 do not fit its registers)
     } else {
         if (p.waves == 1) TP_ROWS_BY_K(k_gather_rows, 1);
         else if (p.waves == 4) TP_ROWS_BY_K(k_gather_rows, 4);
@@ -517,6 +550,7 @@ hipError_t move_rows(const RouteArgs& a, const void* in_, void* to_, const void*
     return hipGetLastError();
 }
 #undef TP_ROWS
+#undef TP_ROWS_DOT
 #undef TP_ROWS_BY_K
 
 }  // namespace
