@@ -563,10 +563,12 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
             if (index_at(j) != -1) all -= up_at(j);
         all = wave_sum(all) + dL;
         // the gradient of score f without what is given or listed there, c p (all - dH (ln p + H)); 0 where not allowed,
-        // and everywhere in a row that allows nothing; NaN in a row with a NaN or +inf
+        // and everywhere in a row that allows nothing; NaN where allowed in a row with a NaN or +inf
         const bool plain = !none && ls == ls;
         const float at_0 = plain ? c * __builtin_fmaf(-dH, H, all) : none ? 0.0f : __builtin_nanf("");
         const float slope = plain ? c * -dH * kLn2 : 0.0f;
+        // (where a factor is not finite, 0 times it is not 0)
+        const bool all_finite = !__ballot(!isfinite(at_0) || !isfinite(slope));
         auto smooth = [&](float f) {
             const float lp2 = fmaxf((f - m) * c2 - ls2, -200.0f);
             return __builtin_amdgcn_exp2f(lp2) * __builtin_fmaf(slope, lp2, at_0);
@@ -579,6 +581,10 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
                 Pack<S> w;
 #pragma unroll
                 for (int i = 0; i < P; ++i) w.v[i] = S::round(smooth(f[p * P + i]));
+                if (!all_finite)
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        if (f[p * P + i] == neg_inf()) w.v[i] = 0;
                 const int64_t v = tile_index<S>(v0, lane, p * P);
                 if (v + P <= end) {
                     if (stream) stream_pack<S>(d + v, w);
