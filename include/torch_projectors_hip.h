@@ -348,7 +348,8 @@ int tp_log_probs(int dtype, const void* scores, int64_t rows, int64_t candidates
                  void* top_index, void* stats, void* work, int64_t work_bytes, void* stream);
 
 /* d_scores [rows, candidates] (row-major, of `dtype`) from the upstream gradients
- * of the four fp32 outputs, each optional; zero where masked. */
+ * of the four fp32 outputs, each optional; zero where masked.  A given index out
+ * of range other than -1 makes its row's NaN unless its upstream gradient is 0. */
 int tp_log_probs_back(int dtype, const void* scores, int64_t rows, int64_t candidates, int64_t row_stride,
                       const void* given, int64_t givens, const void* mask, int64_t mask_stride, int64_t top,
                       double temperature, const void* top_index, const void* stats, const void* d_given,

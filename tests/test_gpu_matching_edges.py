@@ -41,3 +41,33 @@ def test_masked_places_have_no_gradient_in_rows_that_are_not_finite(m, V, dtype)
     allowed[7] = False
     assert torch.isfinite(d[0]).all() and d[1:4, allowed].isnan().all()
     assert not torch.isfinite(d[4, allowed]).any()
+
+
+@pytest.mark.parametrize("G", [1, 3, 90])
+@pytest.mark.parametrize("index", [300, 10 ** 12, -2, -(2 ** 63)])
+def test_gradient_of_given_candidates_out_of_range(m, index, G):
+    """Their log probability is NaN, and so is the gradient of their row, but for masked places; of a result that has no
+    share in the loss (an upstream gradient of 0) there is none."""
+    V = 300
+    x = torch.randn(4, V, generator=gen(2))
+    mask = torch.rand(V, generator=gen(3)) < 0.8
+    given = torch.randint(0, V, (4, G), generator=gen(4))
+    mask[given.flatten()] = True
+    mask[5] = False
+    given[given == 5] = -1
+    fine = given.clone()
+    given[1:, G // 2] = index
+    fine[1:, G // 2] = -1
+    up = torch.randn(4, G, generator=gen(5))
+    up[2, G // 2] = 0.0
+
+    def gradient(which):
+        s = x.to(DEV).requires_grad_()
+        out = m.log_probs(s, which.to(DEV), mask=mask.to(DEV))
+        return out.given.detach().cpu(), torch.autograd.grad(out.given, s, up.to(DEV))[0].cpu()
+
+    got, d = gradient(given)
+    want, d_fine = gradient(fine)
+    assert got[1:, G // 2].isnan().all() and int(got.isnan().sum()) == 3
+    assert torch.equal(d[[0, 2]], d_fine[[0, 2]]) and torch.isfinite(d[[0, 2]]).all()
+    assert d[[1, 3]][:, mask].isnan().all() and (d[:, ~mask] == 0).all()

@@ -548,6 +548,11 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
         const int64_t n = G + K;
         auto index_at = [&](int64_t j) { return j < G ? a.given[t * G + j] : top_index[t * K + j - G]; };
         auto up_at = [&](int64_t j) { return j < G ? d_given[t * G + j] : d_top[t * K + j - G]; };
+        // what a candidate takes from the row's sum: nothing for -1, and of one out of range, whose log probability
+        // is NaN, a NaN unless its upstream gradient is 0
+        auto share = [&](int64_t v, float up) {
+            return v == -1 ? 0.0f : (v >= 0 && v < a.V) || up == 0.0f ? up : __builtin_nanf("");
+        };
         const int64_t mine = lane < n ? index_at(lane) : -1;
         const float up = lane < n ? up_at(lane) : 0.0f;
         const float4 st = *reinterpret_cast<const float4*>(stats + t * kProbsStats);
@@ -558,9 +563,8 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
         const float at_mine = fix ? S::widen(x[mine]) : 0.0f;
         const float m = st.x, ls = st.y, H = st.z, ls2 = ls * kLog2e;
         const bool none = m == neg_inf();
-        float all = mine != -1 ? -up : 0.0f;
-        for (int64_t j = lane + 64; j < n; j += 64)
-            if (index_at(j) != -1) all -= up_at(j);
+        float all = -share(mine, up);
+        for (int64_t j = lane + 64; j < n; j += 64) all -= share(index_at(j), up_at(j));
         all = wave_sum(all) + dL;
         // the gradient of score f without what is given or listed there, c p (all - dH (ln p + H)); 0 where not allowed,
         // and everywhere in a row that allows nothing; NaN where allowed in a row with a NaN or +inf

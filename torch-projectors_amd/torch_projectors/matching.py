@@ -103,7 +103,8 @@ def log_probs(scores: torch.Tensor, given: Optional[torch.Tensor] = None, top: i
     """Log probabilities of the softmax of scores [..., V] / temperature (float32, float16 or bfloat16).
 
     given   int64 [...] or [..., G]: the candidates whose log probability is wanted; -1 for none (its
-            result is 0 and has no gradient), NaN for any other index out of range
+            result is 0 and has no gradient); any other index out of range gives NaN, and a row of NaN
+            gradients unless its own upstream gradient is 0
     top     how many of the best candidates to list, at most 64
     mask    bool [V] or of the scores' shape, True where allowed; what masked scores hold is not used
 
