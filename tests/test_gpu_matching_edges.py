@@ -71,3 +71,71 @@ def test_gradient_of_given_candidates_out_of_range(m, index, G):
     assert got[1:, G // 2].isnan().all() and int(got.isnan().sum()) == 3
     assert torch.equal(d[[0, 2]], d_fine[[0, 2]]) and torch.isfinite(d[[0, 2]]).all()
     assert d[[1, 3]][:, mask].isnan().all() and (d[:, ~mask] == 0).all()
+
+
+def _gradient_in_64_bits(x, given, mask, top_index, temperature, d_given, d_top):
+    """(d_scores, tolerance) from the formula, on the GPU.  An fp32 sum of n values is at most n 2^-24 of their
+    magnitudes off; p is 1e-5 off, as are its logarithm and the entropy (which carry no gradient here)."""
+    z = x.double() / temperature
+    if mask is not None:
+        z = z.masked_fill(~mask, -math.inf)
+    p = torch.softmax(z, 1)
+    at, mag, count = (torch.zeros_like(p) for _ in range(3))
+    for index, up in ((given, d_given.double()), (top_index, d_top.double())):
+        ok = index >= 0
+        safe = index.clamp_min(0)
+        up = torch.where(ok, up, 0.0)
+        at.scatter_add_(1, safe, up)
+        mag.scatter_add_(1, safe, up.abs())
+        count.scatter_add_(1, safe, ok.double())
+    n = given.shape[1] + top_index.shape[1]
+    total, size = at.sum(1, keepdim=True), mag.sum(1, keepdim=True)
+    if mask is not None:
+        at, mag = at.masked_fill(~mask, 0.0), mag.masked_fill(~mask, 0.0)
+    want = (at - p * total) / temperature
+    u = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}[x.dtype]
+    tol = ((count + 4) * 2.0 ** -24 * mag + p * (1e-5 + (n / 64 + 8) * 2.0 ** -24) * size) / temperature
+    return want, tol + 1.01 * u * want.abs() + (2.0 ** -25 if x.dtype == F16 else 1e-37)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T,V,G,places", [(3, 700, 5000, 700), (2, 5003, 3000, 5003), (2, 9000, 3001, 7), (5, 2049, 61, 2049),
+                                          (2, 40001, 40001, 40001), (3, 1, 200, 1), (300, 3100, 130, 3100)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_gradient_of_thousands_of_given_candidates(m, T, V, G, places, masked, dtype):
+    """More given and listed candidates than lanes, with repeats within and between groups of lanes, -1 among them."""
+    g = gen(V + G)
+    x = (torch.randn(T, V, generator=g) * 2).to(dtype).to(DEV)
+    given = (torch.randint(0, places, (T, G), generator=g) * 131 % V).to(DEV)
+    given[torch.rand(T, G, generator=g).to(DEV) < 0.1] = -1
+    mask = (torch.rand(T, V, generator=g) < 0.7).to(DEV) if masked and V > 1 else None
+    if mask is not None:
+        mask[:, 0] = True
+    top = min(V, 7)
+    d_given, d_top = torch.randn(T, G, generator=g).to(DEV), torch.randn(T, top, generator=g).to(DEV)
+    s = x.clone().requires_grad_()
+    out = m.log_probs(s, given, top=top, temperature=1.7, mask=mask)
+    (d,) = torch.autograd.grad([out.given, out.top], [s], [d_given, d_top], retain_graph=True)
+    want, tol = _gradient_in_64_bits(x, given, mask, out.top_index, 1.7, d_given, d_top)
+    off = (d.double() - want).abs() - tol
+    assert float(off.max()) <= 0, float(off.max())
+    (again,) = torch.autograd.grad([out.given, out.top], [s], [d_given, d_top])
+    assert torch.equal(d, again)
+
+
+def test_gradient_of_given_candidates_is_not_quadratic_in_their_number(m):
+    """Every candidate given: 16384 of 16384 in four rows are 1 MB of inputs, a fraction of a millisecond's work; each
+    walked for each other would be 1e9 loads, over a tenth of a second."""
+    T, V = 4, 16384
+    x = torch.randn(T, V, generator=gen(6)).to(DEV).requires_grad_()
+    out = m.log_probs(x, torch.randint(0, V, (T, V), generator=gen(7)).to(DEV))
+    up = torch.ones_like(out.given)
+    ms = []
+    for _ in range(4):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        torch.autograd.grad(out.given, x, up, retain_graph=True)
+        end.record()
+        torch.cuda.synchronize()
+        ms.append(start.elapsed_time(end))
+    assert min(ms) < 10, ms

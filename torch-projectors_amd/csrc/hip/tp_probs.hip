@@ -523,9 +523,20 @@ ProbsPlan probs_plan(int64_t T, int64_t V) {
 // The gradient: a wavefront per stretch of a row.  Every score's share but that of the given and listed ones first,
 // then those scores' once more with it, each by one lane.  Memory bound: reads and writes each score once
 // (4096 x 36864 fp32 192 us, 6.3 TB/s).
+//
+// MANY, more than 64 given and listed candidates of a row: each wavefront walks all of them once, 64 at a time, and adds
+// what falls into its stretch up in LDS, in the order of the candidates (so that the result is always the same): lanes
+// with places of their own at once, of lanes that share a place all of them by one.  Each candidate is so read once for
+// each 2048 scores of its row (or fewer, a stretch), and added once: 4096 x 4300 fp32 with 65 given 26 us, 1024 57; 512 x
+// 36864 with 65 27, 4096 137, 36864 1250, bound by the walks (18 of each row's candidates).
 constexpr int kBackBlock = 256, kBackWaves = kBackBlock / 64;
+constexpr int kManySpan = 2048;
+struct alignas(16) ManyRoom {
+    float added[kManySpan];  // upstream gradients at the places of the stretch
+    uint8_t owner[kManySpan];
+};
 
-template <class S>
+template <class S, bool MANY>
 __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t span, bool stream, const float* __restrict__ stats,
                                                             const int64_t* __restrict__ top_index,
                                                             const float* __restrict__ d_given,
@@ -533,6 +544,7 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
                                                             const float* __restrict__ d_log_sum,
                                                             const float* __restrict__ d_top,
                                                             typename S::Bits* __restrict__ d_scores) {
+    __shared__ ManyRoom rooms[MANY ? kBackWaves : 1];
     const int lane = threadIdx.x & 63;
     const float c = a.c, c2 = a.c2;
     const int64_t G = d_given ? a.G : 0;
@@ -544,27 +556,57 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
         const auto* x = static_cast<const typename S::Bits*>(a.scores) + t * a.stride;
         auto* d = d_scores + t * a.V;
         const uint8_t* mask = a.mask ? a.mask + t * a.mask_stride : nullptr;
-        // a lane's given or listed candidate and its upstream gradient (the first 64; more are read again below)
         const int64_t n = G + K;
-        auto index_at = [&](int64_t j) { return j < G ? a.given[t * G + j] : top_index[t * K + j - G]; };
-        auto up_at = [&](int64_t j) { return j < G ? d_given[t * G + j] : d_top[t * K + j - G]; };
+        auto index_at = [&](int64_t j) { return j < G ? a.given[t * G + j] : j < n ? top_index[t * K + j - G] : -1; };
+        auto up_at = [&](int64_t j) { return j < G ? d_given[t * G + j] : j < n ? d_top[t * K + j - G] : 0.0f; };
         // what a candidate takes from the row's sum: nothing for -1, and of one out of range, whose log probability
         // is NaN, a NaN unless its upstream gradient is 0
         auto share = [&](int64_t v, float up) {
             return v == -1 ? 0.0f : (v >= 0 && v < a.V) || up == 0.0f ? up : __builtin_nanf("");
         };
-        const int64_t mine = lane < n ? index_at(lane) : -1;
-        const float up = lane < n ? up_at(lane) : 0.0f;
+        // a lane's given or listed candidate and its upstream gradient
+        const int64_t mine = MANY ? -1 : index_at(lane);
+        const float up = MANY ? 0.0f : up_at(lane);
         const float4 st = *reinterpret_cast<const float4*>(stats + t * kProbsStats);
         const float dL = d_log_sum ? d_log_sum[t] : 0.0f, dH = d_entropy ? d_entropy[t] : 0.0f;
         float f[kLaneScores];
         load_tile<S>(x, mask, first, end, stream, lane, f);
-        const bool fix = mine >= first && mine < end && !(mask && !mask[mine]);
+        auto here = [&](int64_t v) { return v >= first && v < end && !(mask && !mask[v]); };
+        const bool fix = here(mine);
         const float at_mine = fix ? S::widen(x[mine]) : 0.0f;
         const float m = st.x, ls = st.y, H = st.z, ls2 = ls * kLog2e;
         const bool none = m == neg_inf();
         float all = -share(mine, up);
-        for (int64_t j = lane + 64; j < n; j += 64) all -= share(index_at(j), up_at(j));
+        if constexpr (MANY) {
+            ManyRoom& room = rooms[threadIdx.x >> 6];
+            for (int i = 4 * lane; i < kManySpan; i += 256) *reinterpret_cast<float4*>(room.added + i) = float4{};
+            lds_order();
+            for (int64_t j0 = 0; j0 < n; j0 += 64) {
+                const int64_t v = index_at(j0 + lane);
+                const float u = up_at(j0 + lane);
+                all -= share(v, u);
+                const bool in = here(v);
+                uint64_t left = __ballot(in);
+                if (!left) continue;
+                const int place = in ? int(v - first) : 0;
+                // one lane's number stays at a place that several share
+                if (in) room.owner[place] = uint8_t(lane);
+                lds_order();
+                uint64_t shared = __ballot(in && room.owner[place] != lane);
+                lds_order();
+                while (shared) {
+                    const int at = int(read_lane(uint32_t(place), __ffsll(static_cast<unsigned long long>(shared)) - 1));
+                    const uint64_t same = __ballot(in && place == at);
+                    const float sum = wave_sum(in && place == at ? u : 0.0f);
+                    if (lane == 0) room.added[at] += sum;
+                    lds_order();
+                    left &= ~same;
+                    shared &= ~same;
+                }
+                if (left >> lane & 1) room.added[place] += u;
+                lds_order();
+            }
+        }
         all = wave_sum(all) + dL;
         // the gradient of score f without what is given or listed there, c p (all - dH (ln p + H)); 0 where not allowed,
         // and everywhere in a row that allows nothing; NaN where allowed in a row with a NaN or +inf
@@ -582,14 +624,22 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
             constexpr int P = Pack<S>::n;
 #pragma unroll
             for (int p = 0; p < kLaneScores / P; ++p) {
-                Pack<S> w;
+                const int64_t v = tile_index<S>(v0, lane, p * P);
+                float g[P];
 #pragma unroll
-                for (int i = 0; i < P; ++i) w.v[i] = S::round(smooth(f[p * P + i]));
+                for (int i = 0; i < P; ++i) g[i] = smooth(f[p * P + i]);
                 if (!all_finite)
 #pragma unroll
                     for (int i = 0; i < P; ++i)
-                        if (f[p * P + i] == neg_inf()) w.v[i] = 0;
-                const int64_t v = tile_index<S>(v0, lane, p * P);
+                        if (f[p * P + i] == neg_inf()) g[i] = 0.0f;
+                if constexpr (MANY)
+                    if (plain)
+#pragma unroll
+                        for (int i = 0; i < P; ++i)
+                            g[i] = __builtin_fmaf(c, rooms[threadIdx.x >> 6].added[v - first + i], g[i]);
+                Pack<S> w;
+#pragma unroll
+                for (int i = 0; i < P; ++i) w.v[i] = S::round(g[i]);
                 if (v + P <= end) {
                     if (stream) stream_pack<S>(d + v, w);
                     else store_pack<S>(d + v, w);
@@ -600,10 +650,11 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
                 }
             }
         }
-        if (!plain) continue;
-        // (the stores above come before those below: one wavefront's, in order)
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (n <= 64) {
+        if constexpr (MANY) {
+            lds_order();
+        } else if (plain) {
+            // (the stores above come before those below: one wavefront's, in order)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             // what is given or listed at the same score is summed by the first lane that holds it
             float sum = 0.0f;
             bool is_first = true;
@@ -613,19 +664,6 @@ __global__ __launch_bounds__(kBackBlock) void k_probs_back(ProbsArgs a, int64_t 
                 if (same && l < lane) is_first = false;
             }
             if (fix && is_first) d[mine] = S::round(__builtin_fmaf(c, sum, smooth(at_mine)));
-            continue;
-        }
-        for (int64_t i = lane; i < n; i += 64) {
-            const int64_t v = index_at(i);
-            if (v < first || v >= end || (mask && !mask[v])) continue;
-            float sum = 0.0f;
-            bool is_first = true;
-            for (int64_t j = 0; j < n; ++j)
-                if (index_at(j) == v) {
-                    if (j < i) is_first = false;
-                    sum += up_at(j);
-                }
-            if (is_first) d[v] = S::round(__builtin_fmaf(c, sum, smooth(S::widen(x[v]))));
         }
     }
 }
@@ -671,8 +709,10 @@ template <class S>
 hipError_t probs_back(const ProbsArgs& a, const float* stats, const int64_t* top_index, const float* d_given,
                       const float* d_entropy, const float* d_log_sum, const float* d_top, void* d_scores,
                       hipStream_t s) {
-    const int64_t span = back_span(a, sizeof(typename S::Bits)), items = a.T * ((a.V + span - 1) / span);
-    k_probs_back<S><<<match_grid((items + kBackWaves - 1) / kBackWaves), kBackBlock, 0, s>>>(
+    const bool many = (d_given ? a.G : 0) + (d_top ? a.top : 0) > 64;
+    const int64_t best = back_span(a, sizeof(typename S::Bits)), span = many ? std::min<int64_t>(best, kManySpan) : best;
+    const int64_t items = a.T * ((a.V + span - 1) / span);
+    (many ? k_probs_back<S, true> : k_probs_back<S, false>)<<<match_grid((items + kBackWaves - 1) / kBackWaves), kBackBlock, 0, s>>>(
         a, span, streams(a, sizeof(typename S::Bits)), stats, top_index, d_given, d_entropy, d_log_sum, d_top, static_cast<typename S::Bits*>(d_scores));
     return hipGetLastError();
 }
