@@ -139,3 +139,26 @@ def test_gradient_of_given_candidates_is_not_quadratic_in_their_number(m):
         torch.cuda.synchronize()
         ms.append(start.elapsed_time(end))
     assert min(ms) < 10, ms
+
+
+@pytest.mark.parametrize("T,D", [(4, 33), (600, 2049)])
+def test_places_from_elsewhere_leave_the_last_row_alone(m, T, D):
+    """Slots outside the sorted rows write nothing: not to the last place either, which is another row's."""
+    order = m.sort_by_class(torch.zeros(T, dtype=torch.int64, device=DEV), 1)
+    slot = torch.arange(T, dtype=torch.int32).flip(0).view(T, 1)
+    bad = torch.arange(1, T, 2)
+    slot[bad, 0] = torch.tensor([-5, T, 1 << 30, -(2 ** 31)], dtype=torch.int32)[torch.arange(len(bad)) % 4]
+    foreign = order._replace(slot=slot.to(DEV))
+    x = torch.randn(T, D, generator=gen(8))
+    w = torch.rand(T, 1, generator=gen(9))
+    gx, gw = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    s = m.dispatch(gx, foreign, gw)
+    good = torch.arange(0, T, 2)
+    at = slot[good, 0].long()
+    assert at.max() == T - 1
+    assert torch.equal(s.detach().cpu()[at], w[good] * x[good])
+    up = torch.randn(T, D, generator=gen(10))
+    dx, dw = torch.autograd.grad(s, (gx, gw), up.to(DEV))
+    assert torch.equal(dx.cpu()[good], w[good] * up[at]) and (dx[bad] == 0).all() and (dw[bad] == 0).all()
+    y = m.combine(s.detach(), foreign, gw).detach().cpu()
+    assert torch.equal(y[good], w[good] * (w[good] * x[good])) and (y[bad] == 0).all()

@@ -292,7 +292,7 @@ __device__ __forceinline__ void store_values(typename S::Bits* p, int64_t left, 
 template <int KB> struct Places {
     int64_t at[KB];  // first value of the row there
     float w[KB];
-    bool in[KB], real[KB];  // is not dropped; is a choice at all
+    bool in[KB], real[KB];  // is not dropped; has a place at all
 };
 template <int KB>
 __device__ __forceinline__ Places<KB> places_of(const RouteArgs& a, int64_t t, int j0, int kept) {
@@ -300,12 +300,14 @@ __device__ __forceinline__ Places<KB> places_of(const RouteArgs& a, int64_t t, i
 #pragma unroll
     for (int u = 0; u < KB; ++u) {
         const int64_t s = t * a.k + j0 + u;
-        p.real[u] = j0 + u < a.k;
-        const uint32_t at = p.real[u] ? uint32_t(a.slot[s]) : 0u, last = uint32_t(a.T * a.k) - 1u;
-        // (a place from elsewhere is read nowhere, and not written outside the sorted rows)
-        p.in[u] = p.real[u] && at < uint32_t(kept) && at <= last;
+        const bool choice = j0 + u < a.k;
+        const uint32_t at = choice ? uint32_t(a.slot[s]) : 0u, last = uint32_t(a.T * a.k) - 1u;
+        // (a place outside the sorted rows, of an order from elsewhere, is neither read nor written: a row of zeros for
+        // it at the last place would meet the row that has that place)
+        p.real[u] = choice && at <= last;
+        p.in[u] = p.real[u] && at < uint32_t(kept);
         p.at[u] = int64_t(min(at, last)) * a.D;
-        p.w[u] = p.real[u] && a.weights ? a.weights[s] : 1.0f;
+        p.w[u] = choice && a.weights ? a.weights[s] : 1.0f;
     }
     return p;
 }
@@ -394,7 +396,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int
                 if (lane == 0)
 #pragma unroll
                     for (int u = 0; u < KB; ++u)
-                        if (p.real[u]) d_weights[r.t * a.k + j0 + u] = dot[u];
+                        if (j0 + u < a.k) d_weights[r.t * a.k + j0 + u] = dot[u];
             }
         }
     }
@@ -482,7 +484,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
             if (lane == 0)
 #pragma unroll
                 for (int u = 0; u < KB; ++u)
-                    if (p.real[u]) d_weights[r.t * a.k + j0 + u] = dot[u];
+                    if (j0 + u < a.k) d_weights[r.t * a.k + j0 + u] = dot[u];
         }
     }
 }
