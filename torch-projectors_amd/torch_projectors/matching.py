@@ -67,17 +67,19 @@ def block_scores(images, references, bias: Optional[torch.Tensor] = None,
                  out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """scores[m, n] = <image m, reference n> + bias[n], from 8-bit blocks, summed in float32.
 
-    images [M, ...] and references [N, ...] are BlockScaled, or rows that are quantised here; of complex
+    images [M, ...] and references [N, ...] are BlockScaled, or rows that are quantised here, of as many
+    values on both sides (BlockScaled rows hold zeros past theirs: of them the numbers of blocks are compared); of complex
     rows the real part of the inner product is taken (their real pairs' product).  With rfft images,
     which hold one half of a symmetric plane, scale either side's columns other than x = 0 and n / 2 by two for the
     whole plane's product; with bias = -|reference|^2 / 2 the scores are the log likelihoods of unit noise
     up to a constant per image.  bias float32 [N]; out_dtype float32 or bfloat16.  Not differentiable."""
+    rows = None if isinstance(images, BlockScaled) else _real_rows(images, "images")
     if not isinstance(references, BlockScaled):
+        references = _real_rows(references, "references")
+        if rows is not None and rows.shape[1] != references.shape[1]:
+            raise ValueError(f"Images of {rows.shape[1]} values do not fit references of {references.shape[1]}")
         references = quantize_blocks(references)
-    if isinstance(images, BlockScaled):
-        images, image_scales = images
-    else:
-        images, image_scales = _real_rows(images, "images"), None
+    images, image_scales = images if rows is None else (rows, None)
     return _OPS.block_scores.default(images, image_scales, references.codes, references.scales, bias, out_dtype)
 
 
