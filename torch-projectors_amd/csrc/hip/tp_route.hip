@@ -524,6 +524,7 @@ RowPlan row_plan(const RouteArgs& a, int size, bool dot) {
 #define TP_ROWS(kernel, W, KB)                                                                                       \
     (dot ? TP_ROWS_DOT(kernel, W, KB)                                                                                \
          : kernel<S, W, KB, false><<<grid, row_block<W>(), 0, s>>>(a, p.span, p.parts, stream, in, to, nullptr, nullptr))
+#define TP_ROWS_16(kernel) (a.k <= 2 ? TP_ROWS_DOT(kernel, 16, 2) : TP_ROWS_DOT(kernel, 16, 4))  // (by the gradient only)
 #define TP_ROWS_BY_K(kernel, W) (a.k <= 2 ? TP_ROWS(kernel, W, 2) : TP_ROWS(kernel, W, 4))
 
 template <class S, bool SPREAD>
@@ -540,7 +541,7 @@ hipError_t move_rows(const RouteArgs& a, const void* in_, void* to_, const void*
     if (SPREAD) {
         if (p.waves == 1) TP_ROWS_BY_K(k_spread_rows, 1);
         else if (p.waves == 4) TP_ROWS_BY_K(k_spread_rows, 4);
-        else TP_ROWS_BY_K(k_spread_rows, 16);
+        else TP_ROWS_16(k_spread_rows);
     } else if (dot && a.k > 4) {
         if (p.waves == 1) TP_ROWS_DOT(k_gather_rows, 1, 8);
         else if (p.waves == 4) TP_ROWS_DOT(k_gather_rows, 4, 8);
@@ -548,12 +549,13 @@ hipError_t move_rows(const RouteArgs& a, const void* in_, void* to_, const void*
     } else {
         if (p.waves == 1) TP_ROWS_BY_K(k_gather_rows, 1);
         else if (p.waves == 4) TP_ROWS_BY_K(k_gather_rows, 4);
-        else TP_ROWS_BY_K(k_gather_rows, 16);
+        else TP_ROWS_16(k_gather_rows);
     }
     return hipGetLastError();
 }
 #undef TP_ROWS
 #undef TP_ROWS_DOT
+#undef TP_ROWS_16
 #undef TP_ROWS_BY_K
 
 }  // namespace
