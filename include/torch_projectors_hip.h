@@ -315,7 +315,9 @@ int tp_quantize_blocks(int dtype, const void* x, int64_t rows, int64_t cols, int
 
 /* scores[m, n] = bias[n] + <row m of a, row n of b>, both in 8-bit blocks, summed
  * in fp32 (bias fp32, optional; scores TP_F32 or TP_BF16; at most 2^26 rows on
- * either side, 1 to 65536 blocks). */
+ * either side, 1 to 65536 blocks).  A value is exact where its scale byte is 3
+ * to 246, a multiple of 2^-133 with bytes 0 to 2, and infinite from 2^128 on;
+ * byte 255 is no scale. */
 int64_t tp_block_scores_work(int64_t rows_a, int64_t rows_b, int64_t blocks);
 int tp_block_scores(const void* codes_a, const void* scales_a, int64_t rows_a, const void* codes_b,
                     const void* scales_b, int64_t rows_b, int64_t blocks, const void* bias, int out_dtype,

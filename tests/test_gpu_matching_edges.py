@@ -162,3 +162,58 @@ def test_places_from_elsewhere_leave_the_last_row_alone(m, T, D):
     assert torch.equal(dx.cpu()[good], w[good] * up[at]) and (dx[bad] == 0).all() and (dw[bad] == 0).all()
     y = m.combine(s.detach(), foreign, gw).detach().cpu()
     assert torch.equal(y[good], w[good] * (w[good] * x[good])) and (y[bad] == 0).all()
+
+
+def _random_blocks(m, rows, K, lo, hi, g):
+    """BlockScaled with every finite code and scale bytes lo .. hi."""
+    codes = torch.randint(0, 256, (rows, K), generator=g, dtype=torch.int64).to(torch.uint8)
+    codes[(codes & 127) == 127] = 0
+    scales = torch.full((K // 128, -(-rows // 16) * 16), 127, dtype=torch.uint8)
+    scales[:, :rows] = torch.randint(lo, hi + 1, (K // 128, rows), generator=g).to(torch.uint8)
+    value = codes.view(torch.float8_e4m3fn).float().double().view(rows, K // 128, 128)
+    value = (value * torch.exp2(scales[:, :rows].t().double() - 127)[:, :, None]).view(rows, K)
+    return m.BlockScaled(codes.to(DEV).view(torch.float8_e4m3fn), scales.to(DEV)), value
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 1280), (9, 130, 512), (20, 33, 256), (70, 100, 768)])
+@pytest.mark.parametrize("a,b", [((3, 6), (243, 246)), ((243, 246), (3, 6)), ((3, 60), (200, 230))])
+def test_scores_of_blocks_at_the_ends_of_the_exact_range(m, M, N, K, a, b):
+    """Scale bytes 3 .. 246: every code times its scale is a bfloat16, and the scores are exact but for the sum's
+    roundings (nb + 8 of 2^-23 of the magnitudes' sum)."""
+    g = gen(M)
+    qa, va = _random_blocks(m, M, K, *a, g)
+    qb, vb = _random_blocks(m, N, K, *b, g)
+    want, mag = va @ vb.t(), va.abs() @ vb.abs().t()
+    assert float(mag.max()) < 3e38
+    got = m.block_scores(qa, qb).double().cpu()
+    assert ((got - want).abs() <= (K // 128 + 8) * 2.0 ** -23 * mag).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 1280), (9, 130, 512), (70, 100, 768)])
+def test_scores_of_blocks_below_the_exact_range(m, M, N, K):
+    """Scale bytes 0 .. 2: each value to a multiple of 2^-133, bfloat16's least, at most one off."""
+    g = gen(M)
+    qa, va = _random_blocks(m, M, K, 0, 2, g)
+    qb, vb = _random_blocks(m, N, K, 230, 240, g)
+    want, mag = va @ vb.t(), va.abs() @ vb.abs().t()
+    got = m.block_scores(qa, qb).double().cpu()
+    tol = (K // 128 + 8) * 2.0 ** -23 * mag + 2.0 ** -133 * vb.abs().sum(1)[None]
+    assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("M", [1, 5, 40])
+def test_scores_of_the_largest_float32(m, M):
+    """Values from 248 2^120 = 3.297e38 up are nearest to the code 256 at that scale, 2^128, and count as infinite;
+    those below as 240 2^120, finite."""
+    x, b = torch.zeros(M, 200), torch.full((20, 200), 2.0 ** -30)
+    limit = 248 * 2.0 ** 120
+    x[:, 3], b[7, 3] = torch.nextafter(torch.tensor(limit), torch.tensor(0.0)), 0.0
+    got = m.block_scores(x.to(DEV), b.to(DEV)).cpu()
+    want = torch.full((M, 20), 240 * 2.0 ** 90)
+    want[:, 7] = 0.0
+    assert torch.equal(got, want)
+    x[:, 3] = limit
+    got = m.block_scores(x.to(DEV), b.to(DEV)).cpu()
+    assert (got[:, [i for i in range(20) if i != 7]] == math.inf).all() and got[:, 7].isnan().all()
+    x[:, 3] = -torch.finfo(F32).max
+    assert (m.block_scores(x.to(DEV), b.to(DEV)).cpu()[:, 0] == -math.inf).all()

@@ -59,7 +59,11 @@ def quantize_blocks(x: torch.Tensor) -> BlockScaled:
 
     A block's scale is the least power of two that keeps its largest finite magnitude within 448 times
     it; the codes are rounded to nearest even.  Values that are not finite become NaN.  Not
-    differentiable."""
+    differentiable.
+
+    Products take a value exactly where its block's scale byte is 3 to 246.  In blocks whose largest value is
+    below 1.05e-35 (bytes 0 to 2) values count as multiples of 2^-133; values from 3.297e38 up count as infinite, as
+    does what is past 2^128 in blocks from elsewhere."""
     return BlockScaled(*_OPS.quantize_blocks.default(_real_rows(x, "x")))
 
 
