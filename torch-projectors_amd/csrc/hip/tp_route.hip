@@ -489,29 +489,43 @@ __global__ __launch_bounds__(row_block<W>()) void k_gather_rows(RouteArgs a, int
     }
 }
 
-// Sorted rows of at least this size, what the XCDs' L2s hold together, are streamed past the caches.  Measured: 16384 x 4
-// rows of 4096 bfloat16 (537 MB) weighted gather 134 us through the caches, 121 streamed (spread 123 and 126); 2048 x 2
-// rows of 4224 fp32 (69 MB), spread then gather of one input after another 20 + 30 us through the caches, which the
-// gather finds full of what is yet to be written, 22 + 23 streamed (of the same input again and again 18 + 19 and
-// 22 + 23).
+// Sorted rows of at least this size, what the XCDs' L2s hold together, are streamed past the caches.  Which side is the
+// faster one depends on what a program does around the call, too.  Measured, streamed and through the caches, us: inputs
+// and outputs that were not in the caches (many in turn), weighted spread and gather of 2048 x 2 rows of 2112 fp32 (35
+// MB) 13.4 and 14.8, 11.7 and 13.1, of 4224 (69 MB) 24 and 27, 20 and 24, 16384 x 4 of 1024 bfloat16 (134 MB) 33.5 and
+// 34.5, 34 and 39, 9000 x 2 of 2560 fp32 (184 MB) 52 and 54, 47 and 53; the same input again and again, 69 MB 23 and 17,
+// 18 and 17, 184 MB 51 and 49, 45 and 43, 268 MB and more: streamed or equal; a spread, a pass over the sorted rows and a
+// gather, 35 MB 36.4 and 36.2, 69 MB 65 and 63, 105 MB 101 and 97, 134 MB 100 and 105, 268 MB 204 and 214, 537 MB 430 and
+// 450.  Against it: 65536 x 2 rows of 300 fp32 (157 MB), spread 59 and 54 (of 200, 33 and 38).
 constexpr int64_t kStreamBytes = int64_t(32) << 20;
 
 // Wavefronts of a row: one while a row is at most 2.5 KB, else 4 (16384 x 2 rows of 2560 bytes: spread 25.3 us by one,
-// 26.1 by four, with the weights' gradient 38 and 44; of 4096 bytes 45 and 35, 66 and 58), or 16 where rows are so few
-// that CUs would idle (with the weights' gradient, whose sums need the whole row in one workgroup); without it a
-// row of few is cut into stretches instead (100 x 2 rows of 66560 bytes: 5.5 us, whole 9.3).
+// 26.1 by four, with the weights' gradient 38 and 44; of 4096 bytes 45 and 35, 66 and 58).
+// With fewer than 2048 of them a row is cut into stretches for 2048 (100 x 2 rows of 66560 bytes, spread, whole and cut: 13.3
+// and 6.4 us; 500 x 2 of 8448 5.0 and 4.7, 1000 x 4 of 2500 7.2 and 6.3, but 2000 x 2 of 8448, already 8000
+// wavefronts, 12.8 and 14.1).
+// The weights' gradient needs whole rows.  It takes 4 wavefronts for short rows that are fewer than 1024 (spread by one
+// and four: 512 x 2 of 2500 bytes 5.3 and 4.1 us, 1024 4.8 and 5.1 of 1800, 6.1 and 5.6 of 2500, 2000 6.3 and 8.1, 7.8 and
+// 8.5), and 16 for long rows of which each has a CU of its own (by four and 16: 64 x 2 of 4400 bytes 4.3 and 4.0, of
+// 2800 3.6 and 3.8; 256 x 2 of 8448 5.8 and 5.2, 300 6.2 and 8.3), beyond 32 KB up to two a CU (512 x 2 of 33280 21.8
+// and 20.1, of 24000 13.2 and 14.4; 700 of 33280 26.7 and 27.3).  Gathering more than four choices, which 16 wavefronts
+// do four at a time and fewer eight, pays for 16 beyond 16 KB only (64 x 8 of 8448 12.7 and 13.1, of 16896 23.7 and 20.4;
+// 300 of 66560 104 and 154).
 struct RowPlan {
     int waves, parts;
     int64_t span;
 };
-RowPlan row_plan(const RouteArgs& a, int size, bool dot) {
+RowPlan row_plan(const RouteArgs& a, int size, bool spread, bool dot) {
     const int64_t bytes = a.D * size;
     RowPlan p{bytes <= 2560 ? 1 : 4, 1, a.D};
-    if (a.T * p.waves >= 2048 || bytes <= 1024) return p;
+    if (bytes <= 1024) return p;
     if (dot) {
-        p.waves = bytes <= 4096 ? 4 : 16;
+        const int64_t long_row = spread || a.k <= 4 ? (a.T <= 256 ? 4096 : 32768) : 16384;
+        if (bytes <= 2560) p.waves = a.T < 1024 ? 4 : 1;
+        else if (a.T <= (spread || a.k <= 4 ? 512 : 256) && bytes > long_row) p.waves = 16;
         return p;
     }
+    if (a.T * p.waves >= 2048) return p;
     p.waves = 1;
     const int64_t want = (2048 + a.T - 1) / a.T, step = 1024 / size;  // a wavefront's values at once
     p.span = ((a.D + want - 1) / want + step - 1) / step * step;
@@ -534,7 +548,7 @@ hipError_t move_rows(const RouteArgs& a, const void* in_, void* to_, const void*
     auto* to = static_cast<B*>(to_);
     const auto* other = static_cast<const B*>(other_);
     const bool dot = d_weights != nullptr;
-    const RowPlan p = row_plan(a, sizeof(B), dot);
+    const RowPlan p = row_plan(a, sizeof(B), SPREAD, dot);
     const int64_t items = a.T * p.parts;
     const bool stream = a.T * a.k * a.D * int64_t(sizeof(B)) >= kStreamBytes;
     const unsigned grid = match_grid(p.waves == 1 ? (items + 3) / 4 : items);
