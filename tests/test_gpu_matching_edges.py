@@ -217,3 +217,37 @@ def test_scores_of_the_largest_float32(m, M):
     assert (got[:, [i for i in range(20) if i != 7]] == math.inf).all() and got[:, 7].isnan().all()
     x[:, 3] = -torch.finfo(F32).max
     assert (m.block_scores(x.to(DEV), b.to(DEV)).cpu()[:, 0] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,k,D", [(5, 2, 40), (700, 3, 1301), (40, 5, 4099), (300, 8, 129)])
+def test_rows_with_some_places_from_elsewhere(m, T, k, D, dtype):
+    """Choices without a place beside ones that have theirs, dropped ones among them, both ways and with the weights'
+    gradient: the others' rows are as they are without them."""
+    g = gen(T)
+    classes = torch.randint(-1, 4, (T, k), generator=g)
+    order = m.sort_by_class(classes.to(DEV), 4)
+    slot = order.slot.cpu()
+    away = torch.rand(T, k, generator=g) < 0.3
+    away[0], away[1, 0] = True, False
+    away |= slot == T * k - 1
+    away[T // 2, k - 1] = False
+    far = torch.tensor([-1, T * k, 1 << 30, -(2 ** 31)], dtype=torch.int32)
+    foreign = torch.where(away, far[torch.arange(T * k).view(T, k) % 4], slot)
+    order = order._replace(slot=foreign.to(DEV))
+    held = ~away
+    kept = held & (slot < int(order.offsets[-1]))
+    x, up = torch.randn(T, D, generator=g).to(dtype), torch.randn(T, D, generator=g).to(dtype)
+    w = torch.rand(T, k, generator=g)
+    s = m.dispatch(x.to(DEV), order, w.to(DEV)).cpu()
+    row = torch.arange(T)[:, None].expand(T, k)
+    want = torch.where(kept[:, :, None], w[:, :, None] * x.float()[:, None], 0.0).to(dtype)
+    assert torch.equal(s[slot[held].long()], want[held])
+    y = torch.randn(T * k, D, generator=g).to(dtype)
+    gy, gw = y.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    dy, dw = torch.autograd.grad(m.combine(gy, order, gw), (gy, gw), up.to(DEV))
+    want = torch.where(kept[:, :, None], w[:, :, None] * up.float()[:, None], 0.0).to(dtype)
+    assert torch.equal(dy.cpu()[slot[held].long()], want[held])
+    part = up.double()[row] * y.double()[slot.long()]
+    want, mag = torch.where(kept, part.sum(2), 0.0), part.abs().sum(2)
+    assert ((dw.double().cpu() - want).abs() <= (D / 64 + 16) * 2.0 ** -24 * mag).all() and (dw.cpu()[~kept] == 0).all()

@@ -292,7 +292,8 @@ __device__ __forceinline__ void store_values(typename S::Bits* p, int64_t left, 
 template <int KB> struct Places {
     int64_t at[KB];  // first value of the row there
     float w[KB];
-    bool in[KB], real[KB];  // is not dropped; has a place at all
+    bool in[KB], real[KB];  // is not dropped; is a choice at all
+    bool held[KB];          // is a choice with a place among the sorted rows
 };
 template <int KB>
 __device__ __forceinline__ Places<KB> places_of(const RouteArgs& a, int64_t t, int j0, int kept) {
@@ -300,16 +301,34 @@ __device__ __forceinline__ Places<KB> places_of(const RouteArgs& a, int64_t t, i
 #pragma unroll
     for (int u = 0; u < KB; ++u) {
         const int64_t s = t * a.k + j0 + u;
-        const bool choice = j0 + u < a.k;
-        const uint32_t at = choice ? uint32_t(a.slot[s]) : 0u, last = uint32_t(a.T * a.k) - 1u;
-        // (a place outside the sorted rows, of an order from elsewhere, is neither read nor written: a row of zeros for
-        // it at the last place would meet the row that has that place)
-        p.real[u] = choice && at <= last;
-        p.in[u] = p.real[u] && at < uint32_t(kept);
-        p.at[u] = int64_t(min(at, last)) * a.D;
-        p.w[u] = choice && a.weights ? a.weights[s] : 1.0f;
+        p.real[u] = j0 + u < a.k;
+        const uint32_t at = p.real[u] ? uint32_t(a.slot[s]) : 0u, last = uint32_t(a.T * a.k) - 1u;
+        p.held[u] = p.real[u] && at <= last;
+        p.in[u] = p.held[u] && at < uint32_t(kept);
+        p.at[u] = int64_t(min(at, last)) * a.D;  // (read where `in`)
+        p.w[u] = p.real[u] && a.weights ? a.weights[s] : 1.0f;
     }
     return p;
+}
+// For writing: a choice without a place, of an order from elsewhere, writes what another one of these writes, to the
+// same place (zeros at the last place would meet the row that has it; a branch for each store makes the loads ahead wait
+// for the stores, 16384 x 4 rows of 4096 bfloat16 141 us, so 120; a path of its own takes registers from the other one,
+// 16384 x 8 of 512 with the weights' gradient 72 us, so 59).  False where none has a place.
+template <int KB> __device__ __forceinline__ bool placed(Places<KB>& p) {
+    bool any = true;
+#pragma unroll
+    for (int u = 0; u < KB; ++u) any = any && p.held[u] == p.real[u];
+    if (any) return true;  // (the weights are not waited for)
+    bool in = false;
+    int64_t at = 0;
+    float w = 0.0f;
+#pragma unroll
+    for (int u = 0; u < KB; ++u)
+        if (p.held[u]) any = true, in = p.in[u], at = p.at[u], w = p.w[u];
+#pragma unroll
+    for (int u = 0; u < KB; ++u)
+        if (!p.held[u]) p.in[u] = in, p.at[u] = at, p.w[u] = w;
+    return any;
 }
 
 // Sums of the W wavefronts of a row, the same in all of them.
@@ -358,9 +377,10 @@ __global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int
         RowItem r;
         if (!row_item<W>(a, item0, span, parts, r)) break;
         for (int j0 = 0; j0 < a.k; j0 += KB) {
-            const Places<KB> p = places_of<KB>(a, r.t, j0, kept);
+            Places<KB> p = places_of<KB>(a, r.t, j0, kept);
+            const int64_t end = placed(p) ? r.d1 : r.d0;
             float dot[KB] = {};
-            for (int64_t d0 = r.d0 + lane * n; d0 < r.d1; d0 += U * step) {
+            for (int64_t d0 = r.d0 + lane * n; d0 < end; d0 += U * step) {
                 Values<S> v[U];
 #pragma unroll
                 for (int e = 0; e < U; ++e)
@@ -396,7 +416,7 @@ __global__ __launch_bounds__(row_block<W>()) void k_spread_rows(RouteArgs a, int
                 if (lane == 0)
 #pragma unroll
                     for (int u = 0; u < KB; ++u)
-                        if (j0 + u < a.k) d_weights[r.t * a.k + j0 + u] = dot[u];
+                        if (p.real[u]) d_weights[r.t * a.k + j0 + u] = p.held[u] ? dot[u] : 0.0f;
             }
         }
     }
