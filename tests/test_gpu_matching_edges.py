@@ -251,3 +251,19 @@ def test_rows_with_some_places_from_elsewhere(m, T, k, D, dtype):
     part = up.double()[row] * y.double()[slot.long()]
     want, mag = torch.where(kept, part.sum(2), 0.0), part.abs().sum(2)
     assert ((dw.double().cpu() - want).abs() <= (D / 64 + 16) * 2.0 ** -24 * mag).all() and (dw.cpu()[~kept] == 0).all()
+
+
+def test_forward_mode_is_refused(m):
+    """A forward-mode tangent of what is differentiable is refused, with and without grad mode, not dropped."""
+    import torch.autograd.forward_ad as fw
+    x = torch.randn(4, 20, device=DEV)
+    order = m.sort_by_class(torch.tensor([0, 1, 0, 1], device=DEV), 2)
+    w = torch.rand(4, 1, device=DEV)
+    calls = [lambda d: m.log_probs(d), lambda d: m.dispatch(d, order), lambda d: m.combine(d, order, w),
+             lambda d: m.dispatch(x, order, d[:, :1]), lambda d: m.combine(x, order, d[:, :1])]
+    for call in calls:
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), fw.dual_level():
+                with pytest.raises(NotImplementedError):
+                    call(fw.make_dual(x, torch.ones_like(x)))
+    assert torch.isfinite(m.log_probs(x).log_sum).all()

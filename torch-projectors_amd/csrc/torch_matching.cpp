@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 #include <torch/torch.h>
 
@@ -342,6 +343,11 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads) {
 optional<Tensor> given_or_none(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
 bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
+// There are no forward-mode derivatives: a tangent would be lost without a word.
+void refuse_forward_mode(const optional<Tensor>& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t),
+                                "torch_projectors: the matching operators have no forward-mode derivatives");
+}
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -373,6 +379,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs_grad(const 
                                                                           const optional<Tensor>& given,
                                                                           const optional<Tensor>& mask, int64_t top,
                                                                           double temperature) {
+    refuse_forward_mode(scores);
     if (!at::GradMode::is_enabled() || !wants(scores))  // (no statistics: None)
         return log_probs_of(scores, given, mask, top, temperature, false);
     auto r = LogProbsGrad::apply(scores, given, mask, top, temperature);
@@ -404,6 +411,8 @@ template <bool SPREAD>
 std::tuple<Tensor, Tensor> rows_grad(const Tensor& x, const Tensor& slot, const Tensor& offsets,
                                      const optional<Tensor>& weights, const optional<Tensor>& other) {
     using F = RowsGrad<SPREAD>;
+    refuse_forward_mode(x);
+    refuse_forward_mode(weights);
     if (!at::GradMode::is_enabled() || other.has_value() || !(wants(x) || wants(weights)))
         return F::move(SPREAD, x, slot, offsets, weights, other);
     return {F::apply(x, slot, offsets, weights), Tensor()};

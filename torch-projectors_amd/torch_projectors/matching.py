@@ -16,7 +16,8 @@ with its weights.  In training, `log_probs` of `images @ projections.T` carries 
 likelihood (`log_sum`) back to volumes and poses.
 
 All run on the GPU only (a CPU tensor raises NotImplementedError), on the current stream, without a
-synchronisation; they can be captured in a graph.  What is differentiable is so once.
+synchronisation; they can be captured in a graph.  What is differentiable is so once, backwards (forward-mode
+tangents raise NotImplementedError).
 """
 from typing import NamedTuple, Optional
 
