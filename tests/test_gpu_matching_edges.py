@@ -267,3 +267,95 @@ def test_forward_mode_is_refused(m):
                 with pytest.raises(NotImplementedError):
                     call(fw.make_dual(x, torch.ones_like(x)))
     assert torch.isfinite(m.log_probs(x).log_sum).all()
+
+
+def test_log_probs_of_arguments_of_any_layout(m):
+    """Masks, given candidates and upstream gradients that are views: strided, transposed, expanded."""
+    g = gen(12)
+    T, V = 9, 1500
+    x = torch.randn(T, V, generator=g).to(DEV)
+    ups = torch.randn(T, 3, generator=g).to(DEV), torch.randn(T, generator=g).to(DEV)
+
+    def results(mask, given, up_given, up_sum):
+        s = x.clone().requires_grad_()
+        out = m.log_probs(s, given, top=6, mask=mask)
+        (d,) = torch.autograd.grad([out.given, out.log_sum], [s], [up_given, up_sum])
+        return [*out, d]
+
+    wide = (torch.rand(T, V + 77, generator=g) < 0.6).to(DEV)
+    tall = (torch.rand(V, T, generator=g) < 0.6).to(DEV)
+    one = (torch.rand(V, generator=g) < 0.6).to(DEV)
+    given = torch.randint(0, V, (3, T), generator=g).to(DEV)
+    up_wide = torch.zeros(T, 9, device=DEV)
+    up_wide[:, ::3] = ups[0]
+    up_sum = torch.zeros(2 * T, device=DEV)
+    up_sum[::2] = ups[1]
+    for mask in (wide[:, 50:50 + V], tall.t(), one.expand(T, V), one.repeat_interleave(2)[::2]):
+        want = results(mask.contiguous(), given.t().contiguous(), *ups)
+        got = results(mask, given.t(), up_wide[:, ::3], up_sum[::2])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    scalar = results(one, given.t(), torch.ones((), device=DEV).expand(T, 3), torch.ones((), device=DEV).expand(T))
+    plain = results(one, given.t(), torch.ones(T, 3, device=DEV), torch.ones(T, device=DEV))
+    assert all(torch.equal(a, b) for a, b in zip(scalar, plain))
+
+
+def test_log_probs_of_more_dimensions_with_masks(m):
+    g = gen(13)
+    x = torch.randn(4, 5, 70, generator=g).to(DEV).requires_grad_()
+    mask = (torch.rand(4, 5, 70, generator=g) < 0.5).to(DEV)
+    given = torch.randint(0, 70, (4, 5, 2), generator=g).to(DEV)
+    out = m.log_probs(x, given, top=3, mask=mask)
+    flat = m.log_probs(x.view(20, 70), given.view(20, 2), top=3, mask=mask.view(20, 70))
+    assert out.given.shape == (4, 5, 2) and out.top.shape == (4, 5, 3) and out.entropy.shape == (4, 5)
+    for a, b in zip(out, flat):
+        assert torch.equal(a.reshape(b.shape), b)
+    a, b = (torch.autograd.grad(o.given.exp().sum() + o.top.sum() + o.entropy.sum(), x)[0] for o in (out, flat))
+    assert torch.equal(a, b) and (a[~mask] == 0).all()
+    line = x.detach()[0, 0]
+    one = m.log_probs(line, given[0, 0], top=3, mask=mask[0, 0])
+    assert torch.equal(one.given, out.given[0, 0]) and torch.equal(one.top_index, out.top_index[0, 0])
+
+
+def test_nothing_to_do(m):
+    """No rows, no choices, no candidates wanted: empty or zero results and gradients of the right shapes."""
+    x = torch.empty(0, 70, device=DEV, requires_grad=True)
+    out = m.log_probs(x, torch.empty(0, 2, dtype=torch.int64, device=DEV), top=3)
+    (d,) = torch.autograd.grad([out.given, out.log_sum, out.top], [x], [out.given, out.log_sum, out.top])
+    assert d.shape == (0, 70)
+    x = torch.randn(3, 70, device=DEV, requires_grad=True)
+    out = m.log_probs(x, torch.empty(3, 0, dtype=torch.int64, device=DEV))
+    assert out.given.shape == (3, 0) and out.top.shape == (3, 0)
+    (d,) = torch.autograd.grad(out.given.sum() + out.top.sum(), x)
+    assert (d == 0).all()
+    order = m.sort_by_class(torch.empty(4, 0, dtype=torch.int64, device=DEV), 3)
+    assert order.slot.shape == (4, 0) and order.offsets.tolist() == [0, 0, 0, 0]
+    x = torch.randn(4, 30, device=DEV, requires_grad=True)
+    y = torch.empty(0, 30, device=DEV, requires_grad=True)
+    w = torch.empty(4, 0, device=DEV, requires_grad=True)
+    s, total = m.dispatch(x, order, w), m.combine(y, order, w)
+    assert s.shape == (0, 30) and total.shape == (4, 30) and (total == 0).all()
+    dx, dw = torch.autograd.grad(s, (x, w), torch.empty(0, 30, device=DEV))
+    assert (dx == 0).all() and dw.shape == (4, 0)
+    dy, dw = torch.autograd.grad(total, (y, w), torch.ones(4, 30, device=DEV))
+    assert dy.shape == (0, 30) and dw.shape == (4, 0)
+
+
+def test_rows_of_arguments_of_any_layout(m):
+    """Weights and upstream gradients that are views, complex rows whose gradient comes in conjugate."""
+    g = gen(14)
+    classes = torch.randint(-1, 5, (3, 40), generator=g).to(DEV)
+    order = m.sort_by_class(classes.t(), 5)
+    same = m.sort_by_class(classes.t().contiguous(), 5)
+    assert all(torch.equal(a, b) for a, b in zip(order, same))
+    x = torch.randn(40, 12, 7, dtype=torch.complex64, generator=g).to(DEV)
+    w = torch.rand(3, 40, generator=g).to(DEV).t()
+    up = torch.randn(120, 7, 12, dtype=torch.complex64, generator=g).to(DEV).transpose(1, 2).conj()
+
+    def results(x, w, up):
+        gx, gw = x.detach().requires_grad_(), w.detach().requires_grad_()
+        s = m.dispatch(gx, order, gw)
+        return [s, *torch.autograd.grad(s, (gx, gw), up)]
+
+    got = results(x.transpose(1, 2), w, up.transpose(1, 2))
+    want = results(x.transpose(1, 2).contiguous(), w.contiguous(), up.transpose(1, 2).resolve_conj().contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
