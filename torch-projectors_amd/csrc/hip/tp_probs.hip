@@ -20,7 +20,7 @@
 //
 // Split: a row is one wavefront's, or 2, 4 or 8 of a workgroup's, or, where rows are few, several workgroups',
 // whose sums and keys k_probs_join joins.  Large calls are bound by memory (4096 x 36864 fp32 with 8 alternatives
-// 96 us, 6.3 TB/s; bfloat16 73 us, by the instructions of a score), small ones by the chain from launch to result: of
+// 96 us, 6.3 TB/s; bfloat16 66 to 73 us, 4.1 to 4.6 TB/s, by the instructions of a score), small ones by the chain from launch to result: of
 // the 5.3 us of 1 x 4096 a fifth each goes to the start, the loads and sums, and the selection, the rest to the joins.
 //
 // Scores of -inf count as not allowed.  A NaN makes the row's results NaN.

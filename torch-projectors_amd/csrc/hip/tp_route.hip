@@ -23,8 +23,9 @@ namespace {
 // A workgroup of W wavefronts sorts up to 64 W kGroups slots: each wavefront takes consecutive groups of 64, keeps
 // their classes and their ranks among its own slots of that class in registers, and its counts per class in
 // LDS.  Few slots are one workgroup's; of more, a first kernel counts each workgroup's stretch, and the last,
-// knowing every stretch's counts, places it.  Bound by the chain of launches, counts and scans, not by its bytes: 4096
-// slots 7 us, 65536 12, 8388608 115.  (Loops over wavefronts' counts are not unrolled: instructions are fetched once
+// knowing every stretch's counts, places it.  Up to some 10^5 slots bound by the chain of launches, counts and scans:
+// 4096 slots 7 us, 65536 12.  Millions are bound by their bytes' way, not their number (1048576 24 us, 8388608 112,
+// where 8 bytes in and 8 out are 20): ids are read twice, and `order` is written four bytes at a time.  (Loops over wavefronts' counts are not unrolled: instructions are fetched once
 // per launch, and 4096 slots took 8.3 us with more loads on their way at once.)
 constexpr int kGroups = 8, kMaxSortWaves = 16;
 

@@ -166,7 +166,8 @@ template <class O> __global__ __launch_bounds__(256) void k_scores_join(ScoreArg
 // Few images (at most 16 FM): as fast as the references' codes can be read.  A workgroup takes 16 references,
 // each of its wavefronts every eighth block of them, straight from memory into operands: kAhead blocks'
 // loads are in flight at once (8 KB a wavefront, 64 KB a CU).  One image against 4096 references of 16640
-// values: 14.9 us, 4.6 TB/s; against 64 to 2048 12 us, as 16 wavefronts take, too: what a CU can have on its way.
+// values: 14.9 us, 4.6 TB/s; against 64 to 2048 12 us, as 16 wavefronts take, too: what a CU can have on its way, the
+// other CUs being idle, as a row's blocks are not dealt out over workgroups (the bytes of 1024 references are 2.6 us).
 constexpr int kFewWaves = 8, kAhead = 4;
 
 // A row that a wavefront quantises itself, block by block: no launch and no memory for its codes.

@@ -73,11 +73,15 @@ def block_scores(images, references, bias: Optional[torch.Tensor] = None,
     """scores[m, n] = <image m, reference n> + bias[n], from 8-bit blocks, summed in float32.
 
     images [M, ...] and references [N, ...] are BlockScaled, or rows that are quantised here, of as many
-    values on both sides (BlockScaled rows hold zeros past theirs: of them the numbers of blocks are compared); of complex
-    rows the real part of the inner product is taken (their real pairs' product).  With rfft images,
+    values on both sides (BlockScaled rows hold zeros past theirs: of them the numbers of blocks are
+    compared); of complex rows the real part of the inner product is taken (their real pairs' product).  With rfft images,
     which hold one half of a symmetric plane, scale either side's columns other than x = 0 and n / 2 by two for the
     whole plane's product; with bias = -|reference|^2 / 2 the scores are the log likelihoods of unit noise
-    up to a constant per image.  bias float32 [N]; out_dtype float32 or bfloat16.  Not differentiable."""
+    up to a constant per image, where every image has the same transfer function (in the references).  With functions
+    of their own, score images times theirs without a bias and subtract the half product of the squared functions
+    and the references' squared magnitudes, which depends on the pair, too.
+
+    bias float32 [N]; out_dtype float32 or bfloat16.  Not differentiable."""
     rows = None if isinstance(images, BlockScaled) else _real_rows(images, "images")
     if not isinstance(references, BlockScaled):
         references = _real_rows(references, "references")
