@@ -314,7 +314,8 @@ __device__ __forceinline__ Places<KB> places_of(const RouteArgs& a, int64_t t, i
 // For writing: a choice without a place, of an order from elsewhere, writes what another one of these writes, to the
 // same place (zeros at the last place would meet the row that has it; a branch for each store makes the loads ahead wait
 // for the stores, 16384 x 4 rows of 4096 bfloat16 141 us, so 120; a path of its own takes registers from the other one,
-// 16384 x 8 of 512 with the weights' gradient 72 us, so 59).  False where none has a place.
+// 16384 x 8 of 512 with the weights' gradient 72 us, so 59; what it costs, 2048 x 2 of 4224 fp32 with that gradient 37.1
+// us, 35.8 without it, otherwise at most 2 %).  False where none has a place.
 template <int KB> __device__ __forceinline__ bool placed(Places<KB>& p) {
     bool any = true;
 #pragma unroll
