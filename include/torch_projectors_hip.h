@@ -299,8 +299,8 @@ int tp_normalize_reconstruction(int dtype, const void* data, const void* weights
  * and images in class order.  No counterpart in the reference.  `work` is
  * device memory of at least the matching tp_*_work() bytes (uninitialised,
  * free again once the call's work on the stream is done; it may be NULL where
- * that is 0).  work, codes, scales and stats are 16-byte aligned, everything
- * else as its type. */
+ * that is 0).  work, codes, scales of blocks, stats and state are 16-byte aligned,
+ * everything else as its type. */
 
 /* Rows in 8-bit blocks: x [rows, cols] (TP_F32, TP_F16 or TP_BF16; rows
  * `row_stride` elements apart, values of a row adjacent) becomes
@@ -329,6 +329,64 @@ int64_t tp_score_images_work(int64_t rows_a, int64_t rows_b, int64_t cols);
 int tp_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, int64_t row_stride, const void* codes_b,
                     const void* scales_b, int64_t rows_b, const void* bias, int out_dtype, void* scores, void* work,
                     int64_t work_bytes, void* stream);
+
+/* Rows in 8-bit integers: x [rows, cols] (TP_F32, TP_F16 or TP_BF16; rows
+ * `row_stride` elements apart, values of a row adjacent, cols at most 2^17) becomes
+ *   codes   [rows, cols padded to a multiple of 128] int8, zero past cols
+ *   scales  [rows] fp32: the row's largest magnitude / 127, at least 2^-126
+ * with a value's code that of x / scale to the nearest integer, half to even, both
+ * quotients rounded to fp32.  A row with a value that is not finite has scale NaN
+ * and codes 0.  codes are 16-byte aligned. */
+int tp_quantize_rows(int dtype, const void* x, int64_t rows, int64_t cols, int64_t row_stride, void* codes,
+                     void* scales, void* stream);
+
+/* scores[m, n] = (sum of codes_a[m] codes_b[n]) * scales_a[m] * scales_b[n] +
+ * bias[n], both sides as tp_quantize_rows leaves rows of `cols` values, the sum
+ * exact (codes from -127 to 127), the rest in fp32 (bias fp32, optional; scores
+ * TP_F32 or TP_BF16; at most 2^26 rows on either side and 2^38 scores). */
+int64_t tp_row_scores_work(int64_t rows_a, int64_t rows_b, int64_t cols);
+int tp_row_scores(const void* codes_a, const void* scales_a, int64_t rows_a, const void* codes_b,
+                  const void* scales_b, int64_t rows_b, int64_t cols, const void* bias, int out_dtype, void* scores,
+                  void* work, int64_t work_bytes, void* stream);
+
+/* The same with rows x [rows_a, cols] (`row_stride` elements apart) for a, quantised
+ * as tp_quantize_rows does on the way. */
+int64_t tp_row_score_images_work(int64_t rows_a, int64_t rows_b, int64_t cols);
+int tp_row_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, int64_t row_stride,
+                        const void* codes_b, const void* scales_b, int64_t rows_b, const void* bias, int out_dtype,
+                        void* scores, void* work, int64_t work_bytes, void* stream);
+
+/* Log probabilities of pairs without their scores in memory: p = softmax over the
+ * allowed references of (<image, reference> + bias) / temperature.
+ *   images      [image_rows, cols], references [reference_rows, cols] of `dtype`
+ *               (TP_F32, TP_F16 or TP_BF16), rows a stride apart (0 to 2^21), values of
+ *               a row adjacent; at most 2^26 rows each, 2^38 pairs, 2^21 cols
+ *   given       [image_rows] int64, optional: the reference whose log probability is
+ *               wanted; -1 for none (0 is returned), NaN for any other out of range
+ *   bias        [reference_rows] fp32, optional; -inf rules the reference out
+ *   mask        [reference_rows] bytes, optional, nonzero where allowed; what a
+ *               reference that is ruled out by it holds is not used
+ * Outputs fp32: given_log_probs [image_rows] (with given), log_sum [image_rows] (of exp(score));
+ * state, tp_pair_state() floats that the gradient reads (optional: NULL where none will).
+ * An image with no allowed reference has log_sum and log probabilities -inf. */
+int64_t tp_pair_state(int64_t image_rows, int64_t reference_rows);
+int64_t tp_pair_log_probs_work(int dtype, int64_t image_rows, int64_t reference_rows, int64_t cols);
+int tp_pair_log_probs(int dtype, const void* images, int64_t image_rows, int64_t cols, int64_t image_stride,
+                      const void* references, int64_t reference_rows, int64_t reference_stride, const void* given,
+                      const void* bias, const void* mask, double temperature, void* given_log_probs, void* log_sum,
+                      void* state, void* work, int64_t work_bytes, void* stream);
+
+/* Gradients, each optional: d_images [image_rows, cols] and d_references
+ * [reference_rows, cols] (row-major, of `dtype`), d_bias [reference_rows] fp32, from
+ * the upstream gradients of the two outputs (fp32, each optional); zero where ruled out.  A given index
+ * out of range other than -1 makes its image's NaN unless its upstream gradient is 0. */
+int64_t tp_pair_log_probs_back_work(int dtype, int64_t image_rows, int64_t reference_rows, int64_t cols,
+                                    int want_images, int want_references);
+int tp_pair_log_probs_back(int dtype, const void* images, int64_t image_rows, int64_t cols, int64_t image_stride,
+                           const void* references, int64_t reference_rows, int64_t reference_stride,
+                           const void* given, const void* bias, const void* mask, double temperature,
+                           const void* state, const void* d_given, const void* d_log_sum, void* d_images,
+                           void* d_references, void* d_bias, void* work, int64_t work_bytes, void* stream);
 
 /* Log probabilities of rows of scores [rows, candidates] (TP_F32, TP_F16 or
  * TP_BF16, rows `row_stride` apart): p = softmax(scores / temperature) over

@@ -24,6 +24,7 @@
 #include "../../../include/torch_projectors_hip.h"
 #include "tp_launch.hh"
 #include "tp_match.hh"
+#include "tp_pairs.hh"
 
 namespace {
 
@@ -1074,6 +1075,26 @@ int probs_args(int dtype, const void* scores, int64_t rows, int64_t candidates, 
     return TP_OK;
 }
 
+int pair_args(int dtype, const void* images, int64_t image_rows, int64_t cols, int64_t image_stride,
+              const void* references, int64_t reference_rows, int64_t reference_stride, const void* given,
+              const void* bias, const void* mask, double temperature, tp::PairArgs& a) {
+    TP_TRY(match_dtype(dtype));
+    if (image_rows < 0 || reference_rows < 0) return fail("row counts must be non-negative");
+    if (image_rows > tp::kMaxPairRows || reference_rows > tp::kMaxPairRows) return fail("row counts must be at most 2^26");
+    if (image_rows * reference_rows > tp::kMaxPairs) return fail("there must be at most 2^38 pairs");
+    if (cols < 1 || cols > tp::kMaxStride) return fail("cols must be in [1, 2^21]");
+    if (image_stride < 0 || reference_stride < 0 || image_stride > tp::kMaxStride || reference_stride > tp::kMaxStride)
+        return fail("row strides must be in [0, 2^21]");
+    const float t = float(temperature);
+    if (!(t >= 1e-30f && t <= 1e30f)) return fail("temperature must be in [1e-30, 1e30]");
+    if (image_rows) TP_TRY(need(images, "images"));
+    if (reference_rows) TP_TRY(need(references, "references"));
+    a = tp::PairArgs{dtype, images, image_rows, cols, image_stride, references, reference_rows, reference_stride,
+                     static_cast<const int64_t*>(given), static_cast<const float*>(bias),
+                     static_cast<const uint8_t*>(mask), 1.0f / t};
+    return TP_OK;
+}
+
 int route_args(int dtype, int64_t rows, int64_t cols, int64_t k, const void* slot, const void* kept,
                const void* weights, const void* other, const void* d_weights, tp::RouteArgs& a) {
     TP_TRY(match_dtype(dtype));
@@ -1453,6 +1474,147 @@ int tp_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, int6
     return launched(tp::launch_score_images(dtype, x, rows_a, cols, row_stride, codes_b, scales_b, rows_b, bias,
                                             out_dtype, scores, work, static_cast<hipStream_t>(stream)),
                     "score launch");
+}
+
+int tp_quantize_rows(int dtype, const void* x, int64_t rows, int64_t cols, int64_t row_stride, void* codes,
+                     void* scales, void* stream) {
+    g_err.clear();
+    TP_TRY(match_dtype(dtype));
+    if (rows < 0 || rows > kInt32Max) return fail("rows must be in [0, 2^31)");
+    if (cols < 1 || cols > tp::kMaxRowValues) return fail("cols must be in [1, 2^17]");
+    if (row_stride < 0) return fail("row_stride must be non-negative");
+    if (rows == 0) return TP_OK;
+    TP_TRY(need(x, "x"));
+    TP_TRY(need(codes, "codes"));
+    TP_TRY(need(scales, "scales"));
+    TP_TRY(aligned16(codes, "codes"));
+    return launched(tp::launch_quantize_rows(dtype, x, rows, cols, row_stride, codes, scales,
+                                             static_cast<hipStream_t>(stream)),
+                    "quantisation launch");
+}
+
+int64_t tp_row_scores_work(int64_t rows_a, int64_t rows_b, int64_t cols) {
+    if (rows_a <= 0 || rows_b <= 0 || cols <= 0 || cols > tp::kMaxRowValues) return 0;
+    return tp::row_scores_work(rows_a, rows_b, tp::row_bytes(cols));
+}
+
+int tp_row_scores(const void* codes_a, const void* scales_a, int64_t rows_a, const void* codes_b,
+                  const void* scales_b, int64_t rows_b, int64_t cols, const void* bias, int out_dtype, void* scores,
+                  void* work, int64_t work_bytes, void* stream) {
+    g_err.clear();
+    if (out_dtype != TP_F32 && out_dtype != TP_BF16) return fail("out_dtype must be TP_F32 or TP_BF16");
+    if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
+    if (rows_a > tp::kMaxScoreRows || rows_b > tp::kMaxScoreRows) return fail("row counts must be at most 2^26");
+    if (rows_a * rows_b > tp::kMaxPairs) return fail("there must be at most 2^38 scores");
+    if (cols < 1 || cols > tp::kMaxRowValues) return fail("cols must be in [1, 2^17]");
+    if (rows_a == 0 || rows_b == 0) return TP_OK;
+    TP_TRY(need(codes_a, "codes_a"));
+    TP_TRY(need(scales_a, "scales_a"));
+    TP_TRY(need(codes_b, "codes_b"));
+    TP_TRY(need(scales_b, "scales_b"));
+    TP_TRY(need(scores, "scores"));
+    TP_TRY(aligned16(codes_a, "codes_a"));
+    TP_TRY(aligned16(codes_b, "codes_b"));
+    TP_TRY(aligned16(work, "work"));
+    const int64_t need_bytes = tp_row_scores_work(rows_a, rows_b, cols);
+    if (need_bytes) TP_TRY(need(work, "work"));
+    if (work_bytes < need_bytes) return fail("work is smaller than tp_row_scores_work");
+    return launched(tp::launch_row_scores(codes_a, scales_a, rows_a, codes_b, scales_b, rows_b, tp::row_bytes(cols),
+                                          bias, out_dtype, scores, work, static_cast<hipStream_t>(stream)),
+                    "score launch");
+}
+
+int64_t tp_row_score_images_work(int64_t rows_a, int64_t rows_b, int64_t cols) {
+    if (rows_a <= 0 || rows_b <= 0 || cols <= 0 || cols > tp::kMaxRowValues) return 0;
+    return tp::row_score_images_work(rows_a, rows_b, cols);
+}
+
+int tp_row_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, int64_t row_stride,
+                        const void* codes_b, const void* scales_b, int64_t rows_b, const void* bias, int out_dtype,
+                        void* scores, void* work, int64_t work_bytes, void* stream) {
+    g_err.clear();
+    TP_TRY(match_dtype(dtype));
+    if (out_dtype != TP_F32 && out_dtype != TP_BF16) return fail("out_dtype must be TP_F32 or TP_BF16");
+    if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
+    if (row_stride < 0) return fail("row_stride must be non-negative");
+    if (rows_a > tp::kMaxScoreRows || rows_b > tp::kMaxScoreRows) return fail("row counts must be at most 2^26");
+    if (rows_a * rows_b > tp::kMaxPairs) return fail("there must be at most 2^38 scores");
+    if (cols < 1 || cols > tp::kMaxRowValues) return fail("cols must be in [1, 2^17]");
+    if (rows_a == 0 || rows_b == 0) return TP_OK;
+    TP_TRY(need(x, "x"));
+    TP_TRY(need(codes_b, "codes_b"));
+    TP_TRY(need(scales_b, "scales_b"));
+    TP_TRY(need(scores, "scores"));
+    TP_TRY(aligned16(codes_b, "codes_b"));
+    TP_TRY(aligned16(work, "work"));
+    const int64_t need_bytes = tp::row_score_images_work(rows_a, rows_b, cols);
+    if (need_bytes) TP_TRY(need(work, "work"));
+    if (work_bytes < need_bytes) return fail("work is smaller than tp_row_score_images_work");
+    return launched(tp::launch_row_score_images(dtype, x, rows_a, cols, row_stride, codes_b, scales_b, rows_b, bias,
+                                                out_dtype, scores, work, static_cast<hipStream_t>(stream)),
+                    "score launch");
+}
+
+int64_t tp_pair_state(int64_t image_rows, int64_t reference_rows) {
+    return image_rows <= 0 || reference_rows < 0 ? 0 : tp::pair_state(image_rows, reference_rows);
+}
+
+int64_t tp_pair_log_probs_work(int dtype, int64_t image_rows, int64_t reference_rows, int64_t cols) {
+    if (image_rows <= 0 || reference_rows <= 0 || cols <= 0) return 0;
+    return tp::pair_work(dtype, image_rows, reference_rows, cols);
+}
+
+int tp_pair_log_probs(int dtype, const void* images, int64_t image_rows, int64_t cols, int64_t image_stride,
+                      const void* references, int64_t reference_rows, int64_t reference_stride, const void* given,
+                      const void* bias, const void* mask, double temperature, void* given_log_probs, void* log_sum,
+                      void* state, void* work, int64_t work_bytes, void* stream) {
+    g_err.clear();
+    tp::PairArgs a;
+    TP_TRY(pair_args(dtype, images, image_rows, cols, image_stride, references, reference_rows, reference_stride, given,
+                     bias, mask, temperature, a));
+    if (image_rows == 0) return TP_OK;
+    if (given) TP_TRY(need(given_log_probs, "given_log_probs"));
+    TP_TRY(need(log_sum, "log_sum"));
+    TP_TRY(aligned16(state, "state"));
+    TP_TRY(aligned16(work, "work"));
+    const int64_t need_bytes = tp::pair_work(dtype, image_rows, reference_rows, cols);
+    if (need_bytes) TP_TRY(need(work, "work"));
+    if (work_bytes < need_bytes) return fail("work is smaller than tp_pair_log_probs_work");
+    return launched(tp::launch_pair_log_probs(a, given ? static_cast<float*>(given_log_probs) : nullptr,
+                                              static_cast<float*>(log_sum), static_cast<float*>(state), work,
+                                              static_cast<hipStream_t>(stream)),
+                    "pair log probability launch");
+}
+
+int64_t tp_pair_log_probs_back_work(int dtype, int64_t image_rows, int64_t reference_rows, int64_t cols,
+                                    int want_images, int want_references) {
+    if (image_rows <= 0 || reference_rows <= 0 || cols <= 0) return 0;
+    return tp::pair_back_work(dtype, image_rows, reference_rows, cols, want_images != 0, want_references != 0);
+}
+
+int tp_pair_log_probs_back(int dtype, const void* images, int64_t image_rows, int64_t cols, int64_t image_stride,
+                           const void* references, int64_t reference_rows, int64_t reference_stride,
+                           const void* given, const void* bias, const void* mask, double temperature,
+                           const void* state, const void* d_given, const void* d_log_sum, void* d_images,
+                           void* d_references, void* d_bias, void* work, int64_t work_bytes, void* stream) {
+    g_err.clear();
+    tp::PairArgs a;
+    TP_TRY(pair_args(dtype, images, image_rows, cols, image_stride, references, reference_rows, reference_stride, given,
+                     bias, mask, temperature, a));
+    if (image_rows) TP_TRY(need(state, "state"));
+    TP_TRY(aligned16(state, "state"));
+    TP_TRY(aligned16(work, "work"));
+    const int64_t need_bytes = tp_pair_log_probs_back_work(dtype, image_rows, reference_rows, cols, d_images != nullptr,
+                                                           d_references != nullptr);
+    if (need_bytes) TP_TRY(need(work, "work"));
+    if (work_bytes < need_bytes) return fail("work is smaller than tp_pair_log_probs_back_work");
+    if (!d_images && !d_references && !d_bias) return TP_OK;
+    return launched(tp::launch_pair_log_probs_back(a, static_cast<const float*>(state),
+                                                   static_cast<const float*>(d_given),
+                                                   static_cast<const float*>(d_log_sum), d_images, d_references,
+                                                   static_cast<float*>(d_bias), work,
+                                                   static_cast<hipStream_t>(stream)),
+                    "pair log probability gradient launch");
 }
 
 int64_t tp_log_probs_work(int64_t rows, int64_t candidates, int64_t top) {

@@ -35,6 +35,24 @@ hipError_t launch_score_images(int dt, const void* x, int64_t M, int64_t cols, i
                                const void* sb, int64_t N, const void* bias, int out_dt, void* out, void* work,
                                hipStream_t s);
 
+// ------------------------------------------------------------------ 8-bit integers (tp_rows8.hip)
+constexpr int kRowPad = 128;                      // rows of codes are padded with zeros to a multiple of this
+constexpr int64_t kMaxRowValues = int64_t(1) << 17;  // of a row: their products' sum stays below 2^31
+
+inline int64_t row_bytes(int64_t cols) { return (cols + kRowPad - 1) / kRowPad * kRowPad; }
+
+// x [rows, cols] of `dt`, rows `stride` elements apart -> codes [rows, row_bytes(cols)] int8, scales [rows] fp32.
+hipError_t launch_quantize_rows(int dt, const void* x, int64_t rows, int64_t cols, int64_t stride, void* codes,
+                                void* scales, hipStream_t s);
+// out [M, N] (TP_F32 or TP_BF16) of codes of `bytes` a row; the same for rows x [M, cols] of `dt`, rounded first.
+int64_t row_scores_work(int64_t M, int64_t N, int64_t bytes);
+hipError_t launch_row_scores(const void* a, const void* sa, int64_t M, const void* b, const void* sb, int64_t N,
+                             int64_t bytes, const void* bias, int out_dt, void* out, void* work, hipStream_t s);
+int64_t row_score_images_work(int64_t M, int64_t N, int64_t cols);
+hipError_t launch_row_score_images(int dt, const void* x, int64_t M, int64_t cols, int64_t stride, const void* b,
+                                   const void* sb, int64_t N, const void* bias, int out_dt, void* out, void* work,
+                                   hipStream_t s);
+
 // ------------------------------------------------------------------ log probabilities (tp_probs.hip)
 constexpr int kMaxTop = 64;  // a wavefront keeps one alternative per lane
 

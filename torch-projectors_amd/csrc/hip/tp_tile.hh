@@ -1,0 +1,379 @@
+// Tiled matrix products of the pair log probabilities: operands staged in LDS, multiplied by the matrix units, and
+// handed as fragments to an epilogue.
+//
+//   D[i, j] = sum over k of A(i, k) B(j, k)
+//
+// An operand lies in memory with its contraction adjacent (row i holds k = 0, 1, ...) or across (row k holds i = 0,
+// 1, ...); the latter is transposed on its way from LDS by ds_read_tr16_b64.  16-bit values go through the bfloat16 or
+// half precision units as they are.  float32 values x are cut into three bfloat16 pieces, x = h + m + l exactly (8
+// bits of the mantissa each, cut off, not rounded), and a product is the six largest of the nine products of pieces:
+// what is left out is below 2^-21 of each product and has its sign, so that the sum is off by some 1e-7 of itself.  Six products at
+// the bfloat16 rate are 2.5 times as fast as the float32 units' one.
+#pragma once
+
+#include "tp_match.hh"
+
+namespace tp {
+
+using v8bf = __attribute__((ext_vector_type(8))) __bf16;
+using v8h = __attribute__((ext_vector_type(8))) _Float16;
+using v16f = __attribute__((ext_vector_type(16))) float;
+using v4s = __attribute__((ext_vector_type(4))) short;
+using LocalTr = __attribute__((address_space(3))) v4s*;
+
+// How values of a storage type go through the matrix units: in `planes` pieces, `bk` of the contraction at a time
+// (128 bytes of each row in LDS, 192 in three planes).
+template <class S> struct Units;
+template <> struct Units<BF16> {
+    static constexpr int planes = 1, bk = 64;
+    static __device__ __forceinline__ v16f mfma(int4 a, int4 b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+    }
+};
+template <> struct Units<F16> {
+    static constexpr int planes = 1, bk = 64;
+    static __device__ __forceinline__ v16f mfma(int4 a, int4 b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    }
+};
+template <> struct Units<F32> {
+    static constexpr int planes = 3, bk = 32;
+    static __device__ __forceinline__ v16f mfma(int4 a, int4 b, v16f c) { return Units<BF16>::mfma(a, b, c); }
+};
+
+// A workgroup's tile of BM x BN of D, by WM x WN wavefronts.
+template <int BM_, int BN_, int WM_, int WN_> struct TileShape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NT = 64 * WM * WN;
+    static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;  // fragments of a wavefront
+};
+
+// Eight neighbouring values on their way from memory to LDS.
+template <class S> struct Eight {
+    Pack<S> w[8 / Pack<S>::n];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) set(i, 0);
+    }
+    __device__ __forceinline__ void set(int i, typename S::Bits b) { w[i / Pack<S>::n].v[i % Pack<S>::n] = b; }
+    __device__ __forceinline__ typename S::Bits get(int i) const { return w[i / Pack<S>::n].v[i % Pack<S>::n]; }
+    __device__ __forceinline__ void read(const typename S::Bits* p) {
+#pragma unroll
+        for (int i = 0; i < 8 / Pack<S>::n; ++i) w[i] = load_pack<S>(p + i * Pack<S>::n);
+    }
+    // as the units take them, plane by plane
+    __device__ __forceinline__ void planes(int4 (&out)[Units<S>::planes]) const {
+        if constexpr (Units<S>::planes == 1) {
+            out[0] = __builtin_bit_cast(int4, w[0]);
+        } else {
+            uint32_t part[3][4];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                uint32_t lo = get(i), hi = get(i + 1);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    part[p][i / 2] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);  // the upper halves of both
+                    if (p == 2) break;
+                    lo = __float_as_uint(__uint_as_float(lo) - __uint_as_float(lo & 0xffff0000u));
+                    hi = __float_as_uint(__uint_as_float(hi) - __uint_as_float(hi & 0xffff0000u));
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < 3; ++p) out[p] = int4{int(part[p][0]), int(part[p][1]), int(part[p][2]), int(part[p][3])};
+        }
+    }
+};
+
+// One operand of a product.
+struct Operand {
+    const void* p;
+    int64_t ld;           // elements between its rows in memory, at most kMaxStride
+    const uint8_t* keep;  // (contraction across only) zero: the row counts as zeros, whatever it holds; null: all do not
+};
+
+// An operand's part of a tile: DIM rows of D's side by bk of the contraction, CH chunks of eight values a thread.
+//   adjacent: LDS row i holds its bk values; chunk c of row i at place c ^ (i / rows in 256 bytes), so that 16 lanes
+//             reading one chunk of 16 rows reach each of the 64 banks once
+//   across:   LDS row k holds DIM values; four rows of 64 bytes, as 32 lanes read them, at places that differ by 64
+template <class S, bool ACROSS, int DIM, int NT> struct Side {
+    static constexpr int BK = Units<S>::bk, PL = Units<S>::planes;
+    static constexpr int CPR = ACROSS ? DIM / 8 : BK / 8, CH = DIM * BK / 8 / NT;
+    static constexpr int kPlane = DIM * BK * 2;  // bytes
+    static_assert(CH * 8 * NT == DIM * BK, "whole chunks");
+    using Bits = typename S::Bits;
+
+    const char* base;  // the tile's first value at contraction 0
+    int64_t ld, dim, kdim;
+    const uint8_t* keep;
+    uint32_t off[CH];  // bytes from base (+ the step) of each chunk
+    int tid;
+    Eight<S> reg[CH];
+    uint32_t kept[CH];  // (across, with keep) nonzero where the chunk's row counts
+
+    static __device__ __forceinline__ int row_of(int slot) { return slot / CPR; }
+    static __device__ __forceinline__ int chunk_of(int slot) { return slot % CPR; }
+    static __device__ __forceinline__ int swizzle(int row) {
+        if (ACROSS) return DIM >= 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+        return (row / (128 / BK)) & (CPR - 1);
+    }
+
+    // first: of the tile along D's side; dim_all, kdim_all: what there is of both
+    __device__ __forceinline__ void init(const Operand& o, int64_t first, int64_t dim_all, int64_t kdim_all, int t) {
+        tid = t;
+        ld = o.ld;
+        keep = o.keep;
+        dim = min(dim_all - first, int64_t(DIM));
+        kdim = kdim_all;
+        base = static_cast<const char*>(o.p) + (ACROSS ? first : first * ld) * int64_t(sizeof(Bits));
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
+            // rows and chunks past the end read the last one: what comes of them is not stored
+            const uint32_t at = ACROSS ? uint32_t(row) * uint32_t(ld) + min(c * 8, (int(dim) - 1) & ~7)
+                                       : uint32_t(min(row, int(dim) - 1)) * uint32_t(ld) + c * 8;
+            off[i] = at * uint32_t(sizeof(Bits));
+        }
+    }
+    // Whole chunks only: every row of the step is there, and the last chunk's read ends inside the operand.
+    __device__ __forceinline__ bool whole(int64_t k0) const {
+        if (k0 + BK > kdim) return false;
+        return !ACROSS || (k0 + BK - 1) * ld + ((dim + 7) & ~int64_t(7)) <= (kdim - 1) * ld + dim;
+    }
+    __device__ __forceinline__ void load(int64_t k0) {
+        const char* at = base + (ACROSS ? k0 * ld : k0) * int64_t(sizeof(Bits));
+        if (whole(k0)) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) reg[i].read(reinterpret_cast<const Bits*>(at + off[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
+                reg[i].zero();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool there = ACROSS ? k0 + row < kdim && c * 8 + j < dim : k0 + c * 8 + j < kdim;
+                    if (there) reg[i].set(j, reinterpret_cast<const Bits*>(at + off[i])[j]);
+                }
+            }
+        }
+        if (ACROSS && keep) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) kept[i] = keep[min(k0 + row_of(i * NT + tid), kdim - 1)];
+        }
+    }
+    __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
+            int4 v[PL];
+            reg[i].planes(v);
+            if (ACROSS && keep && !kept[i]) {
+#pragma unroll
+                for (int p = 0; p < PL; ++p) v[p] = int4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int p = 0; p < PL; ++p)
+                *reinterpret_cast<int4*>(lds + p * kPlane + row * (CPR * 16) + (c ^ swizzle(row)) * 16) = v[p];
+        }
+    }
+    // Fragment of rows `first` .. first + 31 of D's side, of the 16 of the contraction from 16 t on: lane r + 32 q has
+    // row r and 8 q .. 8 q + 7 of them.
+    static __device__ __forceinline__ int4 fragment(const char* lds, int first, int t, int lane) {
+        if constexpr (!ACROSS) {
+            const int row = first + (lane & 31), c = 2 * t + (lane >> 5);
+            return *reinterpret_cast<const int4*>(lds + row * (CPR * 16) + (c ^ swizzle(lane & 31)) * 16);
+        } else {
+            // 16 lanes bring 4 rows of 16 values; lane i of them is given value i of each row
+            const int k = 16 * t + 8 * (lane >> 5) + ((lane & 15) >> 2);
+            const int c = first / 8 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+            const char* at = lds + k * (CPR * 16) + (c ^ swizzle(k)) * 16 + (lane & 1) * 8;
+            // (four rows on the swizzle is the same)
+            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LocalTr)(at));
+            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LocalTr)(at + 4 * (CPR * 16)));
+            return __builtin_bit_cast(int4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+// What the products' kernels share: [splits] ranges of the contraction are one workgroup each, and where there are
+// several their fragments go to part, which k_tile_join adds up.
+struct Product {
+    Operand a, b;
+    int64_t rows, cols, kdim;
+    int splits;
+    float* part;
+    uint32_t tm, tn;
+};
+
+template <class T> using Acc = v16f[T::FM][T::FN];
+
+// Where a lane's results lie in the tile: element e of fragment (i, j) of its wavefront.
+template <class T> struct Place {
+    int wm, wn, r, q;
+    __device__ __forceinline__ explicit Place(int tid) {
+        const int wave = tid >> 6;
+        wm = wave / T::WN;
+        wn = wave % T::WN;
+        r = tid & 31;
+        q = (tid >> 5) & 1;
+    }
+    __device__ __forceinline__ int row(int i, int e) const { return (wm * T::FM + i) * 32 + (e >> 2) * 8 + q * 4 + (e & 3); }
+    __device__ __forceinline__ int col(int j) const { return (wn * T::FN + j) * 32 + r; }
+};
+
+// Workgroups are dealt to the XCDs in turn: each XCD takes a contiguous run of the items, whose tiles share rows and
+// columns in its L2; tiles in bands of 4 along the rows, column by column.
+__device__ __forceinline__ void tile_at(uint32_t item, uint32_t tm, uint32_t tn, uint32_t& im, uint32_t& in) {
+    const uint32_t band = item / (4 * tn), at = item - band * 4 * tn, height = min(4u, tm - band * 4);
+    im = band * 4 + at % height;
+    in = at / height;
+}
+__device__ __forceinline__ uint32_t xcd_item(uint32_t block, uint32_t items) {
+    const uint32_t x = block & 7, per = items >> 3, more = items & 7;
+    return x * per + min(x, more) + (block >> 3);
+}
+
+template <class S, class T> constexpr int tile_lds() { return 2 * Units<S>::planes * (T::BM + T::BN) * Units<S>::bk * 2; }
+
+// Epi: static void run(const Args&, Acc<T>&, im, in, char* lds) of the tile (im, in).
+template <class S, class T, bool ATR, bool BTR, class Epi>
+__global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea) {
+    constexpr int BK = Units<S>::bk, PL = Units<S>::planes;
+    using SA = Side<S, ATR, T::BM, T::NT>;
+    using SB = Side<S, BTR, T::BN, T::NT>;
+    constexpr int kA = PL * SA::kPlane, kStage = kA + PL * SB::kPlane;
+    __shared__ __attribute__((aligned(16))) char lds[tile_lds<S, T>()];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const Place<T> place(tid);
+    uint32_t item = xcd_item(blockIdx.x, gridDim.x), im, in;
+    const uint32_t split = item / (g.tm * g.tn);
+    item -= split * g.tm * g.tn;
+    tile_at(item, g.tm, g.tn, im, in);
+    SA a;
+    SB b;
+    a.init(g.a, int64_t(im) * T::BM, g.rows, g.kdim, tid);
+    b.init(g.b, int64_t(in) * T::BN, g.cols, g.kdim, tid);
+    const int64_t steps = (g.kdim + BK - 1) / BK;
+    const int64_t k0 = steps * split / g.splits * BK, k1 = steps * (split + 1) / g.splits * BK;
+
+    Acc<T> acc;
+#pragma unroll
+    for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+    if (k0 < k1) {
+        a.load(k0);
+        b.load(k0);
+        a.store(lds);
+        b.store(lds + kA);
+    }
+    int cur = 0;
+#pragma unroll 1
+    for (int64_t k = k0; k < k1; k += BK) {
+        __syncthreads();
+        const bool more = k + BK < k1;
+        if (more) {
+            a.load(k + BK);
+            b.load(k + BK);
+        }
+        const char* sa = lds + cur * kStage;
+        const char* sb = sa + kA;
+#pragma unroll
+        for (int t = 0; t < BK / 16; ++t) {
+            int4 fa[PL][T::FM], fb[PL][T::FN];
+#pragma unroll
+            for (int p = 0; p < PL; ++p) {
+#pragma unroll
+                for (int i = 0; i < T::FM; ++i) fa[p][i] = SA::fragment(sa + p * SA::kPlane, (place.wm * T::FM + i) * 32, t, lane);
+#pragma unroll
+                for (int j = 0; j < T::FN; ++j) fb[p][j] = SB::fragment(sb + p * SB::kPlane, (place.wn * T::FN + j) * 32, t, lane);
+            }
+            // the small products of pieces first
+#pragma unroll
+            for (int s = PL - 1; s >= 0; --s)
+#pragma unroll
+                for (int p = 0; p <= s; ++p)
+#pragma unroll
+                    for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+                        for (int j = 0; j < T::FN; ++j) acc[i][j] = Units<S>::mfma(fa[p][i], fb[s - p][j], acc[i][j]);
+        }
+        cur ^= 1;
+        if (more) {
+            a.store(lds + cur * kStage);
+            b.store(lds + cur * kStage + kA);
+        }
+    }
+    if (g.splits > 1) {
+        float* out = g.part + ((int64_t(split) * g.tm + im) * g.tn + in) * (T::BM * T::BN) + tid * 4;
+#pragma unroll
+        for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4*>(out + ((i * T::FN + j) * 4 + e / 4) * (T::NT * 4)) =
+                        float4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+        return;
+    }
+    __syncthreads();
+    Epi::template run<S, T>(ea, acc, im, in, lds);
+}
+
+// The ranges' fragments added up, then the epilogue.
+template <class S, class T, class Epi>
+__global__ __launch_bounds__(T::NT) void k_tile_join(Product g, typename Epi::Args ea) {
+    __shared__ __attribute__((aligned(16))) char lds[tile_lds<S, T>()];
+    uint32_t im, in;
+    tile_at(xcd_item(blockIdx.x, gridDim.x), g.tm, g.tn, im, in);
+    Acc<T> acc;
+#pragma unroll
+    for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    for (int s = 0; s < g.splits; ++s) {
+        const float* p = g.part + ((int64_t(s) * g.tm + im) * g.tn + in) * (T::BM * T::BN) + threadIdx.x * 4;
+#pragma unroll
+        for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(p + ((i * T::FN + j) * 4 + e / 4) * (T::NT * 4));
+                    acc[i][j][e] += v.x;
+                    acc[i][j][e + 1] += v.y;
+                    acc[i][j][e + 2] += v.z;
+                    acc[i][j][e + 3] += v.w;
+                }
+    }
+    Epi::template run<S, T>(ea, acc, im, in, lds);
+}
+
+// A row of fragments of a wavefront through its own part of LDS: use(row in the tile, first column, four neighbouring values)
+// for each four of its 32 x 32 FN values, 8 FN lanes a row.  (The workgroup is done with LDS before the first.)
+template <class T> struct Rows4 {
+    static constexpr int kStride = T::FN * 32 + 4, kLanes = T::FN * 8, kBytes = 32 * kStride * 4;  // bytes of a wavefront
+    template <class Use> static __device__ __forceinline__ void run(v16f (&acc)[T::FN], int i, char* lds, Use use) {
+        const int tid = threadIdx.x, lane = tid & 63;
+        const Place<T> place(tid);
+        float* mine = reinterpret_cast<float*>(lds + (tid >> 6) * kBytes);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mine[((e >> 2) * 8 + place.q * 4 + (e & 3)) * kStride + j * 32 + place.r] = acc[j][e];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int row = 0; row < 32; row += 64 / kLanes) {
+            const int at = row + lane / kLanes, c = lane % kLanes * 4;
+            const float4 v = *reinterpret_cast<const float4*>(mine + at * kStride + c);
+            use((place.wm * T::FM + i) * 32 + at, place.wn * T::FN * 32 + c, v);
+        }
+    }
+};
+
+}  // namespace tp

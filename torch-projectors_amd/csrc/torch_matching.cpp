@@ -1,6 +1,6 @@
 // PyTorch dispatcher registration of the matching operators
-// (torch_projectors/matching.py): scores in 8-bit blocks, log probabilities,
-// rows sorted by class.  No counterpart in the reference.  The ops join the
+// (torch_projectors/matching.py): scores in 8-bit blocks and integers, log
+// probabilities of scores and of pairs, rows sorted by class.  No counterpart in the reference.  The ops join the
 // namespace that torch_projectors.cpp defines; each checks its arguments,
 // allocates its outputs and workspace from PyTorch's allocator, and calls the
 // C ABI on PyTorch's current stream.
@@ -140,6 +140,182 @@ Tensor block_scores(const Tensor& images, const optional<Tensor>& image_scales, 
     check_rc(tp_score_images(dt, a.data_ptr(), M, a.size(1), a.stride(0), b.data_ptr(), sb.data_ptr(), N, ptr(f),
                              out_dt, out.data_ptr(), ptr(work), bytes, current_stream(dev)));
     return out;
+}
+
+// ------------------------------------------------------------------ 8-bit integers
+std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
+    const int dt = dtype_code(x, "quantize_rows: x");
+    const auto dev = x.device();
+    const Scope scope(dev);
+    const Tensor v = rows_of(x, "quantize_rows: x");
+    const int64_t R = v.size(0), padded = (v.size(1) + kBlock - 1) / kBlock * kBlock;
+    Tensor codes = fresh({R, padded}, at::kChar, dev), scales = fresh({R}, at::kFloat, dev);
+    check_rc(tp_quantize_rows(dt, v.data_ptr(), R, v.size(1), v.stride(0), codes.data_ptr(), scales.data_ptr(),
+                              current_stream(dev)));
+    return {codes, scales};
+}
+
+void check_rows8(const Tensor& codes, const Tensor& scales, const char* what) {
+    TORCH_CHECK(codes.scalar_type() == at::kChar && codes.dim() == 2 && codes.size(1) >= kBlock &&
+                    codes.size(1) % kBlock == 0,
+                what, ": codes must be int8 (rows, a multiple of 128)");
+    TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.dim() == 1 && scales.size(0) == codes.size(0),
+                what, ": scales must be float32 (rows)");
+}
+
+// images: float rows, quantised on the way, or codes with their scales
+Tensor row_scores(const Tensor& images, const optional<Tensor>& image_scales, const Tensor& codes,
+                  const Tensor& scales, const optional<Tensor>& bias, at::ScalarType out_dtype) {
+    check_rows8(codes, scales, "references");
+    TORCH_CHECK(out_dtype == at::kFloat || out_dtype == at::kBFloat16,
+                "row_scores: out_dtype must be float32 or bfloat16");
+    const auto dev = codes.device();
+    same_device(scales, dev);
+    same_device(images, dev);
+    const Scope scope(dev);
+    const int64_t N = codes.size(0), padded = codes.size(1);
+    Tensor f;
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N && bias->scalar_type() == at::kFloat,
+                    "row_scores: bias must be float32 (references)");
+        same_device(*bias, dev);
+        f = as_held(*bias).contiguous();
+    }
+    const Tensor b = adjacent16(codes), sb = as_held(scales).contiguous();
+    const int out_dt = out_dtype == at::kFloat ? TP_F32 : TP_BF16;
+    auto same_size = [&](int64_t size) {
+        TORCH_CHECK(size == padded, "row_scores: images have ", size, " codes a row, references ", padded);
+    };
+    if (image_scales.has_value()) {
+        check_rows8(images, *image_scales, "images");
+        same_size(images.size(1));
+        same_device(*image_scales, dev);
+        const Tensor a = adjacent16(images), sa = as_held(*image_scales).contiguous();
+        const int64_t M = a.size(0), bytes = tp_row_scores_work(M, N, padded);
+        Tensor out = fresh({M, N}, out_dtype, dev);
+        const Tensor work = workspace(bytes, dev);
+        check_rc(tp_row_scores(a.data_ptr(), sa.data_ptr(), M, b.data_ptr(), sb.data_ptr(), N, padded, ptr(f), out_dt,
+                               out.data_ptr(), ptr(work), bytes, current_stream(dev)));
+        return out;
+    }
+    const int dt = dtype_code(images, "row_scores: images");
+    const Tensor a = rows_of(images, "row_scores: images");
+    same_size((a.size(1) + kBlock - 1) / kBlock * kBlock);
+    const int64_t M = a.size(0), bytes = tp_row_score_images_work(M, N, a.size(1));
+    Tensor out = fresh({M, N}, out_dtype, dev);
+    const Tensor work = workspace(bytes, dev);
+    check_rc(tp_row_score_images(dt, a.data_ptr(), M, a.size(1), a.stride(0), b.data_ptr(), sb.data_ptr(), N, ptr(f),
+                                 out_dt, out.data_ptr(), ptr(work), bytes, current_stream(dev)));
+    return out;
+}
+
+// ------------------------------------------------------------------ log probabilities of pairs
+constexpr int64_t kPairStride = int64_t(1) << 21;  // elements between rows that the kernels take
+
+struct Pairs {
+    int dt;
+    Tensor images, references, given, bias, mask;
+    int64_t M, N, K;
+};
+Pairs pairs(const Tensor& images, const Tensor& references, const optional<Tensor>& given,
+            const optional<Tensor>& bias, const optional<Tensor>& mask) {
+    Pairs p;
+    p.dt = dtype_code(images, "pair_log_probs: images");
+    TORCH_CHECK(references.scalar_type() == images.scalar_type(),
+                "pair_log_probs: images and references must have the same dtype, got ", images.scalar_type(), " and ",
+                references.scalar_type());
+    const auto dev = images.device();
+    same_device(references, dev);
+    auto rows = [](const Tensor& x, const char* what) {
+        const Tensor v = rows_of(x, what);
+        return v.size(0) > 1 && v.stride(0) > kPairStride ? v.contiguous() : v;
+    };
+    p.images = rows(images, "pair_log_probs: images");
+    p.references = rows(references, "pair_log_probs: references");
+    p.M = images.size(0);
+    p.N = references.size(0);
+    p.K = images.size(1);
+    TORCH_CHECK(references.size(1) == p.K, "pair_log_probs: images of ", p.K, " values do not fit references of ",
+                references.size(1));
+    if (given.has_value()) {
+        TORCH_CHECK(given->scalar_type() == at::kLong && given->dim() == 1 && given->size(0) == p.M,
+                    "pair_log_probs: given must be int64 (images)");
+        same_device(*given, dev);
+        p.given = given->contiguous();
+    }
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == p.N,
+                    "pair_log_probs: bias must be float32 (references)");
+        same_device(*bias, dev);
+        p.bias = as_held(*bias).contiguous();
+    }
+    if (mask.has_value()) {
+        TORCH_CHECK(mask->scalar_type() == at::kBool && mask->dim() == 1 && mask->size(0) == p.N,
+                    "pair_log_probs: mask must be bool (references)");
+        same_device(*mask, dev);
+        p.mask = mask->contiguous();
+    }
+    return p;
+}
+// (one row: its stride means nothing, and may be anything)
+int64_t pair_stride(const Tensor& t, int64_t K) { return t.size(0) > 1 ? t.stride(0) : K; }
+
+std::tuple<Tensor, Tensor, Tensor> pair_log_probs_of(const Tensor& images, const Tensor& references,
+                                                     const optional<Tensor>& given, const optional<Tensor>& bias,
+                                                     const optional<Tensor>& mask, double temperature,
+                                                     bool with_state) {
+    const auto dev = images.device();
+    const Scope scope(dev);
+    const Pairs p = pairs(images, references, given, bias, mask);
+    Tensor given_out = given.has_value() ? fresh({p.M}, at::kFloat, dev) : Tensor();
+    Tensor log_sum = fresh({p.M}, at::kFloat, dev);
+    Tensor state = with_state ? fresh({tp_pair_state(p.M, p.N)}, at::kFloat, dev) : Tensor();
+    const int64_t bytes = tp_pair_log_probs_work(p.dt, p.M, p.N, p.K);
+    const Tensor work = workspace(bytes, dev);
+    check_rc(tp_pair_log_probs(p.dt, p.images.data_ptr(), p.M, p.K, pair_stride(p.images, p.K),
+                               p.references.data_ptr(), p.N, pair_stride(p.references, p.K), ptr(p.given), ptr(p.bias),
+                               ptr(p.mask), temperature, ptr(given_out), log_sum.data_ptr(), ptr(state), ptr(work),
+                               bytes, current_stream(dev)));
+    return {given_out, log_sum, state};
+}
+
+std::tuple<Tensor, Tensor, Tensor> pair_log_probs(const Tensor& images, const Tensor& references,
+                                                  const optional<Tensor>& given, const optional<Tensor>& bias,
+                                                  const optional<Tensor>& mask, double temperature) {
+    return pair_log_probs_of(images, references, given, bias, mask, temperature, true);
+}
+
+std::tuple<Tensor, Tensor, Tensor> pair_log_probs_back(const Tensor& images, const Tensor& references,
+                                                       const optional<Tensor>& given, const optional<Tensor>& bias,
+                                                       const optional<Tensor>& mask, double temperature,
+                                                       const Tensor& state, const optional<Tensor>& d_given,
+                                                       const optional<Tensor>& d_log_sum, bool want_images,
+                                                       bool want_references, bool want_bias) {
+    const auto dev = images.device();
+    const Scope scope(dev);
+    const Pairs p = pairs(images, references, given, bias, mask);
+    TORCH_CHECK(state.scalar_type() == at::kFloat && state.dim() == 1 && state.size(0) == tp_pair_state(p.M, p.N),
+                "pair_log_probs_back: state must be the forward call's");
+    same_device(state, dev);
+    auto upstream = [&](const optional<Tensor>& g, const char* what) {
+        if (!g.has_value()) return Tensor();
+        TORCH_CHECK(g->scalar_type() == at::kFloat && g->dim() == 1 && g->size(0) == p.M, "pair_log_probs_back: ",
+                    what, " must be float32 (images)");
+        same_device(*g, dev);
+        return as_held(*g).contiguous();
+    };
+    const Tensor dg = upstream(d_given, "d_given"), dl = upstream(d_log_sum, "d_log_sum"), st = adjacent16(state);
+    Tensor dx, dr, db;
+    if (want_images) dx = fresh({p.M, p.K}, images.scalar_type(), dev);
+    if (want_references) dr = fresh({p.N, p.K}, images.scalar_type(), dev);
+    if (want_bias) db = fresh({p.N}, at::kFloat, dev);
+    const int64_t bytes = tp_pair_log_probs_back_work(p.dt, p.M, p.N, p.K, want_images, want_references);
+    const Tensor work = workspace(bytes, dev);
+    check_rc(tp_pair_log_probs_back(p.dt, p.images.data_ptr(), p.M, p.K, pair_stride(p.images, p.K),
+                                    p.references.data_ptr(), p.N, pair_stride(p.references, p.K), ptr(p.given),
+                                    ptr(p.bias), ptr(p.mask), temperature, st.data_ptr(), ptr(dg), ptr(dl), ptr(dx),
+                                    ptr(dr), ptr(db), ptr(work), bytes, current_stream(dev)));
+    return {dx, dr, db};
 }
 
 // ------------------------------------------------------------------ log probabilities
@@ -386,6 +562,47 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> log_probs_grad(const 
     return {r.size() > 5 ? r[5] : Tensor(), r[0], r[1], r[2], r[3], r[4]};
 }
 
+struct PairLogProbsGrad : torch::autograd::Function<PairLogProbsGrad> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& images, const Tensor& references,
+                                 const optional<Tensor>& given, const optional<Tensor>& bias,
+                                 const optional<Tensor>& mask, double temperature) {
+        auto [g, log_sum, state] = pair_log_probs(images, references, given, bias, mask, temperature);
+        ctx->save_for_backward({images, references, given.value_or(Tensor()), bias.value_or(Tensor()),
+                                mask.value_or(Tensor()), state});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->mark_non_differentiable({state});
+        ctx->set_materialize_grads(false);
+        if (!g.defined()) return {log_sum, state};
+        return {log_sum, state, g};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list d) {
+        const auto v = ctx->get_saved_variables();
+        // (inputs in their order: images, references, given, bias)
+        const bool wx = ctx->needs_input_grad(0), wr = ctx->needs_input_grad(1),
+                   wb = v[3].defined() && ctx->needs_input_grad(v[2].defined() ? 3 : 2);
+        Tensor dx, dr, db;
+        const auto d_given = d.size() > 2 ? given_or_none(d[2]) : c10::nullopt, d_log_sum = given_or_none(d[0]);
+        if (d_given.has_value() || d_log_sum.has_value()) {
+            at::AutoGradMode off(false);
+            std::tie(dx, dr, db) = pair_log_probs_back(v[0], v[1], given_or_none(v[2]), given_or_none(v[3]),
+                                                       given_or_none(v[4]), ctx->saved_data["temperature"].toDouble(),
+                                                       v[5], d_given, d_log_sum, wx, wr, wb);
+        }
+        return once({dx, dr, Tensor(), db, Tensor(), Tensor()});
+    }
+};
+std::tuple<Tensor, Tensor, Tensor> pair_log_probs_grad(const Tensor& images, const Tensor& references,
+                                                       const optional<Tensor>& given, const optional<Tensor>& bias,
+                                                       const optional<Tensor>& mask, double temperature) {
+    refuse_forward_mode(images);
+    refuse_forward_mode(references);
+    refuse_forward_mode(bias);
+    if (!at::GradMode::is_enabled() || !(wants(images) || wants(references) || wants(bias)))  // (no state: None)
+        return pair_log_probs_of(images, references, given, bias, mask, temperature, false);
+    auto r = PairLogProbsGrad::apply(images, references, given, bias, mask, temperature);
+    return {r.size() > 2 ? r[2] : Tensor(), r[0], r[1]};
+}
+
 // SPREAD: rows to their places; else back.  Each one's backward is the other.
 template <bool SPREAD> struct RowsGrad : torch::autograd::Function<RowsGrad<SPREAD>> {
     static std::tuple<Tensor, Tensor> move(bool spread, const Tensor& x, const Tensor& slot, const Tensor& offsets,
@@ -423,6 +640,10 @@ std::tuple<Tensor, Tensor> rows_grad(const Tensor& x, const Tensor& slot, const 
 TORCH_LIBRARY_FRAGMENT(torch_projectors, m) {
     m.def("quantize_blocks(Tensor x) -> (Tensor, Tensor)");
     m.def("block_scores(Tensor images, Tensor? image_scales, Tensor codes, Tensor scales, Tensor? bias, ScalarType out_dtype) -> Tensor");
+    m.def("quantize_rows(Tensor x) -> (Tensor, Tensor)");
+    m.def("row_scores(Tensor images, Tensor? image_scales, Tensor codes, Tensor scales, Tensor? bias, ScalarType out_dtype) -> Tensor");
+    m.def("pair_log_probs(Tensor images, Tensor references, Tensor? given, Tensor? bias, Tensor? mask, float temperature) -> (Tensor, Tensor, Tensor)");
+    m.def("pair_log_probs_back(Tensor images, Tensor references, Tensor? given, Tensor? bias, Tensor? mask, float temperature, Tensor state, Tensor? d_given, Tensor? d_log_sum, bool want_images, bool want_references, bool want_bias) -> (Tensor, Tensor, Tensor)");
     m.def("log_probs(Tensor scores, Tensor? given, Tensor? mask, int top, float temperature) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("log_probs_back(Tensor scores, Tensor? given, Tensor? mask, Tensor top_index, Tensor stats, float temperature, Tensor? d_given, Tensor? d_entropy, Tensor? d_log_sum, Tensor? d_top) -> Tensor");
     m.def("sort_by_class(Tensor classes, int num_classes) -> (Tensor, Tensor, Tensor)");
@@ -433,6 +654,10 @@ TORCH_LIBRARY_FRAGMENT(torch_projectors, m) {
 TORCH_LIBRARY_IMPL(torch_projectors, CUDA, m) {
     m.impl("quantize_blocks", &quantize_blocks);
     m.impl("block_scores", &block_scores);
+    m.impl("quantize_rows", &quantize_rows);
+    m.impl("row_scores", &row_scores);
+    m.impl("pair_log_probs", &pair_log_probs);
+    m.impl("pair_log_probs_back", &pair_log_probs_back);
     m.impl("log_probs", &log_probs);
     m.impl("log_probs_back", &log_probs_back);
     m.impl("sort_by_class", &sort_by_class);
@@ -443,8 +668,9 @@ TORCH_LIBRARY_IMPL(torch_projectors, CUDA, m) {
 // What is differentiable takes its gradient from above; the others are called as they are.
 TORCH_LIBRARY_IMPL(torch_projectors, AutogradCUDA, m) {
     m.impl("log_probs", &log_probs_grad);
+    m.impl("pair_log_probs", &pair_log_probs_grad);
     m.impl("spread_rows", &rows_grad<true>);
     m.impl("gather_rows", &rows_grad<false>);
-    for (const char* name : {"quantize_blocks", "block_scores", "log_probs_back", "sort_by_class"})
+    for (const char* name : {"quantize_blocks", "block_scores", "quantize_rows", "row_scores", "log_probs_back", "pair_log_probs_back", "sort_by_class"})
         m.impl(name, torch::CppFunction::makeFallthrough());
 }

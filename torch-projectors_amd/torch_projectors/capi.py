@@ -45,6 +45,11 @@ SIGNATURES = {
     "tp_quantize_blocks": [_I, _P, _L, _L, _L, _P, _P, _P],
     "tp_block_scores": [_P, _P, _L, _P, _P, _L, _L, _P, _I, _P, _P, _L, _P],
     "tp_score_images": [_I, _P, _L, _L, _L, _P, _P, _L, _P, _I, _P, _P, _L, _P],
+    "tp_quantize_rows": [_I, _P, _L, _L, _L, _P, _P, _P],
+    "tp_row_scores": [_P, _P, _L, _P, _P, _L, _L, _P, _I, _P, _P, _L, _P],
+    "tp_row_score_images": [_I, _P, _L, _L, _L, _P, _P, _L, _P, _I, _P, _P, _L, _P],
+    "tp_pair_log_probs": [_I, _P, _L, _L, _L, _P, _L, _L, _P, _P, _P, _D, _P, _P, _P, _P, _L, _P],
+    "tp_pair_log_probs_back": [_I, _P, _L, _L, _L, _P, _L, _L, _P, _P, _P, _D, _P, _P, _P, _P, _P, _P, _P, _L, _P],
     "tp_log_probs": [_I, _P, _L, _L, _L, _P, _L, _P, _L, _L, _D, _P, _P, _P, _P, _P, _P, _P, _L, _P],
     "tp_log_probs_back": [_I, _P, _L, _L, _L, _P, _L, _P, _L, _L, _D, _P, _P, _P, _P, _P, _P, _P, _P],
     "tp_sort_by_class": [_I, _P, _L, _L, _P, _P, _P, _P, _L, _P],
@@ -60,6 +65,11 @@ SIZE_HELPERS = {
     "tp_scale_rows": [_L],
     "tp_block_scores_work": [_L, _L, _L],
     "tp_score_images_work": [_L, _L, _L],
+    "tp_row_scores_work": [_L, _L, _L],
+    "tp_row_score_images_work": [_L, _L, _L],
+    "tp_pair_state": [_L, _L],
+    "tp_pair_log_probs_work": [_I, _L, _L, _L],
+    "tp_pair_log_probs_back_work": [_I, _L, _L, _L, _I, _I],
     "tp_log_probs_work": [_L, _L, _L],
     "tp_sort_by_class_work": [_L, _L],
 }

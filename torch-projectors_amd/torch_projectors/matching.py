@@ -2,8 +2,12 @@
 
     quantize_blocks(x)                    rows in 8-bit floating point, a scale for each 128 values
     block_scores(images, references)      <image, reference> of every pair, from such rows
+    quantize_rows(x)                      rows in 8-bit integers, a scale for each row
+    row_scores(images, references)        <image, reference> of every pair, from such rows
     log_probs(scores, given, top, ...)    log probabilities of given candidates, entropy, log sum and the
                                           best alternatives of each row; differentiable
+    pair_log_probs(images, references)    log probabilities of given references and log sums of each image, without
+                                          the scores in memory; differentiable
     sort_by_class(classes, num_classes)   rows sorted by the classes that they go to
     dispatch(x, order) / combine(y, order)  rows into that order, and back with weights; differentiable
 
@@ -12,8 +16,9 @@ stack against the projections of every class and pose (`block_scores`), turns th
 (`log_probs`: `top_index` and `top` are the best hypotheses and their weights), and hands each image to the
 classes it goes to (`sort_by_class` of the hypotheses' classes, `dispatch`); each class's stretch
 `offsets[c] : offsets[c + 1]` is then one call of a projection operator, and `combine` sums a row's results
-with its weights.  In training, `log_probs` of `images @ projections.T` carries the gradient of the marginal
-likelihood (`log_sum`) back to volumes and poses.
+with its weights.  In training, `pair_log_probs` of images and projections carries the gradient of the marginal
+likelihood (`log_sum`) back to volumes and poses; where scores with more terms are formed by other means, `log_probs`
+of them does.
 
 All run on the GPU only (a CPU tensor raises NotImplementedError), on the current stream, without a
 synchronisation; they can be captured in a graph.  What is differentiable is so once, backwards (forward-mode
@@ -90,6 +95,88 @@ def block_scores(images, references, bias: Optional[torch.Tensor] = None,
         references = quantize_blocks(references)
     images, image_scales = images if rows is None else (rows, None)
     return _OPS.block_scores.default(images, image_scales, references.codes, references.scales, bias, out_dtype)
+
+
+# ----------------------------------------------------------------------------- scores in 8-bit integers
+class RowScaled(NamedTuple):
+    """Rows [R, K] in 8-bit integers: value = code * scale of its row.
+
+    codes   [R, K padded to a multiple of 128] int8, -127 to 127, zero past K
+    scales  [R] float32
+    """
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def quantize_rows(x: torch.Tensor) -> RowScaled:
+    """Rows [R, ...] (float32, float16, bfloat16 or complex64, at most 131072 values each) in 8-bit integers.
+
+    A row's scale is its largest magnitude / 127 (2^-126 at least), a code its value / scale to the nearest integer,
+    half to even; both quotients are those of float32.  A row with a value that is not finite has scale NaN and codes
+    0, so that its scores are NaN.  Not differentiable.
+
+    The steps are even, 1/127 of a row's largest value: finer than those of `quantize_blocks` for rows whose values
+    are all of a size (whitened images), coarser where they fall by orders of magnitude along a row."""
+    return RowScaled(*_OPS.quantize_rows.default(_real_rows(x, "x")))
+
+
+def row_scores(images, references, bias: Optional[torch.Tensor] = None,
+               out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """scores[m, n] = <image m, reference n> + bias[n], from rows of 8-bit integers: their products' sum is exact,
+    times the image's scale, times the reference's, plus the bias in float32.
+
+    images [M, ...] and references [N, ...] are RowScaled, or rows that are quantised here, of as many values on both
+    sides (of RowScaled rows the padded sizes are compared); of complex rows the real part of the inner product is
+    taken (their real pairs' product).  bias float32 [N]; out_dtype float32 or bfloat16.  Not differentiable."""
+    rows = None if isinstance(images, RowScaled) else _real_rows(images, "images")
+    if not isinstance(references, RowScaled):
+        references = _real_rows(references, "references")
+        if rows is not None and rows.shape[1] != references.shape[1]:
+            raise ValueError(f"Images of {rows.shape[1]} values do not fit references of {references.shape[1]}")
+        references = quantize_rows(references)
+    images, image_scales = images if rows is None else (rows, None)
+    return _OPS.row_scores.default(images, image_scales, references.codes, references.scales, bias, out_dtype)
+
+
+# ----------------------------------------------------------------------------- log probabilities of pairs
+class PairLogProbs(NamedTuple):
+    """Results of pair_log_probs, float32 [M].
+
+    given    log probabilities of the given references (None without)
+    log_sum  ln sum exp(score) over the allowed references
+    """
+    given: Optional[torch.Tensor]
+    log_sum: torch.Tensor
+
+
+def pair_log_probs(images: torch.Tensor, references: torch.Tensor, given: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                   mask: Optional[torch.Tensor] = None) -> PairLogProbs:
+    """What `log_probs` says of scores (<image m, reference n> + bias[n]) / temperature, without the scores in memory:
+    the log probability of each image's given reference and the log sum over its references.
+
+    images [M, ...] and references [N, ...] have the same dtype (float32, float16, bfloat16 or complex64) and as many
+    values each; of complex rows the real part of the inner product is taken (their real pairs' product).
+
+    given   int64 [M]: -1 for none (its result is 0 and has no gradient); any other index out of range gives NaN, and a
+            NaN gradient of its image unless its upstream gradient is 0
+    bias    float32 [N]; -inf rules a reference out, as the mask does
+    mask    bool [N], True where allowed; what a reference that is ruled out by it holds is not used
+
+    An image with no allowed reference has log_sum and log probabilities -inf and no gradient.  Values that are not
+    finite among the allowed make scores that are not, which make their image's results NaN, but for scores of -inf
+    of float16 and bfloat16 rows, which count as ruled out.
+
+    The gradient reaches images, references (in their dtype) and bias from both results.  It forms the scores
+    again, a piece of the references after the other; a piece's share of the gradient of the scores is kept in the
+    rows' dtype (at most 128 MB or 256 references' worth).  Up to 8 images keep their scores instead."""
+    x, r = _real_rows(images, "images"), _real_rows(references, "references")
+    if x.shape[1] != r.shape[1]:
+        raise ValueError(f"Images of {x.shape[1]} values do not fit references of {r.shape[1]}")
+    for what, t, n in (("Given references", given, x.shape[0]), ("Bias", bias, r.shape[0]), ("Mask", mask, r.shape[0])):
+        if t is not None and t.shape != (n,):
+            raise ValueError(f"{what} {tuple(t.shape)} must be ({n},)")
+    return PairLogProbs(*_OPS.pair_log_probs.default(x, r, given, bias, mask, temperature)[:2])
 
 
 # ----------------------------------------------------------------------------- log probabilities
