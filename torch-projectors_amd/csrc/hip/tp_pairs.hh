@@ -42,25 +42,31 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
 // What an image's gradient is made of: G = d score / d(<image, reference> + bias) = a exp(score - most), at_given
 // where the reference is the given one.
 struct PairCoef {
-    float most, a, at_given;
-    int given;  // -1: none
+    float most, a, at_given;  // (most in powers of two, as below)
+    int given;                // -1: none
 };
 struct PairTile {
-    int tile, splits;
+    bool direct;     // operands go straight to LDS (16-bit rows that start at 16-byte boundaries)
+    int tile;
+    uint32_t whole;  // tiles that are not split
+    int splits;      // ranges of the contraction of the others
 };
+// Scores are formed and summed in powers of two: score * log2 e, so that a product and a sum become one multiply-add and
+// the exponential one instruction.
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 struct ScorePart {
-    float most, sum;  // of a tile's references: the largest score, and sum exp(score - most) without the given one
+    float most, sum;  // of a tile's references: the largest score, and sum 2^(score - most) without the given one
 };
 // rows (of D), columns and contraction of a product -> its tile and ranges
-PairTile pair_plan(int dt, int64_t rows, int64_t cols, int64_t kdim);
+PairTile pair_plan(int dt, bool direct, int64_t rows, int64_t cols, int64_t kdim);
 int64_t pair_part_bytes(int dt, const PairTile& t, int64_t rows, int64_t cols);
-int64_t pair_tiles(int dt, int tile, int64_t rows, bool of_rows);  // along the rows or the columns
+int64_t pair_tiles(int dt, const PairTile& t, int64_t n, bool of_rows);  // along the rows or the columns
 
 struct PairOff {  // what a tile's references add to their scores
     const float* bias;
     const uint8_t* mask;
     int64_t N;
-    float c;
+    float c;  // log2 e over the temperature
 };
 // stats: parts [reference tiles][M] and given_score [M]
 struct StatsOut {

@@ -19,11 +19,11 @@
 namespace tp {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kStats = 4;  // largest, others, own, and the given reference's score
 
-__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
-// a, b: (largest, sum of exp(z - largest)) of two sets of scores
+// (scores in powers of two)
+__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z); }
+// (largest, sum of 2^(z - largest)) of two sets of scores
 __device__ __forceinline__ void join(float& most, float& sum, float most2, float sum2) {
     const float both = fmaxf(most, most2), base = both == -INFINITY ? 0.0f : both;
     sum = sum * exp_of(most - base) + sum2 * exp_of(most2 - base);
@@ -39,10 +39,10 @@ __device__ __forceinline__ void finish(const PairArgs& a, int64_t m, float most,
     const float own = valid ? exp_of(z - base) : 0.0f, total = others + own;
     // (1 + x) - 1 is what logf sees of a sum near one: the others by themselves
     const float log_total = own == 1.0f && others < 0.5f ? log1pf(others) : logf(total);
-    log_sum[m] = base + log_total;
+    log_sum[m] = fmaf(base, kLn2, log_total);
     if (total == 0.0f) log_sum[m] = -INFINITY;
     if (given_out) {
-        float v = own > others ? -log1pf(others / own) : (z - base) - log_total;
+        float v = own > others ? -log1pf(others / own) : (z - base) * kLn2 - log_total;
         if (total == 0.0f) v = -INFINITY;
         given_out[m] = valid ? v : g == -1 ? 0.0f : NAN;
     }
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
             if (v == -INFINITY) continue;
             float s = 0.0f;
             for (int t = 0; t < splits; ++t) s += part[(int64_t(t) * a.M + m) * a.N + n];
-            z[k] = (s + v) * a.c;
+            z[k] = fmaf(s, a.c * kLog2e, v * (a.c * kLog2e));
         }
         float here = most;
 #pragma unroll
@@ -418,12 +418,15 @@ int64_t few_per(int64_t N, int64_t K) {
 }
 
 struct TileKind {
-    int bm, bn, bk;
+    int bm, bn, bk, per_cu;  // per_cu: workgroups that a CU holds at once
     double step_us, alone_us;
 };
-constexpr TileKind kTiles16[] = {{64, 64, 64, 0.20, 0.45}, {128, 128, 64, 0.55, 0.8}, {256, 256, 64, 1.9, 1.7}};
-constexpr TileKind kTiles32[] = {{64, 64, 32, 0.45, 0.7}, {128, 128, 32, 1.6, 1.6}, {256, 128, 32, 2.9, 2.5}};
-const TileKind& kind_of(int dt, int t) { return dt == TP_F32 ? kTiles32[t] : kTiles16[t]; }
+constexpr TileKind kTiles16[] = {{64, 64, 64, 5, 0.20, 0.62}, {128, 128, 64, 2, 0.55, 1.00}, {256, 256, 64, 1, 1.75, 1.75}};
+constexpr TileKind kTilesStaged[] = {{64, 64, 64, 4, 0.22, 0.75}, {128, 128, 64, 2, 0.60, 0.95}};
+constexpr TileKind kTiles32[] = {{64, 64, 32, 3, 0.40, 0.62}, {128, 128, 32, 1, 1.40, 1.20}, {256, 128, 32, 1, 2.45, 2.10}};
+const TileKind& kind_of(int dt, const PairTile& t) {
+    return dt == TP_F32 ? kTiles32[t.tile] : t.direct ? kTiles16[t.tile] : kTilesStaged[t.tile];
+}
 constexpr int kMaxSplits = 32;
 
 // A piece's G is at most this large: 128 MB stay in the last cache between the product that writes it and those that read it.
@@ -437,18 +440,24 @@ int64_t piece_of(int dt, int64_t M, int64_t N) {
     return each < N ? each : N;
 }
 
+// Whether all products' operands of these images and references go straight to LDS.
+bool pair_direct(const PairArgs& a) {
+    auto fits = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
+    return a.dt != TP_F32 && a.K % 8 == 0 && fits(a.x, a.ldx) && fits(a.r, a.ldr);
+}
+
 struct BackLayout {
     int64_t piece, ldg;
     PairTile grad, refs, images;
     int64_t coef, scale, g, sums, part, dx, bytes;
 };
-BackLayout back_layout(int dt, int64_t M, int64_t N, int64_t K, bool d_x, bool d_r) {
+BackLayout back_layout(int dt, bool direct, int64_t M, int64_t N, int64_t K, bool d_x, bool d_r) {
     BackLayout b{};
     b.piece = piece_of(dt, M, N);
     b.ldg = (M + 7) / 8 * 8;
-    b.grad = pair_plan(dt, b.piece, M, K);
-    b.refs = pair_plan(dt, b.piece, K, M);
-    b.images = pair_plan(dt, M, K, b.piece);
+    b.grad = pair_plan(dt, direct, b.piece, M, K);
+    b.refs = pair_plan(dt, direct, b.piece, K, M);
+    b.images = pair_plan(dt, direct, M, K, b.piece);
     int64_t at = 0;
     auto room = [&](int64_t bytes) {
         const int64_t here = at;
@@ -458,7 +467,7 @@ BackLayout back_layout(int dt, int64_t M, int64_t N, int64_t K, bool d_x, bool d
     b.coef = room(M * int64_t(sizeof(PairCoef)));
     b.scale = room(16);
     b.g = room(b.piece * b.ldg * size_of(dt));
-    b.sums = room(pair_tiles(dt, b.grad.tile, M, false) * b.piece * 4);
+    b.sums = room(pair_tiles(dt, b.grad, M, false) * b.piece * 4);
     int64_t part = pair_part_bytes(dt, b.grad, b.piece, M);
     if (d_r) part = part > pair_part_bytes(dt, b.refs, b.piece, K) ? part : pair_part_bytes(dt, b.refs, b.piece, K);
     if (d_x) part = part > pair_part_bytes(dt, b.images, M, K) ? part : pair_part_bytes(dt, b.images, M, K);
@@ -492,43 +501,63 @@ __global__ __launch_bounds__(256) void k_pairs_none(PairArgs a, float* given_out
 
 }  // namespace
 
-// The tile and the number of ranges of the contraction with the least time by a count of steps.
-PairTile pair_plan(int dt, int64_t rows, int64_t cols, int64_t kdim) {
-    PairTile best{0, 1};
+// The tile, and the tiles and ranges that are split, with the least time by a count of steps (one bk of the contraction for one
+// tile).  The CUs hold per_cu tiles each; tiles that fill them all run whole, round after round; those that are left over are
+// split so that they do, too.
+PairTile pair_plan(int dt, bool direct, int64_t rows, int64_t cols, int64_t kdim) {
+    PairTile best{direct, 0, 0, 1};
     double least = 1e300;
-    for (int t = 0; t < 3; ++t) {
-        const TileKind& k = kind_of(dt, t);
+    for (int t = 0; t < (dt == TP_F32 || direct ? 3 : 2); ++t) {
+        const TileKind& k = kind_of(dt, PairTile{direct, t, 0, 1});
         const int64_t tiles = ((rows + k.bm - 1) / k.bm) * ((cols + k.bn - 1) / k.bn);
-        const int64_t steps = (kdim + k.bk - 1) / k.bk;
         if (tiles > kMaxTiles) continue;
+        const int64_t steps = (kdim + k.bk - 1) / k.bk, slots = int64_t(kCus) * k.per_cu;
+        const int64_t rounds = tiles / slots, rest = tiles - rounds * slots;
+        // a step of as many workgroups as there are on a CU
+        auto step = [&](int64_t groups) {
+            const double each = double((groups + kCus - 1) / kCus) * k.step_us;
+            return each > k.alone_us ? each : k.alone_us;
+        };
+        const double whole_us = 3.0 + rounds * (steps + 4) * step(slots);
         for (int s = 1; s <= kMaxSplits && s <= steps; ++s) {
-            if (s > 1 && tiles * s > 8 * kCus) break;
-            const double each = double((tiles * s + kCus - 1) / kCus);
-            const double step = each * k.step_us > k.alone_us ? each * k.step_us : k.alone_us;
-            double us = 3.0 + ((steps + s - 1) / s + 3) * step;
-            if (s > 1) us += 4.0 + double(tiles) * k.bm * k.bn * (8.0 * s) / 4.0e6;
+            const int64_t groups = rest * s, full = groups / slots, over = groups - full * slots;
+            if (s > 1 && groups > 4 * slots) break;
+            const double each = double((steps + s - 1) / s + 4);
+            double us = whole_us + each * (full * step(slots) + (over ? step(over) : 0.0));
+            if (s > 1 && rest) us += 4.0 + double(rest) * k.bm * k.bn * (8.0 * s) / 4.0e6;
             if (us < least) {
                 least = us;
-                best = {t, s};
+                best = {direct, t, uint32_t(rounds * slots), s};
             }
+            if (!rest) break;
         }
     }
     return best;
 }
 int64_t pair_part_bytes(int dt, const PairTile& t, int64_t rows, int64_t cols) {
-    const TileKind& k = kind_of(dt, t.tile);
-    return t.splits > 1 ? pair_tiles(dt, t.tile, rows, true) * pair_tiles(dt, t.tile, cols, false) * t.splits * k.bm * k.bn * 4 : 0;
+    const TileKind& k = kind_of(dt, t);
+    const int64_t rest = pair_tiles(dt, t, rows, true) * pair_tiles(dt, t, cols, false) - int64_t(t.whole);
+    return t.splits > 1 && rest > 0 ? rest * t.splits * k.bm * k.bn * 4 : 0;
 }
-int64_t pair_tiles(int dt, int tile, int64_t n, bool of_rows) {
-    const int size = of_rows ? kind_of(dt, tile).bm : kind_of(dt, tile).bn;
+int64_t pair_tiles(int dt, const PairTile& t, int64_t n, bool of_rows) {
+    const int size = of_rows ? kind_of(dt, t).bm : kind_of(dt, t).bn;
     return (n + size - 1) / size;
 }
 
+// (rows may turn out not to start at 16-byte boundaries: room for either plan)
+template <class F> int64_t either_plan(int dt, int64_t K, F bytes) {
+    const int64_t staged = bytes(false);
+    if (dt == TP_F32 || K % 8) return staged;
+    const int64_t straight = bytes(true);
+    return staged > straight ? staged : straight;
+}
 int64_t pair_work(int dt, int64_t M, int64_t N, int64_t K) {
     if (M == 0 || N == 0) return 0;
     if (pair_few(M)) return up16(few_splits(dt, N, K) * M * N * 4);
-    const PairTile t = pair_plan(dt, N, M, K);
-    return up16(M * 4) + up16(pair_tiles(dt, t.tile, N, true) * M * int64_t(sizeof(ScorePart))) + pair_part_bytes(dt, t, N, M);
+    return either_plan(dt, K, [&](bool direct) {
+        const PairTile t = pair_plan(dt, direct, N, M, K);
+        return up16(M * 4) + up16(pair_tiles(dt, t, N, true) * M * int64_t(sizeof(ScorePart))) + pair_part_bytes(dt, t, N, M);
+    });
 }
 
 hipError_t launch_pair_log_probs(const PairArgs& a, float* given_out, float* log_sum, float* state, void* work,
@@ -551,12 +580,12 @@ hipError_t launch_pair_log_probs(const PairArgs& a, float* given_out, float* log
                                                              given_out, log_sum, state);
         return hipGetLastError();
     }
-    const PairTile t = pair_plan(a.dt, a.N, a.M, a.K);
-    const int64_t tiles = pair_tiles(a.dt, t.tile, a.N, true);
+    const PairTile t = pair_plan(a.dt, pair_direct(a), a.N, a.M, a.K);
+    const int64_t tiles = pair_tiles(a.dt, t, a.N, true);
     auto* given_score = static_cast<float*>(work);
     auto* parts = reinterpret_cast<ScorePart*>(static_cast<char*>(work) + up16(a.M * 4));
     auto* part = reinterpret_cast<float*>(reinterpret_cast<char*>(parts) + up16(tiles * a.M * int64_t(sizeof(ScorePart))));
-    const StatsOut o{{a.bias, a.mask, a.N, a.c}, a.given, a.M, parts, given_score};
+    const StatsOut o{{a.bias, a.mask, a.N, a.c * kLog2e}, a.given, a.M, parts, given_score};
     const hipError_t e = by_type(a.dt, [&](auto S) { return PairProducts<decltype(S)>::stats(a, t, o, part, s); });
     if (e) return e;
     k_pairs_join<<<dim3(unsigned((a.M + 15) / 16)), 256, 0, s>>>(a, parts, int(tiles), given_score, given_out, log_sum, state);
@@ -566,7 +595,7 @@ hipError_t launch_pair_log_probs(const PairArgs& a, float* given_out, float* log
 int64_t pair_back_work(int dt, int64_t M, int64_t N, int64_t K, bool d_x, bool d_r) {
     if (M == 0 || N == 0) return 0;
     if (pair_few(M)) return d_x ? up16((N + few_per(N, K) - 1) / few_per(N, K) * M * K * 4) : 0;
-    return back_layout(dt, M, N, K, d_x, d_r).bytes;
+    return either_plan(dt, K, [&](bool direct) { return back_layout(dt, direct, M, N, K, d_x, d_r).bytes; });
 }
 
 hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, const float* d_given,
@@ -597,7 +626,7 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
         });
         return hipGetLastError();
     }
-    const BackLayout b = back_layout(a.dt, a.M, a.N, a.K, d_x, d_r);
+    const BackLayout b = back_layout(a.dt, pair_direct(a), a.M, a.N, a.K, d_x, d_r);
     char* w = static_cast<char*>(work);
     auto* coef = reinterpret_cast<PairCoef*>(w + b.coef);
     auto* scale = reinterpret_cast<float*>(w + b.scale);
@@ -612,7 +641,7 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
         const int64_t n = a.N - first < b.piece ? a.N - first : b.piece;
         const char* r = static_cast<const char*>(a.r) + first * a.ldr * size;
         const uint8_t* mask = a.mask ? a.mask + first : nullptr;
-        const GradOut go{{a.bias ? a.bias + first : nullptr, mask, n, a.c}, coef, a.M, first, w + b.g, b.ldg, d_bias ? sums : nullptr};
+        const GradOut go{{a.bias ? a.bias + first : nullptr, mask, n, a.c * kLog2e}, coef, a.M, first, w + b.g, b.ldg, d_bias ? sums : nullptr};
         const MatrixOut ro{scale, n, a.K, nullptr, nullptr, d_r ? static_cast<char*>(d_r) + first * a.K * size : nullptr, a.K};
         const MatrixOut xo{scale, a.M, a.K, first ? dx : nullptr, first + n < a.N ? dx : nullptr, d_x, a.K};
         const hipError_t e = by_type(a.dt, [&](auto S) {
@@ -624,7 +653,7 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
         });
         if (e) return e;
         if (d_bias) {
-            k_pairs_bias<<<match_grid((n + 255) / 256), 256, 0, s>>>(sums, int(pair_tiles(a.dt, b.grad.tile, a.M, false)), n,
+            k_pairs_bias<<<match_grid((n + 255) / 256), 256, 0, s>>>(sums, int(pair_tiles(a.dt, b.grad, a.M, false)), n,
                                                                      scale, d_bias + first);
             if (hipError_t f = hipGetLastError()) return f;
         }

@@ -4,20 +4,26 @@
 #include "tp_pairs.hh"
 #include "tp_tile.hh"
 
+#include <type_traits>
+
 namespace tp {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
-
-// LDS behind what the epilogue's other parts use: a tile's offsets, -inf where the reference is ruled out.
-template <class T> __device__ __forceinline__ void tile_offsets(const PairOff& o, int64_t first, float* off) {
+// What a reference adds to its scores, in LDS: score = min(sum c + add, limit), where the limit of one that is ruled out
+// is -inf, whatever its sum is (the minimum with a NaN is the other), and that of the others +inf (a NaN becomes
+// +inf, which makes its image's results NaN all the same).
+struct alignas(8) Offset {
+    float add, limit;
+};
+template <class T> __device__ __forceinline__ void tile_offsets(const PairOff& o, int64_t first, Offset* off) {
     for (int i = threadIdx.x; i < T::BM; i += T::NT) {
         const int64_t n = first + i;
-        off[i] = n < o.N && (!o.mask || o.mask[n]) ? (o.bias ? o.bias[n] : 0.0f) : -INFINITY;
+        const float b = n < o.N && (!o.mask || o.mask[n]) ? (o.bias ? o.bias[n] : 0.0f) : -INFINITY;
+        off[i] = b == -INFINITY ? Offset{0.0f, -INFINITY} : Offset{b * o.c, INFINITY};
     }
 }
-// (what the product of a reference that is ruled out came to does not matter)
-__device__ __forceinline__ float score(float sum, float off, float c) { return off == -INFINITY ? -INFINITY : (sum + off) * c; }
+__device__ __forceinline__ float score(float sum, const Offset& o, float c) { return fminf(fmaf(sum, c, o.add), o.limit); }
+__device__ __forceinline__ float base_of(float most) { return most == -INFINITY ? 0.0f : most; }
 
 // A lane holds 16 FM references of each of its FN images: their maximum and sum in registers, then over the two
 // halves of the wavefront and the WM wavefronts.
@@ -28,41 +34,68 @@ struct StatsEpi {
         const int tid = threadIdx.x;
         const Place<T> place(tid);
         const int64_t n0 = int64_t(im) * T::BM, m0 = int64_t(in) * T::BN;
-        float* off = reinterpret_cast<float*>(lds);
+        Offset* off = reinterpret_cast<Offset*>(lds);
         ScorePart* part = reinterpret_cast<ScorePart*>(off + T::BM);  // [WM][BN]
         tile_offsets<T>(g.off, n0, off);
-        __syncthreads();
+        float most[T::FN], sum[T::FN];
+        int at[T::FN];  // the given reference, relative to the lane's first row as at() counts
 #pragma unroll
         for (int j = 0; j < T::FN; ++j) {
             const int64_t m = m0 + place.col(j);
-            const int64_t given = g.given && m < g.M ? g.given[m] - n0 : -1;
-            const int at = given >= 0 && given < T::BM && given + n0 < g.off.N ? int(given) : -1;
-            float most = -INFINITY, sum = 0.0f, z_given = 0.0f;
-            asm volatile("" ::: "memory");  // (the offsets are read again: kept for the next column they would fill the registers)
+            const int64_t given = g.given && m < g.M ? g.given[m] : -1;
+            at[j] = given >= n0 && given < n0 + T::BM && given < g.off.N ? int(given - n0) - place.first() : -1;
+            most[j] = -INFINITY;
+            sum[j] = 0.0f;
+        }
+        __syncthreads();
+        const Offset* mine = off + place.first();
+        // (the scores are formed twice: kept, they would need the registers of the sums once more)
 #pragma unroll
-            for (int i = 0; i < T::FM; ++i) {
+        for (int i = 0; i < T::FM; ++i) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    acc[i][j][e] = score(acc[i][j][e], off[place.row(i, e)], g.off.c);
-                    most = fmaxf(most, acc[i][j][e]);
-                }
-                __builtin_amdgcn_sched_barrier(0);  // (else all offsets of the tile wait in registers)
+            for (int e = 0; e < 16; ++e) {
+                const Offset o = mine[place.at(i, e)];
+#pragma unroll
+                for (int j = 0; j < T::FN; ++j) most[j] = fmaxf(most[j], score(acc[i][j][e], o, g.off.c));
             }
-            most = fmaxf(most, __shfl_xor(most, 32));
-            const float base = most == -INFINITY ? 0.0f : most;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float base[T::FN];
 #pragma unroll
-            for (int i = 0; i < T::FM; ++i)
+        for (int j = 0; j < T::FN; ++j) {
+            most[j] = fmaxf(most[j], __shfl_xor(most[j], 32));
+            base[j] = base_of(most[j]);
+        }
+        asm volatile("" ::: "memory");  // (the offsets are read again)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float z = acc[i][j][e];
-                    const bool is = place.row(i, e) == at;
-                    const float p = __builtin_amdgcn_exp2f((z - base) * kLog2e);
-                    sum += is ? 0.0f : p;
-                    z_given = is ? z : z_given;
+        for (int i = 0; i < T::FM; ++i) {
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j) {
+                const int here = at[j] - i * 32;
+                const bool any = here >= 0 && here < 32 && !(here & 4);
+                if (__builtin_amdgcn_ballot_w64(any) == 0) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        sum[j] += __builtin_amdgcn_exp2f(score(acc[i][j][e], mine[place.at(i, e)], g.off.c) - base[j]);
+                } else {  // the given reference's score goes out, and is not among the others
+                    float given = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const bool is = here == place.at(0, e);
+                        const float z = score(acc[i][j][e], mine[place.at(i, e)], g.off.c);
+                        const float p = __builtin_amdgcn_exp2f(z - base[j]);
+                        given = is ? z : given;
+                        sum[j] += is ? 0.0f : p;
+                    }
+                    if (any) g.given_score[m0 + place.col(j)] = given;
                 }
-            if (at >= 0 && at / (T::FM * 32) == place.wm && ((at >> 2) & 1) == place.q) g.given_score[m] = z_given;
-            sum += __shfl_xor(sum, 32);
-            if (place.q == 0) part[place.wm * T::BN + place.col(j)] = ScorePart{most, sum};
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < T::FN; ++j) {
+            sum[j] += __shfl_xor(sum[j], 32);
+            if (place.q == 0) part[place.wm * T::BN + place.col(j)] = ScorePart{most[j], sum[j]};
         }
         __syncthreads();
         for (int i = tid; i < T::BN; i += T::NT) {
@@ -71,15 +104,27 @@ struct StatsEpi {
 #pragma unroll
             for (int w = 1; w < T::WM; ++w) {
                 const ScorePart p = part[w * T::BN + i];
-                const float most = fmaxf(all.most, p.most), base = most == -INFINITY ? 0.0f : most;
-                all.sum = all.sum * __builtin_amdgcn_exp2f((all.most - base) * kLog2e) +
-                          p.sum * __builtin_amdgcn_exp2f((p.most - base) * kLog2e);
-                all.most = most;
+                const float both = fmaxf(all.most, p.most), base = base_of(both);
+                all.sum = all.sum * __builtin_amdgcn_exp2f(all.most - base) + p.sum * __builtin_amdgcn_exp2f(p.most - base);
+                all.most = both;
             }
             g.parts[int64_t(im) * g.M + m0 + i] = all;
         }
     }
 };
+
+// Sum over 16 (or 8) neighbouring lanes, in each of them: adds whose second operand comes from another lane.
+template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
+    auto plus = [&](auto ctrl) {
+        v += __uint_as_float(__builtin_amdgcn_update_dpp(0, int(__float_as_uint(v)), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    static_assert(LANES == 16 || LANES == 8, "a row of DPP lanes or half of one");
+    if (LANES == 16) plus(std::integral_constant<int, 0x140>{});  // mirrored row
+    plus(std::integral_constant<int, 0x141>{});                   // mirrored half row
+    plus(std::integral_constant<int, 0x4e>{});                    // pairs of four swapped
+    plus(std::integral_constant<int, 0xb1>{});                    // neighbours swapped
+    return v;
+}
 
 struct GradEpi {
     using Args = GradOut;
@@ -89,44 +134,61 @@ struct GradEpi {
         const Place<T> place(tid);
         const int64_t n0 = int64_t(im) * T::BM, m0 = int64_t(in) * T::BN;
         char* rows = lds;
-        float* off = reinterpret_cast<float*>(lds + (T::NT / 64) * Rows4<T>::kBytes);
-        float* sums = off + T::BM;  // [WN][BM]
-        static_assert((T::NT / 64) * Rows4<T>::kBytes + 4 * T::BM * (1 + T::WN) <= tile_lds<S, T>(), "LDS of the products");
+        Offset* off = reinterpret_cast<Offset*>(lds + (T::NT / 64) * Rows4<T>::kBytes);
+        float* sums = reinterpret_cast<float*>(off + T::BM);  // [WN][BM]
+        static_assert((T::NT / 64) * Rows4<T>::kBytes + 4 * T::BM * (2 + T::WN) <= tile_lds<S, T>(), "LDS of the products");
         tile_offsets<T>(g.off, n0, off);
-        __syncthreads();
+        float most[T::FN], a[T::FN], at_given[T::FN];
+        int at[T::FN];
 #pragma unroll
         for (int j = 0; j < T::FN; ++j) {
             const int64_t m = m0 + place.col(j);
             PairCoef k{0.0f, 0.0f, 0.0f, -1};
             if (m < g.M) k = g.coef[m];
-            const int64_t given = k.given - g.first - n0;
-            const int at = k.given >= 0 && given >= 0 && given < T::BM ? int(given) : -1;
-            asm volatile("" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < T::FM; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int row = place.row(i, e);
-                    const float z = score(acc[i][j][e], off[row], g.off.c);
-                    float v = k.a * __builtin_amdgcn_exp2f((z - k.most) * kLog2e);
-                    v = row == at ? k.at_given : v;
-                    acc[i][j][e] = m < g.M && off[row] != -INFINITY ? v : 0.0f;
-                    if (e == 15) __builtin_amdgcn_sched_barrier(0);
-                }
+            const int64_t given = k.given - g.first;
+            at[j] = k.given >= 0 && given >= n0 && given < n0 + T::BM ? int(given - n0) - place.first() : -1;
+            most[j] = k.most;
+            a[j] = k.a;
+            at_given[j] = k.at_given;
         }
+        __syncthreads();
+        const Offset* mine = off + place.first();
         auto* out = static_cast<typename S::Bits*>(g.g);
 #pragma unroll
-        for (int i = 0; i < T::FM; ++i)
-            Rows4<T>::run(acc[i], i, rows, [&](int row, int col, float4 v) {
-                float sum = (v.x + v.y) + (v.z + v.w);
+        for (int i = 0; i < T::FM; ++i) {
+            v16f row[T::FN];
 #pragma unroll
-                for (int d = Rows4<T>::kLanes / 2; d; d >>= 1) sum += __shfl_xor(sum, d);
+            for (int e = 0; e < 16; ++e) {
+                const Offset o = mine[place.at(i, e)];
+#pragma unroll
+                for (int j = 0; j < T::FN; ++j) {
+                    const float z = score(acc[i][j][e], o, g.off.c);
+                    const float v = a[j] * __builtin_amdgcn_exp2f(z - most[j]);
+                    row[j][e] = z == -INFINITY ? 0.0f : v;  // (a may be NaN)
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j) {
+                const int here = at[j] - i * 32;
+                if (__builtin_amdgcn_ballot_w64(here >= 0 && here < 32) != 0)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const bool is = here == place.at(0, e) && mine[place.at(i, e)].limit != -INFINITY;
+                        row[j][e] = is ? at_given[j] : row[j][e];
+                    }
+                if (m0 + place.col(j) >= g.M)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) row[j][e] = 0.0f;
+            }
+            Rows4<T>::run(row, i, rows, [&](int row, int col, float4 v) {
+                const float sum = lanes_sum<Rows4<T>::kLanes>((v.x + v.y) + (v.z + v.w));
                 if ((tid & (Rows4<T>::kLanes - 1)) == 0) sums[place.wn * T::BM + row] = sum;
                 const int64_t n = n0 + row, m = m0 + col;
                 if (n >= g.off.N || m >= g.ldg) return;  // (ldg is a multiple of 8)
                 const typename S::Bits b[4] = {S::round(v.x), S::round(v.y), S::round(v.z), S::round(v.w)};
                 __builtin_memcpy(__builtin_assume_aligned(out + n * g.ldg + m, sizeof b), b, sizeof b);
             });
+        }
         if (!g.sums) return;
         __syncthreads();
         for (int i = tid; i < T::BM; i += T::NT) {
@@ -183,7 +245,7 @@ struct MatrixEpi {
 template <class S> struct Shapes {
     using Small = TileShape<64, 64, 2, 2>;
     using Middle = TileShape<128, 128, 2, 4>;
-    using Large = TileShape<256, 256, 2, 4>;
+    using Large = TileShape<256, 256, 2, 4>;  // (straight to LDS only: there are no registers for what is on its way)
 };
 template <> struct Shapes<F32> {  // (three planes of 256 x 128 are 144 KB in two stages)
     using Small = TileShape<64, 64, 2, 2>;
@@ -191,46 +253,64 @@ template <> struct Shapes<F32> {  // (three planes of 256 x 128 are 144 KB in tw
     using Large = TileShape<256, 128, 4, 2>;
 };
 
-template <class S, class T, bool ATR, bool BTR, class Epi>
+// Whether an operand's chunks of eight 16-bit values can go straight to LDS.
+template <bool ACROSS> bool direct(const Operand& o) {
+    return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % 8 == 0 && (ACROSS || o.kdim % 8 == 0);
+}
+
+template <class S, class T, bool ATR, bool BTR, bool DIRECT, class Epi>
 hipError_t product_of(Product g, const typename Epi::Args& ea, hipStream_t s) {
     g.tm = uint32_t((g.rows + T::BM - 1) / T::BM);
     g.tn = uint32_t((g.cols + T::BN - 1) / T::BN);
-    k_tile<S, T, ATR, BTR, Epi><<<dim3(g.tm * g.tn * g.splits), T::NT, 0, s>>>(g, ea);
+    const uint32_t tiles = g.tm * g.tn, rest = tiles > g.whole ? tiles - g.whole : 0;
+    g.whole = tiles - rest;
+    k_tile<S, T, ATR, BTR, DIRECT, Epi><<<dim3(g.whole + rest * g.splits), T::NT, 0, s>>>(g, ea);
     if (hipError_t e = hipGetLastError()) return e;
-    if (g.splits > 1) k_tile_join<S, T, Epi><<<dim3(g.tm * g.tn), T::NT, 0, s>>>(g, ea);
+    if (rest && g.splits > 1) k_tile_join<S, T, Epi><<<dim3(rest), T::NT, 0, s>>>(g, ea);
     return hipGetLastError();
 }
 template <class S, bool ATR, bool BTR, class Epi>
-hipError_t product(const Product& g, int tile, const typename Epi::Args& ea, hipStream_t s) {
-    switch (tile) {
-        case 0: return product_of<S, typename Shapes<S>::Small, ATR, BTR, Epi>(g, ea, s);
-        case 1: return product_of<S, typename Shapes<S>::Middle, ATR, BTR, Epi>(g, ea, s);
-        default: return product_of<S, typename Shapes<S>::Large, ATR, BTR, Epi>(g, ea, s);
+hipError_t product(const Product& g, const PairTile& t, const typename Epi::Args& ea, hipStream_t s) {
+    using Small = typename Shapes<S>::Small;
+    using Middle = typename Shapes<S>::Middle;
+    using Large = typename Shapes<S>::Large;
+    if constexpr (Units<S>::planes == 1) {
+        if (t.direct && direct<ATR>(g.a) && direct<BTR>(g.b)) {
+            if (t.tile == 0) return product_of<S, Small, ATR, BTR, true, Epi>(g, ea, s);
+            if (t.tile == 1) return product_of<S, Middle, ATR, BTR, true, Epi>(g, ea, s);
+            return product_of<S, Large, ATR, BTR, true, Epi>(g, ea, s);
+        }
+    } else if (t.tile == 2) {
+        return product_of<S, Large, ATR, BTR, false, Epi>(g, ea, s);
     }
+    if (t.tile == 0) return product_of<S, Small, ATR, BTR, false, Epi>(g, ea, s);
+    if (t.tile == 1) return product_of<S, Middle, ATR, BTR, false, Epi>(g, ea, s);
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
 
 template <class S> hipError_t PairProducts<S>::stats(const PairArgs& a, const PairTile& t, const StatsOut& o, float* part, hipStream_t s) {
-    const Product g{{a.r, a.ldr, nullptr}, {a.x, a.ldx, nullptr}, a.N, a.M, a.K, t.splits, part, 0, 0};
-    return product<S, false, false, StatsEpi>(g, t.tile, o, s);
+    const Product g{{a.r, a.ldr, a.K, nullptr}, {a.x, a.ldx, a.K, nullptr}, a.N, a.M, a.K, 0, 0, t.whole, t.splits, part};
+    return product<S, false, false, StatsEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::grad(const PairArgs& a, const void* r, int64_t n, const PairTile& t, const GradOut& o, float* part, hipStream_t s) {
-    const Product g{{r, a.ldr, nullptr}, {a.x, a.ldx, nullptr}, n, a.M, a.K, t.splits, part, 0, 0};
-    return product<S, false, false, GradEpi>(g, t.tile, o, s);
+    const Product g{{r, a.ldr, a.K, nullptr}, {a.x, a.ldx, a.K, nullptr}, n, a.M, a.K, 0, 0, t.whole, t.splits, part};
+    return product<S, false, false, GradEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::d_references(const PairArgs& a, const void* gr, int64_t ldg, int64_t n, const PairTile& t,
                                          const MatrixOut& o, float* part, hipStream_t s) {
-    const Product g{{gr, ldg, nullptr}, {a.x, a.ldx, nullptr}, n, a.K, a.M, t.splits, part, 0, 0};
-    return product<S, false, true, MatrixEpi>(g, t.tile, o, s);
+    // (g holds zeros from M to ldg: whole chunks)
+    const Product g{{gr, ldg, ldg, nullptr}, {a.x, a.ldx, a.M, nullptr}, n, a.K, a.M, 0, 0, t.whole, t.splits, part};
+    return product<S, false, true, MatrixEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::d_images(const PairArgs& a, const void* gr, int64_t ldg, const void* r, const uint8_t* mask,
                                      int64_t n, const PairTile& t, const MatrixOut& o, float* part, hipStream_t s) {
-    const Product g{{gr, ldg, nullptr}, {r, a.ldr, mask}, a.M, a.K, n, t.splits, part, 0, 0};
-    return product<S, true, true, MatrixEpi>(g, t.tile, o, s);
+    const Product g{{gr, ldg, n, nullptr}, {r, a.ldr, n, mask}, a.M, a.K, n, 0, 0, t.whole, t.splits, part};
+    return product<S, true, true, MatrixEpi>(g, t, o, s);
 }
 
 }  // namespace tp

@@ -12,6 +12,7 @@
 #pragma once
 
 #include "tp_match.hh"
+#include "tp_stage.hh"
 
 namespace tp {
 
@@ -87,6 +88,7 @@ template <class S> struct Eight {
 struct Operand {
     const void* p;
     int64_t ld;           // elements between its rows in memory, at most kMaxStride
+    int64_t kdim;         // contraction that there is (zeros count as being there)
     const uint8_t* keep;  // (contraction across only) zero: the row counts as zeros, whatever it holds; null: all do not
 };
 
@@ -94,7 +96,9 @@ struct Operand {
 //   adjacent: LDS row i holds its bk values; chunk c of row i at place c ^ (i / rows in 256 bytes), so that 16 lanes
 //             reading one chunk of 16 rows reach each of the 64 banks once
 //   across:   LDS row k holds DIM values; four rows of 64 bytes, as 32 lanes read them, at places that differ by 64
-template <class S, bool ACROSS, int DIM, int NT> struct Side {
+// DIRECT: from memory straight to LDS, without registers between (16-bit values whose rows start at 16-byte
+// boundaries; an adjacent contraction is a whole number of chunks).
+template <class S, bool ACROSS, int DIM, int NT, bool DIRECT> struct Side {
     static constexpr int BK = Units<S>::bk, PL = Units<S>::planes;
     static constexpr int CPR = ACROSS ? DIM / 8 : BK / 8, CH = DIM * BK / 8 / NT;
     static constexpr int kPlane = DIM * BK * 2;  // bytes
@@ -106,8 +110,6 @@ template <class S, bool ACROSS, int DIM, int NT> struct Side {
     const uint8_t* keep;
     uint32_t off[CH];  // bytes from base (+ the step) of each chunk
     int tid;
-    Eight<S> reg[CH];
-    uint32_t kept[CH];  // (across, with keep) nonzero where the chunk's row counts
 
     static __device__ __forceinline__ int row_of(int slot) { return slot / CPR; }
     static __device__ __forceinline__ int chunk_of(int slot) { return slot % CPR; }
@@ -116,51 +118,87 @@ template <class S, bool ACROSS, int DIM, int NT> struct Side {
         return (row / (128 / BK)) & (CPR - 1);
     }
 
-    // first: of the tile along D's side; dim_all, kdim_all: what there is of both
-    __device__ __forceinline__ void init(const Operand& o, int64_t first, int64_t dim_all, int64_t kdim_all, int t) {
+    // first: of the tile along D's side; dim_all: what there is of that
+    __device__ __forceinline__ void init(const Operand& o, int64_t first, int64_t dim_all, int t) {
         tid = t;
         ld = o.ld;
         keep = o.keep;
         dim = min(dim_all - first, int64_t(DIM));
-        kdim = kdim_all;
+        kdim = o.kdim;
         base = static_cast<const char*>(o.p) + (ACROSS ? first : first * ld) * int64_t(sizeof(Bits));
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
+            if (DIRECT) {  // (a place in LDS, and the chunk that belongs there)
+                const int from = (c ^ swizzle(row)) * 8;
+                off[i] = (uint32_t(row) * uint32_t(ld) + from) * uint32_t(sizeof(Bits));
+                continue;
+            }
             // rows and chunks past the end read the last one: what comes of them is not stored
             const uint32_t at = ACROSS ? uint32_t(row) * uint32_t(ld) + min(c * 8, (int(dim) - 1) & ~7)
                                        : uint32_t(min(row, int(dim) - 1)) * uint32_t(ld) + c * 8;
             off[i] = at * uint32_t(sizeof(Bits));
         }
     }
-    // Whole chunks only: every row of the step is there, and the last chunk's read ends inside the operand.
-    __device__ __forceinline__ bool whole(int64_t k0) const {
-        if (k0 + BK > kdim) return false;
-        return !ACROSS || (k0 + BK - 1) * ld + ((dim + 7) & ~int64_t(7)) <= (kdim - 1) * ld + dim;
-    }
-    __device__ __forceinline__ void load(int64_t k0) {
-        const char* at = base + (ACROSS ? k0 * ld : k0) * int64_t(sizeof(Bits));
-        if (whole(k0)) {
-#pragma unroll
-            for (int i = 0; i < CH; ++i) reg[i].read(reinterpret_cast<const Bits*>(at + off[i]));
-        } else {
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
-                reg[i].zero();
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bool there = ACROSS ? k0 + row < kdim && c * 8 + j < dim : k0 + c * 8 + j < kdim;
-                    if (there) reg[i].set(j, reinterpret_cast<const Bits*>(at + off[i])[j]);
-                }
-            }
-        }
+    // which rows of the step at k0 count (across, with keep: nonzero where the chunk's does)
+    __device__ __forceinline__ void look(int64_t k0, uint32_t (&kept)[CH]) const {
         if (ACROSS && keep) {
 #pragma unroll
             for (int i = 0; i < CH; ++i) kept[i] = keep[min(k0 + row_of(i * NT + tid), kdim - 1)];
         }
     }
-    __device__ __forceinline__ void store(char* lds) const {
+    // The step at k0 straight to LDS; what lies outside the operand arrives as zeros, and so do rows that do not count (look
+    // has been called for this step, and is for the next).
+    __device__ __forceinline__ void fill(int64_t k0, char* lds, uint32_t (&kept)[CH]) const {
+        constexpr uint32_t kNowhere = 0x80000000u;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const char* at = base + (ACROSS ? k0 * ld * int64_t(sizeof(Bits)) : 0);
+        const int64_t values = ACROSS ? (kdim - k0 - 1) * ld + dim : (dim - 1) * ld + kdim;
+        const auto src = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(at), 0, int(min(values * int64_t(sizeof(Bits)), int64_t(0x7fffffff))), 0x00027000);
+        const int step = ACROSS ? 0 : int(k0 * int64_t(sizeof(Bits)));
+        const bool tail = !ACROSS && k0 + BK > kdim;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            uint32_t o = off[i];
+            if (tail) {
+                const int slot = i * NT + tid;
+                if (k0 + (chunk_of(slot) ^ swizzle(row_of(slot))) * 8 >= kdim) o = kNowhere;
+            }
+            if (ACROSS && keep && !kept[i]) o = kNowhere;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (LocalPtr)(lds + (i * NT + wave * 64) * 16), 16, int(o), step, 0, 0);
+        }
+        look(k0 + BK, kept);
+    }
+    // The contraction up to here can be read in whole chunks: every row of a step is there, and the last chunk's read
+    // ends inside the operand.
+    __device__ __forceinline__ int64_t whole() const {
+        const int64_t past = ACROSS ? -dim & 7 : 0;  // values that a row's last chunk reads of the next rows
+        return max(kdim - (past ? (past + ld - 1) / max(ld, int64_t(1)) : 0), int64_t(0)) / BK * BK;
+    }
+    using Regs = Eight<S>[CH];
+    __device__ __forceinline__ void load(int64_t k0, Regs& reg, uint32_t (&kept)[CH]) const {
+        const char* at = base + (ACROSS ? k0 * ld : k0) * int64_t(sizeof(Bits));
+#pragma unroll
+        for (int i = 0; i < CH; ++i) reg[i].read(reinterpret_cast<const Bits*>(at + off[i]));
+        look(k0, kept);
+    }
+    // The same for a step that is not whole.
+    __device__ __forceinline__ void load_some(int64_t k0, Regs& reg, uint32_t (&kept)[CH]) const {
+        const char* at = base + (ACROSS ? k0 * ld : k0) * int64_t(sizeof(Bits));
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
+            reg[i].zero();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool there = ACROSS ? k0 + row < kdim && c * 8 + j < dim : k0 + c * 8 + j < kdim;
+                if (there) reg[i].set(j, reinterpret_cast<const Bits*>(at + off[i])[j]);
+            }
+        }
+        look(k0, kept);
+    }
+    __device__ __forceinline__ void store(char* lds, const Regs& reg, const uint32_t (&kept)[CH]) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
@@ -194,14 +232,14 @@ template <class S, bool ACROSS, int DIM, int NT> struct Side {
     }
 };
 
-// What the products' kernels share: [splits] ranges of the contraction are one workgroup each, and where there are
-// several their fragments go to part, which k_tile_join adds up.
+// What the products' kernels share: the first `whole` tiles are one workgroup each; of the others [splits] ranges of
+// the contraction are one each, and where there are several their fragments go to part, which k_tile_join adds up.
 struct Product {
     Operand a, b;
     int64_t rows, cols, kdim;
+    uint32_t tm, tn, whole;
     int splits;
     float* part;
-    uint32_t tm, tn;
 };
 
 template <class T> using Acc = v16f[T::FM][T::FN];
@@ -216,7 +254,9 @@ template <class T> struct Place {
         r = tid & 31;
         q = (tid >> 5) & 1;
     }
-    __device__ __forceinline__ int row(int i, int e) const { return (wm * T::FM + i) * 32 + (e >> 2) * 8 + q * 4 + (e & 3); }
+    // the row of the tile is first() + at(i, e), the latter known to the compiler
+    __device__ __forceinline__ int first() const { return wm * T::FM * 32 + q * 4; }
+    static __device__ constexpr int at(int i, int e) { return i * 32 + (e >> 2) * 8 + (e & 3); }
     __device__ __forceinline__ int col(int j) const { return (wn * T::FN + j) * 32 + r; }
 };
 
@@ -235,61 +275,84 @@ __device__ __forceinline__ uint32_t xcd_item(uint32_t block, uint32_t items) {
 template <class S, class T> constexpr int tile_lds() { return 2 * Units<S>::planes * (T::BM + T::BN) * Units<S>::bk * 2; }
 
 // Epi: static void run(const Args&, Acc<T>&, im, in, char* lds) of the tile (im, in).
-template <class S, class T, bool ATR, bool BTR, class Epi>
+template <class S, class T, bool ATR, bool BTR, bool DIRECT, class Epi>
 __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea) {
     constexpr int BK = Units<S>::bk, PL = Units<S>::planes;
-    using SA = Side<S, ATR, T::BM, T::NT>;
-    using SB = Side<S, BTR, T::BN, T::NT>;
+    using SA = Side<S, ATR, T::BM, T::NT, DIRECT>;
+    using SB = Side<S, BTR, T::BN, T::NT, DIRECT>;
     constexpr int kA = PL * SA::kPlane, kStage = kA + PL * SB::kPlane;
     __shared__ __attribute__((aligned(16))) char lds[tile_lds<S, T>()];
     const int tid = threadIdx.x, lane = tid & 63;
     const Place<T> place(tid);
-    uint32_t item = xcd_item(blockIdx.x, gridDim.x), im, in;
-    const uint32_t split = item / (g.tm * g.tn);
-    item -= split * g.tm * g.tn;
+    const uint32_t rest = g.tm * g.tn - g.whole;
+    uint32_t item, split = 0, im, in;
+    int splits = 1;
+    if (blockIdx.x < g.whole) {
+        item = xcd_item(blockIdx.x, g.whole);
+    } else {
+        item = xcd_item(blockIdx.x - g.whole, rest * g.splits);
+        split = item / rest;
+        item += g.whole - split * rest;
+        splits = g.splits;
+    }
     tile_at(item, g.tm, g.tn, im, in);
     SA a;
     SB b;
-    a.init(g.a, int64_t(im) * T::BM, g.rows, g.kdim, tid);
-    b.init(g.b, int64_t(in) * T::BN, g.cols, g.kdim, tid);
+    a.init(g.a, int64_t(im) * T::BM, g.rows, tid);
+    b.init(g.b, int64_t(in) * T::BN, g.cols, tid);
     const int64_t steps = (g.kdim + BK - 1) / BK;
-    const int64_t k0 = steps * split / g.splits * BK, k1 = steps * (split + 1) / g.splits * BK;
+    const int64_t k0 = steps * split / splits * BK, k1 = steps * (split + 1) / splits * BK;
 
     Acc<T> acc;
+    auto clear = [](Acc<T>& v) {
 #pragma unroll
-    for (int i = 0; i < T::FM; ++i)
+        for (int i = 0; i < T::FM; ++i)
 #pragma unroll
-        for (int j = 0; j < T::FN; ++j)
+            for (int j = 0; j < T::FN; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+                for (int e = 0; e < 16; ++e) v[i][j][e] = 0.0f;
+    };
+    clear(acc);
+    // A sum over thousands of products in one go loses what its own size is to each of them: every kFlush of the contraction it is
+    // added to another set of registers and begun anew (where there are registers: not in 16-bit tiles of 256 x 256, nor where
+    // both operands come across, whose sums are gradients of images).  Of 2048
+    // x 8192 float32 pairs of 16640 values log_sum is 4.8e-6 off without and 3.4e-7 with it.
+    constexpr bool kTwo = T::FM * T::FN <= 4 && !(ATR && BTR);
+    constexpr int kFlush = 512;
+    Acc<T> total;
+    if constexpr (kTwo) clear(total);
+    auto flush = [&] {
+#pragma unroll
+        for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) total[i][j][e] += acc[i][j][e];
+        clear(acc);
+    };
 
-    if (k0 < k1) {
-        a.load(k0);
-        b.load(k0);
-        a.store(lds);
-        b.store(lds + kA);
-    }
-    int cur = 0;
-#pragma unroll 1
-    for (int64_t k = k0; k < k1; k += BK) {
-        __syncthreads();
-        const bool more = k + BK < k1;
-        if (more) {
-            a.load(k + BK);
-            b.load(k + BK);
-        }
-        const char* sa = lds + cur * kStage;
-        const char* sb = sa + kA;
-#pragma unroll
-        for (int t = 0; t < BK / 16; ++t) {
-            int4 fa[PL][T::FM], fb[PL][T::FN];
+    // one step's products from a stage: the operands of a sixteenth are read while those of the one before are multiplied
+    // (in planes that has no registers, and needs none: six products for each operand)
+    constexpr int D = PL == 1 ? 2 : 1;
+    auto multiply = [&](const char* stage, auto between) {
+        const char *sa = stage, *sb = stage + kA;
+        int4 fa[D][PL][T::FM], fb[D][PL][T::FN];
+        auto read = [&](int t) {
 #pragma unroll
             for (int p = 0; p < PL; ++p) {
 #pragma unroll
-                for (int i = 0; i < T::FM; ++i) fa[p][i] = SA::fragment(sa + p * SA::kPlane, (place.wm * T::FM + i) * 32, t, lane);
+                for (int i = 0; i < T::FM; ++i)
+                    fa[t % D][p][i] = SA::fragment(sa + p * SA::kPlane, (place.wm * T::FM + i) * 32, t, lane);
 #pragma unroll
-                for (int j = 0; j < T::FN; ++j) fb[p][j] = SB::fragment(sb + p * SB::kPlane, (place.wn * T::FN + j) * 32, t, lane);
+                for (int j = 0; j < T::FN; ++j)
+                    fb[t % D][p][j] = SB::fragment(sb + p * SB::kPlane, (place.wn * T::FN + j) * 32, t, lane);
             }
+        };
+        if (D == 2) read(0);
+        between();
+#pragma unroll
+        for (int t = 0; t < BK / 16; ++t) {
+            if (t + D - 1 < BK / 16) read(t + D - 1);
             // the small products of pieces first
 #pragma unroll
             for (int s = PL - 1; s >= 0; --s)
@@ -298,16 +361,85 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
 #pragma unroll
                     for (int i = 0; i < T::FM; ++i)
 #pragma unroll
-                        for (int j = 0; j < T::FN; ++j) acc[i][j] = Units<S>::mfma(fa[p][i], fb[s - p][j], acc[i][j]);
+                        for (int j = 0; j < T::FN; ++j)
+                            acc[i][j] = Units<S>::mfma(fa[t % D][p][i], fb[t % D][s - p][j], acc[i][j]);
+            if (DIRECT) __builtin_amdgcn_sched_barrier(0);
         }
-        cur ^= 1;
-        if (more) {
-            a.store(lds + cur * kStage);
-            b.store(lds + cur * kStage + kA);
+    };
+    if constexpr (DIRECT) {
+        uint32_t ka[SA::CH], kb[SB::CH];
+        if (k0 < k1) {
+            a.look(k0, ka);
+            b.look(k0, kb);
+            a.fill(k0, lds, ka);
+            b.fill(k0, lds + kA, kb);
+        }
+        int cur = 0;
+#pragma unroll 1
+        for (int64_t k = k0; k < k1; k += BK) {
+            if (kTwo && k % kFlush == 0) flush();
+            stage_ready();
+            char* next = lds + (cur ^ 1) * kStage;
+            multiply(lds + cur * kStage, [&] {
+                if (k + BK < k1) {
+                    a.fill(k + BK, next, ka);
+                    b.fill(k + BK, next + kA, kb);
+                }
+            });
+            cur ^= 1;
+        }
+    } else {
+        // two steps are on their way to registers while a third is multiplied
+        typename SA::Regs ra[2];
+        typename SB::Regs rb[2];
+        uint32_t ka[2][SA::CH], kb[2][SB::CH];
+        auto load = [&](int64_t k, int r) {
+            a.load(k, ra[r], ka[r]);
+            b.load(k, rb[r], kb[r]);
+        };
+        auto store = [&](int r) {
+            a.store(lds + r * kStage, ra[r], ka[r]);
+            b.store(lds + r * kStage + kA, rb[r], kb[r]);
+        };
+        const int64_t kw = max(k0, min(k1, min(a.whole(), b.whole()))), last = kw - BK;
+        if (k0 < kw) {
+            load(k0, 0);
+            load(min(k0 + BK, last), 1);
+            store(0);
+        }
+#pragma unroll 1
+        for (int64_t k = k0; k < kw; k += 2 * BK) {
+            if (kTwo && k % kFlush < 2 * BK) flush();
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int64_t at = k + r * BK;
+                if (at >= kw) break;
+                __syncthreads();
+                load(min(at + 2 * BK, last), r);  // (past the end: the last one again, not used)
+                multiply(lds + r * kStage, [] {});
+                if (at + BK < kw) store(r ^ 1);
+            }
+        }
+        // what is left of the contraction
+#pragma unroll 1
+        for (int64_t k = kw; k < k1; k += BK) {
+            a.load_some(k, ra[0], ka[0]);
+            b.load_some(k, rb[0], kb[0]);
+            __syncthreads();
+            store(0);
+            __syncthreads();
+            multiply(lds, [] {});
         }
     }
-    if (g.splits > 1) {
-        float* out = g.part + ((int64_t(split) * g.tm + im) * g.tn + in) * (T::BM * T::BN) + tid * 4;
+    if constexpr (kTwo) {
+        flush();
+#pragma unroll
+        for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j) acc[i][j] = total[i][j];
+    }
+    if (splits > 1) {
+        float* out = g.part + (int64_t(split) * rest + item - g.whole) * (T::BM * T::BN) + tid * 4;
 #pragma unroll
         for (int i = 0; i < T::FM; ++i)
 #pragma unroll
@@ -326,8 +458,9 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
 template <class S, class T, class Epi>
 __global__ __launch_bounds__(T::NT) void k_tile_join(Product g, typename Epi::Args ea) {
     __shared__ __attribute__((aligned(16))) char lds[tile_lds<S, T>()];
+    const uint32_t item = xcd_item(blockIdx.x, gridDim.x);
     uint32_t im, in;
-    tile_at(xcd_item(blockIdx.x, gridDim.x), g.tm, g.tn, im, in);
+    tile_at(g.whole + item, g.tm, g.tn, im, in);
     Acc<T> acc;
 #pragma unroll
     for (int i = 0; i < T::FM; ++i)
@@ -336,7 +469,7 @@ __global__ __launch_bounds__(T::NT) void k_tile_join(Product g, typename Epi::Ar
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     for (int s = 0; s < g.splits; ++s) {
-        const float* p = g.part + ((int64_t(s) * g.tm + im) * g.tn + in) * (T::BM * T::BN) + threadIdx.x * 4;
+        const float* p = g.part + (int64_t(s) * gridDim.x + item) * (T::BM * T::BN) + threadIdx.x * 4;
 #pragma unroll
         for (int i = 0; i < T::FM; ++i)
 #pragma unroll
@@ -373,6 +506,7 @@ template <class T> struct Rows4 {
             const float4 v = *reinterpret_cast<const float4*>(mine + at * kStride + c);
             use((place.wm * T::FM + i) * 32 + at, place.wn * T::FN * 32 + c, v);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (rows of fragments one after the other: registers)
     }
 };
 
