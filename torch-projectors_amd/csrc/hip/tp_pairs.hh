@@ -85,6 +85,7 @@ struct GradOut {
     void* g;
     int64_t ldg;
     float* sums;
+    int* look;  // set to 1 where a reference that the mask rules out made a product that is not finite
 };
 // rows x cols times *scale: float32 sums [rows][cols] are added where `before`, and kept where `after`, else out
 struct MatrixOut {
@@ -103,7 +104,7 @@ template <class S> struct PairProducts {
     static hipError_t d_references(const PairArgs& a, const void* g, int64_t ldg, int64_t n, const PairTile& t,
                                    const MatrixOut& o, float* part, hipStream_t s);
     static hipError_t d_images(const PairArgs& a, const void* g, int64_t ldg, const void* r, const uint8_t* mask,
-                               int64_t n, const PairTile& t, const MatrixOut& o, float* part, hipStream_t s);
+                               const int* look, int64_t n, const PairTile& t, const MatrixOut& o, float* part, hipStream_t s);
 };
 
 }  // namespace tp

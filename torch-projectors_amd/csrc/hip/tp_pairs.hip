@@ -16,6 +16,8 @@
 #include "../../../include/torch_projectors_hip.h"
 #include "tp_pairs.hh"
 
+#include <algorithm>
+
 namespace tp {
 namespace {
 
@@ -99,7 +101,7 @@ __device__ __forceinline__ PairCoef coefficients(const PairArgs& a, const float*
 // numbers start at 2^-14: what is 2^-28 of the largest, or more, keeps all bits), and back by scale[0].
 constexpr float kHalfMost = 16384.0f;
 __global__ __launch_bounds__(1024) void k_pairs_coef(PairArgs a, const float* __restrict__ state, const float* d_given,
-                                                     const float* d_log_sum, bool half, PairCoef* coef, float* scale) {
+                                                     const float* d_log_sum, bool half, PairCoef* coef, float* scale, int* look) {
     __shared__ float room[16];
     float up = 1.0f;
     if (half) {
@@ -119,7 +121,10 @@ __global__ __launch_bounds__(1024) void k_pairs_coef(PairArgs a, const float* __
         frexpf(most, &e);  // most < 2^e
         up = most > 0.0f ? ldexpf(1.0f, max(min(14 - e, 100), -100)) : 1.0f;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) scale[0] = 1.0f / up;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        scale[0] = 1.0f / up;
+        *look = 0;
+    }
     for (int64_t m = int64_t(blockIdx.x) * 1024 + threadIdx.x; m < a.M; m += int64_t(gridDim.x) * 1024) {
         PairCoef k = coefficients(a, state, m, d_given, d_log_sum);
         k.a *= up;
@@ -417,13 +422,15 @@ int64_t few_per(int64_t N, int64_t K) {
     return per < 16 ? 16 : per;
 }
 
+// One step (bk of the contraction) of a tile, and its start and end: among as many as a CU holds, and alone.  Measured on products of
+// 1024 to 16384 along the contraction with every CU at work.
 struct TileKind {
-    int bm, bn, bk, per_cu;  // per_cu: workgroups that a CU holds at once
-    double step_us, alone_us;
+    int bm, bn, bk;
+    double step_us, over_us, alone_us, alone_over_us;
 };
-constexpr TileKind kTiles16[] = {{64, 64, 64, 5, 0.20, 0.62}, {128, 128, 64, 2, 0.55, 1.00}, {256, 256, 64, 1, 1.75, 1.75}};
-constexpr TileKind kTilesStaged[] = {{64, 64, 64, 4, 0.22, 0.75}, {128, 128, 64, 2, 0.60, 0.95}};
-constexpr TileKind kTiles32[] = {{64, 64, 32, 3, 0.40, 0.62}, {128, 128, 32, 1, 1.40, 1.20}, {256, 128, 32, 1, 2.45, 2.10}};
+constexpr TileKind kTiles16[] = {{64, 64, 64, 0.174, 2.2, 0.50, 5}, {128, 128, 64, 0.395, 5, 0.75, 6}, {256, 256, 64, 1.62, 10, 1.62, 10}};
+constexpr TileKind kTilesStaged[] = {{64, 64, 64, 0.24, 1.4, 0.75, 5}, {128, 128, 64, 0.48, 5, 0.85, 6}};
+constexpr TileKind kTiles32[] = {{64, 64, 32, 0.44, 0.5, 0.62, 4}, {128, 128, 32, 1.42, 3, 1.42, 4}, {256, 128, 32, 2.40, 11, 2.40, 11}};
 const TileKind& kind_of(int dt, const PairTile& t) {
     return dt == TP_F32 ? kTiles32[t.tile] : t.direct ? kTiles16[t.tile] : kTilesStaged[t.tile];
 }
@@ -501,9 +508,10 @@ __global__ __launch_bounds__(256) void k_pairs_none(PairArgs a, float* given_out
 
 }  // namespace
 
-// The tile, and the tiles and ranges that are split, with the least time by a count of steps (one bk of the contraction for one
-// tile).  The CUs hold per_cu tiles each; tiles that fill them all run whole, round after round; those that are left over are
-// split so that they do, too.
+// The tile, and the tiles and ranges that are split, with the least time by a count of steps.  Every CU computes as many whole
+// tiles; those that are left over are split along the contraction so that they give every CU something to do, too, which
+// costs their sums written and read (by one workgroup a tile, at some 70 GB/s).  Against all tiles and 1 to 16 ranges
+// on 88 products from 20 x 5000 to 4096 x 12288 the choice is 3 % from the best on average, at most 28 %.
 PairTile pair_plan(int dt, bool direct, int64_t rows, int64_t cols, int64_t kdim) {
     PairTile best{direct, 0, 0, 1};
     double least = 1e300;
@@ -511,25 +519,21 @@ PairTile pair_plan(int dt, bool direct, int64_t rows, int64_t cols, int64_t kdim
         const TileKind& k = kind_of(dt, PairTile{direct, t, 0, 1});
         const int64_t tiles = ((rows + k.bm - 1) / k.bm) * ((cols + k.bn - 1) / k.bn);
         if (tiles > kMaxTiles) continue;
-        const int64_t steps = (kdim + k.bk - 1) / k.bk, slots = int64_t(kCus) * k.per_cu;
-        const int64_t rounds = tiles / slots, rest = tiles - rounds * slots;
-        // a step of as many workgroups as there are on a CU
-        auto step = [&](int64_t groups) {
-            const double each = double((groups + kCus - 1) / kCus) * k.step_us;
-            return each > k.alone_us ? each : k.alone_us;
-        };
-        const double whole_us = 3.0 + rounds * (steps + 4) * step(slots);
-        for (int s = 1; s <= kMaxSplits && s <= steps; ++s) {
-            const int64_t groups = rest * s, full = groups / slots, over = groups - full * slots;
-            if (s > 1 && groups > 4 * slots) break;
-            const double each = double((steps + s - 1) / s + 4);
-            double us = whole_us + each * (full * step(slots) + (over ? step(over) : 0.0));
-            if (s > 1 && rest) us += 4.0 + double(rest) * k.bm * k.bn * (8.0 * s) / 4.0e6;
+        const int64_t steps = (kdim + k.bk - 1) / k.bk;
+        auto weigh = [&](int64_t each, int s) {  // `each` whole tiles on a CU, the others in s ranges
+            const int64_t rest = tiles - each * kCus, groups = (rest * s + kCus - 1) / kCus, part = (steps + s - 1) / s;
+            double us = each * (steps * k.step_us + k.over_us) + groups * (part * k.step_us + k.over_us);
+            us = std::max(us, (each ? steps : part) * k.alone_us + k.alone_over_us);
+            if (s > 1) us += 6.0 + 0.1 * s + (s + 1) * (k.bm * k.bn * 6e-5) * double((rest + kCus - 1) / kCus);
             if (us < least) {
                 least = us;
-                best = {direct, t, uint32_t(rounds * slots), s};
+                best = {direct, t, uint32_t(each * kCus), s};
             }
-            if (!rest) break;
+        };
+        weigh(tiles / kCus, 1);
+        for (int s = 2; s <= kMaxSplits && s <= steps; ++s) {
+            if (tiles % kCus) weigh(tiles / kCus, s);
+            if (tiles >= kCus && tiles * s <= 8 * kCus) weigh(0, s);
         }
     }
     return best;
@@ -630,18 +634,19 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
     char* w = static_cast<char*>(work);
     auto* coef = reinterpret_cast<PairCoef*>(w + b.coef);
     auto* scale = reinterpret_cast<float*>(w + b.scale);
+    auto* look = reinterpret_cast<int*>(scale + 1);
     auto* sums = reinterpret_cast<float*>(w + b.sums);
     auto* part = reinterpret_cast<float*>(w + b.part);
     auto* dx = reinterpret_cast<float*>(w + b.dx);
     const bool half = a.dt == TP_F16;
     const int64_t blocks = (a.M + 1023) / 1024;
-    k_pairs_coef<<<dim3(unsigned(blocks < 64 ? blocks : 64)), 1024, 0, s>>>(a, state, d_given, d_log_sum, half, coef, scale);
+    k_pairs_coef<<<dim3(unsigned(blocks < 64 ? blocks : 64)), 1024, 0, s>>>(a, state, d_given, d_log_sum, half, coef, scale, look);
     if (hipError_t e = hipGetLastError()) return e;
     for (int64_t first = 0; first < a.N; first += b.piece) {
         const int64_t n = a.N - first < b.piece ? a.N - first : b.piece;
         const char* r = static_cast<const char*>(a.r) + first * a.ldr * size;
         const uint8_t* mask = a.mask ? a.mask + first : nullptr;
-        const GradOut go{{a.bias ? a.bias + first : nullptr, mask, n, a.c * kLog2e}, coef, a.M, first, w + b.g, b.ldg, d_bias ? sums : nullptr};
+        const GradOut go{{a.bias ? a.bias + first : nullptr, mask, n, a.c * kLog2e}, coef, a.M, first, w + b.g, b.ldg, d_bias ? sums : nullptr, look};
         const MatrixOut ro{scale, n, a.K, nullptr, nullptr, d_r ? static_cast<char*>(d_r) + first * a.K * size : nullptr, a.K};
         const MatrixOut xo{scale, a.M, a.K, first ? dx : nullptr, first + n < a.N ? dx : nullptr, d_x, a.K};
         const hipError_t e = by_type(a.dt, [&](auto S) {
@@ -649,7 +654,7 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
             if (hipError_t f = P::grad(a, r, n, b.grad, go, part, s)) return f;
             if (d_r)
                 if (hipError_t f = P::d_references(a, w + b.g, b.ldg, n, b.refs, ro, part, s)) return f;
-            return d_x ? P::d_images(a, w + b.g, b.ldg, r, mask, n, b.images, xo, part, s) : hipSuccess;
+            return d_x ? P::d_images(a, w + b.g, b.ldg, r, mask, look, n, b.images, xo, part, s) : hipSuccess;
         });
         if (e) return e;
         if (d_bias) {

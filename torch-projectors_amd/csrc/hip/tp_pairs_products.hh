@@ -153,6 +153,20 @@ struct GradEpi {
         }
         __syncthreads();
         const Offset* mine = off + place.first();
+        // What a reference holds that the mask rules out is not used: a product that is not finite says that it may hold what
+        // a factor of zero would not take out of the images' gradients, which then look at the mask.
+        if (g.off.mask) {
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const bool out = mine[place.at(i, e)].limit == -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < T::FN; ++j) bad |= out && !(fabsf(acc[i][j][e]) < INFINITY);
+                }
+            if (bad) *g.look = 1;
+        }
         auto* out = static_cast<typename S::Bits*>(g.g);
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
@@ -245,7 +259,7 @@ struct MatrixEpi {
 template <class S> struct Shapes {
     using Small = TileShape<64, 64, 2, 2>;
     using Middle = TileShape<128, 128, 2, 4>;
-    using Large = TileShape<256, 256, 2, 4>;  // (straight to LDS only: there are no registers for what is on its way)
+    using Large = TileShape<256, 256, 2, 4, true>;  // (straight to LDS only: there are no registers for what is on its way)
 };
 template <> struct Shapes<F32> {  // (three planes of 256 x 128 are 144 KB in two stages)
     using Small = TileShape<64, 64, 2, 2>;
@@ -291,25 +305,25 @@ hipError_t product(const Product& g, const PairTile& t, const typename Epi::Args
 }  // namespace
 
 template <class S> hipError_t PairProducts<S>::stats(const PairArgs& a, const PairTile& t, const StatsOut& o, float* part, hipStream_t s) {
-    const Product g{{a.r, a.ldr, a.K, nullptr}, {a.x, a.ldx, a.K, nullptr}, a.N, a.M, a.K, 0, 0, t.whole, t.splits, part};
+    const Product g{{a.r, a.ldr, a.K, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr}, a.N, a.M, a.K, 0, 0, t.whole, t.splits, part};
     return product<S, false, false, StatsEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::grad(const PairArgs& a, const void* r, int64_t n, const PairTile& t, const GradOut& o, float* part, hipStream_t s) {
-    const Product g{{r, a.ldr, a.K, nullptr}, {a.x, a.ldx, a.K, nullptr}, n, a.M, a.K, 0, 0, t.whole, t.splits, part};
+    const Product g{{r, a.ldr, a.K, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr}, n, a.M, a.K, 0, 0, t.whole, t.splits, part};
     return product<S, false, false, GradEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::d_references(const PairArgs& a, const void* gr, int64_t ldg, int64_t n, const PairTile& t,
                                          const MatrixOut& o, float* part, hipStream_t s) {
     // (g holds zeros from M to ldg: whole chunks)
-    const Product g{{gr, ldg, ldg, nullptr}, {a.x, a.ldx, a.M, nullptr}, n, a.K, a.M, 0, 0, t.whole, t.splits, part};
+    const Product g{{gr, ldg, ldg, nullptr, nullptr}, {a.x, a.ldx, a.M, nullptr, nullptr}, n, a.K, a.M, 0, 0, t.whole, t.splits, part};
     return product<S, false, true, MatrixEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::d_images(const PairArgs& a, const void* gr, int64_t ldg, const void* r, const uint8_t* mask,
-                                     int64_t n, const PairTile& t, const MatrixOut& o, float* part, hipStream_t s) {
-    const Product g{{gr, ldg, n, nullptr}, {r, a.ldr, n, mask}, a.M, a.K, n, 0, 0, t.whole, t.splits, part};
+                                     const int* look, int64_t n, const PairTile& t, const MatrixOut& o, float* part, hipStream_t s) {
+    const Product g{{gr, ldg, n, nullptr, nullptr}, {r, a.ldr, n, mask, look}, a.M, a.K, n, 0, 0, t.whole, t.splits, part};
     return product<S, true, true, MatrixEpi>(g, t, o, s);
 }
 

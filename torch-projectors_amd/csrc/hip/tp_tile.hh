@@ -20,6 +20,8 @@ using v8bf = __attribute__((ext_vector_type(8))) __bf16;
 using v8h = __attribute__((ext_vector_type(8))) _Float16;
 using v16f = __attribute__((ext_vector_type(16))) float;
 using v4s = __attribute__((ext_vector_type(4))) short;
+using v4u = __attribute__((ext_vector_type(4))) uint32_t;
+using LocalBytes = const __attribute__((address_space(3))) char*;
 using LocalTr = __attribute__((address_space(3))) v4s*;
 
 // How values of a storage type go through the matrix units: in `planes` pieces, `bk` of the contraction at a time
@@ -42,8 +44,10 @@ template <> struct Units<F32> {
     static __device__ __forceinline__ v16f mfma(int4 a, int4 b, v16f c) { return Units<BF16>::mfma(a, b, c); }
 };
 
-// A workgroup's tile of BM x BN of D, by WM x WN wavefronts.
-template <int BM_, int BN_, int WM_, int WN_> struct TileShape {
+// A workgroup's tile of BM x BN of D, by WM x WN wavefronts.  DEEP: operands that go straight to LDS do so in four stages of 32 of
+// the contraction, else in two of 64.
+template <int BM_, int BN_, int WM_, int WN_, bool DEEP_ = false> struct TileShape {
+    static constexpr bool DEEP = DEEP_;
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NT = 64 * WM * WN;
     static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;  // fragments of a wavefront
 };
@@ -89,7 +93,9 @@ struct Operand {
     const void* p;
     int64_t ld;           // elements between its rows in memory, at most kMaxStride
     int64_t kdim;         // contraction that there is (zeros count as being there)
-    const uint8_t* keep;  // (contraction across only) zero: the row counts as zeros, whatever it holds; null: all do not
+    // (contraction across only) where *look is not 0, rows whose byte is zero count as zeros, whatever they hold; null: none does
+    const uint8_t* keep;
+    const int* look;
 };
 
 // An operand's part of a tile: DIM rows of D's side by bk of the contraction, CH chunks of eight values a thread.
@@ -98,8 +104,8 @@ struct Operand {
 //   across:   LDS row k holds DIM values; four rows of 64 bytes, as 32 lanes read them, at places that differ by 64
 // DIRECT: from memory straight to LDS, without registers between (16-bit values whose rows start at 16-byte
 // boundaries; an adjacent contraction is a whole number of chunks).
-template <class S, bool ACROSS, int DIM, int NT, bool DIRECT> struct Side {
-    static constexpr int BK = Units<S>::bk, PL = Units<S>::planes;
+template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Side {
+    static constexpr int PL = Units<S>::planes;
     static constexpr int CPR = ACROSS ? DIM / 8 : BK / 8, CH = DIM * BK / 8 / NT;
     static constexpr int kPlane = DIM * BK * 2;  // bytes
     static_assert(CH * 8 * NT == DIM * BK, "whole chunks");
@@ -122,7 +128,7 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT> struct Side {
     __device__ __forceinline__ void init(const Operand& o, int64_t first, int64_t dim_all, int t) {
         tid = t;
         ld = o.ld;
-        keep = o.keep;
+        keep = ACROSS && o.keep && *o.look ? o.keep : nullptr;
         dim = min(dim_all - first, int64_t(DIM));
         kdim = o.kdim;
         base = static_cast<const char*>(o.p) + (ACROSS ? first : first * ld) * int64_t(sizeof(Bits));
@@ -147,28 +153,44 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT> struct Side {
             for (int i = 0; i < CH; ++i) kept[i] = keep[min(k0 + row_of(i * NT + tid), kdim - 1)];
         }
     }
-    // The step at k0 straight to LDS; what lies outside the operand arrives as zeros, and so do rows that do not count (look
-    // has been called for this step, and is for the next).
-    __device__ __forceinline__ void fill(int64_t k0, char* lds, uint32_t (&kept)[CH]) const {
+    // The step at k0 straight to LDS; what lies outside the operand arrives as zeros, and so do rows that do not count.
+    // The loads are written out: behind a builtin the compiler waits for all of them before it reads any transposed fragment, of
+    // whichever stage.  They have no registers to return to; arrive() waits for them.
+    __device__ __forceinline__ void fill(int64_t k0, const char* lds) const {
         constexpr uint32_t kNowhere = 0x80000000u;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const char* at = base + (ACROSS ? k0 * ld * int64_t(sizeof(Bits)) : 0);
         const int64_t values = ACROSS ? (kdim - k0 - 1) * ld + dim : (dim - 1) * ld + kdim;
-        const auto src = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<char*>(at), 0, int(min(values * int64_t(sizeof(Bits)), int64_t(0x7fffffff))), 0x00027000);
+        const int64_t bytes = min(values * int64_t(sizeof(Bits)), int64_t(0x7fffffff));
+        // a raw buffer: base address, its upper half, size, and the data format of 32-bit words
+        const uint64_t address = reinterpret_cast<uint64_t>(at);
+        const v4u src{uint32_t(address), uint32_t(address >> 32) & 0xffffu, uint32_t(bytes), 0x00027000u};
         const int step = ACROSS ? 0 : int(k0 * int64_t(sizeof(Bits)));
-        const bool tail = !ACROSS && k0 + BK > kdim;
+        const int left = int(min(kdim - k0, int64_t(BK)));
+        uint32_t o[CH];
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            uint32_t o = off[i];
-            if (tail) {
-                const int slot = i * NT + tid;
-                if (k0 + (chunk_of(slot) ^ swizzle(row_of(slot))) * 8 >= kdim) o = kNowhere;
-            }
-            if (ACROSS && keep && !kept[i]) o = kNowhere;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (LocalPtr)(lds + (i * NT + wave * 64) * 16), 16, int(o), step, 0, 0);
+            const int slot = i * NT + tid;
+            o[i] = ACROSS || (chunk_of(slot) ^ swizzle(row_of(slot))) * 8 < left ? off[i] : kNowhere;
         }
-        look(k0 + BK, kept);
+        if (ACROSS && keep) {
+            uint32_t kept[CH];
+            look(k0, kept);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                o[i] = kept[i] ? o[i] : kNowhere;
+                asm volatile("" : "+v"(o[i]));  // (waited for here, not by those who do not look)
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const uint32_t to = __builtin_amdgcn_readfirstlane(
+                uint32_t(reinterpret_cast<uintptr_t>((LocalBytes)(lds + (i * NT + wave * 64) * 16))));
+            asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                         :
+                         : "s"(to), "v"(o[i]), "s"(src), "s"(step)
+                         : "memory");
+        }
     }
     // The contraction up to here can be read in whole chunks: every row of a step is there, and the last chunk's read
     // ends inside the operand.
@@ -272,14 +294,23 @@ __device__ __forceinline__ uint32_t xcd_item(uint32_t block, uint32_t items) {
     return x * per + min(x, more) + (block >> 3);
 }
 
+// Wait until all but N of this wavefront's loads to LDS have arrived, and its reads of LDS, then for the other wavefronts.
+template <int N> __device__ __forceinline__ void arrive() {
+    static_assert(N < 64, "vmcnt has six bits");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070);  // vmcnt(N) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <class S, class T> constexpr int tile_lds() { return 2 * Units<S>::planes * (T::BM + T::BN) * Units<S>::bk * 2; }
 
 // Epi: static void run(const Args&, Acc<T>&, im, in, char* lds) of the tile (im, in).
 template <class S, class T, bool ATR, bool BTR, bool DIRECT, class Epi>
 __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea) {
-    constexpr int BK = Units<S>::bk, PL = Units<S>::planes;
-    using SA = Side<S, ATR, T::BM, T::NT, DIRECT>;
-    using SB = Side<S, BTR, T::BN, T::NT, DIRECT>;
+    constexpr int BK = DIRECT && T::DEEP ? 32 : Units<S>::bk, PL = Units<S>::planes;
+    using SA = Side<S, ATR, T::BM, T::NT, DIRECT, BK>;
+    using SB = Side<S, BTR, T::BN, T::NT, DIRECT, BK>;
     constexpr int kA = PL * SA::kPlane, kStage = kA + PL * SB::kPlane;
     __shared__ __attribute__((aligned(16))) char lds[tile_lds<S, T>()];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -331,64 +362,108 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
         clear(acc);
     };
 
-    // one step's products from a stage: the operands of a sixteenth are read while those of the one before are multiplied
-    // (in planes that has no registers, and needs none: six products for each operand)
-    constexpr int D = PL == 1 ? 2 : 1;
-    auto multiply = [&](const char* stage, auto between) {
-        const char *sa = stage, *sb = stage + kA;
-        int4 fa[D][PL][T::FM], fb[D][PL][T::FN];
-        auto read = [&](int t) {
-#pragma unroll
-            for (int p = 0; p < PL; ++p) {
-#pragma unroll
-                for (int i = 0; i < T::FM; ++i)
-                    fa[t % D][p][i] = SA::fragment(sa + p * SA::kPlane, (place.wm * T::FM + i) * 32, t, lane);
-#pragma unroll
-                for (int j = 0; j < T::FN; ++j)
-                    fb[t % D][p][j] = SB::fragment(sb + p * SB::kPlane, (place.wn * T::FN + j) * 32, t, lane);
-            }
-        };
-        if (D == 2) read(0);
-        between();
-#pragma unroll
-        for (int t = 0; t < BK / 16; ++t) {
-            if (t + D - 1 < BK / 16) read(t + D - 1);
-            // the small products of pieces first
-#pragma unroll
-            for (int s = PL - 1; s >= 0; --s)
-#pragma unroll
-                for (int p = 0; p <= s; ++p)
-#pragma unroll
-                    for (int i = 0; i < T::FM; ++i)
-#pragma unroll
-                        for (int j = 0; j < T::FN; ++j)
-                            acc[i][j] = Units<S>::mfma(fa[t % D][p][i], fb[t % D][s - p][j], acc[i][j]);
-            if (DIRECT) __builtin_amdgcn_sched_barrier(0);
-        }
-    };
     if constexpr (DIRECT) {
-        uint32_t ka[SA::CH], kb[SB::CH];
-        if (k0 < k1) {
-            a.look(k0, ka);
-            b.look(k0, kb);
-            a.fill(k0, lds, ka);
-            b.fill(k0, lds + kA, kb);
-        }
-        int cur = 0;
+        constexpr int kStages = T::DEEP ? 4 : 2, L = SA::CH + SB::CH;  // L: a wavefront's loads for a stage
+        const int n = int((k1 - k0 + BK - 1) / BK);
+        int4 fa[2][T::FM], fb[2][T::FN];
+        auto stage = [&](int s) { return lds + s % kStages * kStage; };
+        auto fill = [&](int s) {
+            a.fill(k0 + int64_t(s) * BK, stage(s));
+            b.fill(k0 + int64_t(s) * BK, stage(s) + kA);
+        };
+        auto read = [&](int s, int t) {
+            const char *sa = stage(s), *sb = sa + kA;
+#pragma unroll
+            for (int i = 0; i < T::FM; ++i) fa[t % 2][i] = SA::fragment(sa, (place.wm * T::FM + i) * 32, t, lane);
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j) fb[t % 2][j] = SB::fragment(sb, (place.wn * T::FN + j) * 32, t, lane);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto multiply = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+                for (int j = 0; j < T::FN; ++j) acc[i][j] = Units<S>::mfma(fa[t % 2][i], fb[t % 2][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if constexpr (!T::DEEP) {
+            // one stage is multiplied while the other is filled
+            if (n > 0) fill(0);
 #pragma unroll 1
-        for (int64_t k = k0; k < k1; k += BK) {
-            if (kTwo && k % kFlush == 0) flush();
-            stage_ready();
-            char* next = lds + (cur ^ 1) * kStage;
-            multiply(lds + cur * kStage, [&] {
-                if (k + BK < k1) {
-                    a.fill(k + BK, next, ka);
-                    b.fill(k + BK, next + kA, kb);
+            for (int s = 0; s < n; ++s) {
+                if (kTwo && s % (kFlush / BK) == 0) flush();
+                arrive<0>();
+                read(s, 0);
+                if (s + 1 < n) fill(s + 1);
+#pragma unroll
+                for (int t = 0; t < BK / 16; ++t) {
+                    if (t + 1 < BK / 16) read(s, t + 1);
+                    multiply(t);
                 }
-            });
-            cur ^= 1;
+            }
+        } else {
+            // While one stage is multiplied the next has arrived and two are on their way.  A step's first operands are
+            // read behind the barrier of the step before, so that products are at hand while wavefronts wait for each
+            // other.  (4096 x 12288 bfloat16 pairs of 4224 values: 384 us for the images' gradients, 429 in two stages;
+            // tiles of 128 x 128 are slower that way, 516 and 441 for the scores' gradient: twice the barriers)
+            if (n > 0) fill(0);
+            if (n > 1) fill(1);
+            if (n > 2) fill(2);
+            if (n > 2)
+                arrive<2 * L>();
+            else
+                arrive<0>();
+            if (n > 0) read(0, 0);
+#pragma unroll 1
+            for (int s = 0; s < n; ++s) {
+                if (kTwo && s % (kFlush / BK) == 0) flush();
+                if (s + 3 < n) fill(s + 3);  // (where the stage before this one was)
+                read(s, 1);
+                multiply(0);
+                if (s + 1 < n) {
+                    if (s + 3 < n)
+                        arrive<2 * L>();
+                    else
+                        arrive<0>();
+                    read(s + 1, 0);
+                }
+                multiply(1);
+            }
         }
     } else {
+        // one step's products from a stage: the operands of a sixteenth are read while those of the one before are multiplied
+        // (in planes there are no registers for that, and no need: six products for each operand)
+        constexpr int D = PL == 1 ? 2 : 1;
+        auto multiply = [&](const char* stage) {
+            const char *sa = stage, *sb = stage + kA;
+            int4 fa[D][PL][T::FM], fb[D][PL][T::FN];
+            auto read = [&](int t) {
+#pragma unroll
+                for (int p = 0; p < PL; ++p) {
+#pragma unroll
+                    for (int i = 0; i < T::FM; ++i)
+                        fa[t % D][p][i] = SA::fragment(sa + p * SA::kPlane, (place.wm * T::FM + i) * 32, t, lane);
+#pragma unroll
+                    for (int j = 0; j < T::FN; ++j)
+                        fb[t % D][p][j] = SB::fragment(sb + p * SB::kPlane, (place.wn * T::FN + j) * 32, t, lane);
+                }
+            };
+            if (D == 2) read(0);
+#pragma unroll
+            for (int t = 0; t < BK / 16; ++t) {
+                if (t + D - 1 < BK / 16) read(t + D - 1);
+                // the small products of pieces first
+#pragma unroll
+                for (int s = PL - 1; s >= 0; --s)
+#pragma unroll
+                    for (int p = 0; p <= s; ++p)
+#pragma unroll
+                        for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+                            for (int j = 0; j < T::FN; ++j)
+                                acc[i][j] = Units<S>::mfma(fa[t % D][p][i], fb[t % D][s - p][j], acc[i][j]);
+            }
+        };
         // two steps are on their way to registers while a third is multiplied
         typename SA::Regs ra[2];
         typename SB::Regs rb[2];
@@ -416,7 +491,7 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
                 if (at >= kw) break;
                 __syncthreads();
                 load(min(at + 2 * BK, last), r);  // (past the end: the last one again, not used)
-                multiply(lds + r * kStage, [] {});
+                multiply(lds + r * kStage);
                 if (at + BK < kw) store(r ^ 1);
             }
         }
@@ -428,7 +503,7 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
             __syncthreads();
             store(0);
             __syncthreads();
-            multiply(lds, [] {});
+            multiply(lds);
         }
     }
     if constexpr (kTwo) {
@@ -468,6 +543,8 @@ __global__ __launch_bounds__(T::NT) void k_tile_join(Product g, typename Epi::Ar
         for (int j = 0; j < T::FN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    constexpr int kUnroll = T::FM * T::FN <= 2 ? 4 : 1;  // (ranges on their way; the others have no registers)
+#pragma unroll kUnroll
     for (int s = 0; s < g.splits; ++s) {
         const float* p = g.part + (int64_t(s) * gridDim.x + item) * (T::BM * T::BN) + threadIdx.x * 4;
 #pragma unroll
