@@ -3,13 +3,13 @@
 #pragma once
 
 #include "tp_match.hh"
+#include "tp_tile_plan.hh"
 
 namespace tp {
 
 constexpr int64_t kMaxStride = int64_t(1) << 21;    // elements between rows, and values of a row
 constexpr int64_t kMaxPairRows = int64_t(1) << 26;  // of either side
 constexpr int64_t kMaxPairs = int64_t(1) << 38;     // images times references
-constexpr int64_t kMaxTiles = int64_t(1) << 22;     // of a product (a launch has fewer than 2^32 lanes)
 constexpr int kFewImages = 8;                       // up to here the references are streamed past the images
 
 struct PairArgs {
@@ -45,23 +45,12 @@ struct PairCoef {
     float most, a, at_given;  // (most in powers of two, as below)
     int given;                // -1: none
 };
-struct PairTile {
-    bool direct;     // operands go straight to LDS (16-bit rows that start at 16-byte boundaries)
-    int tile;
-    uint32_t whole;  // tiles that are not split
-    int splits;      // ranges of the contraction of the others
-};
 // Scores are formed and summed in powers of two: score * log2 e, so that a product and a sum become one multiply-add and
 // the exponential one instruction.
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 struct ScorePart {
     float most, sum;  // of a tile's references: the largest score, and sum 2^(score - most) without the given one
 };
-// rows (of D), columns and contraction of a product -> its tile and ranges
-PairTile pair_plan(int dt, bool direct, int64_t rows, int64_t cols, int64_t kdim);
-int64_t pair_part_bytes(int dt, const PairTile& t, int64_t rows, int64_t cols);
-int64_t pair_tiles(int dt, const PairTile& t, int64_t n, bool of_rows);  // along the rows or the columns
-
 struct PairOff {  // what a tile's references add to their scores
     const float* bias;
     const uint8_t* mask;
@@ -98,13 +87,13 @@ struct MatrixOut {
 };
 template <class S> struct PairProducts {
     // references x images
-    static hipError_t stats(const PairArgs& a, const PairTile& t, const StatsOut& o, float* part, hipStream_t s);
-    static hipError_t grad(const PairArgs& a, const void* r, int64_t n, const PairTile& t, const GradOut& o, float* part, hipStream_t s);
+    static hipError_t stats(const PairArgs& a, const TilePlan& t, const StatsOut& o, float* part, hipStream_t s);
+    static hipError_t grad(const PairArgs& a, const void* r, int64_t n, const TilePlan& t, const GradOut& o, float* part, hipStream_t s);
     // out [n][K] = g x, out [M][K] = g^t r
-    static hipError_t d_references(const PairArgs& a, const void* g, int64_t ldg, int64_t n, const PairTile& t,
+    static hipError_t d_references(const PairArgs& a, const void* g, int64_t ldg, int64_t n, const TilePlan& t,
                                    const MatrixOut& o, float* part, hipStream_t s);
     static hipError_t d_images(const PairArgs& a, const void* g, int64_t ldg, const void* r, const uint8_t* mask,
-                               const int* look, int64_t n, const PairTile& t, const MatrixOut& o, float* part, hipStream_t s);
+                               const int* look, int64_t n, const TilePlan& t, const MatrixOut& o, float* part, hipStream_t s);
 };
 
 }  // namespace tp

@@ -250,6 +250,7 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
             float v = a.bias ? a.bias[n] : 0.0f;
             if (v == -INFINITY) continue;
             float s = 0.0f;
+#pragma unroll 4
             for (int t = 0; t < splits; ++t) s += part[(int64_t(t) * a.M + m) * a.N + n];
             z[k] = fmaf(s, a.c * kLog2e, v * (a.c * kLog2e));
         }
@@ -292,6 +293,7 @@ __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float*
                                                         void* d_r, float* d_bias) {
     using Bits = typename S::Bits;
     __shared__ float G[kBackRows][MB];
+    __shared__ bool counts[kBackRows];
     __shared__ PairCoef coef[MB];
     const int tid = threadIdx.x;
     const int64_t first = int64_t(blockIdx.y) * per, last = min(first + per, a.N);
@@ -307,8 +309,25 @@ __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float*
             dx[m][k] = 0.0f;
             x[m][k] = d_r && m < a.M && k < have ? S::widen(static_cast<const Bits*>(a.x)[m * a.ldx + c + k]) : 0.0f;
         }
+    constexpr int W = 8;  // rows on their way
+    Bits next[W][kBackCols];
     for (int64_t n0 = first; n0 < last; n0 += kBackRows) {
         const int rows = int(min(last - n0, int64_t(kBackRows)));
+        const Bits* r = static_cast<const Bits*>(a.r) + n0 * a.ldr + c;
+        auto fetch = [&](int row) {
+            if (!dx_part) return;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const Bits* p = r + min(row + w, rows - 1) * a.ldr;
+                if (have == kBackCols) {
+                    __builtin_memcpy(next[w], p, sizeof next[w]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kBackCols; ++k) next[w][k] = k < have ? p[k] : Bits(0);
+                }
+            }
+        };
+        fetch(0);
         __syncthreads();
         for (int i = tid; i < kBackRows * MB; i += 256) {
             const int m = i / kBackRows, row = i % kBackRows;
@@ -319,6 +338,7 @@ __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float*
             }
             G[row][m] = v;
         }
+        if (tid < rows) counts[tid] = !a.mask || a.mask[n0 + tid];
         __syncthreads();
         if (blockIdx.x == 0 && d_bias && tid < rows) {
             float v = 0.0f;
@@ -327,57 +347,42 @@ __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float*
             d_bias[n0 + tid] = v;
         }
         if (!have) continue;
-        const Bits* r = static_cast<const Bits*>(a.r) + n0 * a.ldr + c;
         Bits* o = static_cast<Bits*>(d_r) + (d_r ? n0 * a.K + c : 0);
-        auto one = [&](int row, const Bits (&v)[kBackCols]) {
-            float up[kBackCols] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int row0 = 0; row0 < rows; row0 += W) {
+            Bits now[W][kBackCols];
 #pragma unroll
-            for (int m = 0; m < MB; ++m) {
-                const float w = G[row][m];
+            for (int w = 0; w < W; ++w)
 #pragma unroll
-                for (int k = 0; k < kBackCols; ++k) {
-                    dx[m][k] += w * S::widen(v[k]);
-                    up[k] += w * x[m][k];
+                for (int k = 0; k < kBackCols; ++k) now[w][k] = dx_part ? next[w][k] : Bits(0);
+            if (row0 + W < rows) fetch(row0 + W);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const int row = row0 + w;
+                if (row >= rows) break;
+                // (what a reference that the mask rules out holds is not used)
+                const bool use = counts[row];
+                float up[kBackCols] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int m = 0; m < MB; ++m) {
+                    const float g = G[row][m];
+#pragma unroll
+                    for (int k = 0; k < kBackCols; ++k) {
+                        dx[m][k] += g * (use ? S::widen(now[w][k]) : 0.0f);
+                        up[k] += g * x[m][k];
+                    }
+                }
+                if (!d_r) continue;
+                Bits b[kBackCols];
+#pragma unroll
+                for (int k = 0; k < kBackCols; ++k) b[k] = S::round(up[k]);
+                if (have == kBackCols) {
+                    __builtin_memcpy(o + row * a.K, b, sizeof b);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kBackCols; ++k)
+                        if (k < have) o[row * a.K + k] = b[k];
                 }
             }
-            if (!d_r) return;
-            Bits b[kBackCols];
-#pragma unroll
-            for (int k = 0; k < kBackCols; ++k) b[k] = S::round(up[k]);
-            if (have == kBackCols) {
-                __builtin_memcpy(o + row * a.K, b, sizeof b);
-            } else {
-#pragma unroll
-                for (int k = 0; k < kBackCols; ++k)
-                    if (k < have) o[row * a.K + k] = b[k];
-            }
-        };
-        auto fetch = [&](int row, Bits (&v)[kBackCols]) {
-#pragma unroll
-            for (int k = 0; k < kBackCols; ++k) v[k] = 0;
-            // (what a reference that is ruled out holds is not used)
-            if (!dx_part || (a.mask && !a.mask[n0 + row])) return;
-            if (have == kBackCols) {
-                __builtin_memcpy(v, r + row * a.ldr, sizeof v);
-            } else {
-#pragma unroll
-                for (int k = 0; k < kBackCols; ++k)
-                    if (k < have) v[k] = r[row * a.ldr + k];
-            }
-        };
-        constexpr int W = 8;  // rows on their way
-        int row = 0;
-        for (; row + W <= rows; row += W) {
-            Bits v[W][kBackCols];
-#pragma unroll
-            for (int w = 0; w < W; ++w) fetch(row + w, v[w]);
-#pragma unroll
-            for (int w = 0; w < W; ++w) one(row + w, v[w]);
-        }
-        for (; row < rows; ++row) {
-            Bits v[kBackCols];
-            fetch(row, v);
-            one(row, v);
         }
     }
     if (!dx_part) return;
@@ -422,20 +427,6 @@ int64_t few_per(int64_t N, int64_t K) {
     return per < 16 ? 16 : per;
 }
 
-// One step (bk of the contraction) of a tile, and its start and end: among as many as a CU holds, and alone.  Measured on products of
-// 1024 to 16384 along the contraction with every CU at work.
-struct TileKind {
-    int bm, bn, bk;
-    double step_us, over_us, alone_us, alone_over_us;
-};
-constexpr TileKind kTiles16[] = {{64, 64, 64, 0.174, 2.2, 0.50, 5}, {128, 128, 64, 0.395, 5, 0.75, 6}, {256, 256, 64, 1.62, 10, 1.62, 10}};
-constexpr TileKind kTilesStaged[] = {{64, 64, 64, 0.24, 1.4, 0.75, 5}, {128, 128, 64, 0.48, 5, 0.85, 6}};
-constexpr TileKind kTiles32[] = {{64, 64, 32, 0.44, 0.5, 0.62, 4}, {128, 128, 32, 1.42, 3, 1.42, 4}, {256, 128, 32, 2.40, 11, 2.40, 11}};
-const TileKind& kind_of(int dt, const PairTile& t) {
-    return dt == TP_F32 ? kTiles32[t.tile] : t.direct ? kTiles16[t.tile] : kTilesStaged[t.tile];
-}
-constexpr int kMaxSplits = 32;
-
 // A piece's G is at most this large: 128 MB stay in the last cache between the product that writes it and those that read it.
 constexpr int64_t kPieceBytes = int64_t(1) << 27;
 int64_t piece_of(int dt, int64_t M, int64_t N) {
@@ -455,16 +446,16 @@ bool pair_direct(const PairArgs& a) {
 
 struct BackLayout {
     int64_t piece, ldg;
-    PairTile grad, refs, images;
+    TilePlan grad, refs, images;
     int64_t coef, scale, g, sums, part, dx, bytes;
 };
 BackLayout back_layout(int dt, bool direct, int64_t M, int64_t N, int64_t K, bool d_x, bool d_r) {
     BackLayout b{};
     b.piece = piece_of(dt, M, N);
     b.ldg = (M + 7) / 8 * 8;
-    b.grad = pair_plan(dt, direct, b.piece, M, K);
-    b.refs = pair_plan(dt, direct, b.piece, K, M);
-    b.images = pair_plan(dt, direct, M, K, b.piece);
+    b.grad = tile_plan(dt, direct, b.piece, M, K);
+    b.refs = tile_plan(dt, direct, b.piece, K, M);
+    b.images = tile_plan(dt, direct, M, K, b.piece);
     int64_t at = 0;
     auto room = [&](int64_t bytes) {
         const int64_t here = at;
@@ -474,10 +465,10 @@ BackLayout back_layout(int dt, bool direct, int64_t M, int64_t N, int64_t K, boo
     b.coef = room(M * int64_t(sizeof(PairCoef)));
     b.scale = room(16);
     b.g = room(b.piece * b.ldg * size_of(dt));
-    b.sums = room(pair_tiles(dt, b.grad, M, false) * b.piece * 4);
-    int64_t part = pair_part_bytes(dt, b.grad, b.piece, M);
-    if (d_r) part = part > pair_part_bytes(dt, b.refs, b.piece, K) ? part : pair_part_bytes(dt, b.refs, b.piece, K);
-    if (d_x) part = part > pair_part_bytes(dt, b.images, M, K) ? part : pair_part_bytes(dt, b.images, M, K);
+    b.sums = room(tile_count(dt, b.grad, M, false) * b.piece * 4);
+    int64_t part = tile_part_bytes(dt, b.grad, b.piece, M);
+    if (d_r) part = part > tile_part_bytes(dt, b.refs, b.piece, K) ? part : tile_part_bytes(dt, b.refs, b.piece, K);
+    if (d_x) part = part > tile_part_bytes(dt, b.images, M, K) ? part : tile_part_bytes(dt, b.images, M, K);
     b.part = room(part);
     b.dx = room(d_x && b.piece < N ? M * K * 4 : 0);
     b.bytes = at;
@@ -508,46 +499,6 @@ __global__ __launch_bounds__(256) void k_pairs_none(PairArgs a, float* given_out
 
 }  // namespace
 
-// The tile, and the tiles and ranges that are split, with the least time by a count of steps.  Every CU computes as many whole
-// tiles; those that are left over are split along the contraction so that they give every CU something to do, too, which
-// costs their sums written and read (by one workgroup a tile, at some 70 GB/s).  Against all tiles and 1 to 16 ranges
-// on 88 products from 20 x 5000 to 4096 x 12288 the choice is 3 % from the best on average, at most 28 %.
-PairTile pair_plan(int dt, bool direct, int64_t rows, int64_t cols, int64_t kdim) {
-    PairTile best{direct, 0, 0, 1};
-    double least = 1e300;
-    for (int t = 0; t < (dt == TP_F32 || direct ? 3 : 2); ++t) {
-        const TileKind& k = kind_of(dt, PairTile{direct, t, 0, 1});
-        const int64_t tiles = ((rows + k.bm - 1) / k.bm) * ((cols + k.bn - 1) / k.bn);
-        if (tiles > kMaxTiles) continue;
-        const int64_t steps = (kdim + k.bk - 1) / k.bk;
-        auto weigh = [&](int64_t each, int s) {  // `each` whole tiles on a CU, the others in s ranges
-            const int64_t rest = tiles - each * kCus, groups = (rest * s + kCus - 1) / kCus, part = (steps + s - 1) / s;
-            double us = each * (steps * k.step_us + k.over_us) + groups * (part * k.step_us + k.over_us);
-            us = std::max(us, (each ? steps : part) * k.alone_us + k.alone_over_us);
-            if (s > 1) us += 6.0 + 0.1 * s + (s + 1) * (k.bm * k.bn * 6e-5) * double((rest + kCus - 1) / kCus);
-            if (us < least) {
-                least = us;
-                best = {direct, t, uint32_t(each * kCus), s};
-            }
-        };
-        weigh(tiles / kCus, 1);
-        for (int s = 2; s <= kMaxSplits && s <= steps; ++s) {
-            if (tiles % kCus) weigh(tiles / kCus, s);
-            if (tiles >= kCus && tiles * s <= 8 * kCus) weigh(0, s);
-        }
-    }
-    return best;
-}
-int64_t pair_part_bytes(int dt, const PairTile& t, int64_t rows, int64_t cols) {
-    const TileKind& k = kind_of(dt, t);
-    const int64_t rest = pair_tiles(dt, t, rows, true) * pair_tiles(dt, t, cols, false) - int64_t(t.whole);
-    return t.splits > 1 && rest > 0 ? rest * t.splits * k.bm * k.bn * 4 : 0;
-}
-int64_t pair_tiles(int dt, const PairTile& t, int64_t n, bool of_rows) {
-    const int size = of_rows ? kind_of(dt, t).bm : kind_of(dt, t).bn;
-    return (n + size - 1) / size;
-}
-
 // (rows may turn out not to start at 16-byte boundaries: room for either plan)
 template <class F> int64_t either_plan(int dt, int64_t K, F bytes) {
     const int64_t staged = bytes(false);
@@ -559,8 +510,8 @@ int64_t pair_work(int dt, int64_t M, int64_t N, int64_t K) {
     if (M == 0 || N == 0) return 0;
     if (pair_few(M)) return up16(few_splits(dt, N, K) * M * N * 4);
     return either_plan(dt, K, [&](bool direct) {
-        const PairTile t = pair_plan(dt, direct, N, M, K);
-        return up16(M * 4) + up16(pair_tiles(dt, t, N, true) * M * int64_t(sizeof(ScorePart))) + pair_part_bytes(dt, t, N, M);
+        const TilePlan t = tile_plan(dt, direct, N, M, K);
+        return up16(M * 4) + up16(tile_count(dt, t, N, true) * M * int64_t(sizeof(ScorePart))) + tile_part_bytes(dt, t, N, M);
     });
 }
 
@@ -584,8 +535,8 @@ hipError_t launch_pair_log_probs(const PairArgs& a, float* given_out, float* log
                                                              given_out, log_sum, state);
         return hipGetLastError();
     }
-    const PairTile t = pair_plan(a.dt, pair_direct(a), a.N, a.M, a.K);
-    const int64_t tiles = pair_tiles(a.dt, t, a.N, true);
+    const TilePlan t = tile_plan(a.dt, pair_direct(a), a.N, a.M, a.K);
+    const int64_t tiles = tile_count(a.dt, t, a.N, true);
     auto* given_score = static_cast<float*>(work);
     auto* parts = reinterpret_cast<ScorePart*>(static_cast<char*>(work) + up16(a.M * 4));
     auto* part = reinterpret_cast<float*>(reinterpret_cast<char*>(parts) + up16(tiles * a.M * int64_t(sizeof(ScorePart))));
@@ -658,7 +609,7 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
         });
         if (e) return e;
         if (d_bias) {
-            k_pairs_bias<<<match_grid((n + 255) / 256), 256, 0, s>>>(sums, int(pair_tiles(a.dt, b.grad, a.M, false)), n,
+            k_pairs_bias<<<match_grid((n + 255) / 256), 256, 0, s>>>(sums, int(tile_count(a.dt, b.grad, a.M, false)), n,
                                                                      scale, d_bias + first);
             if (hipError_t f = hipGetLastError()) return f;
         }

@@ -256,65 +256,19 @@ struct MatrixEpi {
     }
 };
 
-template <class S> struct Shapes {
-    using Small = TileShape<64, 64, 2, 2>;
-    using Middle = TileShape<128, 128, 2, 4>;
-    using Large = TileShape<256, 256, 2, 4, true>;  // (straight to LDS only: there are no registers for what is on its way)
-};
-template <> struct Shapes<F32> {  // (three planes of 256 x 128 are 144 KB in two stages)
-    using Small = TileShape<64, 64, 2, 2>;
-    using Middle = TileShape<128, 128, 2, 4>;
-    using Large = TileShape<256, 128, 4, 2>;
-};
-
-// Whether an operand's chunks of eight 16-bit values can go straight to LDS.
-template <bool ACROSS> bool direct(const Operand& o) {
-    return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % 8 == 0 && (ACROSS || o.kdim % 8 == 0);
-}
-
-template <class S, class T, bool ATR, bool BTR, bool DIRECT, class Epi>
-hipError_t product_of(Product g, const typename Epi::Args& ea, hipStream_t s) {
-    g.tm = uint32_t((g.rows + T::BM - 1) / T::BM);
-    g.tn = uint32_t((g.cols + T::BN - 1) / T::BN);
-    const uint32_t tiles = g.tm * g.tn, rest = tiles > g.whole ? tiles - g.whole : 0;
-    g.whole = tiles - rest;
-    k_tile<S, T, ATR, BTR, DIRECT, Epi><<<dim3(g.whole + rest * g.splits), T::NT, 0, s>>>(g, ea);
-    if (hipError_t e = hipGetLastError()) return e;
-    if (rest && g.splits > 1) k_tile_join<S, T, Epi><<<dim3(rest), T::NT, 0, s>>>(g, ea);
-    return hipGetLastError();
-}
-template <class S, bool ATR, bool BTR, class Epi>
-hipError_t product(const Product& g, const PairTile& t, const typename Epi::Args& ea, hipStream_t s) {
-    using Small = typename Shapes<S>::Small;
-    using Middle = typename Shapes<S>::Middle;
-    using Large = typename Shapes<S>::Large;
-    if constexpr (Units<S>::planes == 1) {
-        if (t.direct && direct<ATR>(g.a) && direct<BTR>(g.b)) {
-            if (t.tile == 0) return product_of<S, Small, ATR, BTR, true, Epi>(g, ea, s);
-            if (t.tile == 1) return product_of<S, Middle, ATR, BTR, true, Epi>(g, ea, s);
-            return product_of<S, Large, ATR, BTR, true, Epi>(g, ea, s);
-        }
-    } else if (t.tile == 2) {
-        return product_of<S, Large, ATR, BTR, false, Epi>(g, ea, s);
-    }
-    if (t.tile == 0) return product_of<S, Small, ATR, BTR, false, Epi>(g, ea, s);
-    if (t.tile == 1) return product_of<S, Middle, ATR, BTR, false, Epi>(g, ea, s);
-    return hipErrorInvalidValue;
-}
-
 }  // namespace
 
-template <class S> hipError_t PairProducts<S>::stats(const PairArgs& a, const PairTile& t, const StatsOut& o, float* part, hipStream_t s) {
+template <class S> hipError_t PairProducts<S>::stats(const PairArgs& a, const TilePlan& t, const StatsOut& o, float* part, hipStream_t s) {
     const Product g{{a.r, a.ldr, a.K, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr}, a.N, a.M, a.K, 0, 0, t.whole, t.splits, part};
     return product<S, false, false, StatsEpi>(g, t, o, s);
 }
 template <class S>
-hipError_t PairProducts<S>::grad(const PairArgs& a, const void* r, int64_t n, const PairTile& t, const GradOut& o, float* part, hipStream_t s) {
+hipError_t PairProducts<S>::grad(const PairArgs& a, const void* r, int64_t n, const TilePlan& t, const GradOut& o, float* part, hipStream_t s) {
     const Product g{{r, a.ldr, a.K, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr}, n, a.M, a.K, 0, 0, t.whole, t.splits, part};
     return product<S, false, false, GradEpi>(g, t, o, s);
 }
 template <class S>
-hipError_t PairProducts<S>::d_references(const PairArgs& a, const void* gr, int64_t ldg, int64_t n, const PairTile& t,
+hipError_t PairProducts<S>::d_references(const PairArgs& a, const void* gr, int64_t ldg, int64_t n, const TilePlan& t,
                                          const MatrixOut& o, float* part, hipStream_t s) {
     // (g holds zeros from M to ldg: whole chunks)
     const Product g{{gr, ldg, ldg, nullptr, nullptr}, {a.x, a.ldx, a.M, nullptr, nullptr}, n, a.K, a.M, 0, 0, t.whole, t.splits, part};
@@ -322,7 +276,7 @@ hipError_t PairProducts<S>::d_references(const PairArgs& a, const void* gr, int6
 }
 template <class S>
 hipError_t PairProducts<S>::d_images(const PairArgs& a, const void* gr, int64_t ldg, const void* r, const uint8_t* mask,
-                                     const int* look, int64_t n, const PairTile& t, const MatrixOut& o, float* part, hipStream_t s) {
+                                     const int* look, int64_t n, const TilePlan& t, const MatrixOut& o, float* part, hipStream_t s) {
     const Product g{{gr, ldg, n, nullptr, nullptr}, {r, a.ldr, n, mask, look}, a.M, a.K, n, 0, 0, t.whole, t.splits, part};
     return product<S, true, true, MatrixEpi>(g, t, o, s);
 }

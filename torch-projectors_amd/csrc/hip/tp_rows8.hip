@@ -9,15 +9,13 @@
 // that is finer than 8-bit floating point's 3-bit mantissa, at twice the rate of the bfloat16 units which those need.
 #include "../../../include/torch_projectors_hip.h"
 #include "tp_match.hh"
-#include "tp_stage.hh"
+#include "tp_tile.hh"
 
 #include <type_traits>
 
 namespace tp {
 namespace {
 
-using v4i = __attribute__((ext_vector_type(4))) int;
-using v16i = __attribute__((ext_vector_type(16))) int;
 constexpr int kRow = kRowPad;  // bytes of a row that a step of the products takes
 
 // ------------------------------------------------------------------ quantize
@@ -59,25 +57,55 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
     return v;
 }
 
-// W wavefronts per row, which read it twice: the second time it comes from the caches.
-template <class S, int W>
-__global__ __launch_bounds__(256) void k_quantize_rows(const typename S::Bits* __restrict__ x, int64_t rows, int64_t cols,
-                                                       int64_t stride, int64_t padded, uint8_t* __restrict__ codes,
-                                                       float* __restrict__ scales) {
-    __shared__ uint32_t room[4];
-    const int wave = threadIdx.x >> 6, t = threadIdx.x & (64 * W - 1);
-    for (int64_t r0 = int64_t(blockIdx.x) * (4 / W); r0 < rows; r0 += int64_t(gridDim.x) * (4 / W)) {
+// Eight codes.  The quotient by the reciprocal is within 2^-15 of the right one (three roundings of numbers up to 127): where it is
+// not that close to a border between two codes both have the same, and the right quotient, some ten instructions, is not formed.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float scale, float inverse) {
+    float c[8];
+    bool close = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float q = v[i] * inverse;
+        c[i] = rintf(q);
+        close = close || !(fabsf(q - c[i]) < 0.5f - 0x1p-14f);
+    }
+    if (__builtin_amdgcn_ballot_w64(close) != 0) return codes8(v, scale);
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i / 4] |= (uint32_t(int(c[i])) & 255u) << (i % 4 * 8);
+    return uint2{w[0], w[1]};
+}
+__device__ __forceinline__ float row_inverse(float scale) { return 1.0f / scale; }
+
+// W wavefronts per row.  A row of at most 2048 W values stays in registers between its largest and its codes; a longer one is
+// read twice.
+constexpr int kHeld = 4;  // chunks of eight values that a lane holds
+template <class S, int W, bool HELD>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_quantize_rows(const typename S::Bits* __restrict__ x, int64_t rows, int64_t cols,
+                                                                        int64_t stride, int64_t padded, uint8_t* __restrict__ codes,
+                                                                        float* __restrict__ scales) {
+    constexpr int kWaves = W > 4 ? W : 4, kRows = kWaves / W;
+    __shared__ uint32_t room[kWaves];
+    const int wave = threadIdx.x >> 6, t = threadIdx.x % (64 * W);
+    for (int64_t r0 = int64_t(blockIdx.x) * kRows; r0 < rows; r0 += int64_t(gridDim.x) * kRows) {
         const int64_t r = r0 + wave / W;
         const bool there = r < rows;
         const typename S::Bits* p = x + (there ? r : 0) * stride;
         uint32_t most = 0;
-        float v[8];
-        if (there)
+        float held[HELD ? kHeld : 1][8];
+        if (there) {
+            if constexpr (HELD) {
+#pragma unroll
+                for (int k = 0; k < kHeld; ++k) load8<S>(p + 8 * t + k * 512 * W, cols - 8 * t - k * 512 * W, held[k]);
+#pragma unroll
+                for (int k = 0; k < kHeld; ++k) most = max8(held[k], most);
+            } else {
 #pragma unroll 4
-            for (int64_t c = 8 * t; c < cols; c += 512 * W) {
-                load8<S>(p + c, cols - c, v);
-                most = max8(v, most);
+                for (int64_t c = 8 * t; c < cols; c += 512 * W) {
+                    load8<S>(p + c, cols - c, held[0]);
+                    most = max8(held[0], most);
+                }
             }
+        }
         most = wave_most(most);
         if (W > 1) {
             __syncthreads();
@@ -87,19 +115,28 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const typename S::Bits* _
             for (int i = 0; i < W; ++i) most = max(most, room[wave / W * W + i]);
         }
         if (!there) continue;
-        const float scale = row_scale(most);
+        const float scale = row_scale(most), inverse = row_inverse(scale);
         if (t == 0) scales[r] = scale;
+        uint8_t* out = codes + r * padded;
+        if constexpr (HELD) {
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) {
+                const int64_t c = 8 * t + k * 512 * W;
+                if (c < padded) *reinterpret_cast<uint2*>(out + c) = codes8(held[k], scale, inverse);
+            }
+        } else {
 #pragma unroll 4
-        for (int64_t c = 8 * t; c < padded; c += 512 * W) {
-            load8<S>(p + c, cols - c, v);
-            *reinterpret_cast<uint2*>(codes + r * padded + c) = codes8(v, scale);
+            for (int64_t c = 8 * t; c < padded; c += 512 * W) {
+                load8<S>(p + c, cols - c, held[0]);
+                *reinterpret_cast<uint2*>(out + c) = codes8(held[0], scale, inverse);
+            }
         }
     }
 }
 
 // ------------------------------------------------------------------ scores
-// [splits] ranges of the rows' steps are one workgroup each, and where there are several their sums go to part
-// [splits][M][N], which k_rows8_join adds up.
+// Few images: [splits] ranges of the rows' steps are one workgroup each, and where there are several their sums go to
+// part [splits][M][N], which k_rows8_join adds up.
 struct Rows8Args {
     const uint8_t* a;
     const float* sa;
@@ -173,9 +210,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_rows8_few(Rows8Args g, OneRo
     float scale = 0.0f;
     if constexpr (kOne) {
         const auto* x = static_cast<const typename S::Bits*>(one.x);
+        // the first kKept x 4096 values stay in registers between their largest and their codes
+        constexpr int kKept = 5;
         uint32_t most = 0;
-        float v[8];
-        for (int64_t c = 8 * tid; c < one.cols; c += 512 * kFewWaves) {
+        float kept[kKept][8], v[8];
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) load8<S>(x + 8 * tid + i * 4096, one.cols - 8 * tid - i * 4096, kept[i]);
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) most = max8(kept[i], most);
+        for (int64_t c = 8 * tid + kKept * 4096; c < one.cols; c += 4096) {
             load8<S>(x + c, one.cols - c, v);
             most = max8(v, most);
         }
@@ -185,9 +228,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_rows8_few(Rows8Args g, OneRo
 #pragma unroll
         for (int w = 0; w < kFewWaves; ++w) most = max(most, mosts[w]);
         scale = row_scale(most);
-        for (int64_t c = int64_t(k0) * kRow + 8 * tid; c < int64_t(k1) * kRow; c += 512 * kFewWaves) {
+        const float inverse = row_inverse(scale);
+#pragma unroll
+        for (int i = 0; i < kKept; ++i)
+            if (8 * tid + i * 4096 < K) *reinterpret_cast<uint2*>(room + 8 * tid + i * 4096) = codes8(kept[i], scale, inverse);
+        for (int64_t c = 8 * tid + kKept * 4096; c < K; c += 4096) {
             load8<S>(x + c, one.cols - c, v);
-            *reinterpret_cast<uint2*>(room + (c - int64_t(k0) * kRow)) = codes8(v, scale);
+            *reinterpret_cast<uint2*>(room + c) = codes8(v, scale, inverse);
         }
         __syncthreads();
     }
@@ -201,7 +248,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_rows8_few(Rows8Args g, OneRo
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int f = 0; f < FM; ++f) {
-                    const v4i a = kOne ? *reinterpret_cast<const v4i*>(room + (at - k0) * kRow + h * 64 + q * 16) : ca[u][f][h];
+                    const v4i a = kOne ? *reinterpret_cast<const v4i*>(room + at * kRow + h * 64 + q * 16) : ca[u][f][h];
                     acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, cb[u][h], acc[f], 0, 0, 0);
                 }
         }
@@ -225,225 +272,90 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_rows8_few(Rows8Args g, OneRo
     }
 }
 
-// The product in tiles: a workgroup of WM x WN x KW wavefronts computes BM x BN scores.  One step of a tile's rows in
-// LDS is 128 bytes each, fragment after fragment (fragment f of a part of the tile has its rows F r + f, r < 32), and the
-// 16-byte chunks of a row permuted among themselves (chunk c of row r of a fragment at place c ^ ((r / 2) & 7)), so
-// that the 16 lanes that read one chunk of 16 rows at a time reach each of the 64 banks once.
-template <int BM, int BN> struct alignas(16) Stage8 {
-    uint8_t a[BM * kRow], b[BN * kRow];
+// Many images: the products in tiles of tp_tile.hh, scaled on their way out.
+struct ScaledOut {
+    const float *sa, *sb;  // of the tile's rows (images) and columns (references)
+    const float* bias;
+    void* out;
+    int64_t M, N;
 };
-
-template <int BM, int BN, int WM, int WN, int KW, class O>
-__global__ __launch_bounds__(64 * WM * WN * KW, BM * BN == 128 * 128 ? 4 : 1) void k_rows8_tile(Rows8Args g, uint32_t tm, uint32_t tn) {
-    constexpr int W = WM * WN * KW, FM = BM / WM / 32, FN = BN / WN / 32, NT = 4 / KW;
-    constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // loads of a wavefront for a stage
-    static_assert(LA * W * 8 == BM && LB * W * 8 == BN, "whole loads");
-    __shared__ Stage8<BM, BN> stages[2];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, q = lane >> 5;
-    const int kw = wave % KW, wm = wave / KW / WN, wn = wave / KW % WN;
-    // workgroups are dealt to the XCDs in turn: each XCD takes a contiguous run of the items, whose tiles
-    // share rows and columns in its L2
-    const uint32_t items = gridDim.x, x = blockIdx.x & 7, per = items >> 3, more = items & 7;
-    uint32_t item = x * per + min(x, more) + (blockIdx.x >> 3);
-    const uint32_t split = item / (tm * tn);
-    item -= split * tm * tn;
-    // tiles in bands of 4 along M, column by column
-    const uint32_t band = item / (4 * tn), at = item - band * 4 * tn, height = min(4u, tm - band * 4);
-    const int64_t m0 = int64_t(band * 4u + at % height) * BM, n0 = int64_t(at / height) * BN;
-    const int k0 = g.first(split), k1 = g.first(split + 1);
-    const int64_t K = int64_t(g.steps) * kRow;
-
-    uint32_t oa[LA], ob[LB];
-    const int row8 = lane >> 3, place = lane & 7;
-    auto offset = [&](int slot, int F) {  // of a row's place in LDS and this lane's chunk there
-        const int rr = slot & 31, f = (slot >> 5) % F, part = (slot >> 5) / F;
-        return uint32_t(((part * 32 + rr) * F + f) * K) + (place ^ ((rr >> 1) & 7)) * 16;
-    };
+template <class O> struct ScaledEpi {
+    using Args = ScaledOut;
+    template <class S, class T>
+    static __device__ __forceinline__ void run(const Args& g, Acc<T>& acc, uint32_t im, uint32_t in, char* lds) {
+        const Place<T> place(threadIdx.x);
+        const int64_t m0 = int64_t(im) * T::BM, n0 = int64_t(in) * T::BN;
+        float sb[T::FN], off[T::FN];
 #pragma unroll
-    for (int i = 0; i < LA; ++i) oa[i] = offset((wave * LA + i) * 8 + row8, FM);
-#pragma unroll
-    for (int i = 0; i < LB; ++i) ob[i] = offset((wave * LB + i) * 8 + row8, FN);
-    // rows past the end read zeros
-    const auto ga = codes_buffer(g.a + m0 * K, min(int64_t(BM), g.M - m0), K);
-    const auto gb = codes_buffer(g.b + n0 * K, min(int64_t(BN), g.N - n0), K);
-    v16i acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-    auto load = [&](Stage8<BM, BN>& st, int k) {
-        to_lds(ga, oa, k * kRow, st.a + wave * LA * 1024);
-        to_lds(gb, ob, k * kRow, st.b + wave * LB * 1024);
-    };
-    const int key = (r >> 1) & 7;
-    load(stages[0], k0);
-#pragma unroll 1
-    for (int k = k0; k < k1; ++k) {
-        const int cur = (k - k0) & 1;
-        stage_ready();
-        const uint8_t* sa = stages[cur].a + (wm * 32 * FM + r) * kRow;
-        const uint8_t* sb = stages[cur].b + (wn * 32 * FN + r) * kRow;
-        v4i fa[2][FM], fb[2][FN];
-        auto read = [&](int t) {
-            const int c = ((2 * (kw * NT + t) + q) ^ key) * 16;
-#pragma unroll
-            for (int f = 0; f < FM; ++f) fa[t & 1][f] = *reinterpret_cast<const v4i*>(sa + f * 32 * kRow + c);
-#pragma unroll
-            for (int f = 0; f < FN; ++f) fb[t & 1][f] = *reinterpret_cast<const v4i*>(sb + f * 32 * kRow + c);
-        };
-        read(0);
-        if (k + 1 < k1) load(stages[cur ^ 1], k + 1);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (t + 1 < NT) read(t + 1);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[t & 1][i], fb[t & 1][j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < T::FN; ++j) {
+            const int64_t n = n0 + place.col(j);
+            sb[j] = n < g.N ? g.sb[n] : 0.0f;
+            off[j] = g.bias && n < g.N ? g.bias[n] : 0.0f;
         }
-    }
-
-    // a wavefront's share of its part's results: elements e0 .. e0 + EN - 1 of each fragment
-    constexpr int EN = 16 / KW;
-    const int e0 = kw * EN;
-    int sum[FM][FN][EN];
-    if constexpr (KW == 1) {
+        float* sa = reinterpret_cast<float*>(lds + T::NT / 64 * Rows4<T>::kBytes);  // (behind the fragments' rows)
+        static_assert(T::NT / 64 * Rows4<T>::kBytes + T::BM * 4 <= tile_lds<S, T>(), "LDS of the products");
+        for (int i = threadIdx.x; i < T::BM; i += T::NT) sa[i] = m0 + i < g.M ? g.sa[m0 + i] : 0.0f;
+        __syncthreads();
+        const float* mine = sa + place.first();
+        auto* out = static_cast<typename O::Bits*>(g.out);
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < T::FM; ++i) {
+            v16f row[T::FN];
 #pragma unroll
-            for (int j = 0; j < FN; ++j)
+            for (int e = 0; e < 16; ++e)
 #pragma unroll
-                for (int e = 0; e < EN; ++e) sum[i][j][e] = acc[i][j][e];
-    } else {
-        int* room = reinterpret_cast<int*>(stages);
-        static_assert(sizeof(stages) >= size_t(W) * 4096, "a fragment of every wavefront");
-        const int* part = room + (wave - kw) * 1024 + e0 * 64 + lane;
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < 16; ++e) room[wave * 1024 + e * 64 + lane] = acc[i][j][e];
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < EN; ++e) {
-                    int v = part[e * 64];
-#pragma unroll
-                    for (int w = 1; w < KW; ++w) v += part[w * 1024 + e * 64];
-                    sum[i][j][e] = v;
-                }
-            }
-    }
-
-    const int64_t n = n0 + (wn * 32 + r) * FN;
-    const bool whole = n + FN <= g.N;
-    float off[FN], sb[FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const bool there = n + j < g.N;
-        off[j] = g.bias && there ? g.bias[n + j] : 0.0f;
-        sb[j] = there ? g.sb[n + j] : 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int e = 0; e < EN; ++e) {
-            const int at_e = e0 + e;
-            const int64_t m = m0 + (wm * 32 + (at_e / 4) * 8 + q * 4 + at_e % 4) * FM + i;
-            if (m >= g.M) continue;
-            if (g.splits > 1) {
-                int* p = g.part + (int64_t(split) * g.M + m) * g.N + n;
-                if (whole) {
-                    int v[FN];
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) v[j] = sum[i][j][e];
-                    __builtin_memcpy(p, v, sizeof v);
+                for (int j = 0; j < T::FN; ++j)
+                    row[j][e] = scaled(int(__float_as_uint(acc[i][j][e])), mine[place.at(i, e)], sb[j], off[j]);
+            Rows4<T>::run(row, i, lds, [&](int at, int col, float4 v) {
+                const int64_t m = m0 + at, n = n0 + col;
+                if (m >= g.M || n >= g.N) return;
+                const typename O::Bits b[4] = {O::round(v.x), O::round(v.y), O::round(v.z), O::round(v.w)};
+                if (n + 4 <= g.N) {
+                    __builtin_memcpy(out + m * g.N + n, b, sizeof b);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < FN; ++j)
-                        if (n + j < g.N) p[j] = sum[i][j][e];
+                    for (int k = 0; k < 3; ++k)
+                        if (n + k < g.N) out[m * g.N + n + k] = b[k];
                 }
-                continue;
-            }
-            const float sa = g.sa[m];
-            auto* p = static_cast<typename O::Bits*>(g.out) + m * g.N + n;
-            typename O::Bits v[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) v[j] = O::round(scaled(sum[i][j][e], sa, sb[j], off[j]));
-            if (whole) {
-                __builtin_memcpy(p, v, sizeof v);
-            } else {
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    if (n + j < g.N) p[j] = v[j];
-            }
+            });
         }
-}
+    }
+};
 
 // ------------------------------------------------------------------ which kernel
 struct Rows8Plan {
-    int few, tile, splits;  // few: FM of k_rows8_few, or 0; tile: index of kTiles
+    int few, splits;  // FM of k_rows8_few and its ranges, or 0: tiles
 };
-struct TileKind {
-    int bm, bn;
-    double step_us, alone_us;
-};
-constexpr TileKind kTiles[] = {{64, 64, 0.14, 0.40}, {128, 128, 0.45, 0.7}, {256, 256, 1.6, 1.4}};
-constexpr int kCus = 256, kMaxSplits = 16;
-constexpr int64_t kMaxTiles = int64_t(1) << 22;  // (a launch has fewer than 2^32 lanes)
+constexpr int kCus = 256;
 
+// The tiles' plan is that of 16-bit products: their steps are as long, as many bytes go through LDS for as many instructions.
+TilePlan rows8_tiles(int64_t M, int64_t N, int64_t steps) { return tile_plan(TP_BF16, true, M, N, steps * kRow / 2); }
+
+// Up to 16 images: k_rows8_few.  Up to 32 it takes two fragments of images, as long as its workgroups are on the card at once (24 x
+// 1000 x 4224 @@ us, in tiles @@; 24 x 36864 x 4224 @@ and @@).
 Rows8Plan rows8_plan(int64_t M, int64_t N, int64_t steps) {
-    Rows8Plan best{M <= 16 ? 1 : 2, 0, 1};
-    double least = 1e300;
-    if (M == 1) return best;  // (its image is rounded in the same launch)
-    if (M <= 32) {
-        const int64_t groups = (N + 15) / 16;
-        int64_t s = (kCus + groups - 1) / groups;
-        const int64_t most = (steps + kFewWaves * kAhead - 1) / (kFewWaves * kAhead);
-        best.splits = int(s > most ? most : s);
-        if (M <= 16) return best;
-        least = (2.5 + 0.15 * steps) * double((N + 16 * kCus - 1) / (16 * kCus));
-    }
-    for (int t = 0; t < 3; ++t) {
-        const TileKind& kind = kTiles[t];
-        const int64_t tiles = ((M + kind.bm - 1) / kind.bm) * ((N + kind.bn - 1) / kind.bn);
-        if (tiles > kMaxTiles) continue;
-        for (int s = 1; s <= kMaxSplits && s <= steps; ++s) {
-            if (s > 1 && tiles * s > 8 * kCus) break;
-            const double each = double((tiles * s + kCus - 1) / kCus);
-            double us = 2.0 + ((steps + s - 1) / s + 2) * (each * kind.step_us > kind.alone_us ? each * kind.step_us : kind.alone_us);
-            if (s > 1) us += 4.0 + double(M) * N * (8 * s + 4) / 4.5e6;
-            if (us < least) {
-                least = us;
-                best = {0, t, s};
-            }
-        }
-    }
-    return best;
+    Rows8Plan p{M <= 16 ? 1 : 2, 1};
+    if (M == 1) return p;  // (its image is rounded in the same launch)
+    const int64_t groups = (N + 15) / 16;
+    if (M > 32 || (M > 16 && groups > kCus)) return {0, 1};
+    const int64_t wanted = (kCus + groups - 1) / groups, most = (steps + kFewWaves * kAhead - 1) / (kFewWaves * kAhead);
+    p.splits = int(wanted > most ? most : wanted);
+    return p;
 }
 
 template <class O> hipError_t row_scores(const Rows8Args& g, const Rows8Plan& p, hipStream_t s) {
-    if (p.few) {
-        const dim3 grid(unsigned((g.N + 15) / 16), unsigned(p.splits));
-        if (p.few == 1)
-            k_rows8_few<1, O, void><<<grid, 64 * kFewWaves, 0, s>>>(g, OneRow{});
-        else
-            k_rows8_few<2, O, void><<<grid, 64 * kFewWaves, 0, s>>>(g, OneRow{});
-    } else {
-        const TileKind& kind = kTiles[p.tile];
-        const uint32_t tm = uint32_t((g.M + kind.bm - 1) / kind.bm), tn = uint32_t((g.N + kind.bn - 1) / kind.bn);
-        const dim3 grid(tm * tn * p.splits);
-        if (p.tile == 0)
-            k_rows8_tile<64, 64, 1, 1, 4, O><<<grid, 256, 0, s>>>(g, tm, tn);
-        else if (p.tile == 1)
-            k_rows8_tile<128, 128, 2, 2, 2, O><<<grid, 512, 0, s>>>(g, tm, tn);
-        else
-            k_rows8_tile<256, 256, 2, 4, 1, O><<<grid, 512, 0, s>>>(g, tm, tn);
+    if (!p.few) {
+        const int64_t half = int64_t(g.steps) * kRow / 2;  // (pairs of codes)
+        const TilePlan t = rows8_tiles(g.M, g.N, g.steps);
+        const Product product{{g.a, half, half, nullptr, nullptr}, {g.b, half, half, nullptr, nullptr}, g.M, g.N, half, 0, 0,
+                              t.whole, t.splits, reinterpret_cast<float*>(g.part)};
+        return tp::product<I8x2, false, false, ScaledEpi<O>>(product, t, ScaledOut{g.sa, g.sb, g.bias, g.out, g.M, g.N}, s);
     }
+    const dim3 grid(unsigned((g.N + 15) / 16), unsigned(p.splits));
+    if (p.few == 1)
+        k_rows8_few<1, O, void><<<grid, 64 * kFewWaves, 0, s>>>(g, OneRow{});
+    else
+        k_rows8_few<2, O, void><<<grid, 64 * kFewWaves, 0, s>>>(g, OneRow{});
     if (hipError_t e = hipGetLastError()) return e;
     if (p.splits > 1) k_rows8_join<O><<<match_grid((g.M * g.N + 255) / 256), 256, 0, s>>>(g);
     return hipGetLastError();
@@ -454,10 +366,19 @@ template <class S> void quantize(const void* x, int64_t rows, int64_t cols, int6
     auto* c = static_cast<uint8_t*>(codes);
     auto* f = static_cast<float*>(scales);
     const int64_t padded = row_bytes(cols);
-    if (cols <= 2048)
-        k_quantize_rows<S, 1><<<match_grid((rows + 3) / 4), 256, 0, s>>>(p, rows, cols, stride, padded, c, f);
+    // (rows of 512, 4096, 16640 float32 values: 1, 2 and 16 wavefronts a row)
+    if (cols <= 512 * kHeld)
+        k_quantize_rows<S, 1, true><<<match_grid((rows + 3) / 4), 256, 0, s>>>(p, rows, cols, stride, padded, c, f);
+    else if (cols <= 1024 * kHeld)
+        k_quantize_rows<S, 2, true><<<match_grid((rows + 1) / 2), 256, 0, s>>>(p, rows, cols, stride, padded, c, f);
+    else if (cols <= 2048 * kHeld)
+        k_quantize_rows<S, 4, true><<<match_grid(rows), 256, 0, s>>>(p, rows, cols, stride, padded, c, f);
+    else if (cols <= 4096 * kHeld)
+        k_quantize_rows<S, 8, true><<<match_grid(rows), 512, 0, s>>>(p, rows, cols, stride, padded, c, f);
+    else if (cols <= 8192 * kHeld)
+        k_quantize_rows<S, 16, true><<<match_grid(rows), 1024, 0, s>>>(p, rows, cols, stride, padded, c, f);
     else
-        k_quantize_rows<S, 4><<<match_grid(rows), 256, 0, s>>>(p, rows, cols, stride, padded, c, f);
+        k_quantize_rows<S, 16, false><<<match_grid(rows), 1024, 0, s>>>(p, rows, cols, stride, padded, c, f);
 }
 
 // One image is rounded by the product's own kernel where its codes fit LDS beside others.
@@ -479,6 +400,7 @@ hipError_t launch_quantize_rows(int dt, const void* x, int64_t rows, int64_t col
 
 int64_t row_scores_work(int64_t M, int64_t N, int64_t bytes) {
     const Rows8Plan p = rows8_plan(M, N, bytes / kRow);
+    if (!p.few) return tile_part_bytes(TP_BF16, rows8_tiles(M, N, bytes / kRow), M, N);
     return p.splits > 1 ? up16(p.splits * M * N * int64_t(sizeof(int))) : 0;
 }
 

@@ -13,6 +13,7 @@
 
 #include "tp_match.hh"
 #include "tp_stage.hh"
+#include "tp_tile_plan.hh"
 
 namespace tp {
 
@@ -20,27 +21,44 @@ using v8bf = __attribute__((ext_vector_type(8))) __bf16;
 using v8h = __attribute__((ext_vector_type(8))) _Float16;
 using v16f = __attribute__((ext_vector_type(16))) float;
 using v4s = __attribute__((ext_vector_type(4))) short;
+using v4i = __attribute__((ext_vector_type(4))) int;
+using v16i = __attribute__((ext_vector_type(16))) int;
 using v4u = __attribute__((ext_vector_type(4))) uint32_t;
 using LocalBytes = const __attribute__((address_space(3))) char*;
 using LocalTr = __attribute__((address_space(3))) v4s*;
 
 // How values of a storage type go through the matrix units: in `planes` pieces, `bk` of the contraction at a time
-// (128 bytes of each row in LDS, 192 in three planes).
+// (128 bytes of each row in LDS, 192 in three planes).  whole: the sums are integers, in the bits of the fragments.
 template <class S> struct Units;
+// Pairs of 8-bit integers: laid out like 16-bit values, half as many as there are integers.
+struct I8x2 {
+    using Bits = uint16_t;
+};
+template <> struct Units<I8x2> {
+    static constexpr int planes = 1, bk = 64;
+    static constexpr bool whole = true;
+    static __device__ __forceinline__ v16f mfma(int4 a, int4 b, v16f c) {
+        return __builtin_bit_cast(v16f, __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(v4i, a), __builtin_bit_cast(v4i, b),
+                                                                              __builtin_bit_cast(v16i, c), 0, 0, 0));
+    }
+};
 template <> struct Units<BF16> {
     static constexpr int planes = 1, bk = 64;
+    static constexpr bool whole = false;
     static __device__ __forceinline__ v16f mfma(int4 a, int4 b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
     }
 };
 template <> struct Units<F16> {
     static constexpr int planes = 1, bk = 64;
+    static constexpr bool whole = false;
     static __device__ __forceinline__ v16f mfma(int4 a, int4 b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
     }
 };
 template <> struct Units<F32> {
     static constexpr int planes = 3, bk = 32;
+    static constexpr bool whole = false;
     static __device__ __forceinline__ v16f mfma(int4 a, int4 b, v16f c) { return Units<BF16>::mfma(a, b, c); }
 };
 
@@ -345,10 +363,10 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
     };
     clear(acc);
     // A sum over thousands of products in one go loses what its own size is to each of them: every kFlush of the contraction it is
-    // added to another set of registers and begun anew (where there are registers: not in 16-bit tiles of 256 x 256, nor where
-    // both operands come across, whose sums are gradients of images).  Of 2048
-    // x 8192 float32 pairs of 16640 values log_sum is 4.8e-6 off without and 3.4e-7 with it.
-    constexpr bool kTwo = T::FM * T::FN <= 4 && !(ATR && BTR);
+    // added to another set of registers and begun anew (for scores, whose differences count, and where there are registers: not in
+    // 16-bit tiles of 256 x 256).  Of 2048 x 8192 float32 pairs of 16640 values log_sum is 4.8e-6 off without and 3.4e-7
+    // with it.
+    constexpr bool kTwo = !Units<S>::whole && T::FM * T::FN <= 4 && !BTR;
     constexpr int kFlush = 512;
     Acc<T> total;
     if constexpr (kTwo) clear(total);
@@ -529,6 +547,10 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
     Epi::template run<S, T>(ea, acc, im, in, lds);
 }
 
+template <class S> __device__ __forceinline__ float plus(float a, float b) {
+    return Units<S>::whole ? __uint_as_float(__float_as_uint(a) + __float_as_uint(b)) : a + b;
+}
+
 // The ranges' fragments added up, then the epilogue.
 template <class S, class T, class Epi>
 __global__ __launch_bounds__(T::NT) void k_tile_join(Product g, typename Epi::Args ea) {
@@ -554,10 +576,10 @@ __global__ __launch_bounds__(T::NT) void k_tile_join(Product g, typename Epi::Ar
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     const float4 v = *reinterpret_cast<const float4*>(p + ((i * T::FN + j) * 4 + e / 4) * (T::NT * 4));
-                    acc[i][j][e] += v.x;
-                    acc[i][j][e + 1] += v.y;
-                    acc[i][j][e + 2] += v.z;
-                    acc[i][j][e + 3] += v.w;
+                    acc[i][j][e] = plus<S>(acc[i][j][e], v.x);
+                    acc[i][j][e + 1] = plus<S>(acc[i][j][e + 1], v.y);
+                    acc[i][j][e + 2] = plus<S>(acc[i][j][e + 2], v.z);
+                    acc[i][j][e + 3] = plus<S>(acc[i][j][e + 3], v.w);
                 }
     }
     Epi::template run<S, T>(ea, acc, im, in, lds);
@@ -586,5 +608,56 @@ template <class T> struct Rows4 {
         __builtin_amdgcn_sched_barrier(0);  // (rows of fragments one after the other: registers)
     }
 };
+
+template <class S> struct Shapes {
+    using Small = TileShape<64, 64, 2, 2>;
+    using Middle = TileShape<128, 128, 2, 4>;
+    using Large = TileShape<256, 256, 2, 4, true>;  // (straight to LDS only: there are no registers for what is on its way)
+};
+template <> struct Shapes<I8x2> {
+    using Small = TileShape<64, 64, 2, 2>;
+    using Middle = TileShape<128, 128, 2, 4>;
+    using Large = TileShape<256, 256, 2, 4>;  // (4096 x 8192 x 16640: 470 to 490 us, in four stages 505)
+};
+template <> struct Shapes<F32> {  // (three planes of 256 x 128 are 144 KB in two stages)
+    using Small = TileShape<64, 64, 2, 2>;
+    using Middle = TileShape<128, 128, 2, 4>;
+    using Large = TileShape<256, 128, 4, 2>;
+};
+
+// Whether an operand's chunks of eight 16-bit values can go straight to LDS.
+template <bool ACROSS> bool direct(const Operand& o) {
+    return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.ld % 8 == 0 && (ACROSS || o.kdim % 8 == 0);
+}
+
+template <class S, class T, bool ATR, bool BTR, bool DIRECT, class Epi>
+hipError_t product_of(Product g, const typename Epi::Args& ea, hipStream_t s) {
+    g.tm = uint32_t((g.rows + T::BM - 1) / T::BM);
+    g.tn = uint32_t((g.cols + T::BN - 1) / T::BN);
+    const uint32_t tiles = g.tm * g.tn, rest = tiles > g.whole ? tiles - g.whole : 0;
+    g.whole = tiles - rest;
+    k_tile<S, T, ATR, BTR, DIRECT, Epi><<<dim3(g.whole + rest * g.splits), T::NT, 0, s>>>(g, ea);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (rest && g.splits > 1) k_tile_join<S, T, Epi><<<dim3(rest), T::NT, 0, s>>>(g, ea);
+    return hipGetLastError();
+}
+template <class S, bool ATR, bool BTR, class Epi>
+hipError_t product(const Product& g, const TilePlan& t, const typename Epi::Args& ea, hipStream_t s) {
+    using Small = typename Shapes<S>::Small;
+    using Middle = typename Shapes<S>::Middle;
+    using Large = typename Shapes<S>::Large;
+    if constexpr (Units<S>::planes == 1) {
+        if (t.direct && direct<ATR>(g.a) && direct<BTR>(g.b)) {
+            if (t.tile == 0) return product_of<S, Small, ATR, BTR, true, Epi>(g, ea, s);
+            if (t.tile == 1) return product_of<S, Middle, ATR, BTR, true, Epi>(g, ea, s);
+            return product_of<S, Large, ATR, BTR, true, Epi>(g, ea, s);
+        }
+    } else if (t.tile == 2) {
+        return product_of<S, Large, ATR, BTR, false, Epi>(g, ea, s);
+    }
+    if (t.tile == 0) return product_of<S, Small, ATR, BTR, false, Epi>(g, ea, s);
+    if (t.tile == 1) return product_of<S, Middle, ATR, BTR, false, Epi>(g, ea, s);
+    return hipErrorInvalidValue;
+}
 
 }  // namespace tp
