@@ -233,30 +233,33 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_pairs_few(PairArgs a, int sp
 __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float* part, int splits, float* scores,
                                                          float* given_out, float* log_sum, float* state) {
     __shared__ ScorePart all[16];
+    __shared__ float z_given;
     const int64_t m = blockIdx.x;
     const int64_t g = a.given ? a.given[m] : -1;
+    const float c = a.c * kLog2e;
     float most = -INFINITY, sum = 0.0f;
-    __shared__ float z_given;
-    if (threadIdx.x == 0) z_given = -INFINITY;
-    __syncthreads();
     constexpr int V = 4;
     for (int64_t n0 = threadIdx.x; n0 < a.N; n0 += 1024 * V) {
-        float z[V];
+        // (all of a step's loads, then what they mean)
+        float add[V], s[V];
+        bool counts[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const int64_t n = n0 + k * 1024;
-            z[k] = -INFINITY;
-            if (n >= a.N || (a.mask && !a.mask[n])) continue;
-            float v = a.bias ? a.bias[n] : 0.0f;
-            if (v == -INFINITY) continue;
-            float s = 0.0f;
-#pragma unroll 4
-            for (int t = 0; t < splits; ++t) s += part[(int64_t(t) * a.M + m) * a.N + n];
-            z[k] = fmaf(s, a.c * kLog2e, v * (a.c * kLog2e));
+            const int64_t n = min(n0 + k * 1024, a.N - 1);
+            add[k] = a.bias ? a.bias[n] : 0.0f;
+            counts[k] = !a.mask || a.mask[n];
+            s[k] = part[m * a.N + n];
         }
-        float here = most;
+#pragma unroll 4
+        for (int t = 1; t < splits; ++t)
 #pragma unroll
-        for (int k = 0; k < V; ++k) here = fmaxf(here, z[k]);
+            for (int k = 0; k < V; ++k) s[k] += part[(int64_t(t) * a.M + m) * a.N + min(n0 + k * 1024, a.N - 1)];
+        float z[V], here = most;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            z[k] = counts[k] && add[k] != -INFINITY && n0 + k * 1024 < a.N ? fmaf(s[k], c, add[k] * c) : -INFINITY;
+            here = fmaxf(here, z[k]);
+        }
         const float base = here == -INFINITY ? 0.0f : here;
         sum *= exp_of(most - base);
         most = here;
@@ -271,14 +274,21 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
                 sum += exp_of(z[k] - base);
         }
     }
+    auto shuffled = [&](int from) {
 #pragma unroll
-    for (int d = 32; d; d >>= 1) join(most, sum, __shfl_xor(most, d), __shfl_xor(sum, d));
+        for (int d = from; d; d >>= 1) {
+            const float most2 = __shfl_xor(most, d), sum2 = __shfl_xor(sum, d);
+            join(most, sum, most2, sum2);
+        }
+    };
+    shuffled(32);
     if ((threadIdx.x & 63) == 0) all[threadIdx.x >> 6] = ScorePart{most, sum};
     __syncthreads();
-    if (threadIdx.x) return;
-#pragma unroll
-    for (int i = 1; i < 16; ++i) join(most, sum, all[i].most, all[i].sum);
-    finish(a, m, most, sum, z_given, given_out, log_sum, state);
+    if (threadIdx.x >= 16) return;
+    most = all[threadIdx.x].most;
+    sum = all[threadIdx.x].sum;
+    shuffled(8);
+    if (threadIdx.x == 0) finish(a, m, most, sum, g >= 0 && g < a.N ? z_given : -INFINITY, given_out, log_sum, state);
 }
 
 // ------------------------------------------------------------------ few images: gradient
