@@ -365,7 +365,7 @@ int tp_row_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, 
  *               wanted; -1 for none (0 is returned), NaN for any other out of range
  *   bias        [reference_rows] fp32, optional; -inf rules the reference out
  *   mask        [reference_rows] bytes, optional, nonzero where allowed; what a
- *               reference that is ruled out by it holds is not used
+ *               reference that is ruled out holds is not used
  * Outputs fp32: given_log_probs [image_rows] (with given), log_sum [image_rows] (of exp(score));
  * state, tp_pair_state() floats that the gradient reads (optional: NULL where none will).
  * An image with no allowed reference has log_sum and log probabilities -inf. */

@@ -42,20 +42,26 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
 // What an image's gradient is made of: G = d score / d(<image, reference> + bias) = a exp(score - most), at_given
 // where the reference is the given one.
 struct PairCoef {
-    float most, a, at_given;  // (most in powers of two, as below)
-    int given;                // -1: none
+    float most, a, at_given;
+    int given;  // -1: none
 };
-// Scores are formed and summed in powers of two: score * log2 e, so that a product and a sum become one multiply-add and
-// the exponential one instruction.
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
+#ifdef __HIPCC__
+// What a bias adds to a score.  The type's lowest value is a bias like another: no temperature makes -inf of it, which would
+// rule its reference out.
+__device__ __forceinline__ float times(float bias, float c) {
+    const float v = bias * c;
+    return v < -3.402823466e38f ? -3.402823466e38f : v;
+}
+#endif
 struct ScorePart {
-    float most, sum;  // of a tile's references: the largest score, and sum 2^(score - most) without the given one
+    float most, sum;  // of a tile's references: the largest score, and sum exp(score - most) without the given one
 };
 struct PairOff {  // what a tile's references add to their scores
     const float* bias;
     const uint8_t* mask;
     int64_t N;
-    float c;  // log2 e over the temperature
+    float c;  // 1 / temperature
 };
 // stats: parts [reference tiles][M] and given_score [M]
 struct StatsOut {
@@ -74,10 +80,11 @@ struct GradOut {
     void* g;
     int64_t ldg;
     float* sums;
-    int* look;  // set to 1 where a reference that the mask rules out made a product that is not finite
+    int* look;  // set to 1 where a reference that is ruled out made a product that is not finite
 };
 // rows x cols times *scale: float32 sums [rows][cols] are added where `before`, and kept where `after`, else out
 struct MatrixOut {
+    PairOff ruled;  // of the rows: zeros where they are ruled out (N 0: none is)
     const float* scale;
     int64_t rows, cols;
     const float* before;
@@ -92,8 +99,8 @@ template <class S> struct PairProducts {
     // out [n][K] = g x, out [M][K] = g^t r
     static hipError_t d_references(const PairArgs& a, const void* g, int64_t ldg, int64_t n, const TilePlan& t,
                                    const MatrixOut& o, float* part, hipStream_t s);
-    static hipError_t d_images(const PairArgs& a, const void* g, int64_t ldg, const void* r, const uint8_t* mask,
-                               const int* look, int64_t n, const TilePlan& t, const MatrixOut& o, float* part, hipStream_t s);
+    static hipError_t d_images(const PairArgs& a, const void* g, int64_t ldg, const void* r, const PairOff& off,
+                               const int* look, const TilePlan& t, const MatrixOut& o, float* part, hipStream_t s);
 };
 
 }  // namespace tp

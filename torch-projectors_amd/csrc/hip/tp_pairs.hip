@@ -23,9 +23,8 @@ namespace {
 
 constexpr int kStats = 4;  // largest, others, own, and the given reference's score
 
-// (scores in powers of two)
-__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z); }
-// (largest, sum of 2^(z - largest)) of two sets of scores
+__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
+// (largest, sum of exp(z - largest)) of two sets of scores
 __device__ __forceinline__ void join(float& most, float& sum, float most2, float sum2) {
     const float both = fmaxf(most, most2), base = both == -INFINITY ? 0.0f : both;
     sum = sum * exp_of(most - base) + sum2 * exp_of(most2 - base);
@@ -41,10 +40,10 @@ __device__ __forceinline__ void finish(const PairArgs& a, int64_t m, float most,
     const float own = valid ? exp_of(z - base) : 0.0f, total = others + own;
     // (1 + x) - 1 is what logf sees of a sum near one: the others by themselves
     const float log_total = own == 1.0f && others < 0.5f ? log1pf(others) : logf(total);
-    log_sum[m] = fmaf(base, kLn2, log_total);
+    log_sum[m] = base + log_total;
     if (total == 0.0f) log_sum[m] = -INFINITY;
     if (given_out) {
-        float v = own > others ? -log1pf(others / own) : (z - base) * kLn2 - log_total;
+        float v = own > others ? -log1pf(others / own) : (z - base) - log_total;
         if (total == 0.0f) v = -INFINITY;
         given_out[m] = valid ? v : g == -1 ? 0.0f : NAN;
     }
@@ -99,7 +98,6 @@ __device__ __forceinline__ PairCoef coefficients(const PairArgs& a, const float*
 
 // Half precision: G is scaled by a power of two that brings its largest possible value to 2^13 to 2^14 (its normal
 // numbers start at 2^-14: what is 2^-28 of the largest, or more, keeps all bits), and back by scale[0].
-constexpr float kHalfMost = 16384.0f;
 __global__ __launch_bounds__(1024) void k_pairs_coef(PairArgs a, const float* __restrict__ state, const float* d_given,
                                                      const float* d_log_sum, bool half, PairCoef* coef, float* scale, int* look) {
     __shared__ float room[16];
@@ -236,7 +234,6 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
     __shared__ float z_given;
     const int64_t m = blockIdx.x;
     const int64_t g = a.given ? a.given[m] : -1;
-    const float c = a.c * kLog2e;
     float most = -INFINITY, sum = 0.0f;
     constexpr int V = 4;
     for (int64_t n0 = threadIdx.x; n0 < a.N; n0 += 1024 * V) {
@@ -257,7 +254,7 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
         float z[V], here = most;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            z[k] = counts[k] && add[k] != -INFINITY && n0 + k * 1024 < a.N ? fmaf(s[k], c, add[k] * c) : -INFINITY;
+            z[k] = counts[k] && add[k] != -INFINITY && n0 + k * 1024 < a.N ? fmaf(s[k], a.c, times(add[k], a.c)) : -INFINITY;
             here = fmaxf(here, z[k]);
         }
         const float base = here == -INFINITY ? 0.0f : here;
@@ -348,7 +345,7 @@ __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float*
             }
             G[row][m] = v;
         }
-        if (tid < rows) counts[tid] = !a.mask || a.mask[n0 + tid];
+        if (tid < rows) counts[tid] = (!a.mask || a.mask[n0 + tid]) && (!a.bias || a.bias[n0 + tid] != -INFINITY);
         __syncthreads();
         if (blockIdx.x == 0 && d_bias && tid < rows) {
             float v = 0.0f;
@@ -369,7 +366,7 @@ __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float*
             for (int w = 0; w < W; ++w) {
                 const int row = row0 + w;
                 if (row >= rows) break;
-                // (what a reference that the mask rules out holds is not used)
+                // (what a reference that is ruled out holds is not used, and it has no gradient, whatever images hold)
                 const bool use = counts[row];
                 float up[kBackCols] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -384,7 +381,7 @@ __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float*
                 if (!d_r) continue;
                 Bits b[kBackCols];
 #pragma unroll
-                for (int k = 0; k < kBackCols; ++k) b[k] = S::round(up[k]);
+                for (int k = 0; k < kBackCols; ++k) b[k] = S::round(use ? up[k] : 0.0f);
                 if (have == kBackCols) {
                     __builtin_memcpy(o + row * a.K, b, sizeof b);
                 } else {
@@ -550,7 +547,7 @@ hipError_t launch_pair_log_probs(const PairArgs& a, float* given_out, float* log
     auto* given_score = static_cast<float*>(work);
     auto* parts = reinterpret_cast<ScorePart*>(static_cast<char*>(work) + up16(a.M * 4));
     auto* part = reinterpret_cast<float*>(reinterpret_cast<char*>(parts) + up16(tiles * a.M * int64_t(sizeof(ScorePart))));
-    const StatsOut o{{a.bias, a.mask, a.N, a.c * kLog2e}, a.given, a.M, parts, given_score};
+    const StatsOut o{{a.bias, a.mask, a.N, a.c}, a.given, a.M, parts, given_score};
     const hipError_t e = by_type(a.dt, [&](auto S) { return PairProducts<decltype(S)>::stats(a, t, o, part, s); });
     if (e) return e;
     k_pairs_join<<<dim3(unsigned((a.M + 15) / 16)), 256, 0, s>>>(a, parts, int(tiles), given_score, given_out, log_sum, state);
@@ -606,16 +603,16 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
     for (int64_t first = 0; first < a.N; first += b.piece) {
         const int64_t n = a.N - first < b.piece ? a.N - first : b.piece;
         const char* r = static_cast<const char*>(a.r) + first * a.ldr * size;
-        const uint8_t* mask = a.mask ? a.mask + first : nullptr;
-        const GradOut go{{a.bias ? a.bias + first : nullptr, mask, n, a.c * kLog2e}, coef, a.M, first, w + b.g, b.ldg, d_bias ? sums : nullptr, look};
-        const MatrixOut ro{scale, n, a.K, nullptr, nullptr, d_r ? static_cast<char*>(d_r) + first * a.K * size : nullptr, a.K};
-        const MatrixOut xo{scale, a.M, a.K, first ? dx : nullptr, first + n < a.N ? dx : nullptr, d_x, a.K};
+        const PairOff off{a.bias ? a.bias + first : nullptr, a.mask ? a.mask + first : nullptr, n, a.c};
+        const GradOut go{off, coef, a.M, first, w + b.g, b.ldg, d_bias ? sums : nullptr, look};
+        const MatrixOut ro{off, scale, n, a.K, nullptr, nullptr, d_r ? static_cast<char*>(d_r) + first * a.K * size : nullptr, a.K};
+        const MatrixOut xo{{nullptr, nullptr, 0, 0.0f}, scale, a.M, a.K, first ? dx : nullptr, first + n < a.N ? dx : nullptr, d_x, a.K};
         const hipError_t e = by_type(a.dt, [&](auto S) {
             using P = PairProducts<decltype(S)>;
             if (hipError_t f = P::grad(a, r, n, b.grad, go, part, s)) return f;
             if (d_r)
                 if (hipError_t f = P::d_references(a, w + b.g, b.ldg, n, b.refs, ro, part, s)) return f;
-            return d_x ? P::d_images(a, w + b.g, b.ldg, r, mask, look, n, b.images, xo, part, s) : hipSuccess;
+            return d_x ? P::d_images(a, w + b.g, b.ldg, r, off, look, b.images, xo, part, s) : hipSuccess;
         });
         if (e) return e;
         if (d_bias) {

@@ -15,14 +15,18 @@ namespace {
 struct alignas(8) Offset {
     float add, limit;
 };
+__device__ __forceinline__ bool ruled_out(const PairOff& o, int64_t n) {
+    return (o.mask && !o.mask[n]) || (o.bias && o.bias[n] == -INFINITY);
+}
 template <class T> __device__ __forceinline__ void tile_offsets(const PairOff& o, int64_t first, Offset* off) {
     for (int i = threadIdx.x; i < T::BM; i += T::NT) {
         const int64_t n = first + i;
-        const float b = n < o.N && (!o.mask || o.mask[n]) ? (o.bias ? o.bias[n] : 0.0f) : -INFINITY;
-        off[i] = b == -INFINITY ? Offset{0.0f, -INFINITY} : Offset{b * o.c, INFINITY};
+        const float b = n >= o.N || ruled_out(o, n) ? -INFINITY : o.bias ? o.bias[n] : 0.0f;
+        off[i] = b == -INFINITY ? Offset{0.0f, -INFINITY} : Offset{times(b, o.c), INFINITY};
     }
 }
 __device__ __forceinline__ float score(float sum, const Offset& o, float c) { return fminf(fmaf(sum, c, o.add), o.limit); }
+__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
 __device__ __forceinline__ float base_of(float most) { return most == -INFINITY ? 0.0f : most; }
 
 // A lane holds 16 FM references of each of its FN images: their maximum and sum in registers, then over the two
@@ -76,14 +80,14 @@ struct StatsEpi {
                 if (__builtin_amdgcn_ballot_w64(any) == 0) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        sum[j] += __builtin_amdgcn_exp2f(score(acc[i][j][e], mine[place.at(i, e)], g.off.c) - base[j]);
+                        sum[j] += exp_of(score(acc[i][j][e], mine[place.at(i, e)], g.off.c) - base[j]);
                 } else {  // the given reference's score goes out, and is not among the others
                     float given = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const bool is = here == place.at(0, e);
                         const float z = score(acc[i][j][e], mine[place.at(i, e)], g.off.c);
-                        const float p = __builtin_amdgcn_exp2f(z - base[j]);
+                        const float p = exp_of(z - base[j]);
                         given = is ? z : given;
                         sum[j] += is ? 0.0f : p;
                     }
@@ -105,7 +109,7 @@ struct StatsEpi {
             for (int w = 1; w < T::WM; ++w) {
                 const ScorePart p = part[w * T::BN + i];
                 const float both = fmaxf(all.most, p.most), base = base_of(both);
-                all.sum = all.sum * __builtin_amdgcn_exp2f(all.most - base) + p.sum * __builtin_amdgcn_exp2f(p.most - base);
+                all.sum = all.sum * exp_of(all.most - base) + p.sum * exp_of(p.most - base);
                 all.most = both;
             }
             g.parts[int64_t(im) * g.M + m0 + i] = all;
@@ -153,9 +157,14 @@ struct GradEpi {
         }
         __syncthreads();
         const Offset* mine = off + place.first();
-        // What a reference holds that the mask rules out is not used: a product that is not finite says that it may hold what
-        // a factor of zero would not take out of the images' gradients, which then look at the mask.
-        if (g.off.mask) {
+        // What a reference that is ruled out holds is not used: a product that is not finite says that it may hold what a factor
+        // of zero would not take out of the images' gradients, which then look at who is.
+        bool ruled = false;
+        for (int i = tid & 63; i < T::FM * 32; i += 64) {
+            const int row = place.wm * T::FM * 32 + i;
+            ruled |= n0 + row < g.off.N && off[row].limit == -INFINITY;
+        }
+        if (__builtin_amdgcn_ballot_w64(ruled) != 0) {
             bool bad = false;
 #pragma unroll
             for (int i = 0; i < T::FM; ++i)
@@ -177,7 +186,7 @@ struct GradEpi {
 #pragma unroll
                 for (int j = 0; j < T::FN; ++j) {
                     const float z = score(acc[i][j][e], o, g.off.c);
-                    const float v = a[j] * __builtin_amdgcn_exp2f(z - most[j]);
+                    const float v = a[j] * exp_of(z - most[j]);
                     row[j][e] = z == -INFINITY ? 0.0f : v;  // (a may be NaN)
                 }
             }
@@ -229,6 +238,7 @@ struct MatrixEpi {
                 if (at >= g.rows || c >= g.cols) return;
                 const int n = int(min(g.cols - c, int64_t(4)));
                 float f[4] = {v.x, v.y, v.z, v.w};
+                if (g.ruled.N && ruled_out(g.ruled, at)) f[0] = f[1] = f[2] = f[3] = 0.0f;  // (what images hold does not matter)
                 if (g.before)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -259,25 +269,25 @@ struct MatrixEpi {
 }  // namespace
 
 template <class S> hipError_t PairProducts<S>::stats(const PairArgs& a, const TilePlan& t, const StatsOut& o, float* part, hipStream_t s) {
-    const Product g{{a.r, a.ldr, a.K, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr}, a.N, a.M, a.K, 0, 0, t.whole, t.splits, part};
+    const Product g{{a.r, a.ldr, a.K, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr, nullptr}, a.N, a.M, a.K, 0, 0, t.whole, t.splits, part};
     return product<S, false, false, StatsEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::grad(const PairArgs& a, const void* r, int64_t n, const TilePlan& t, const GradOut& o, float* part, hipStream_t s) {
-    const Product g{{r, a.ldr, a.K, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr}, n, a.M, a.K, 0, 0, t.whole, t.splits, part};
+    const Product g{{r, a.ldr, a.K, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr, nullptr}, n, a.M, a.K, 0, 0, t.whole, t.splits, part};
     return product<S, false, false, GradEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::d_references(const PairArgs& a, const void* gr, int64_t ldg, int64_t n, const TilePlan& t,
                                          const MatrixOut& o, float* part, hipStream_t s) {
     // (g holds zeros from M to ldg: whole chunks)
-    const Product g{{gr, ldg, ldg, nullptr, nullptr}, {a.x, a.ldx, a.M, nullptr, nullptr}, n, a.K, a.M, 0, 0, t.whole, t.splits, part};
+    const Product g{{gr, ldg, ldg, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.M, nullptr, nullptr, nullptr}, n, a.K, a.M, 0, 0, t.whole, t.splits, part};
     return product<S, false, true, MatrixEpi>(g, t, o, s);
 }
 template <class S>
-hipError_t PairProducts<S>::d_images(const PairArgs& a, const void* gr, int64_t ldg, const void* r, const uint8_t* mask,
-                                     const int* look, int64_t n, const TilePlan& t, const MatrixOut& o, float* part, hipStream_t s) {
-    const Product g{{gr, ldg, n, nullptr, nullptr}, {r, a.ldr, n, mask, look}, a.M, a.K, n, 0, 0, t.whole, t.splits, part};
+hipError_t PairProducts<S>::d_images(const PairArgs& a, const void* gr, int64_t ldg, const void* r, const PairOff& off,
+                                     const int* look, const TilePlan& t, const MatrixOut& o, float* part, hipStream_t s) {
+    const Product g{{gr, ldg, off.N, nullptr, nullptr, nullptr}, {r, a.ldr, off.N, look, off.mask, off.bias}, a.M, a.K, off.N, 0, 0, t.whole, t.splits, part};
     return product<S, true, true, MatrixEpi>(g, t, o, s);
 }
 

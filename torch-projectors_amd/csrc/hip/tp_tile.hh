@@ -111,9 +111,11 @@ struct Operand {
     const void* p;
     int64_t ld;           // elements between its rows in memory, at most kMaxStride
     int64_t kdim;         // contraction that there is (zeros count as being there)
-    // (contraction across only) where *look is not 0, rows whose byte is zero count as zeros, whatever they hold; null: none does
-    const uint8_t* keep;
+    // (contraction across only) where *look is not 0, rows whose byte is zero or whose bias is -inf count as zeros, whatever they
+    // hold; each may be null
     const int* look;
+    const uint8_t* keep;
+    const float* bias;
 };
 
 // An operand's part of a tile: DIM rows of D's side by bk of the contraction, CH chunks of eight values a thread.
@@ -131,7 +133,9 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
 
     const char* base;  // the tile's first value at contraction 0
     int64_t ld, dim, kdim;
+    bool looks;
     const uint8_t* keep;
+    const float* bias;
     uint32_t off[CH];  // bytes from base (+ the step) of each chunk
     int tid;
 
@@ -146,7 +150,9 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
     __device__ __forceinline__ void init(const Operand& o, int64_t first, int64_t dim_all, int t) {
         tid = t;
         ld = o.ld;
-        keep = ACROSS && o.keep && *o.look ? o.keep : nullptr;
+        looks = ACROSS && o.look && *o.look;
+        keep = o.keep;
+        bias = o.bias;
         dim = min(dim_all - first, int64_t(DIM));
         kdim = o.kdim;
         base = static_cast<const char*>(o.p) + (ACROSS ? first : first * ld) * int64_t(sizeof(Bits));
@@ -154,8 +160,9 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
         for (int i = 0; i < CH; ++i) {
             const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
             if (DIRECT) {  // (a place in LDS, and the chunk that belongs there)
-                const int from = (c ^ swizzle(row)) * 8;
-                off[i] = (uint32_t(row) * uint32_t(ld) + from) * uint32_t(sizeof(Bits));
+                // (rows past the end read the last one where the contraction is adjacent)
+                const int from = (c ^ swizzle(row)) * 8, at = ACROSS ? row : min(row, int(dim) - 1);
+                off[i] = (uint32_t(at) * uint32_t(ld) + from) * uint32_t(sizeof(Bits));
                 continue;
             }
             // rows and chunks past the end read the last one: what comes of them is not stored
@@ -164,11 +171,14 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
             off[i] = at * uint32_t(sizeof(Bits));
         }
     }
-    // which rows of the step at k0 count (across, with keep: nonzero where the chunk's does)
+    // which rows of the step at k0 count (where it looks: nonzero where the chunk's does)
     __device__ __forceinline__ void look(int64_t k0, uint32_t (&kept)[CH]) const {
-        if (ACROSS && keep) {
+        if (looks) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) kept[i] = keep[min(k0 + row_of(i * NT + tid), kdim - 1)];
+            for (int i = 0; i < CH; ++i) {
+                const int64_t k = min(k0 + row_of(i * NT + tid), kdim - 1);
+                kept[i] = (!keep || keep[k]) && (!bias || bias[k] != -INFINITY);
+            }
         }
     }
     // The step at k0 straight to LDS; what lies outside the operand arrives as zeros, and so do rows that do not count.
@@ -191,7 +201,7 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
             const int slot = i * NT + tid;
             o[i] = ACROSS || (chunk_of(slot) ^ swizzle(row_of(slot))) * 8 < left ? off[i] : kNowhere;
         }
-        if (ACROSS && keep) {
+        if (looks) {
             uint32_t kept[CH];
             look(k0, kept);
 #pragma unroll
@@ -214,7 +224,8 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
     // ends inside the operand.
     __device__ __forceinline__ int64_t whole() const {
         const int64_t past = ACROSS ? -dim & 7 : 0;  // values that a row's last chunk reads of the next rows
-        return max(kdim - (past ? (past + ld - 1) / max(ld, int64_t(1)) : 0), int64_t(0)) / BK * BK;
+        if (past && ld == 0) return 0;               // (there are none)
+        return max(kdim - (past ? (past + ld - 1) / ld : 0), int64_t(0)) / BK * BK;
     }
     using Regs = Eight<S>[CH];
     __device__ __forceinline__ void load(int64_t k0, Regs& reg, uint32_t (&kept)[CH]) const {
@@ -244,7 +255,7 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
             const int slot = i * NT + tid, row = row_of(slot), c = chunk_of(slot);
             int4 v[PL];
             reg[i].planes(v);
-            if (ACROSS && keep && !kept[i]) {
+            if (looks && !kept[i]) {
 #pragma unroll
                 for (int p = 0; p < PL; ++p) v[p] = int4{0, 0, 0, 0};
             }

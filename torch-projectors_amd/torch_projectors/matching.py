@@ -161,7 +161,7 @@ def pair_log_probs(images: torch.Tensor, references: torch.Tensor, given: Option
     given   int64 [M]: -1 for none (its result is 0 and has no gradient); any other index out of range gives NaN, and a
             NaN gradient of its image unless its upstream gradient is 0
     bias    float32 [N]; -inf rules a reference out, as the mask does
-    mask    bool [N], True where allowed; what a reference that is ruled out by it holds is not used
+    mask    bool [N], True where allowed; what a reference that is ruled out holds is not used, and it has no gradient
 
     An image with no allowed reference has log_sum and log probabilities -inf and no gradient.  Values that are not
     finite among the allowed make scores that are not, which make their image's results NaN, but for scores of -inf
