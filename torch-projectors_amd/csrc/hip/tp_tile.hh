@@ -581,7 +581,7 @@ __global__ __launch_bounds__(T::NT) void k_tile_join(Product g, typename Epi::Ar
     for (int s = 0; s < g.splits; ++s) {
         const float* p = g.part + (int64_t(s) * gridDim.x + item) * (T::BM * T::BN) + threadIdx.x * 4;
 #pragma unroll
-        for (int i = 0; i < T::FM; ++i)
+        for (int i = 0; i < T::FM; ++i) {
 #pragma unroll
             for (int j = 0; j < T::FN; ++j)
 #pragma unroll
@@ -592,6 +592,8 @@ __global__ __launch_bounds__(T::NT) void k_tile_join(Product g, typename Epi::Ar
                     acc[i][j][e + 2] = plus<S>(acc[i][j][e + 2], v.z);
                     acc[i][j][e + 3] = plus<S>(acc[i][j][e + 3], v.w);
                 }
+            if (kUnroll == 1 && i % 2) __builtin_amdgcn_sched_barrier(0);
+        }
     }
     Epi::template run<S, T>(ea, acc, im, in, lds);
 }
