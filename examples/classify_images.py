@@ -8,7 +8,7 @@ The steps between the projection operators, as a user runs them:
   sort         images by the classes of their best hypotheses      matching.sort_by_class, dispatch
   backproject  each class's images, weighted by their posterior    backproject_2d_to_3d_forw, reconstruct
   expect       each class's projections back in image order        project_3d_to_2d_forw, matching.combine
-  refine       the volumes by the gradient of the likelihood       matching.log_probs(...).log_sum
+  refine       the volumes by the gradient of the likelihood       matching.pair_log_probs
 
 Run on a GPU: python examples/classify_images.py [--box 32] [--images 512] [--poses 64] [--classes 3]
 """
@@ -103,13 +103,12 @@ def run(box=32, images=512, poses=64, classes=3, noise=1.0, seed=0, device="cuda
     residual = data - matching.combine(expected, order, weights / weights.sum(1, keepdim=True)) * w
     result["noise_power"] = residual.abs().square().mean().item() / 2
 
-    # one step up the marginal likelihood from blurred volumes
+    # one step up the marginal likelihood from blurred volumes, without the scores in memory
     volumes = (0.8 * truth).requires_grad_()
-    real_data = torch.view_as_real(data).reshape(images, -1)
 
     def likelihood(v):
-        r = torch.view_as_real(projections(v, rot, n) * w).reshape(classes * poses, -1)
-        return matching.log_probs(real_data @ r.t() - 0.5 * r.square().sum(1)).log_sum.mean()
+        r = (projections(v, rot, n) * w).flatten(0, 1)
+        return matching.pair_log_probs(data, r, bias=-0.5 * r.abs().square().sum((1, 2))).log_sum.mean()
 
     before = likelihood(volumes)
     (slope,) = torch.autograd.grad(before, volumes)

@@ -294,6 +294,12 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
 // written.
 constexpr int kBackCols = 4, kBackRows = 64;
 
+// Four values as one access, at any address that a value may have.
+template <class B> struct Streamed {
+    using Any = B __attribute__((ext_vector_type(kBackCols)));
+    using At = B __attribute__((ext_vector_type(kBackCols), aligned(sizeof(B))));
+};
+
 template <class S, int MB>
 __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float* __restrict__ state, const float* d_given,
                                                         const float* d_log_sum, int64_t per, float* __restrict__ dx_part,
@@ -383,7 +389,8 @@ __global__ __launch_bounds__(256) void k_pairs_few_back(PairArgs a, const float*
 #pragma unroll
                 for (int k = 0; k < kBackCols; ++k) b[k] = S::round(use ? up[k] : 0.0f);
                 if (have == kBackCols) {
-                    __builtin_memcpy(o + row * a.K, b, sizeof b);
+                    using At = typename Streamed<Bits>::At;
+                    __builtin_nontemporal_store(__builtin_bit_cast(typename Streamed<Bits>::Any, b), reinterpret_cast<At*>(o + row * a.K));
                 } else {
 #pragma unroll
                     for (int k = 0; k < kBackCols; ++k)
@@ -533,11 +540,11 @@ hipError_t launch_pair_log_probs(const PairArgs& a, float* given_out, float* log
         const int splits = few_splits(a.dt, a.N, a.K);
         auto* part = static_cast<float*>(work);
         const dim3 grid(unsigned((a.N + 15) / 16), unsigned(splits));
-        by_type(a.dt, [&](auto S) {
+        const hipError_t e = by_type(a.dt, [&](auto S) {
             k_pairs_few<decltype(S)><<<grid, 64 * kFewWaves, 0, s>>>(a, splits, part);
-            return hipSuccess;
+            return hipGetLastError();
         });
-        if (hipError_t e = hipGetLastError()) return e;
+        if (e) return e;
         k_pairs_few_join<<<dim3(unsigned(a.M)), 1024, 0, s>>>(a, part, splits, state ? state + a.M * kStats : nullptr,
                                                              given_out, log_sum, state);
         return hipGetLastError();
@@ -575,7 +582,7 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
         const int ranges = int((a.N + per - 1) / per);
         auto* part = d_x ? static_cast<float*>(work) : nullptr;
         const dim3 grid(unsigned((a.K + 256 * kBackCols - 1) / (256 * kBackCols)), unsigned(ranges));
-        by_type(a.dt, [&](auto S) {
+        return by_type(a.dt, [&](auto S) {
             using T = decltype(S);
             if (a.M == 1)
                 k_pairs_few_back<T, 1><<<grid, 256, 0, s>>>(a, state, d_given, d_log_sum, per, part, d_r, d_bias);
@@ -584,9 +591,8 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
             else
                 k_pairs_few_back<T, 8><<<grid, 256, 0, s>>>(a, state, d_given, d_log_sum, per, part, d_r, d_bias);
             if (d_x) k_pairs_sum<T><<<match_grid((a.M * a.K + 255) / 256), 256, 0, s>>>(part, ranges, a.M * a.K, d_x);
-            return hipSuccess;
+            return hipGetLastError();
         });
-        return hipGetLastError();
     }
     const BackLayout b = back_layout(a.dt, pair_direct(a), a.M, a.N, a.K, d_x, d_r);
     char* w = static_cast<char*>(work);

@@ -125,7 +125,6 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void k_quantize_rows(const ty
                 if (c < padded) *reinterpret_cast<uint2*>(out + c) = codes8(held[k], scale, inverse);
             }
         } else {
-#pragma unroll 4
             for (int64_t c = 8 * t; c < padded; c += 512 * W) {
                 load8<S>(p + c, cols - c, held[0]);
                 *reinterpret_cast<uint2*>(out + c) = codes8(held[0], scale, inverse);
@@ -331,13 +330,14 @@ constexpr int kCus = 256;
 // The tiles' plan is that of 16-bit products: their steps are as long, as many bytes go through LDS for as many instructions.
 TilePlan rows8_tiles(int64_t M, int64_t N, int64_t steps) { return tile_plan(TP_BF16, true, M, N, steps * kRow / 2); }
 
-// Up to 16 images: k_rows8_few.  Up to 32 it takes two fragments of images, as long as its workgroups are on the card at once (24 x
-// 1000 x 4224 @@ us, in tiles @@; 24 x 36864 x 4224 @@ and @@).
+// One image, and few images of at most 16384 references: k_rows8_few (2 and 16 x 4096 x 16640 14.3 and 18.1 us, in tiles 20; but x 36864
+// x 4224 33 and 44, in tiles 28).  From 17 to 32 images it takes two fragments of them, up to 2048 references (24 x 1000 x 4224 9.0 us, in
+// tiles 10.2; x 4096 x 16640 23.1 and 19.7).
 Rows8Plan rows8_plan(int64_t M, int64_t N, int64_t steps) {
     Rows8Plan p{M <= 16 ? 1 : 2, 1};
     if (M == 1) return p;  // (its image is rounded in the same launch)
     const int64_t groups = (N + 15) / 16;
-    if (M > 32 || (M > 16 && groups > kCus)) return {0, 1};
+    if (M > 32 || groups > (M > 16 ? 128 : 1024)) return {0, 1};
     const int64_t wanted = (kCus + groups - 1) / groups, most = (steps + kFewWaves * kAhead - 1) / (kFewWaves * kAhead);
     p.splits = int(wanted > most ? most : wanted);
     return p;
