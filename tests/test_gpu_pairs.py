@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from tests import own_streams
 from tests import pairs_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -124,6 +125,21 @@ def test_large_tiles(m, M, N, K, dtype):
 def test_references_in_pieces(m, dtype):
     """More references than a piece of the scores' gradient holds (128 MB: 16384 of 16-bit rows of 4096 images)."""
     p = problem(4096, 17000 if dtype == BF16 else 8300, 16, dtype, seed=3)
+    check(m, p)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,N", [(1, 8192), (1, 8193), (3, 12288), (8, 20001)])
+def test_few_images_of_many_references(m, M, N, dtype):
+    """More than 8192 references of few images are joined in steps of 4096: given references in the last one, and steps
+    that allow nothing."""
+    p = problem(M, N, 24, dtype, seed=N)
+    p["given"][0] = N - 1
+    check(m, p)
+    p["mask"][:4096] = False
+    p["mask"][8000:] = False
+    check(m, p)
+    p["mask"][:] = False
     check(m, p)
 
 
@@ -414,7 +430,7 @@ def test_another_stream_and_a_graph(m, M, N, K, dtype):
 
     wanted = [[t.clone() for t in step(p)] for p in states]
     torch.cuda.synchronize()
-    side = torch.cuda.Stream()
+    side = own_streams.stream()
     with torch.cuda.stream(side):
         got = step(states[0])
     side.synchronize()
@@ -436,7 +452,7 @@ def test_two_streams_at_once(m):
     ps = [problem(300, 2000, 520, BF16, seed=s) for s in range(2)]
     wanted = [run(m, p) for p in ps]
     torch.cuda.synchronize()
-    streams = [torch.cuda.Stream() for _ in ps]
+    streams = [own_streams.stream(i) for i in range(len(ps))]
     got = [None, None]
     for _ in range(3):
         for i, s in enumerate(streams):

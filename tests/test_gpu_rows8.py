@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from tests import own_streams
 from tests import pairs_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -197,7 +198,7 @@ def test_another_stream_and_a_graph(m, M):
 
     wanted = [[t.clone() for t in step(s)] for s in states]
     torch.cuda.synchronize()
-    side = torch.cuda.Stream()
+    side = own_streams.stream()
     with torch.cuda.stream(side):
         got = step(states[0])
     side.synchronize()

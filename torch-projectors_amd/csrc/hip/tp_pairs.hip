@@ -226,23 +226,24 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_pairs_few(PairArgs a, int sp
     out[(int64_t(split) * a.M + m) * a.N + n0 + i] = v;
 }
 
-// One image's scores from the ranges' sums, reduced by one workgroup; kept in `scores` (which may be the first range's
-// sums) where the gradient will read them.
+// One image's scores from the ranges' sums, reduced by one workgroup, or by several, each of which leaves a part for
+// k_pairs_join; kept in `scores` where the gradient will read them.
 __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float* part, int splits, float* scores,
-                                                         float* given_out, float* log_sum, float* state) {
+                                                         float* given_out, float* log_sum, float* state, int64_t each,
+                                                         ScorePart* parts, float* given_score) {
     __shared__ ScorePart all[16];
     __shared__ float z_given;
-    const int64_t m = blockIdx.x;
+    const int64_t m = blockIdx.x, first = int64_t(blockIdx.y) * each, end = min(first + each, a.N);
     const int64_t g = a.given ? a.given[m] : -1;
     float most = -INFINITY, sum = 0.0f;
     constexpr int V = 4;
-    for (int64_t n0 = threadIdx.x; n0 < a.N; n0 += 1024 * V) {
+    for (int64_t n0 = first + threadIdx.x; n0 < end; n0 += 1024 * V) {
         // (all of a step's loads, then what they mean)
         float add[V], s[V];
         bool counts[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const int64_t n = min(n0 + k * 1024, a.N - 1);
+            const int64_t n = min(n0 + k * 1024, end - 1);
             add[k] = a.bias ? a.bias[n] : 0.0f;
             counts[k] = !a.mask || a.mask[n];
             s[k] = part[m * a.N + n];
@@ -250,11 +251,11 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
 #pragma unroll 4
         for (int t = 1; t < splits; ++t)
 #pragma unroll
-            for (int k = 0; k < V; ++k) s[k] += part[(int64_t(t) * a.M + m) * a.N + min(n0 + k * 1024, a.N - 1)];
+            for (int k = 0; k < V; ++k) s[k] += part[(int64_t(t) * a.M + m) * a.N + min(n0 + k * 1024, end - 1)];
         float z[V], here = most;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            z[k] = counts[k] && add[k] != -INFINITY && n0 + k * 1024 < a.N ? fmaf(s[k], a.c, times(add[k], a.c)) : -INFINITY;
+            z[k] = counts[k] && add[k] != -INFINITY && n0 + k * 1024 < end ? fmaf(s[k], a.c, times(add[k], a.c)) : -INFINITY;
             here = fmaxf(here, z[k]);
         }
         const float base = here == -INFINITY ? 0.0f : here;
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int64_t n = n0 + k * 1024;
-            if (n >= a.N) continue;
+            if (n >= end) continue;
             if (scores) scores[m * a.N + n] = z[k];
             if (n == g)
                 z_given = z[k];
@@ -285,7 +286,10 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
     most = all[threadIdx.x].most;
     sum = all[threadIdx.x].sum;
     shuffled(8);
-    if (threadIdx.x == 0) finish(a, m, most, sum, g >= 0 && g < a.N ? z_given : -INFINITY, given_out, log_sum, state);
+    if (threadIdx.x) return;
+    if (!parts) return finish(a, m, most, sum, g >= 0 && g < a.N ? z_given : -INFINITY, given_out, log_sum, state);
+    parts[int64_t(blockIdx.y) * a.M + m] = ScorePart{most, sum};
+    if (g >= first && g < end) given_score[m] = z_given;
 }
 
 // ------------------------------------------------------------------ few images: gradient
@@ -432,6 +436,10 @@ int few_splits(int dt, int64_t N, int64_t K) {
     const int64_t most = (units + kFewWaves * kAhead - 1) / (kFewWaves * kAhead);
     return int(s < 1 ? 1 : s > most ? most : s > 16 ? 16 : s);
 }
+// References that a workgroup joins: all of them up to 8192, which it reads in two steps, and a step's each beyond, whose parts take a
+// launch more (1 x 36864 x 1024 bfloat16 29.5 us, in one workgroup 34.1).
+int64_t few_each(int64_t N) { return N <= 8192 ? N : 4096; }
+int64_t few_parts(int64_t N) { return (N + few_each(N) - 1) / few_each(N); }
 // References of a range of the gradient.
 int64_t few_per(int64_t N, int64_t K) {
     const int64_t blocks = (K + 256 * kBackCols - 1) / (256 * kBackCols);
@@ -522,7 +530,7 @@ template <class F> int64_t either_plan(int dt, int64_t K, F bytes) {
 }
 int64_t pair_work(int dt, int64_t M, int64_t N, int64_t K) {
     if (M == 0 || N == 0) return 0;
-    if (pair_few(M)) return up16(few_splits(dt, N, K) * M * N * 4);
+    if (pair_few(M)) return up16(few_splits(dt, N, K) * M * N * 4) + up16(few_parts(N) * M * int64_t(sizeof(ScorePart))) + up16(M * 4);
     return either_plan(dt, K, [&](bool direct) {
         const TilePlan t = tile_plan(dt, direct, N, M, K);
         return up16(M * 4) + up16(tile_count(dt, t, N, true) * M * int64_t(sizeof(ScorePart))) + tile_part_bytes(dt, t, N, M);
@@ -545,8 +553,13 @@ hipError_t launch_pair_log_probs(const PairArgs& a, float* given_out, float* log
             return hipGetLastError();
         });
         if (e) return e;
-        k_pairs_few_join<<<dim3(unsigned(a.M)), 1024, 0, s>>>(a, part, splits, state ? state + a.M * kStats : nullptr,
-                                                             given_out, log_sum, state);
+        const int64_t n = few_parts(a.N);
+        auto* parts = reinterpret_cast<ScorePart*>(static_cast<char*>(work) + up16(int64_t(splits) * a.M * a.N * 4));
+        auto* given_score = reinterpret_cast<float*>(reinterpret_cast<char*>(parts) + up16(n * a.M * int64_t(sizeof(ScorePart))));
+        k_pairs_few_join<<<dim3(unsigned(a.M), unsigned(n)), 1024, 0, s>>>(a, part, splits, state ? state + a.M * kStats : nullptr, given_out,
+                                                                          log_sum, state, few_each(a.N), n > 1 ? parts : nullptr, given_score);
+        if (hipError_t f = hipGetLastError()) return f;
+        if (n > 1) k_pairs_join<<<dim3(1), 256, 0, s>>>(a, parts, int(n), given_score, given_out, log_sum, state);
         return hipGetLastError();
     }
     const TilePlan t = tile_plan(a.dt, pair_direct(a), a.N, a.M, a.K);

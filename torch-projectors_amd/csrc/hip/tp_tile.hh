@@ -1,4 +1,4 @@
-// Tiled matrix products of the pair log probabilities: operands staged in LDS, multiplied by the matrix units, and
+// Tiled matrix products of the pair log probabilities and of the scores in 8-bit integers: operands staged in LDS, multiplied by the matrix units, and
 // handed as fragments to an epilogue.
 //
 //   D[i, j] = sum over k of A(i, k) B(j, k)
@@ -12,7 +12,6 @@
 #pragma once
 
 #include "tp_match.hh"
-#include "tp_stage.hh"
 #include "tp_tile_plan.hh"
 
 namespace tp {
