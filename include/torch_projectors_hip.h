@@ -343,7 +343,7 @@ int tp_quantize_rows(int dtype, const void* x, int64_t rows, int64_t cols, int64
 /* scores[m, n] = (sum of codes_a[m] codes_b[n]) * scales_a[m] * scales_b[n] +
  * bias[n], both sides as tp_quantize_rows leaves rows of `cols` values, the sum
  * exact (codes from -127 to 127), the rest in fp32 (bias fp32, optional; scores
- * TP_F32 or TP_BF16; at most 2^26 rows on either side and 2^38 scores). */
+ * TP_F32 or TP_BF16; at most 2^26 rows on either side and 2^37 scores). */
 int64_t tp_row_scores_work(int64_t rows_a, int64_t rows_b, int64_t cols);
 int tp_row_scores(const void* codes_a, const void* scales_a, int64_t rows_a, const void* codes_b,
                   const void* scales_b, int64_t rows_b, int64_t cols, const void* bias, int out_dtype, void* scores,
@@ -360,7 +360,7 @@ int tp_row_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, 
  * allowed references of (<image, reference> + bias) / temperature.
  *   images      [image_rows, cols], references [reference_rows, cols] of `dtype`
  *               (TP_F32, TP_F16 or TP_BF16), rows a stride apart (0 to 2^21), values of
- *               a row adjacent; at most 2^26 rows each, 2^38 pairs, 2^21 cols
+ *               a row adjacent; at most 2^26 rows each, 2^35 pairs, 2^21 cols
  *   given       [image_rows] int64, optional: the reference whose log probability is
  *               wanted; -1 for none (0 is returned), NaN for any other out of range
  *   bias        [reference_rows] fp32, optional; -inf rules the reference out

@@ -56,7 +56,7 @@ PAIRS = dict(dt=0, x=A, M=20, K=30, sx=30, r=A, N=40, sr=30, given=NULL, bias=NU
 BACK = dict(dt=0, x=A, M=20, K=30, sx=30, r=A, N=40, sr=30, given=NULL, bias=NULL, mask=NULL, temp=1.0, st=A, dg=NULL, dl=A, dx=A, dr=A,
             db=A, work=A, bytes=1 << 40, stream=NULL)
 ROWS = [(dict(dt=1), "dtype"), (dict(M=-1), "non-negative"), (dict(N=-1), "non-negative"), (dict(M=1 << 27), "2^26"), (dict(N=(1 << 26) + 1), "2^26"),
-        (dict(M=1 << 20, N=1 << 19), "2^38"), (dict(K=0), "cols"), (dict(K=(1 << 21) + 1), "cols"), (dict(sx=-1), "strides"),
+        (dict(M=1 << 18, N=(1 << 17) + 1), "2^35"), (dict(K=0), "cols"), (dict(K=(1 << 21) + 1), "cols"), (dict(sx=-1), "strides"),
         (dict(sr=(1 << 21) + 1), "strides"), (dict(temp=0.0), "temperature"), (dict(temp=math.nan), "temperature"), (dict(temp=1e-40), "temperature"),
         (dict(x=NULL), "images"), (dict(r=NULL), "references"), (dict(work=NULL), "work must not be NULL"), (dict(bytes=15), "work is smaller"),
         (dict(work=ODD), "work must be 16-byte aligned"), (dict(st=ODD), "state must be 16-byte aligned")]
@@ -67,7 +67,7 @@ ROWS = [(dict(dt=1), "dtype"), (dict(M=-1), "non-negative"), (dict(N=-1), "non-n
         (dict(dt=1), "dtype"), (dict(rows=-1), "rows"), (dict(cols=0), "cols"), (dict(cols=(1 << 17) + 1), "2^17"), (dict(stride=-1), "row_stride"),
         (dict(x=NULL), "x"), (dict(codes=NULL), "codes"), (dict(scales=NULL), "scales"), (dict(codes=ODD), "codes must be 16-byte aligned")]),
     ("tp_row_scores", SCORES, [
-        (dict(odt=3), "out_dtype"), (dict(M=-1), "non-negative"), (dict(N=1 << 27), "2^26"), (dict(M=1 << 20, N=1 << 20), "2^38"), (dict(cols=0), "cols"),
+        (dict(odt=3), "out_dtype"), (dict(M=-1), "non-negative"), (dict(N=1 << 27), "2^26"), (dict(M=1 << 20, N=(1 << 17) + 1), "2^37"), (dict(cols=0), "cols"),
         (dict(cols=(1 << 17) + 1), "2^17"), (dict(a=NULL), "codes_a"), (dict(sa=NULL), "scales_a"), (dict(b=NULL), "codes_b"), (dict(sb=NULL), "scales_b"),
         (dict(out=NULL), "scores"), (dict(a=ODD), "codes_a must be 16-byte"), (dict(b=ODD), "codes_b must be 16-byte"), (dict(work=ODD), "work must be 16-byte")]),
     ("tp_row_score_images", IMAGES, [

@@ -1081,7 +1081,7 @@ int pair_args(int dtype, const void* images, int64_t image_rows, int64_t cols, i
     TP_TRY(match_dtype(dtype));
     if (image_rows < 0 || reference_rows < 0) return fail("row counts must be non-negative");
     if (image_rows > tp::kMaxPairRows || reference_rows > tp::kMaxPairRows) return fail("row counts must be at most 2^26");
-    if (image_rows * reference_rows > tp::kMaxPairs) return fail("there must be at most 2^38 pairs");
+    if (image_rows * reference_rows > tp::kMaxPairs) return fail("there must be at most 2^35 pairs");
     if (cols < 1 || cols > tp::kMaxStride) return fail("cols must be in [1, 2^21]");
     if (image_stride < 0 || reference_stride < 0 || image_stride > tp::kMaxStride || reference_stride > tp::kMaxStride)
         return fail("row strides must be in [0, 2^21]");
@@ -1505,7 +1505,7 @@ int tp_row_scores(const void* codes_a, const void* scales_a, int64_t rows_a, con
     if (out_dtype != TP_F32 && out_dtype != TP_BF16) return fail("out_dtype must be TP_F32 or TP_BF16");
     if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
     if (rows_a > tp::kMaxScoreRows || rows_b > tp::kMaxScoreRows) return fail("row counts must be at most 2^26");
-    if (rows_a * rows_b > tp::kMaxPairs) return fail("there must be at most 2^38 scores");
+    if (rows_a * rows_b > tp::kMaxRowScores) return fail("there must be at most 2^37 scores");
     if (cols < 1 || cols > tp::kMaxRowValues) return fail("cols must be in [1, 2^17]");
     if (rows_a == 0 || rows_b == 0) return TP_OK;
     TP_TRY(need(codes_a, "codes_a"));
@@ -1538,7 +1538,7 @@ int tp_row_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, 
     if (rows_a < 0 || rows_b < 0) return fail("row counts must be non-negative");
     if (row_stride < 0) return fail("row_stride must be non-negative");
     if (rows_a > tp::kMaxScoreRows || rows_b > tp::kMaxScoreRows) return fail("row counts must be at most 2^26");
-    if (rows_a * rows_b > tp::kMaxPairs) return fail("there must be at most 2^38 scores");
+    if (rows_a * rows_b > tp::kMaxRowScores) return fail("there must be at most 2^37 scores");
     if (cols < 1 || cols > tp::kMaxRowValues) return fail("cols must be in [1, 2^17]");
     if (rows_a == 0 || rows_b == 0) return TP_OK;
     TP_TRY(need(x, "x"));

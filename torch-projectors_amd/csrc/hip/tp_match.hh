@@ -37,6 +37,7 @@ hipError_t launch_score_images(int dt, const void* x, int64_t M, int64_t cols, i
 
 // ------------------------------------------------------------------ 8-bit integers (tp_rows8.hip)
 constexpr int kRowPad = 128;                      // rows of codes are padded with zeros to a multiple of this
+constexpr int64_t kMaxRowScores = int64_t(1) << 37;  // fewer than kMaxTiles tiles of 256 x 256
 constexpr int64_t kMaxRowValues = int64_t(1) << 17;  // of a row: their products' sum stays below 2^31
 
 inline int64_t row_bytes(int64_t cols) { return (cols + kRowPad - 1) / kRowPad * kRowPad; }

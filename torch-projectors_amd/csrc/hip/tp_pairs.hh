@@ -9,7 +9,7 @@ namespace tp {
 
 constexpr int64_t kMaxStride = int64_t(1) << 21;    // elements between rows, and values of a row
 constexpr int64_t kMaxPairRows = int64_t(1) << 26;  // of either side
-constexpr int64_t kMaxPairs = int64_t(1) << 38;     // images times references
+constexpr int64_t kMaxPairs = int64_t(1) << 35;     // images times references: fewer than kMaxTiles tiles of 128 x 128 on both sides
 constexpr int kFewImages = 8;                       // up to here the references are streamed past the images
 
 struct PairArgs {
