@@ -182,7 +182,8 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
     }
     // The step at k0 straight to LDS; what lies outside the operand arrives as zeros, and so do rows that do not count.
     // The loads are written out: behind a builtin the compiler waits for all of them before it reads any transposed fragment, of
-    // whichever stage.  They have no registers to return to; arrive() waits for them.
+    // whichever stage.  They have no registers to return to; arrive() waits for them.  (m0 is reserved: the compiler sets it before each
+    // use of its own)
     __device__ __forceinline__ void fill(int64_t k0, const char* lds) const {
         constexpr uint32_t kNowhere = 0x80000000u;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
