@@ -463,6 +463,56 @@ def test_two_streams_at_once(m):
             assert all(torch.equal(a[k], b[k]) for k in b)
 
 
+@pytest.mark.parametrize("M", [5, 60])
+def test_two_graphs_in_turn(m, M):
+    """Forward and gradient captured twice, with other inputs, and replayed alternately: what each keeps between its kernels is its own."""
+    ps = [problem(M, 700, 264, F32, seed=s) for s in (21, 22)]
+
+    def step(p):
+        x, r, b = (p[k].detach().requires_grad_() for k in ("images", "references", "bias"))
+        out = m.pair_log_probs(x, r, p["given"], bias=b, temperature=p["temperature"], mask=p["mask"])
+        return (out.log_sum.detach(), *torch.autograd.grad((out.given, out.log_sum), (x, r, b), (p["d_given"], p["d_log_sum"])))
+
+    wanted = [[t.clone() for t in step(p)] for p in ps]
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in ps], []
+    for graph, p in zip(graphs, ps):
+        with torch.cuda.graph(graph):
+            outs.append(step(p))
+    for n in (0, 1, 1, 0, 1):
+        for t in outs[n]:
+            t.zero_()
+        graphs[n].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[n], wanted[n])), n
+
+
+@pytest.mark.parametrize("M", [6, 90])
+def test_images_that_are_the_references(m, M):
+    """One tensor on both sides has the gradients of both."""
+    p = problem(M, M, 70, F32, seed=23, bias=False, mask=False, given=False)
+    p["images"] = p["references"]
+    w = want(p)
+    both = p["references"].clone().requires_grad_()
+    (got,) = torch.autograd.grad(m.pair_log_probs(both, both, temperature=p["temperature"]).log_sum, both, p["d_log_sum"])
+    # (their sum is rounded once more)
+    total = w["d_images"] + w["d_references"]
+    near(got, total, w["tol_d_images"] + w["tol_d_references"] + R.U * total.abs(), "both")
+
+
+@pytest.mark.parametrize("M", [2, 20])
+def test_conjugate_rows(m, M):
+    """Conjugates that are only marked as such are what they stand for."""
+    g = gen(24)
+    x = torch.randn(M, 40, dtype=torch.complex64, generator=g, device=DEV)
+    r = torch.randn(70, 40, dtype=torch.complex64, generator=g, device=DEV) * 0.2
+    assert x.conj().is_conj()
+    a = m.pair_log_probs(x.conj(), r.conj())
+    b = m.pair_log_probs(x.conj().resolve_conj(), r.conj().resolve_conj())
+    assert torch.equal(a.log_sum, b.log_sum)
+    assert torch.equal(m.row_scores(x.conj(), m.quantize_rows(r.conj())), m.row_scores(x.conj().resolve_conj(), m.quantize_rows(r.conj().resolve_conj())))
+
+
 # ----------------------------------------------------------------------------- with the other operators
 @pytest.mark.parametrize("M", [6, 40])
 def test_same_as_log_probs_of_the_scores(m, M):
