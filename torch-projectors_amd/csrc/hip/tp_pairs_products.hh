@@ -1,4 +1,10 @@
 // The tiled products of the pair log probabilities for one storage type (included by tp_pairs_*.hip).
+//
+// The matrix units bound them, at some 2.0 GHz under this load.  4096 x 36864 bfloat16 pairs of 4224 values: 1218 us for the scores and
+// their statistics (1.05 PFLOP/s), 1276 formed again for G, 1455 for the references' gradients and 1384 for the images'.
+// 2048 x 8192 float32 pairs of 4224: 709, 715, 788 and 782 us (180 to 200 TFLOP/s of six products each).
+// G is rounded to the rows' type, as a product has both its operands in one; that is of the size of the results' own rounding (bfloat16 gradients
+// 2.3e-3 off, 1.7e-3 with one rounding).
 #pragma once
 
 #include "tp_pairs.hh"
