@@ -1,0 +1,57 @@
+"""Gradients of pair log probabilities of more images than one piece of the scores' gradient holds (32768): pieces of the images
+and of the references, and counts at which a row of all images would pass what the products' offsets reach."""
+import pytest
+import torch
+
+from tests import pairs_plans as P
+from tests import pairs_reference as R
+from tests.test_gpu_pairs import BF16, DEV, F16, F32, NAN, check, gen, m, near, problem, run, want  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(33000, 4200, 16), (40001, 4199, 9), (70000, 40, 24)])
+def test_pieces_of_images(m, M, N, K, dtype):  # noqa: F811
+    b = P.back_layout(P.CODES[str(dtype)], dtype != F32 and K % 8 == 0, M, N, K)
+    assert b.images < M
+    assert b.references < N or N < 1000
+    p = problem(M, N, K, dtype, seed=M)
+    got = check(m, p)
+    # what is ruled out stays out of every piece, whatever it holds
+    p["references"][~p["mask"]] = NAN
+    p["bias"][~p["mask"]] = NAN
+    for k, v in run(m, p).items():
+        assert torch.equal(v, got[k]), k
+
+
+@pytest.mark.parametrize("dtype,M", [(BF16, 20000000), (F16, 9000000), (F32, 5000000)])
+def test_millions_of_images(m, dtype, M):  # noqa: F811
+    """255 rows of 5 million float32 values pass 2^32 bytes, of 9 million 16-bit ones 2^31.
+
+    The terms of a reference's gradient are all positive here, so that what 32 bits lose is relative to the result: scores of
+    at most 20 lose 2 (6 K + 16) 2^-24 20 = 1.6e-4 of a probability, sums of 2^16 products and of 611 pieces 3e-4 at most, the
+    scores' gradient and the result a rounding each."""
+    N, K = 300, 8
+    print(dtype, M, flush=True)
+    g = gen(31)
+    r = (0.3 * torch.randn(N, K, generator=g, device=DEV)).to(dtype).requires_grad_()
+    bias = torch.randn(N, generator=g, device=DEV).requires_grad_()
+    x = (0.5 + torch.rand(M, K, generator=g, device=DEV)).to(dtype).requires_grad_()
+    up = 1e-3 * (0.5 + torch.rand(M, generator=g, device=DEV))
+    out = m.pair_log_probs(x, r, bias=bias)
+    dx, dr, db = torch.autograd.grad(out.log_sum, (x, r, bias), up)
+    x, r, bias = x.detach(), r.detach(), bias.detach()
+    want_r, want_b = torch.zeros(N, K, dtype=torch.float64, device=DEV), torch.zeros(N, dtype=torch.float64, device=DEV)
+    for i in range(0, M, 1 << 20):
+        part = x[i: i + (1 << 20)].double()
+        G = torch.softmax(part @ r.double().t() + bias.double(), 1) * up[i: i + (1 << 20), None].double()
+        want_r += G.t() @ part
+        want_b += G.sum(0)
+    rounding = R.roundoff(dtype) if dtype != F32 else 0.0
+    near(dr, want_r, (5e-4 + 2 * rounding) * want_r, "d_references")
+    near(db, want_b, 5e-4 * want_b, "d_bias")
+    for rows in (slice(0, 500), slice(M // 2 - 250, M // 2 + 250), slice(M - 500, M)):
+        w = R.pair_log_probs(x[rows], r, None, bias, d_log_sum=up[rows])
+        near(out.log_sum[rows], w["log_sum"], w["tol_log_sum"], "log_sum")
+        near(dx[rows], w["d_images"], w["tol_d_images"], "d_images")

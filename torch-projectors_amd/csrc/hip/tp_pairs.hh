@@ -3,14 +3,9 @@
 #pragma once
 
 #include "tp_match.hh"
-#include "tp_tile_plan.hh"
+#include "tp_pairs_plan.hh"
 
 namespace tp {
-
-constexpr int64_t kMaxStride = int64_t(1) << 21;    // elements between rows, and values of a row
-constexpr int64_t kMaxPairRows = int64_t(1) << 26;  // of either side
-constexpr int64_t kMaxPairs = int64_t(1) << 35;     // images times references: fewer than kMaxTiles tiles of 128 x 128 on both sides
-constexpr int kFewImages = 8;                       // up to here the references are streamed past the images
 
 struct PairArgs {
     int dt;  // of images and references (TP_F32, TP_F16, TP_BF16)
@@ -45,6 +40,7 @@ struct PairCoef {
     float most, a, at_given;
     int given;  // -1: none
 };
+static_assert(sizeof(PairCoef) == 16, "the gradient's workspace");
 constexpr float kLog2e = 1.44269504088896340736f;
 #ifdef __HIPCC__
 // What a bias adds to a score.  The type's lowest value is a bias like another: no temperature makes -inf of it, which would

@@ -6,8 +6,8 @@
 //            d_x = G r,  d_r = G^T x,  d_bias = the sums of G over the images
 //
 // Many images: the scores are formed in tiles (tp_tile.hh), a tile's references reduced at once to their largest score and
-// sum per image, and these joined.  The gradient forms the scores again, piece after piece of the references, turns
-// them into G in the products' type, and multiplies it with both sides; a piece's G is all that is kept of M x N.
+// sum per image, and these joined.  The gradient forms the scores again, piece after piece of the references and the images,
+// turns them into G in the products' type, and multiplies it with both sides; a piece's G is all that is kept of M x N.
 // Few images: the references stream past them once, as fast as they can be read; the scores (at most 8 rows) are kept for the
 // gradient, which streams the references and their gradient.
 //
@@ -131,14 +131,15 @@ __global__ __launch_bounds__(1024) void k_pairs_coef(PairArgs a, const float* __
     }
 }
 
-// d_bias of a piece's references from the image tiles' sums.
+// d_bias of a piece's references from the image tiles' sums, those of the images' further pieces on top.
 __global__ __launch_bounds__(256) void k_pairs_bias(const float* __restrict__ sums, int tiles, int64_t n,
-                                                    const float* __restrict__ scale, float* d_bias) {
+                                                    const float* __restrict__ scale, bool more, float* d_bias) {
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
         float v = 0.0f;
 #pragma unroll 4
         for (int t = 0; t < tiles; ++t) v += sums[int64_t(t) * n + i];
-        d_bias[i] = v * scale[0];
+        v *= scale[0];
+        d_bias[i] = more ? d_bias[i] + v : v;
     }
 }
 
@@ -175,7 +176,6 @@ template <class S> __device__ __forceinline__ Pack<S> load_some(const typename S
 // rows), straight from memory into operands: kAhead such units' loads are in flight at once.  Bytes bound it: 4096 references of 16640
 // bfloat16 values take 23 us, 5.9 TB/s.  (A ring of loads that never drains is 4 us slower there, more registers for fewer
 // wavefronts, though 8 us faster for float32, 58 with the join.)
-constexpr int kFewWaves = 8, kAhead = 4, kUnit = 128;
 
 template <class S>
 __global__ __launch_bounds__(64 * kFewWaves) void k_pairs_few(PairArgs a, int splits, float* __restrict__ out) {
@@ -301,7 +301,6 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
 // each reference's row read once, added to the images' gradients in registers (G r) while its own gradient (G^T x) is
 // written.  Bytes bound it: 4096 float32 references of 16640 values and their gradients take about 100 us, 5.3 TB/s read and written (122
 // where the gradient's stores were not streamed past the caches).
-constexpr int kBackCols = 4, kBackRows = 64;
 
 // Four values as one access, at any address that a value may have.
 template <class B> struct Streamed {
@@ -429,77 +428,11 @@ __global__ __launch_bounds__(256) void k_pairs_sum(const float* __restrict__ par
     }
 }
 
-// ------------------------------------------------------------------ plans
-constexpr int kCus = 256;
-int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
-int size_of(int dt) { return dt == TP_F32 ? 4 : 2; }
-
-// Ranges of the rows' values: as many workgroups as hide a load's way.
-int few_splits(int dt, int64_t N, int64_t K) {
-    const int64_t groups = (N + 15) / 16, units = (K * size_of(dt) + kUnit - 1) / kUnit;
-    int64_t s = (2 * kCus + groups - 1) / groups;
-    const int64_t most = (units + kFewWaves * kAhead - 1) / (kFewWaves * kAhead);
-    return int(s < 1 ? 1 : s > most ? most : s > 16 ? 16 : s);
-}
-// References that a workgroup joins: all of them up to 8192, which it reads in two steps, and a step's each beyond, whose parts take a
-// launch more (1 x 36864 x 1024 bfloat16 24 us, in one workgroup 5 us longer).
-int64_t few_each(int64_t N) { return N <= 8192 ? N : 4096; }
-int64_t few_parts(int64_t N) { return (N + few_each(N) - 1) / few_each(N); }
-// References of a range of the gradient.
-int64_t few_per(int64_t N, int64_t K) {
-    const int64_t blocks = (K + 256 * kBackCols - 1) / (256 * kBackCols);
-    int64_t ranges = (4 * kCus + blocks - 1) / blocks;
-    int64_t per = (N + ranges - 1) / ranges;
-    per = (per + 7) / 8 * 8;
-    return per < 16 ? 16 : per;
-}
-
-// A piece's G is at most this large: 128 MB stay in the last cache between the product that writes it and those that read it.
-constexpr int64_t kPieceBytes = int64_t(1) << 27;
-int64_t piece_of(int dt, int64_t M, int64_t N) {
-    const int64_t ld = (M + 7) / 8 * 8;
-    int64_t most = kPieceBytes / (ld * size_of(dt)) / 256 * 256;
-    if (most < 256) most = 256;
-    const int64_t pieces = (N + most - 1) / most;
-    const int64_t each = ((N + pieces - 1) / pieces + 255) / 256 * 256;
-    return each < N ? each : N;
-}
-
+// ------------------------------------------------------------------ launches
 // Whether all products' operands of these images and references go straight to LDS.
 bool pair_direct(const PairArgs& a) {
     auto fits = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
     return a.dt != TP_F32 && a.K % 8 == 0 && fits(a.x, a.ldx) && fits(a.r, a.ldr);
-}
-
-struct BackLayout {
-    int64_t piece, ldg;
-    TilePlan grad, refs, images;
-    int64_t coef, scale, g, sums, part, dx, bytes;
-};
-BackLayout back_layout(int dt, bool direct, int64_t M, int64_t N, int64_t K, bool d_x, bool d_r) {
-    BackLayout b{};
-    b.piece = piece_of(dt, M, N);
-    b.ldg = (M + 7) / 8 * 8;
-    b.grad = tile_plan(dt, direct, b.piece, M, K);
-    b.refs = tile_plan(dt, direct, b.piece, K, M);
-    b.images = tile_plan(dt, direct, M, K, b.piece);
-    int64_t at = 0;
-    auto room = [&](int64_t bytes) {
-        const int64_t here = at;
-        at += up16(bytes);
-        return here;
-    };
-    b.coef = room(M * int64_t(sizeof(PairCoef)));
-    b.scale = room(16);
-    b.g = room(b.piece * b.ldg * size_of(dt));
-    b.sums = room(tile_count(dt, b.grad, M, false) * b.piece * 4);
-    int64_t part = tile_part_bytes(dt, b.grad, b.piece, M);
-    if (d_r) part = part > tile_part_bytes(dt, b.refs, b.piece, K) ? part : tile_part_bytes(dt, b.refs, b.piece, K);
-    if (d_x) part = part > tile_part_bytes(dt, b.images, M, K) ? part : tile_part_bytes(dt, b.images, M, K);
-    b.part = room(part);
-    b.dx = room(d_x && b.piece < N ? M * K * 4 : 0);
-    b.bytes = at;
-    return b;
 }
 
 template <class F> hipError_t by_type(int dt, F f) {
@@ -619,30 +552,39 @@ hipError_t launch_pair_log_probs_back(const PairArgs& a, const float* state, con
     auto* look = reinterpret_cast<int*>(scale + 1);
     auto* sums = reinterpret_cast<float*>(w + b.sums);
     auto* part = reinterpret_cast<float*>(w + b.part);
-    auto* dx = reinterpret_cast<float*>(w + b.dx);
+    auto* dr = reinterpret_cast<float*>(w + b.dr);
     const bool half = a.dt == TP_F16;
     const int64_t blocks = (a.M + 1023) / 1024;
     k_pairs_coef<<<dim3(unsigned(blocks < 64 ? blocks : 64)), 1024, 0, s>>>(a, state, d_given, d_log_sum, half, coef, scale, look);
     if (hipError_t e = hipGetLastError()) return e;
-    for (int64_t first = 0; first < a.N; first += b.piece) {
-        const int64_t n = a.N - first < b.piece ? a.N - first : b.piece;
+    const PairOff none{nullptr, nullptr, 0, 0.0f};
+    for (int64_t first = 0; first < a.N; first += b.references) {
+        const int64_t n = std::min(a.N - first, b.references);
         const char* r = static_cast<const char*>(a.r) + first * a.ldr * size;
         const PairOff off{a.bias ? a.bias + first : nullptr, a.mask ? a.mask + first : nullptr, n, a.c};
-        const GradOut go{off, coef, a.M, first, w + b.g, b.ldg, d_bias ? sums : nullptr, look};
-        const MatrixOut ro{off, scale, n, a.K, nullptr, nullptr, d_r ? static_cast<char*>(d_r) + first * a.K * size : nullptr, a.K};
-        const MatrixOut xo{{nullptr, nullptr, 0, 0.0f}, scale, a.M, a.K, first ? dx : nullptr, first + n < a.N ? dx : nullptr, d_x, a.K};
-        const hipError_t e = by_type(a.dt, [&](auto S) {
-            using P = PairProducts<decltype(S)>;
-            if (hipError_t f = P::grad(a, r, n, b.grad, go, part, s)) return f;
-            if (d_r)
-                if (hipError_t f = P::d_references(a, w + b.g, b.ldg, n, b.refs, ro, part, s)) return f;
-            return d_x ? P::d_images(a, w + b.g, b.ldg, r, off, look, b.images, xo, part, s) : hipSuccess;
-        });
-        if (e) return e;
-        if (d_bias) {
-            k_pairs_bias<<<match_grid((n + 255) / 256), 256, 0, s>>>(sums, int(tile_count(a.dt, b.grad, a.M, false)), n,
-                                                                     scale, d_bias + first);
-            if (hipError_t f = hipGetLastError()) return f;
+        for (int64_t image = 0; image < a.M; image += b.images) {
+            PairArgs p = a;  // (of this piece's images)
+            p.M = std::min(a.M - image, b.images);
+            p.x = static_cast<const char*>(a.x) + image * a.ldx * size;
+            auto* dx = reinterpret_cast<float*>(w + b.dx) + image * a.K;
+            const GradOut go{off, coef + image, p.M, first, w + b.g, b.ldg, d_bias ? sums : nullptr, look};
+            const MatrixOut ro{off, scale, n, a.K, image ? dr : nullptr, image + p.M < a.M ? dr : nullptr,
+                               d_r ? static_cast<char*>(d_r) + first * a.K * size : nullptr, a.K};
+            const MatrixOut xo{none, scale, p.M, a.K, first ? dx : nullptr, first + n < a.N ? dx : nullptr,
+                               d_x ? static_cast<char*>(d_x) + image * a.K * size : nullptr, a.K};
+            const hipError_t e = by_type(a.dt, [&](auto S) {
+                using P = PairProducts<decltype(S)>;
+                if (hipError_t f = P::grad(p, r, n, b.grad, go, part, s)) return f;
+                if (d_r)
+                    if (hipError_t f = P::d_references(p, w + b.g, b.ldg, n, b.refs, ro, part, s)) return f;
+                return d_x ? P::d_images(p, w + b.g, b.ldg, r, off, look, b.imgs, xo, part, s) : hipSuccess;
+            });
+            if (e) return e;
+            if (d_bias) {
+                k_pairs_bias<<<match_grid((n + 255) / 256), 256, 0, s>>>(sums, int(tile_count(a.dt, b.grad, p.M, false)), n,
+                                                                         scale, image != 0, d_bias + first);
+                if (hipError_t f = hipGetLastError()) return f;
+            }
         }
     }
     return hipSuccess;

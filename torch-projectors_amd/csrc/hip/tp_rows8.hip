@@ -328,7 +328,6 @@ template <class O> struct ScaledEpi {
 struct Rows8Plan {
     int few, splits;  // FM of k_rows8_few and its ranges, or 0: tiles
 };
-constexpr int kCus = 256;
 
 // The tiles' plan is that of 16-bit products: their steps are as long, as many bytes go through LDS for as many instructions.
 TilePlan rows8_tiles(int64_t M, int64_t N, int64_t steps) { return tile_plan(TP_BF16, true, M, N, steps * kRow / 2); }

@@ -5,6 +5,8 @@
 
 namespace tp {
 
+constexpr int kCus = 256;
+constexpr int64_t kMaxStride = int64_t(1) << 21;  // elements between an operand's rows, and values of a row
 constexpr int64_t kMaxTiles = int64_t(1) << 22;  // of a product (a launch has fewer than 2^32 lanes)
 
 struct TilePlan {

@@ -8,7 +8,6 @@
 namespace tp {
 namespace {
 
-constexpr int kCus = 256;
 // One step (bk of the contraction) of a tile, and its start and end: among as many as a CU holds, and alone.  Measured on products of
 // 1024 to 16384 along the contraction with every CU at work.
 struct TileKind {

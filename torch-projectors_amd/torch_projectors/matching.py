@@ -168,8 +168,9 @@ def pair_log_probs(images: torch.Tensor, references: torch.Tensor, given: Option
     of float16 and bfloat16 rows, which count as ruled out.
 
     The gradient reaches images, references (in their dtype) and bias from both results.  It forms the scores
-    again, a piece of the references after the other; a piece's share of the gradient of the scores is kept in the
-    rows' dtype (at most 128 MB or 256 references' worth).  Up to 8 images keep their scores instead."""
+    again, for a piece of the references and of the images (32768 at most) after the other; a piece's share of the
+    gradient of the scores is kept in the rows' dtype (at most 128 MB), and sums over several pieces in float32.
+    Up to 8 images keep their scores instead."""
     x, r = _real_rows(images, "images"), _real_rows(references, "references")
     if x.shape[1] != r.shape[1]:
         raise ValueError(f"Images of {x.shape[1]} values do not fit references of {r.shape[1]}")
