@@ -259,7 +259,9 @@ __global__ __launch_bounds__(1024) void k_pairs_few_join(PairArgs a, const float
         float z[V], here = most;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            z[k] = counts[k] && add[k] != -INFINITY && n0 + k * 1024 < end ? fmaf(s[k], a.c, times(add[k], a.c)) : -INFINITY;
+            z[k] = fmaf(s[k], a.c, times(add[k], a.c));
+            if (!(fabsf(z[k]) < INFINITY)) z[k] = NAN;  // (-inf is what is ruled out, and no score)
+            if (!counts[k] || add[k] == -INFINITY || n0 + k * 1024 >= end) z[k] = -INFINITY;
             here = fmaxf(here, z[k]);
         }
         const float base = here == -INFINITY ? 0.0f : here;

@@ -17,7 +17,8 @@ namespace {
 
 // What a reference adds to its scores, in LDS: score = min(sum c + add, limit), where the limit of one that is ruled out
 // is -inf, whatever its sum is (the minimum with a NaN is the other), and that of the others +inf (a NaN becomes
-// +inf, which makes its image's results NaN all the same).
+// +inf, which makes its image's results NaN all the same).  -inf is no score of an allowed reference: max(sum c + add, -limit) is -inf
+// for those that are -inf or NaN, and for no other.
 struct alignas(8) Offset {
     float add, limit;
 };
@@ -32,6 +33,7 @@ template <class T> __device__ __forceinline__ void tile_offsets(const PairOff& o
     }
 }
 __device__ __forceinline__ float score(float sum, const Offset& o, float c) { return fminf(fmaf(sum, c, o.add), o.limit); }
+__device__ __forceinline__ float lowest_of(float sum, const Offset& o, float c) { return fmaxf(fmaf(sum, c, o.add), -o.limit); }
 __device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
 __device__ __forceinline__ float base_of(float most) { return most == -INFINITY ? 0.0f : most; }
 
@@ -47,7 +49,7 @@ struct StatsEpi {
         Offset* off = reinterpret_cast<Offset*>(lds);
         ScorePart* part = reinterpret_cast<ScorePart*>(off + T::BM);  // [WM][BN]
         tile_offsets<T>(g.off, n0, off);
-        float most[T::FN], sum[T::FN];
+        float most[T::FN], least[T::FN], sum[T::FN];
         int at[T::FN];  // the given reference, relative to the lane's first row as at() counts
 #pragma unroll
         for (int j = 0; j < T::FN; ++j) {
@@ -55,6 +57,7 @@ struct StatsEpi {
             const int64_t given = g.given && m < g.M ? g.given[m] : -1;
             at[j] = given >= n0 && given < n0 + T::BM && given < g.off.N ? int(given - n0) - place.first() : -1;
             most[j] = -INFINITY;
+            least[j] = INFINITY;
             sum[j] = 0.0f;
         }
         __syncthreads();
@@ -85,15 +88,20 @@ struct StatsEpi {
                 const bool any = here >= 0 && here < 32 && !(here & 4);
                 if (__builtin_amdgcn_ballot_w64(any) == 0) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        sum[j] += exp_of(score(acc[i][j][e], mine[place.at(i, e)], g.off.c) - base[j]);
+                    for (int e = 0; e < 16; ++e) {
+                        const Offset o = mine[place.at(i, e)];
+                        sum[j] += exp_of(score(acc[i][j][e], o, g.off.c) - base[j]);
+                        least[j] = fminf(least[j], lowest_of(acc[i][j][e], o, g.off.c));
+                    }
                 } else {  // the given reference's score goes out, and is not among the others
                     float given = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const bool is = here == place.at(0, e);
-                        const float z = score(acc[i][j][e], mine[place.at(i, e)], g.off.c);
+                        const Offset o = mine[place.at(i, e)];
+                        const float z = score(acc[i][j][e], o, g.off.c);
                         const float p = exp_of(z - base[j]);
+                        least[j] = fminf(least[j], lowest_of(acc[i][j][e], o, g.off.c));
                         given = is ? z : given;
                         sum[j] += is ? 0.0f : p;
                     }
@@ -104,6 +112,7 @@ struct StatsEpi {
         }
 #pragma unroll
         for (int j = 0; j < T::FN; ++j) {
+            if (least[j] == -INFINITY) sum[j] = NAN;
             sum[j] += __shfl_xor(sum[j], 32);
             if (place.q == 0) part[place.wm * T::BN + place.col(j)] = ScorePart{most[j], sum[j]};
         }
@@ -193,7 +202,7 @@ struct GradEpi {
                 for (int j = 0; j < T::FN; ++j) {
                     const float z = score(acc[i][j][e], o, g.off.c);
                     const float v = a[j] * exp_of(z - most[j]);
-                    row[j][e] = z == -INFINITY ? 0.0f : v;  // (a may be NaN)
+                    row[j][e] = o.limit == -INFINITY ? 0.0f : v;  // (a may be NaN)
                 }
             }
 #pragma unroll

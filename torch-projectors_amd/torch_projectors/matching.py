@@ -163,9 +163,9 @@ def pair_log_probs(images: torch.Tensor, references: torch.Tensor, given: Option
     bias    float32 [N]; -inf rules a reference out, as the mask does
     mask    bool [N], True where allowed; what a reference that is ruled out holds is not used, and it has no gradient
 
-    An image with no allowed reference has log_sum and log probabilities -inf and no gradient.  Values that are not
-    finite among the allowed make scores that are not, which make their image's results NaN, but for scores of -inf
-    of float16 and bfloat16 rows, which count as ruled out.
+    An image with no allowed reference has log_sum and log probabilities -inf and no gradient.  A score of an allowed
+    reference that is not finite, -inf among them (of values that are not finite, or past float32's largest), makes
+    its image's results and gradient NaN, and the gradients of the allowed references and biases.
 
     The gradient reaches images, references (in their dtype) and bias from both results.  It forms the scores
     again, for a piece of the references and of the images (32768 at most) after the other; a piece's share of the
