@@ -82,22 +82,32 @@ __global__ __launch_bounds__(256) void k_pairs_join(PairArgs a, const ScorePart*
 }
 
 // ------------------------------------------------------------------ the gradient's coefficients
+// An image's upstream gradients as they are used.
+struct Upstream {
+    float log_sum, given;
+    int at;  // the given reference, -1: none
+};
+__device__ __forceinline__ Upstream upstream(const PairArgs& a, int64_t m, const float* d_given, const float* d_log_sum) {
+    const int64_t g = a.given ? a.given[m] : -1;
+    const bool valid = g >= 0 && g < a.N;
+    Upstream u{d_log_sum ? d_log_sum[m] : 0.0f, d_given && a.given && g != -1 ? d_given[m] : 0.0f, valid ? int(g) : -1};
+    if (!valid && u.given != 0.0f) u.given = NAN;
+    return u;
+}
 __device__ __forceinline__ PairCoef coefficients(const PairArgs& a, const float* state, int64_t m, const float* d_given,
                                                  const float* d_log_sum) {
     const float* st = state + m * kStats;
     const float others = st[1], own = st[2], total = others + own;
-    const int64_t g = a.given ? a.given[m] : -1;
-    const bool valid = g >= 0 && g < a.N;
-    const float dl = d_log_sum ? d_log_sum[m] : 0.0f;
-    float dg = d_given && a.given && g != -1 ? d_given[m] : 0.0f;
-    if (!valid && dg != 0.0f) dg = NAN;
-    PairCoef k{st[0], a.c * (dl - dg) / total, a.c * (dl * own + dg * others) / total, valid ? int(g) : -1};
+    const Upstream u = upstream(a, m, d_given, d_log_sum);
+    const float dl = u.log_sum, dg = u.given;
+    PairCoef k{st[0], a.c * (dl - dg) / total, a.c * (dl * own + dg * others) / total, u.at};
     if (total == 0.0f) k.a = k.at_given = 0.0f;  // a row that allows nothing
     return k;
 }
 
 // Half precision: G is scaled by a power of two that brings its largest possible value to 2^13 to 2^14 (its normal
-// numbers start at 2^-14: what is 2^-28 of the largest, or more, keeps all bits), and back by scale[0].
+// numbers start at 2^-14: what is 2^-28 of the largest, or more, keeps all bits), and back by scale[0].  Images that have no finite gradient,
+// or none, have no say in it.
 __global__ __launch_bounds__(1024) void k_pairs_coef(PairArgs a, const float* __restrict__ state, const float* d_given,
                                                      const float* d_log_sum, bool half, PairCoef* coef, float* scale, int* look) {
     __shared__ float room[16];
@@ -105,9 +115,9 @@ __global__ __launch_bounds__(1024) void k_pairs_coef(PairArgs a, const float* __
     if (half) {
         float most = 0.0f;
         for (int64_t m = threadIdx.x; m < a.M; m += 1024) {
-            const float dl = d_log_sum ? fabsf(d_log_sum[m]) : 0.0f, dg = d_given ? fabsf(d_given[m]) : 0.0f;
-            const float v = a.c * (dl + dg);
-            if (v < INFINITY) most = fmaxf(most, v);
+            const Upstream u = upstream(a, m, d_given, d_log_sum);
+            const float v = a.c * (fabsf(u.log_sum) + fabsf(u.given)), total = state[m * kStats + 1] + state[m * kStats + 2];
+            if (v < INFINITY && total > 0.0f) most = fmaxf(most, v);
         }
 #pragma unroll
         for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
