@@ -34,8 +34,8 @@ def check(dt, M, N, K):
         pieces = -(-M // b.images) * -(-N // b.references)
         assert pieces <= 1 << 22, where  # (a loop on the host)
         # rows of G as an operand: a tile's 256 rows of either side, or a step's 64, from one base
-        row = b.ldg * SIZES[dt]
-        assert b.ldg <= P.limit(1) and 256 * row + row <= 0x7fffffff, where
+        row = b.ldg * 4  # (of 16 bits in two pieces)
+        assert 2 * b.ldg <= P.limit(1) and 256 * row + row <= 0x7fffffff, where
         assert b.g_bytes <= 1 << 27, where
         for tile in (b.grad, b.refs, b.imgs, P.tile_plan(dt, direct, N, M, K)):
             assert 1 <= tile.tiles <= P.limit(0), where
@@ -76,3 +76,24 @@ def test_small_calls_are_in_one_piece():
     for dt, M, N in ((P.BF16, 4096, 4096), (P.F32, 2048, 8192), (P.F16, 333, 1999)):
         b = P.back_layout(dt, True if dt != P.F32 else False, M, N, 4224)
         assert (b.images, b.references) == (M, N)
+
+
+def forms(sizes, dt):
+    """(product, tile, straight to LDS, in ranges) that calls of these sizes run."""
+    out = set()
+    for M, N, K in sizes:
+        direct = dt != P.F32 and K % 8 == 0
+        b = P.back_layout(dt, direct, M, N, K)
+        for name, t in (("grad", b.grad), ("references", b.refs), ("images", b.imgs), ("scores", P.tile_plan(dt, direct, N, M, K))):
+            out.add((name, t.tile, direct, t.split))
+    return out
+
+
+@pytest.mark.parametrize("dt", [P.F16, P.BF16])
+def test_sizes_of_the_rounding_tests_reach_every_tile(dt):
+    from tests.test_gpu_pairs_rounding import ROUNDED
+    ran = forms(ROUNDED, dt)
+    for name in ("references", "images"):
+        for tile, direct in ((0, True), (1, True), (2, True), (0, False), (1, False)):
+            assert any(f[:3] == (name, tile, direct) for f in ran), (name, tile, direct)
+        assert any(f[0] == name and f[2] and f[3] for f in ran) and any(f[0] == name and not f[2] and f[3] for f in ran), name

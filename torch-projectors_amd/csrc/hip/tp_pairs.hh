@@ -67,8 +67,8 @@ struct StatsOut {
     ScorePart* parts;
     float* given_score;
 };
-// gradient of the scores: g [references][ldg] of the type (rounded; half precision scaled by the coefficients), and the
-// sums over the images [image tiles][N] (or null)
+// gradient of the scores: g [references][pieces][ldg] of the type (half precision scaled by the coefficients; of 16 bits the rounded
+// values, then what rounding left of them, rounded), and the sums over the images [image tiles][N] (or null)
 struct GradOut {
     PairOff off;  // (of this piece's references)
     const PairCoef* coef;

@@ -44,11 +44,14 @@ inline int64_t few_per(int64_t N, int64_t K) {
 // The scores' gradient G is formed for a piece of the references and one of the images at a time.  A piece of G is at most
 // kPieceBytes large (128 MB stay in the last cache between the product that writes it and those that read it), of at
 // most kPieceImages images, whose rows the products' 32-bit offsets and sums of few thousand terms can take, and at least 256 references.
+// 16-bit rows are multiplied with G in two pieces of their type, what the first leaves to the second: four bytes of G either way.
 constexpr int64_t kPieceBytes = int64_t(1) << 27, kPieceImages = int64_t(1) << 15;
+
+inline int g_pieces(int dt) { return dt == TP_F32 ? 1 : 2; }
 
 struct BackLayout {
     int64_t images, references;  // of a piece, at most
-    int64_t ldg;                 // elements between the rows of G, one of each reference
+    int64_t ldg;                 // elements of a row of G (a reference's) or, of 16 bits, of each of its two pieces, the second behind the first
     TilePlan grad, refs, imgs;   // G, the references' gradient, the images'
     // bytes from the workspace's start: coefficients, scale and flag, G, its sums over the images, the split tiles' sums, and sums over
     // the pieces of the images (of a piece's references) and of the references (of all images)
@@ -63,15 +66,15 @@ inline BackLayout back_layout(int dt, bool direct, int64_t M, int64_t N, int64_t
     BackLayout b{};
     b.images = equal_parts(M, kPieceImages);
     b.ldg = up_to(b.images, 8);
-    int64_t most = kPieceBytes / (b.ldg * size_of(dt)) / 256 * 256;
+    int64_t most = kPieceBytes / (b.ldg * 4) / 256 * 256;
     // (tiles of 128 x 128 of a piece's references and their values: 32768 references of the longest rows, as many images as there may be)
     const int64_t fit = kMaxTiles / ((K + 127) / 128) * 128 / 256 * 256;
     if (most > fit) most = fit;
     if (most < 256) most = 256;
     b.references = equal_parts(N, most);
     b.grad = tile_plan(dt, direct, b.references, b.images, K);
-    b.refs = tile_plan(dt, direct, b.references, K, b.images);
-    b.imgs = tile_plan(dt, direct, b.images, K, b.references);
+    b.refs = tile_plan(dt, direct, b.references, K, g_pieces(dt) * b.images);
+    b.imgs = tile_plan(dt, direct, b.images, K, g_pieces(dt) * b.references);
     int64_t at = 0;
     auto room = [&](int64_t bytes) {
         const int64_t here = at;
@@ -80,7 +83,7 @@ inline BackLayout back_layout(int dt, bool direct, int64_t M, int64_t N, int64_t
     };
     b.coef = room(M * 16);
     b.scale = room(16);
-    b.g = room(b.references * b.ldg * size_of(dt));
+    b.g = room(b.references * b.ldg * 4);
     b.sums = room(tile_count(dt, b.grad, b.images, false) * b.references * 4);
     int64_t part = tile_part_bytes(dt, b.grad, b.references, b.images);
     auto also = [&](int64_t bytes) { part = part > bytes ? part : bytes; };

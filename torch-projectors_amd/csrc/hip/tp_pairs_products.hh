@@ -3,8 +3,8 @@
 // The matrix units bound them, at some 2.0 GHz under this load.  4096 x 36864 bfloat16 pairs of 4224 values: 1218 us for the scores and
 // their statistics (1.05 PFLOP/s), 1276 formed again for G, 1455 for the references' gradients and 1384 for the images'.
 // 2048 x 8192 float32 pairs of 4224: 709, 715, 788 and 782 us (180 to 200 TFLOP/s of six products each).
-// G is rounded to the rows' type, as a product has both its operands in one; that is of the size of the results' own rounding (bfloat16 gradients
-// 2.3e-3 off, 1.7e-3 with one rounding).
+// A product has both its operands in one type: G goes through 16-bit units in two pieces, what rounding it leaves being the second.  With the first alone
+// bfloat16 gradients are 2.3e-3 off, and 1.7e-3 with both, which is their own rounding.
 #pragma once
 
 #include "tp_pairs.hh"
@@ -41,6 +41,7 @@ __device__ __forceinline__ float base_of(float most) { return most == -INFINITY 
 // halves of the wavefront and the WM wavefronts.
 struct StatsEpi {
     using Args = StatsOut;
+    template <class S> static constexpr bool kTwice = false;
     template <class S, class T>
     static __device__ __forceinline__ void run(const Args& g, Acc<T>& acc, uint32_t im, uint32_t in, char* lds) {
         const int tid = threadIdx.x;
@@ -145,8 +146,16 @@ template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+// Pieces of G (as g_pieces says on the host), and what rounding left of a value for the second.
+template <class S> constexpr int kPieces = Units<S>::planes == 1 ? 2 : 1;
+template <class S> __device__ __forceinline__ float left_of(float v, typename S::Bits rounded) {
+    const float w = S::widen(rounded);
+    return fabsf(w) < INFINITY ? v - w : 0.0f;
+}
+
 struct GradEpi {
     using Args = GradOut;
+    template <class S> static constexpr bool kTwice = false;
     template <class S, class T>
     static __device__ __forceinline__ void run(const Args& g, Acc<T>& acc, uint32_t im, uint32_t in, char* lds) {
         const int tid = threadIdx.x;
@@ -223,8 +232,16 @@ struct GradEpi {
                 if ((tid & (Rows4<T>::kLanes - 1)) == 0) sums[place.wn * T::BM + row] = sum;
                 const int64_t n = n0 + row, m = m0 + col;
                 if (n >= g.off.N || m >= g.ldg) return;  // (ldg is a multiple of 8)
-                const typename S::Bits b[4] = {S::round(v.x), S::round(v.y), S::round(v.z), S::round(v.w)};
-                __builtin_memcpy(__builtin_assume_aligned(out + n * g.ldg + m, sizeof b), b, sizeof b);
+                auto* to = out + n * (kPieces<S> * g.ldg) + m;
+                typename S::Bits b[4] = {S::round(v.x), S::round(v.y), S::round(v.z), S::round(v.w)};
+                __builtin_memcpy(__builtin_assume_aligned(to, sizeof b), b, sizeof b);
+                if constexpr (kPieces<S> > 1) {
+                    b[0] = S::round(left_of<S>(v.x, b[0]));
+                    b[1] = S::round(left_of<S>(v.y, b[1]));
+                    b[2] = S::round(left_of<S>(v.z, b[2]));
+                    b[3] = S::round(left_of<S>(v.w, b[3]));
+                    __builtin_memcpy(__builtin_assume_aligned(to + g.ldg, sizeof b), b, sizeof b);
+                }
             });
         }
         if (!g.sums) return;
@@ -241,6 +258,7 @@ struct GradEpi {
 
 struct MatrixEpi {
     using Args = MatrixOut;
+    template <class S> static constexpr bool kTwice = kPieces<S> > 1;  // (with each of G's pieces)
     template <class S, class T>
     static __device__ __forceinline__ void run(const Args& g, Acc<T>& acc, uint32_t im, uint32_t in, char* lds) {
         const int64_t i0 = int64_t(im) * T::BM, j0 = int64_t(in) * T::BN;
@@ -284,25 +302,25 @@ struct MatrixEpi {
 }  // namespace
 
 template <class S> hipError_t PairProducts<S>::stats(const PairArgs& a, const TilePlan& t, const StatsOut& o, float* part, hipStream_t s) {
-    const Product g{{a.r, a.ldr, a.K, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr, nullptr}, a.N, a.M, a.K, 0, 0, t.whole, t.splits, part};
+    const Product g{{a.r, a.ldr, a.K, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr, nullptr}, a.N, a.M, a.K, 0, 0, 0, t.whole, t.splits, part};
     return product<S, false, false, StatsEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::grad(const PairArgs& a, const void* r, int64_t n, const TilePlan& t, const GradOut& o, float* part, hipStream_t s) {
-    const Product g{{r, a.ldr, a.K, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr, nullptr}, n, a.M, a.K, 0, 0, t.whole, t.splits, part};
+    const Product g{{r, a.ldr, a.K, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.K, nullptr, nullptr, nullptr}, n, a.M, a.K, 0, 0, 0, t.whole, t.splits, part};
     return product<S, false, false, GradEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::d_references(const PairArgs& a, const void* gr, int64_t ldg, int64_t n, const TilePlan& t,
                                          const MatrixOut& o, float* part, hipStream_t s) {
     // (g holds zeros from M to ldg: whole chunks)
-    const Product g{{gr, ldg, ldg, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.M, nullptr, nullptr, nullptr}, n, a.K, a.M, 0, 0, t.whole, t.splits, part};
+    const Product g{{gr, kPieces<S> * ldg, ldg, nullptr, nullptr, nullptr}, {a.x, a.ldx, a.M, nullptr, nullptr, nullptr}, n, a.K, a.M, ldg, 0, 0, t.whole, t.splits, part};
     return product<S, false, true, MatrixEpi>(g, t, o, s);
 }
 template <class S>
 hipError_t PairProducts<S>::d_images(const PairArgs& a, const void* gr, int64_t ldg, const void* r, const PairOff& off,
                                      const int* look, const TilePlan& t, const MatrixOut& o, float* part, hipStream_t s) {
-    const Product g{{gr, ldg, off.N, nullptr, nullptr, nullptr}, {r, a.ldr, off.N, look, off.mask, off.bias}, a.M, a.K, off.N, 0, 0, t.whole, t.splits, part};
+    const Product g{{gr, kPieces<S> * ldg, off.N, nullptr, nullptr, nullptr}, {r, a.ldr, off.N, look, off.mask, off.bias}, a.M, a.K, off.N, ldg, 0, 0, t.whole, t.splits, part};
     return product<S, true, true, MatrixEpi>(g, t, o, s);
 }
 

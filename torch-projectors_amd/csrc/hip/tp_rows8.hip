@@ -283,6 +283,7 @@ struct ScaledOut {
 };
 template <class O> struct ScaledEpi {
     using Args = ScaledOut;
+    template <class S> static constexpr bool kTwice = false;
     template <class S, class T>
     static __device__ __forceinline__ void run(const Args& g, Acc<T>& acc, uint32_t im, uint32_t in, char* lds) {
         const Place<T> place(threadIdx.x);
@@ -349,7 +350,7 @@ template <class O> hipError_t row_scores(const Rows8Args& g, const Rows8Plan& p,
     if (!p.few) {
         const int64_t half = int64_t(g.steps) * kRow / 2;  // (pairs of codes)
         const TilePlan t = rows8_tiles(g.M, g.N, g.steps);
-        const Product product{{g.a, half, half, nullptr, nullptr, nullptr}, {g.b, half, half, nullptr, nullptr, nullptr}, g.M, g.N, half, 0, 0,
+        const Product product{{g.a, half, half, nullptr, nullptr, nullptr}, {g.b, half, half, nullptr, nullptr, nullptr}, g.M, g.N, half, 0, 0, 0,
                               t.whole, t.splits, reinterpret_cast<float*>(g.part)};
         return tp::product<I8x2, false, false, ScaledEpi<O>>(product, t, ScaledOut{g.sa, g.sb, g.bias, g.out, g.M, g.N}, s);
     }

@@ -184,10 +184,11 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
     // The loads are written out: behind a builtin the compiler waits for all of them before it reads any transposed fragment, of
     // whichever stage.  They have no registers to return to; arrive() waits for them.  (m0 is reserved: the compiler sets it before each
     // use of its own)
-    __device__ __forceinline__ void fill(int64_t k0, const char* lds) const {
+    // from: elements from the operand's first value to those meant
+    __device__ __forceinline__ void fill(int64_t k0, const char* lds, int64_t from) const {
         constexpr uint32_t kNowhere = 0x80000000u;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        const char* at = base + (ACROSS ? k0 * ld * int64_t(sizeof(Bits)) : 0);
+        const char* at = base + (from + (ACROSS ? k0 * ld : 0)) * int64_t(sizeof(Bits));
         const int64_t values = ACROSS ? (kdim - k0 - 1) * ld + dim : (dim - 1) * ld + kdim;
         const int64_t bytes = min(values * int64_t(sizeof(Bits)), int64_t(0x7fffffff));
         // a raw buffer: base address, its upper half, size, and the data format of 32-bit words
@@ -285,9 +286,10 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
 
 // What the products' kernels share: the first `whole` tiles are one workgroup each; of the others [splits] ranges of
 // the contraction are one each, and where there are several their fragments go to part, which k_tile_join adds up.
+// Where the epilogue says so (kTwice) the contraction is gone through once more, with a's values `again` elements further on.
 struct Product {
     Operand a, b;
-    int64_t rows, cols, kdim;
+    int64_t rows, cols, kdim, again;
     uint32_t tm, tn, whole;
     int splits;
     float* part;
@@ -360,7 +362,8 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
     SB b;
     a.init(g.a, int64_t(im) * T::BM, g.rows, tid);
     b.init(g.b, int64_t(in) * T::BN, g.cols, tid);
-    const int64_t steps = (g.kdim + BK - 1) / BK;
+    constexpr bool kTwice = Epi::template kTwice<S>;
+    const int64_t turn = (g.kdim + BK - 1) / BK * BK, steps = turn / BK * (kTwice ? 2 : 1);
     const int64_t k0 = steps * split / splits * BK, k1 = steps * (split + 1) / splits * BK;
 
     Acc<T> acc;
@@ -397,8 +400,10 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
         int4 fa[2][T::FM], fb[2][T::FN];
         auto stage = [&](int s) { return lds + s % kStages * kStage; };
         auto fill = [&](int s) {
-            a.fill(k0 + int64_t(s) * BK, stage(s));
-            b.fill(k0 + int64_t(s) * BK, stage(s) + kA);
+            const int64_t k = k0 + int64_t(s) * BK;
+            const bool again = kTwice && k >= turn;
+            a.fill(again ? k - turn : k, stage(s), again ? g.again : 0);
+            b.fill(again ? k - turn : k, stage(s) + kA, 0);
         };
         auto read = [&](int s, int t) {
             const char *sa = stage(s), *sb = sa + kA;
@@ -505,34 +510,42 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
             a.store(lds + r * kStage, ra[r], ka[r]);
             b.store(lds + r * kStage + kA, rb[r], kb[r]);
         };
-        const int64_t kw = max(k0, min(k1, min(a.whole(), b.whole()))), last = kw - BK;
-        if (k0 < kw) {
-            load(k0, 0);
-            load(min(k0 + BK, last), 1);
-            store(0);
-        }
 #pragma unroll 1
-        for (int64_t k = k0; k < kw; k += 2 * BK) {
-            if (kTwo && k % kFlush < 2 * BK) flush();
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int64_t at = k + r * BK;
-                if (at >= kw) break;
+        for (int pass = 0; pass < (kTwice ? 2 : 1); ++pass) {
+            const int64_t p0 = pass ? max(k0 - turn, int64_t(0)) : k0, p1 = pass ? k1 - turn : kTwice ? min(k1, turn) : k1;
+            if (pass) {
+                a.base += g.again * int64_t(sizeof(typename S::Bits));
                 __syncthreads();
-                load(min(at + 2 * BK, last), r);  // (past the end: the last one again, not used)
-                multiply(lds + r * kStage);
-                if (at + BK < kw) store(r ^ 1);
             }
-        }
-        // what is left of the contraction
+            const int64_t kw = max(p0, min(p1, min(a.whole(), b.whole()))), last = kw - BK;
+            if (p0 < kw) {
+                load(p0, 0);
+                load(min(p0 + BK, last), 1);
+                store(0);
+            }
 #pragma unroll 1
-        for (int64_t k = kw; k < k1; k += BK) {
-            a.load_some(k, ra[0], ka[0]);
-            b.load_some(k, rb[0], kb[0]);
-            __syncthreads();
-            store(0);
-            __syncthreads();
-            multiply(lds);
+            for (int64_t k = p0; k < kw; k += 2 * BK) {
+                if (kTwo && k % kFlush < 2 * BK) flush();
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int64_t at = k + r * BK;
+                    if (at >= kw) break;
+                    __syncthreads();
+                    load(min(at + 2 * BK, last), r);  // (past the end: the last one again, not used)
+                    multiply(lds + r * kStage);
+                    if (at + BK < kw) store(r ^ 1);
+                }
+            }
+            // what is left of the contraction
+#pragma unroll 1
+            for (int64_t k = kw; k < p1; k += BK) {
+                a.load_some(k, ra[0], ka[0]);
+                b.load_some(k, rb[0], kb[0]);
+                __syncthreads();
+                store(0);
+                __syncthreads();
+                multiply(lds);
+            }
         }
     }
     if constexpr (kTwo) {
