@@ -97,3 +97,10 @@ def test_sizes_of_the_rounding_tests_reach_every_tile(dt):
         for tile, direct in ((0, True), (1, True), (2, True), (0, False), (1, False)):
             assert any(f[:3] == (name, tile, direct) for f in ran), (name, tile, direct)
         assert any(f[0] == name and f[2] and f[3] for f in ran) and any(f[0] == name and not f[2] and f[3] for f in ran), name
+
+
+def test_sizes_of_the_long_sums_reach_both_tiles_with_two_sums():
+    from tests.test_gpu_pairs_float32 import LONG_SUMS
+    ran = forms(LONG_SUMS, P.F32)
+    for name in ("images", "references"):
+        assert {f[1] for f in ran if f[0] == name} == {0, 1}, (name, ran)

@@ -380,11 +380,12 @@ __global__ __launch_bounds__(T::NT) void k_tile(Product g, typename Epi::Args ea
                 for (int e = 0; e < 16; ++e) v[i][j][e] = 0.0f;
     };
     clear(acc);
-    // A sum over thousands of products in one go loses what its own size is to each of them: every kFlush of the contraction it is
-    // added to another set of registers and begun anew (for scores, whose differences count, and where there are registers: not in
-    // 16-bit tiles of 256 x 256).  Of 2048 x 8192 float32 pairs of 16640 values log_sum is 4.8e-6 off without and 3.4e-7
-    // with it.
-    constexpr bool kTwo = !Units<S>::whole && T::FM * T::FN <= 4 && !BTR;
+    // A sum over thousands of products in one go loses what its own size is to each of them, and the units round towards zero: every
+    // kFlush of the contraction it is added to another set of registers and begun anew.  For scores, whose differences count, where
+    // there are registers (not in 16-bit tiles of 256 x 256): of 2048 x 8192 float32 pairs of 16640 values log_sum is 4.8e-6 off without and
+    // 3.4e-7 with it.  For gradients of float32 rows where there are (not in tiles of 256 x 128; sums of 100000 terms of one sign 2.8e-6 off
+    // without and 1.3e-7 with it); those of 16-bit rows are rounded to 2^-11 or less.
+    constexpr bool kTwo = !Units<S>::whole && T::FM * T::FN <= 4 && (!BTR || (PL > 1 && T::FM * T::FN <= 2));
     constexpr int kFlush = 512;
     Acc<T> total;
     if constexpr (kTwo) clear(total);
