@@ -48,3 +48,20 @@ def test_long_sums_of_gradients(m, M, N, K):  # noqa: F811
     for name, error in (("d_images", off(dx, p @ r64)), ("d_references", off(dr, p.t() @ x64))):
         print(name, float(error.mean()), float(error.square().mean().sqrt()), float(error.abs().max()))
         assert float(error.mean().abs()) < 3e-7 and float(error.abs().max()) < 2e-6, name
+
+
+# 128 x 128 and 256 x 128 tiles of the scores, in ranges and whole
+LONG_ROWS = [(100, 5000, 8280), (500, 1000, 16640), (1100, 1500, 16640), (2048, 4096, 16640)]
+
+
+@pytest.mark.parametrize("M,N,K", LONG_ROWS)
+def test_long_rows_of_large_tiles(m, M, N, K):  # noqa: F811
+    """Scores of 16640 positive products: 7e-8 off on average.  One of the six products of pieces is 7e-6 of them or more, and one set
+    of registers loses 4.8e-6."""
+    g = gen(63)
+    x, r = torch.rand(M, K, generator=g, device=DEV), 1 + torch.rand(N, K, generator=g, device=DEV)
+    out = m.pair_log_probs(x, r, bias=-(torch.arange(N, device=DEV) % 7 * 100.0), temperature=40.0)
+    z = (x.double() @ r.double().t() - (torch.arange(N, device=DEV) % 7 * 100.0).double()) / 40.0
+    error = off(out.log_sum, torch.logsumexp(z, 1))
+    print(float(error.square().mean().sqrt()), float(error.abs().max()))
+    assert float(error.abs().max()) < 1e-6

@@ -104,3 +104,20 @@ def test_sizes_of_the_long_sums_reach_both_tiles_with_two_sums():
     ran = forms(LONG_SUMS, P.F32)
     for name in ("images", "references"):
         assert {f[1] for f in ran if f[0] == name} == {0, 1}, (name, ran)
+
+
+def test_sizes_of_the_long_rows_reach_the_large_tiles_with_two_sums():
+    from tests.test_gpu_pairs_float32 import LONG_ROWS
+    ran = forms(LONG_ROWS, P.F32)
+    assert {f[1:] for f in ran if f[0] == "scores"} == {(1, False, True), (2, False, False), (2, False, True)}
+
+
+def test_sizes_of_the_masked_tests_reach_the_largest_tiles():
+    from tests.test_gpu_pairs_masked_tiles import LARGE, MASKED
+    for dtype, M, N, K in MASKED:
+        dt = P.CODES[str(dtype)]
+        b = P.back_layout(dt, dt != P.F32, M, N, K)
+        assert b.imgs.tile == 2 and (b.references < N or N == 100), (dtype, M, N, K)
+    for dtype, M, N, K in LARGE:
+        dt = P.CODES[str(dtype)]
+        assert P.tile_plan(dt, dt != P.F32, N, M, K).tile == 2, (dtype, M, N, K)
