@@ -60,3 +60,18 @@ def test_gradients_of_half_rows_are_rounded_once(m, M, N, K, dtype):  # noqa: F8
     for k, other in (("d_images", "references"), ("d_references", "images")):
         tol = w["tol_" + k] + tiny * p[other].double().abs().sum(0)
         near(got[k], w[k], tol + half_step(w[k].abs() + tol, dtype), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(9, 1, 8), (65, 63, 72), (333, 129, 264), (333, 129, 131), (4097, 4095, 72)])
+def test_last_image_and_last_reference(m, M, N, K, dtype):  # noqa: F811
+    """Odd numbers of both: the last value of the scores' gradient is read where its operand ends."""
+    p = problem(M, N, K, dtype, seed=53)
+    p["mask"][:] = False
+    p["mask"][N - 1] = True
+    p["given"][:] = -1
+    p["given"][::2] = N - 1
+    got, w = run(m, p), want(p)
+    assert (w["d_images"][M - 1].abs().max() > 0) and (w["d_references"][N - 1].abs().max() > 0)
+    for k, v in got.items():
+        near(v, w[k], w["tol_" + k], k)

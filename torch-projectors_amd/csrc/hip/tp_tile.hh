@@ -126,7 +126,7 @@ struct Operand {
 //             reading one chunk of 16 rows reach each of the 64 banks once
 //   across:   LDS row k holds DIM values; four rows of 64 bytes, as 32 lanes read them, at places that differ by 64
 // DIRECT: from memory straight to LDS, without registers between (16-bit values whose rows start at 16-byte
-// boundaries; an adjacent contraction is a whole number of chunks).
+// boundaries; a row is a whole number of chunks, or is followed by what makes it one).
 template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Side {
     static constexpr int PL = Units<S>::planes;
     static constexpr int CPR = ACROSS ? DIM / 8 : BK / 8, CH = DIM * BK / 8 / NT;
@@ -193,7 +193,8 @@ template <class S, bool ACROSS, int DIM, int NT, bool DIRECT, int BK> struct Sid
         constexpr uint32_t kNowhere = 0x80000000u;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const char* at = base + (from + (ACROSS ? k0 * ld : 0)) * int64_t(sizeof(Bits));
-        const int64_t values = ACROSS ? (kdim - k0 - 1) * ld + dim : (dim - 1) * ld + kdim;
+        // (whole chunks: of a 32-bit word that the buffer ends in the middle of neither half arrives)
+        const int64_t values = ACROSS ? (kdim - k0 - 1) * ld + ((dim + 7) & ~int64_t(7)) : (dim - 1) * ld + kdim;
         const int64_t bytes = min(values * int64_t(sizeof(Bits)), int64_t(0x7fffffff));
         // a raw buffer: base address, its upper half, size, and the data format of 32-bit words
         const uint64_t address = reinterpret_cast<uint64_t>(at);
