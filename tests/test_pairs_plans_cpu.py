@@ -121,3 +121,14 @@ def test_sizes_of_the_masked_tests_reach_the_largest_tiles():
     for dtype, M, N, K in LARGE:
         dt = P.CODES[str(dtype)]
         assert P.tile_plan(dt, dt != P.F32, N, M, K).tile == 2, (dtype, M, N, K)
+
+
+def test_ranges_of_few_images():
+    """16 at most, and none without a round of loads."""
+    rng = random.Random(3)
+    for _ in range(2000):
+        dt = rng.choice([P.F32, P.F16, P.BF16])
+        N, K = int(math.exp(rng.uniform(0, 14))), int(math.exp(rng.uniform(0, math.log(1 << 21))))
+        s = P.lib().splits(dt, P._L(N), P._L(K))
+        units = -(-K * SIZES[dt] // 128)
+        assert 1 <= s <= 16 and (s == 1 or s <= -(-units // 32)), (dt, N, K, s)

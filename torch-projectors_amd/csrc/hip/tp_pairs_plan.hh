@@ -20,12 +20,14 @@ inline int64_t up16(int64_t bytes) { return up_to(bytes, 16); }
 inline int size_of(int dt) { return dt == TP_F32 ? 4 : 2; }
 
 // ------------------------------------------------------------------ few images
-// Ranges of the rows' values: as many workgroups as hide a load's way.
+// Ranges of the rows' values: as many workgroups as hide a load's way, each of at least a round of loads, and 16 at most, as one workgroup an image
+// adds them up (1 x 16 x 262144 bfloat16 26 us, in 128 ranges 42; 1 x 40 x 16640 float32 13.1, in 17 ranges 13.9).
 inline int few_splits(int dt, int64_t N, int64_t K) {
     const int64_t groups = (N + 15) / 16, units = (K * size_of(dt) + kUnit - 1) / kUnit;
     int64_t s = (2 * kCus + groups - 1) / groups;
     const int64_t most = (units + kFewWaves * kAhead - 1) / (kFewWaves * kAhead);
-    return int(s < 1 ? 1 : s > most ? most : s > 16 ? 16 : s);
+    if (s > most) s = most;
+    return int(s < 1 ? 1 : s > 16 ? 16 : s);
 }
 // References that a workgroup joins: all of them up to 8192, which it reads in two steps, and a step's each beyond, whose parts take a
 // launch more (1 x 36864 x 1024 bfloat16 24 us, in one workgroup 5 us longer).
