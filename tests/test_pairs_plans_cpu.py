@@ -132,3 +132,17 @@ def test_ranges_of_few_images():
         s = P.lib().splits(dt, P._L(N), P._L(K))
         units = -(-K * SIZES[dt] // 128)
         assert 1 <= s <= 16 and (s == 1 or s <= -(-units // 32)), (dt, N, K, s)
+
+
+def test_more_tiles_than_a_launch_holds():
+    """No call is accepted that has them; the plan is the one of the fewest tiles, and the product refuses."""
+    for dt, direct, tile in ((P.F16, False, 1), (P.BF16, True, 2), (P.F32, False, 2)):
+        t = P.tile_plan(dt, direct, 1 << 26, 1 << 21, 64)
+        assert t.tile == tile and t.tiles > P.limit(0)
+
+
+def test_no_kernels_that_no_call_reaches():
+    """Codes go straight to LDS: no tiles that are staged in registers."""
+    from tests.test_kernel_resources_cpu import _kernels, _report
+    tiles = [n for n in _kernels(_report("tp_rows8.hip"), "k_") if "6k_tileI" in n]
+    assert len(tiles) == 6 and all("ELb0ELb0ELb1ENS" in n for n in tiles), tiles

@@ -19,8 +19,8 @@ struct PairArgs {
     float c;               // 1 / temperature
 };
 
-// Floats of the state that the gradient reads: four statistics of each image (largest score, the others' sum of
-// exp(score - largest), the given reference's, and its score), and where there are few images their scores.
+// Floats of the state that the gradient reads: four of each image (largest score, the others' sum of
+// exp(score - largest), the given reference's, and one that is not used), and where there are few images their scores.
 inline bool pair_few(int64_t M) { return M <= kFewImages; }
 inline int64_t pair_state(int64_t M, int64_t N) { return 4 * M + (pair_few(M) ? M * N : 0); }
 

@@ -21,7 +21,7 @@
 namespace tp {
 namespace {
 
-constexpr int kStats = 4;  // largest, others, own, and the given reference's score
+constexpr int kStats = 4;  // largest, others' sum, own, and one to spare: an image's stand in 16 bytes
 
 __device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
 // (largest, sum of exp(z - largest)) of two sets of scores
@@ -52,7 +52,6 @@ __device__ __forceinline__ void finish(const PairArgs& a, int64_t m, float most,
         st[0] = base;
         st[1] = others;
         st[2] = own;
-        st[3] = z;
     }
 }
 

@@ -666,6 +666,7 @@ template <class S, class T, bool ATR, bool BTR, bool DIRECT, class Epi>
 hipError_t product_of(Product g, const typename Epi::Args& ea, hipStream_t s) {
     g.tm = uint32_t((g.rows + T::BM - 1) / T::BM);
     g.tn = uint32_t((g.cols + T::BN - 1) / T::BN);
+    if (int64_t(g.tm) * g.tn > kMaxTiles) return hipErrorInvalidValue;
     const uint32_t tiles = g.tm * g.tn, rest = tiles > g.whole ? tiles - g.whole : 0;
     g.whole = tiles - rest;
     k_tile<S, T, ATR, BTR, DIRECT, Epi><<<dim3(g.whole + rest * g.splits), T::NT, 0, s>>>(g, ea);
@@ -687,8 +688,10 @@ hipError_t product(const Product& g, const TilePlan& t, const typename Epi::Args
     } else if (t.tile == 2) {
         return product_of<S, Large, ATR, BTR, false, Epi>(g, ea, s);
     }
-    if (t.tile == 0) return product_of<S, Small, ATR, BTR, false, Epi>(g, ea, s);
-    if (t.tile == 1) return product_of<S, Middle, ATR, BTR, false, Epi>(g, ea, s);
+    if constexpr (!Units<S>::whole) {  // (codes are rows of whole chunks)
+        if (t.tile == 0) return product_of<S, Small, ATR, BTR, false, Epi>(g, ea, s);
+        if (t.tile == 1) return product_of<S, Middle, ATR, BTR, false, Epi>(g, ea, s);
+    }
     return hipErrorInvalidValue;
 }
 

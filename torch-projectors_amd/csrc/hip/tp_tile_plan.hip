@@ -29,9 +29,10 @@ constexpr int kMaxSplits = 32;
 // costs their sums written and read (by one workgroup a tile, at some 70 GB/s).  Against all tiles and 1 to 16 ranges
 // on 88 products from 20 x 5000 to 4096 x 12288 the choice is 2 % from the best on average, at most 17 %.
 TilePlan tile_plan(int dt, bool direct, int64_t rows, int64_t cols, int64_t kdim) {
-    TilePlan best{direct, 0, 0, 1};
+    const int kinds = dt == TP_F32 || direct ? 3 : 2;
+    TilePlan best{direct, kinds - 1, 0, 1};  // (the fewest tiles: where these are more than a launch holds the product refuses)
     double least = 1e300;
-    for (int t = 0; t < (dt == TP_F32 || direct ? 3 : 2); ++t) {
+    for (int t = 0; t < kinds; ++t) {
         const TileKind& k = kind_of(dt, TilePlan{direct, t, 0, 1});
         const int64_t tiles = ((rows + k.bm - 1) / k.bm) * ((cols + k.bn - 1) / k.bn);
         if (tiles > kMaxTiles) continue;
