@@ -6,7 +6,7 @@
 //             as 127^2 times 131072 values is below 2^31.
 //
 // Codes are evenly spaced, so a row keeps 1 / 254 of its largest value: for whitened images, whose values are all of a size,
-// that is finer than 8-bit floating point's 3-bit mantissa, at twice the rate of the bfloat16 units which those need.
+// that is finer than 8-bit floating point's 3-bit mantissa.  Products run at 2.0 to 2.4 POP/s, 1.6 times a bfloat16 library product's rate.
 #include "../../../include/torch_projectors_hip.h"
 #include "tp_match.hh"
 #include "tp_tile.hh"

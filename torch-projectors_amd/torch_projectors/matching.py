@@ -115,8 +115,10 @@ def quantize_rows(x: torch.Tensor) -> RowScaled:
     half to even; both quotients are those of float32.  A row with a value that is not finite has scale NaN and codes
     0, so that its scores are NaN.  Not differentiable.
 
-    The steps are even, 1/127 of a row's largest value: finer than those of `quantize_blocks` for rows whose values
-    are all of a size (whitened images), coarser where they fall by orders of magnitude along a row."""
+    The steps are even, 1/127 of a row's largest value.  Scores are three times closer than those of `quantize_blocks` where
+    both sides' large values meet: whitened images, and rows that fall by orders of magnitude alike (4224 values: 1.9e-4
+    of |image| |reference| to 5.8e-4, and 4.2e-4 to 1.2e-3 for rows that fall by 100).  Where a side's small values
+    meet the other's large ones, take the blocks, which keep 3 bits of every value."""
     return RowScaled(*_OPS.quantize_rows.default(_real_rows(x, "x")))
 
 
