@@ -1,5 +1,6 @@
 """HIP streams of a test's own, default priority.  PyTorch hands out its pool's 32 in turn, so each taken from there moves which
-of them a later test gets, and with it whether calls that keep something by stream have seen it."""
+of them a later test gets, and with it whether calls that keep something by stream have seen it: tests/test_zz_no_alloc.py captures on two
+that no earlier call may have used.  A test that only needs another stream takes one from here."""
 import ctypes
 import functools
 import os

@@ -333,14 +333,17 @@ struct Rows8Plan {
 // The tiles' plan is that of 16-bit products: their steps are as long, as many bytes go through LDS for as many instructions.
 TilePlan rows8_tiles(int64_t M, int64_t N, int64_t steps) { return tile_plan(TP_BF16, true, M, N, steps * kRow / 2); }
 
-// One image, and few images of at most 16384 references: k_rows8_few (2 and 16 x 4096 x 16640 14.3 and 18.1 us, in tiles 20; but x 36864
-// x 4224 33 and 44, in tiles 28).  From 17 to 32 images it takes two fragments of them, up to 2048 references (24 x 1000 x 4224 7.3 us, in
-// tiles 10.2; x 4096 x 16640 23.1 and 19.7).
+// One image, and few images of not too many references: k_rows8_few, which reads them at up to 5 TB/s but for every 16 images again.  The
+// borders by references and by bytes of their codes, each varied with the other held (us, k_rows8_few / tiles):
+//   8 images    8192 references of 1024, 4224, 16640 codes 4.4 / 5.8, 9.7 / 13.8, 28 / 28; 16384: 7.2 / 5.9, 17 / 19, 56 / 52; 36864: 16 / 9.9, 36 / 27, 133 / 129
+//   16 images   4096: 3.4 / 5.8, 6.1 / 14.2, 17.7 / 19.6; 8192: 5.0 / 6.0, 11.1 / 14.1, 33 / 29; 16384: 8.1 / 6.1, 19.8 / 19.1, 65 / 53
+//   32 images   2048: 4.0 / 6.1, 8.0 / 11.2, 16.3 / 17.0; 4096: 3.9 / 6.0, 7.9 / 14.3, 25 / 20; 8192: 6.3 / 6.1, 15.3 / 14.2, 48 / 29
 Rows8Plan rows8_plan(int64_t M, int64_t N, int64_t steps) {
     Rows8Plan p{M <= 16 ? 1 : 2, 1};
     if (M == 1) return p;  // (its image is rounded in the same launch)
-    const int64_t groups = (N + 15) / 16;
-    if (M > 32 || groups > (M > 16 ? 128 : 1024)) return {0, 1};
+    const int64_t groups = (N + 15) / 16, bytes = N * steps * kRow;
+    const bool streams = M <= 8 ? N <= 16384 : M <= 16 ? N <= 8192 && bytes <= 80 << 20 : M <= 32 && N <= 4096 && bytes <= 36 << 20;
+    if (!streams) return {0, 1};
     const int64_t wanted = (kCus + groups - 1) / groups, most = (steps + kFewWaves * kAhead - 1) / (kFewWaves * kAhead);
     p.splits = int(wanted > most ? most : wanted);
     return p;
