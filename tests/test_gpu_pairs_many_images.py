@@ -55,3 +55,20 @@ def test_millions_of_images(m, dtype, M):  # noqa: F811
         w = R.pair_log_probs(x[rows], r, None, bias, d_log_sum=up[rows])
         near(out.log_sum[rows], w["log_sum"], w["tol_log_sum"], "log_sum")
         near(dx[rows], w["d_images"], w["tol_d_images"], "d_images")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(3, 10000000, 4), (12, 5000000, 8), (12, 3000001, 3)])
+def test_millions_of_references(m, M, N, K, dtype):  # noqa: F811
+    """Thousands of parts of an image's scores, and pieces of the references.
+
+    The native exponential has no subnormal results: probabilities below 2^-126 of the largest count as 0, which takes at most 2^-126 of the
+    upstream gradients times what a gradient's other factors add up to."""
+    print(dtype, M, N, flush=True)
+    p = problem(M, N, K, dtype, seed=32)
+    p["given"][0] = N - 1
+    got, w = run(m, p), want(p)
+    least = 2.0 ** -126 * float((p["d_given"].abs() + p["d_log_sum"].abs()).max()) / p["temperature"]
+    lost = dict(d_images=least * p["references"].double().abs().sum(0), d_references=least * p["images"].double().abs().sum(0), d_bias=least * M)
+    for k, v in got.items():
+        near(v, w[k], w["tol_" + k] + lost.get(k, 0.0), k)
