@@ -65,3 +65,15 @@ def test_long_rows_of_large_tiles(m, M, N, K):  # noqa: F811
     error = off(out.log_sum, torch.logsumexp(z, 1))
     print(float(error.square().mean().sqrt()), float(error.abs().max()))
     assert float(error.abs().max()) < 1e-6
+
+
+@pytest.mark.parametrize("power", [108, 116, 124, 132, 140])
+@pytest.mark.parametrize("M", [8, 64])
+def test_values_next_to_the_smallest(m, M, power):  # noqa: F811
+    """The pieces' last bits end at 2^-133: of more than 8 images a value is off by less than that."""
+    g = gen(64)
+    x = (1 + torch.rand(M, 16, generator=g, device=DEV)) * 2.0 ** min(power - 6, 120)
+    r = ((1 + torch.rand(1, 16, generator=g, device=DEV, dtype=torch.float64)) * 2.0 ** -power).float()
+    z = (x.double() @ r.double().t())[:, 0]
+    error = (m.pair_log_probs(x, r).log_sum.double() - z).abs()
+    assert (error <= 5e-7 * z + (2.0 ** -133 * x.double().sum(1) if M > 8 else 0.0)).all()

@@ -172,7 +172,10 @@ def pair_log_probs(images: torch.Tensor, references: torch.Tensor, given: Option
     The gradient reaches images, references (in their dtype) and bias from both results.  It forms the scores
     again, for a piece of the references and of the images (32768 at most) after the other; a piece's share of the
     gradient of the scores is kept (at most 128 MB; of 16-bit rows in two numbers of their dtype, so that the results are
-    rounded once), and sums over several pieces in float32.  Up to 8 images keep their scores instead."""
+    rounded once), and sums over several pieces in float32.  Up to 8 images keep their scores instead.
+
+    Products of float32 values lose no more than float32 does, but of more than 8 images values count as multiples of
+    2^-133.  Probabilities below 2^-126 of an image's largest count as 0."""
     x, r = _real_rows(images, "images"), _real_rows(references, "references")
     if x.shape[1] != r.shape[1]:
         raise ValueError(f"Images of {x.shape[1]} values do not fit references of {r.shape[1]}")
