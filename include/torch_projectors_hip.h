@@ -368,7 +368,8 @@ int tp_row_score_images(int dtype, const void* x, int64_t rows_a, int64_t cols, 
  *               reference that is ruled out holds is not used
  * Outputs fp32: given_log_probs [image_rows] (with given), log_sum [image_rows] (of exp(score));
  * state, tp_pair_state() floats that the gradient reads (optional: NULL where none will).
- * An image with no allowed reference has log_sum and log probabilities -inf. */
+ * An image with no allowed reference has log_sum and log probabilities -inf; one with a score that is not finite
+ * (-inf among them) of an allowed reference has NaN. */
 int64_t tp_pair_state(int64_t image_rows, int64_t reference_rows);
 int64_t tp_pair_log_probs_work(int dtype, int64_t image_rows, int64_t reference_rows, int64_t cols);
 int tp_pair_log_probs(int dtype, const void* images, int64_t image_rows, int64_t cols, int64_t image_stride,

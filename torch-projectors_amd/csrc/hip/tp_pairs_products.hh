@@ -1,8 +1,10 @@
 // The tiled products of the pair log probabilities for one storage type (included by tp_pairs_*.hip).
 //
-// The matrix units bound them, at some 2.0 GHz under this load.  4096 x 36864 bfloat16 pairs of 4224 values: 1218 us for the scores and
-// their statistics (1.05 PFLOP/s), 1276 formed again for G, 1455 for the references' gradients and 1384 for the images'.
-// 2048 x 8192 float32 pairs of 4224: 709, 715, 788 and 782 us (180 to 200 TFLOP/s of six products each).
+// 4096 x 36864 bfloat16 pairs of 4224 values: 1230 us for the scores and their statistics (1.04 PFLOP/s), 1440 formed again for G in five pieces, 2880
+// for the references' gradients and 3220 for the images' (0.89 and 0.79 PFLOP/s, each with both pieces of G).  The matrix units are 36 to 50 % busy;
+// wavefronts wait 35 to 45 % of their time at a step's barrier, for loads and for each other, and nothing else is on the CU to fill that.
+// 2048 x 8192 float32 pairs of 4224: 720, 717, 816 and 797 us (174 to 198 TFLOP/s of six products each).  Matrix instructions (52 to 61 %) and
+// those that cut values into pieces (34 %) take nearly all of the SIMDs' time between them.
 // A product has both its operands in one type: G goes through 16-bit units in two pieces, what rounding it leaves being the second.  With the first alone
 // bfloat16 gradients are 2.3e-3 off, and 1.7e-3 with both, which is their own rounding.
 #pragma once
