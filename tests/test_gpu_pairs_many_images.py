@@ -72,3 +72,39 @@ def test_millions_of_references(m, M, N, K, dtype):  # noqa: F811
     lost = dict(d_images=least * p["references"].double().abs().sum(0), d_references=least * p["images"].double().abs().sum(0), d_bias=least * M)
     for k, v in got.items():
         near(v, w[k], w["tol_" + k] + lost.get(k, 0.0), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_some_gradients_of_pieces(m, dtype):  # noqa: F811
+    """What is not wanted is not formed, and does not change the rest."""
+    p = problem(33000, 4200, 16, dtype, seed=33)
+    every = run(m, p)
+    for wants in (("images",), ("references",), ("bias",), ("references", "bias")):
+        some = run(m, p, wants=wants)
+        for k in wants:
+            assert torch.equal(some["d_" + k], every["d_" + k]), k
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_pieces_in_two_graphs(m, dtype):  # noqa: F811
+    """Captured twice with other inputs and replayed in turn, with eager calls in between: what pieces add up begins anew each time."""
+    ps = [problem(33000, 4200, 16, dtype, seed=s) for s in (34, 35)]
+
+    def step(p):  # (leaves of its own)
+        x, r, b = (p[k].detach().requires_grad_() for k in ("images", "references", "bias"))
+        out = m.pair_log_probs(x, r, p["given"], bias=b, temperature=p["temperature"], mask=p["mask"])
+        return (out.log_sum.detach(), *torch.autograd.grad((out.given, out.log_sum), (x, r, b), (p["d_given"], p["d_log_sum"])))
+
+    wanted = [[t.clone() for t in step(p)] for p in ps]
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in ps], []
+    for graph, p in zip(graphs, ps):
+        with torch.cuda.graph(graph):
+            outs.append(step(p))
+    for n in (0, 1, 1, 0):
+        for t in outs[n]:
+            t.fill_(NAN)
+        graphs[n].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[n], wanted[n])), n
+        assert all(torch.equal(a, b) for a, b in zip(step(ps[n]), wanted[n])), n
